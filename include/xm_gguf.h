@@ -58,7 +58,8 @@ int xm_abi_version(void);
 const char* xm_last_error(void);
 
 /* Device error word of the current device: a non-zero bit means a bounded wait
- * inside a kernel gave up (XM_DEVERR_TIMEOUT = 1) instead of hanging.  With
+ * inside a kernel gave up (XM_DEVERR_TIMEOUT = 1) instead of hanging, or that a
+ * paged-cache kernel met a position without a page (XM_DEVERR_PAGE = 2).  With
  * clear != 0 the word is reset.  Returns the word (>= 0) or XM_ERR_CUDA. */
 int xm_device_status(int clear);
 
@@ -326,6 +327,80 @@ int xm_attention(const float* d_qkv, int64_t qkv_stride, void* d_kcache, void* d
                  int Lq, int Hq, int Hk, int head_dim, float theta, int64_t max_ctx, float* d_out,
                  int64_t out_stride, void* d_workspace, int64_t workspace_bytes, void* stream);
 int xm_argmax(const float* d_logits, int64_t B, int64_t V, int* d_out, void* stream);
+
+/*
+ * Paged key/value cache (cache of attention.py:99-104 in pages of tokens).
+ *
+ * The pool holds `pages` pages of xm_kv_page_bytes() bytes: [Hk][keys, values]
+ * of page_size tokens (a power of two, 16..1024; head_dim D 64 or 128), 16-byte
+ * aligned.  XM_KV_F16: [page_size][D] fp16.  XM_KV_Q4_0: [page_size][D / 2]
+ * bytes of codes, then [page_size][D / 32] fp16 scales; 32 values are
+ * d (c - 8), the values of GGUF Q4_0 blocks (gguf_dequant.py:25-46).  With
+ * n = D / 32, nibble i of 32-bit word p of a row of keys is value
+ * 32 (p % n) + 8 (p / n) + i, nibble i of 16-bit word h of a row of values is
+ * value 32 (h % n) + 4 (h / n) + i.
+ *
+ * The new tokens of a call are rows 0 .. T - 1.  Row t belongs to the sequence s
+ * with cu[s] <= t < cu[s + 1] (int32 [B + 1], ascending; null: T = B, row t is
+ * sequence t); lens[s] (int32 [B]) counts the tokens of s with its new ones, so
+ * row t is position lens[s] - (cu[s + 1] - t).  Position p of s is slot
+ * p % page_size of page table[s * table_stride + p / page_size], one of
+ * table_width entries.  Rows behind cu[B] are left alone.  A row at a negative
+ * position (more rows than tokens) is not stored and yields zeros.  A position
+ * past the table or the rotation table, or a page outside the pool, is treated
+ * the same and sets XM_DEVERR_PAGE in xm_device_status.
+ *
+ * xm_kv_append: qkv row t = [q | k | v] (Hq, Hk, Hk heads of D, F32 / F16 /
+ * BF16, row pitch qkv_stride elements).  Each query and key head x is normalised
+ * if d_q_norm / d_k_norm (fp32 [D]) is given, x w / sqrt(mean(x^2) + eps), then
+ * rotated if d_rope (fp32 [rope_rows][D / 2][cos, sin], row = position) is
+ * given, rotate-half (attention.py:66-70).  Queries go to d_q (F16 or BF16, row
+ * pitch q_stride), keys and values to the cache.  4-bit blocks:
+ * d = fp16(first value of largest magnitude / -8), c = floor(x / d + 8.5)
+ * clamped to 0..15, decided exactly on the fp32 value (of a key: normalised and
+ * rotated in 64 bits, rounded once).  A non-finite value makes its block NaN.
+ *
+ * xm_kv_read: the cached keys and values of the rows as fp16 [T][Hk][D].
+ *
+ * xm_kv_attention: out row t (type and head layout of q) =
+ * softmax(q K^T scale) V per query head over the positions 0 .. p of its
+ * sequence, p the row's own (with window > 0: positions above p - window and
+ * the first `sinks` ones); Hq / Hk <= 64 query heads per KV head; a row that
+ * sees no key is zeros.  d_ws: xm_kv_attention_workspace_size bytes (max_keys =
+ * table_width * page_size), 16-byte aligned, no initial contents; two calls
+ * that may run at the same time need one each.
+ *
+ * xm_sample: one token per row of logits (F32 / F16 / BF16, row pitch stride)
+ * (sampling.py:94-158).  Weights exp((x - max) / T); in descending order, equal
+ * logits by ascending index, the first top_k tokens are kept (<= 0: all), of
+ * those the ones before which less than top_p of their mass lies (>= 1: all),
+ * of those the ones of weight >= min_p (the largest is 1); the first is always
+ * kept.  ids[b] = the first token, by index, at which the kept mass up to and
+ * with it exceeds u[b] times the kept mass; logprob[b] (may be null) = log of its share.
+ * T <= 0: the first maximum, with logprob 0.  Each of T, top_k, top_p, min_p is
+ * per row where its device pointer is given.  NaN logits count as -inf; a row
+ * of nothing else gives token 0 with logprob -inf.  Same result for any launch.
+ */
+#define XM_KV_F16 0
+#define XM_KV_Q4_0 1
+int64_t xm_kv_page_bytes(int kv_type, int Hk, int head_dim, int page_size);
+int xm_kv_append(const void* d_qkv, int x_dtype, int64_t T, int64_t qkv_stride, int Hq, int Hk, int head_dim,
+                 const float* d_rope, int64_t rope_rows, const float* d_q_norm, const float* d_k_norm, double eps,
+                 void* d_pool, int64_t pages, int kv_type, int page_size, const int* d_table, int64_t table_stride,
+                 int64_t table_width, const int* d_cu, const int* d_lens, int64_t B, void* d_q, int q_dtype,
+                 int64_t q_stride, void* stream);
+int xm_kv_read(const void* d_pool, int64_t pages, int kv_type, int Hk, int head_dim, int page_size,
+               const int* d_table, int64_t table_stride, int64_t table_width, const int* d_cu, const int* d_lens,
+               int64_t B, int64_t T, void* d_k, void* d_v, void* stream);
+int64_t xm_kv_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hk, int head_dim, int64_t max_keys);
+int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, int Hq, int Hk, int head_dim,
+                    float scale, int64_t window, int64_t sinks, const void* d_pool, int64_t pages, int kv_type,
+                    int page_size, const int* d_table, int64_t table_stride, int64_t table_width, const int* d_cu,
+                    const int* d_lens, int64_t B, void* d_out, int64_t out_stride, void* d_ws, int64_t ws_bytes,
+                    void* stream);
+int xm_sample(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t stride, const float* d_u,
+              float temperature, const float* d_temperature, int top_k, const int* d_top_k, float top_p,
+              const float* d_top_p, float min_p, const float* d_min_p, int* d_ids, float* d_logprob, void* stream);
 
 /*
  * Tensor-parallel exchange over NVLink peer memory (one process per GPU of a

@@ -7,6 +7,7 @@ fails with ``ImportError`` when the shared library has not been built
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -18,7 +19,10 @@ XM_ERR_UNSUPPORTED = -2
 XM_ERR_CUDA = -3
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+ERR_TIMEOUT, ERR_PAGE = 1, 2   # bits of the device error word
 PRO_NONE, PRO_RMSNORM, PRO_SWIGLU = 0, 1, 2
+# paged-cache types: fp16, and 4-bit blocks with the values of GGUF Q4_0
+KV = {"F16": 0, "Q4_0": 1}
 # expert activations of the MoE entry points, by the reference's names (primitives.py:52-62)
 ACT = {"silu": 0, "swish": 0, "gelu": 1, "relu": 2, "identity": 3}
 
@@ -26,6 +30,7 @@ _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -69,6 +74,14 @@ SIGNATURES = {
     "xm_comm_open_local": (_int, [_vp, _int, _vp]),
     "xm_comm_set_wait_limit": (_int, [_vp, _i64]),
     "xm_rmsnorm": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _vp]),
+    "xm_kv_page_bytes": (_i64, [_int, _int, _int, _int]),
+    "xm_kv_append": (_int, [_vp, _int, _i64, _i64, _int, _int, _int, _vp, _i64, _vp, _vp, _f64, _vp, _i64, _int, _int,
+                            _vp, _i64, _i64, _vp, _vp, _i64, _vp, _int, _i64, _vp]),
+    "xm_kv_read": (_int, [_vp, _i64, _int, _int, _int, _int, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "xm_kv_attention_workspace_size": (_i64, [_i64, _i64, _int, _int, _int, _i64]),
+    "xm_kv_attention": (_int, [_vp, _int, _i64, _i64, _int, _int, _int, _f32, _i64, _i64, _vp, _i64, _int, _int, _vp,
+                               _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "xm_sample": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _int, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp]),
     "xm_comm_destroy": (_int, [_vp]),
     "xm_allreduce_add": (_int, [_vp, _vp, _vp, _i64, _vp]),
 }
@@ -93,6 +106,14 @@ def _load():
 
 lib = _load()
 
+_HERE = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """A context in which `dev` (with an index) is the current device; free where it already is."""
+    import torch
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
 
 def check_device(what: str = "") -> None:
     """Raise if a bounded wait inside a kernel on the current device gave up
@@ -101,6 +122,9 @@ def check_device(what: str = "") -> None:
     st = lib.xm_device_status(1)
     if st < 0:
         raise XMError(f"{what}: {lib.xm_last_error().decode(errors='replace')}")
+    if st == ERR_PAGE:
+        raise XMError(f"{what}: a paged-cache kernel met a position without a page (device error word {st}); the "
+                      f"results of the calls since the last check are not valid")
     if st:
         raise XMError(f"{what}: a bounded wait inside a kernel gave up (device error word {st}); the results of "
                       f"the calls since the last check are not valid")

@@ -87,6 +87,7 @@ XM_DEV float warp_sum(float v) {
 // error instead of a hung GPU.
 // ---------------------------------------------------------------------------
 #define XM_DEVERR_TIMEOUT 1
+#define XM_DEVERR_PAGE 2
 extern __device__ int g_xm_device_error;
 
 XM_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -6,6 +6,7 @@
 //
 // k_kv_attn: one warp per (row, query head), one pass over the keys with a running maximum and sum;
 // lane l holds values 2l, 2l + 1 of each half of the head (one per half at D = 64).
+#include <algorithm>
 #include <type_traits>
 
 #include "xm_kv.cuh"
@@ -24,6 +25,7 @@ struct AttnArgs {
   int64_t window, sinks;
   void* out;
   int64_t out_stride;
+  bool out_vec;          // rows of out allow stores of four values
 };
 
 constexpr int kAttnWarps = 8;
@@ -106,6 +108,746 @@ __global__ void __launch_bounds__(32 * kAttnWarps) k_kv_attn(const KvView kv, co
     }
 }
 
+// ---------------------------------------------------------------------------
+// Decode: up to 8 NT rows (token, query head) of one KV head of one sequence per CTA; the keys are
+// split over the warps of a CTA, and over CTAs in chunks of `chunk` keys whose partial softmaxes
+// k_kv_merge joins.
+//
+// Bound: memory (the cache is read once); the work per byte decides whether that is reached.  A warp
+// takes 16 keys at a time on mma.sync m16n8k16 (fp16 operands, fp32 sums) with the keys, or the
+// values' dimensions, as the 16 matrix rows and the query rows as the 8 columns:
+//   S^T [16 keys x 8 rows] = K q^T,   O^T [D x 8 rows] += V^T P^T.
+// Operands come from global memory straight into the fragments: the order of the products' inner
+// dimension is free, and the cache's layout was chosen for it.
+//
+// 4-bit rows are never unpacked to values.  The nibbles 0 and 4 (for keys; 0 of two keys, paired by a
+// byte permute, for values) of a word are, after one mask, two fp16 subnormals c 2^-24, the nibbles
+// 1 and 5 are c 2^-20: exact, one instruction for two codes.  The block scale and the offset of the
+// codes stay outside the product:
+//   S  = sum over blocks b of d_kb (sum_i q_i c_i - 8 sum_i q_i)       (the offset is the product's
+//        initial accumulator),
+//   O  = sum_k c_k (p_k d_kb) - 8 sum_k p_k d_kb                       (one more product with constants).
+// q is scaled by a power of two per row into fp16's range (exact for fp16 and nearly so for bf16).
+// p d is rounded to fp16 once (2^-11); so that it neither overflows nor vanishes whatever the scales
+// are, the running reference R of a row is the largest s + log2 of the tile's largest |d|, less 13.
+//
+// A key behind the mask takes no part whatever its bytes are: its score and its p d are selected
+// away, not multiplied by zero.
+// ---------------------------------------------------------------------------
+
+constexpr int kDecWarps = 4;
+constexpr int kMaxSplits = 128;
+
+XM_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+XM_DEV uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+XM_DEV void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transposes an 8 x 8 matrix of 16-bit values held two per lane (row lane / 4, columns 2 (lane % 4), + 1)
+XM_DEV uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <int W>
+XM_DEV void ldg_words(uint32_t (&w)[W], const uint8_t* p) {
+  if constexpr (W == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (W == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+XM_DEV float half_of(uint32_t w, int hi) {
+  return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
+}
+
+// Rows [r0, r0 + R) of (token, query head) pairs of one sequence, and the keys that any of them sees:
+// subtiles of 16 keys, first the ones that hold sinks, then a run up to the last row's position.
+struct TileSpan {
+  int s, rows;            // sequence; valid rows
+  int64_t t0;             // row of the sequence's first new token
+  int r0;
+  int p_first;            // position of the sequence's first new token
+  int pmin, pmax;         // positions of the tile's first and last token
+  int ns, a0, n16;        // sink subtiles; first subtile of the run; subtiles in all
+  bool past_table;        // positions past the page table were asked for
+  XM_DEV int subtile(int v) const { return v < ns ? v : v - ns + a0; }
+};
+
+template <int R>
+XM_DEV TileSpan tile_span(const KvView& kv, const AttnArgs& a, int s, int64_t t0, int q_len, int rt, int G) {
+  TileSpan x;
+  x.s = s;
+  x.t0 = t0;
+  x.r0 = rt * R;
+  x.rows = min(R, q_len * G - x.r0);
+  const int len = __ldg(kv.lens + s);
+  x.p_first = len - q_len;
+  x.pmin = x.p_first + x.r0 / G;
+  x.pmax = x.p_first + (x.r0 + x.rows - 1) / G;
+  const int64_t cap = (int64_t)kv.table_width << kv.page_shift;
+  x.past_table = (int64_t)x.pmax >= cap;
+  const int kend = (int)min((int64_t)x.pmax + 1, cap);
+  int lo = 0, se = 0;
+  if (a.window > 0) {
+    lo = (int)max((int64_t)0, (int64_t)x.pmin - a.window + 1);
+    se = (int)min(a.sinks, (int64_t)lo);
+  }
+  x.a0 = lo >> 4;
+  x.ns = min((se + 15) >> 4, x.a0);
+  x.n16 = kend > 0 ? x.ns + max(0, ((kend + 15) >> 4) - x.a0) : 0;
+  return x;
+}
+
+XM_DEV bool sees(const AttnArgs& a, int pos, int key) {
+  return key <= pos && (a.window == 0 || (int64_t)key > (int64_t)pos - a.window || key < a.sinks);
+}
+
+// The rows of sequence s among the call's T, [t0, t0 + q_len) (none of them outside the call, whatever
+// the offsets say).
+XM_DEV void sequence_rows(const KvView& kv, int64_t T, int s, int64_t& t0, int& q_len) {
+  if (!kv.cu) {
+    t0 = s;
+    q_len = 1;
+    return;
+  }
+  const int first = max(0, min(__ldg(kv.cu + s), (int)T));
+  t0 = first;
+  q_len = max(0, min(__ldg(kv.cu + s + 1), (int)T) - first);
+}
+
+// The tile x of row tiles of R rows over all sequences: its sequence, or -1.  Every thread of the
+// warp calls it.
+template <int R>
+XM_DEV int find_tile(const KvView& kv, int64_t T, int G, int x, int& rt, int64_t& t0, int& q_len) {
+  if (!kv.cu) {
+    const int per = (G + R - 1) / R;
+    const int s = x / per;
+    rt = x % per;
+    t0 = s;
+    q_len = 1;
+    return s < kv.B ? s : -1;
+  }
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < kv.B; s0 += 32) {
+    const int s = s0 + lane;
+    int64_t first = 0;
+    int len = 0;
+    if (s < kv.B) sequence_rows(kv, T, s, first, len);
+    const int tiles = (int)(((int64_t)len * G + R - 1) / R);
+    int c = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, c, o);
+      if (lane >= o) c += n;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + c > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      rt = x - (before + __shfl_sync(0xffffffffu, c - tiles, l));
+      t0 = __shfl_sync(0xffffffffu, first, l);
+      q_len = __shfl_sync(0xffffffffu, len, l);
+      return s0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, c, 31);
+  }
+  return -1;
+}
+
+// One subtile's bytes as they come from the cache.
+template <int KV, int D>
+struct SubTile;
+template <int D>
+struct SubTile<XM_KV_Q4_0, D> {
+  static constexpr int NG = D / 32;
+  uint32_t k[2][NG], v[4][NG / 2], kd[2][NG / 2], vd[2][NG / 2];
+  XM_DEV void load_k(const uint8_t* head, int page_size, int slot0) {
+    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ldg_words<NG>(k[i], head + (slot0 + r + 8 * i) * (D / 2) + kq * (NG * 4));
+      ldg_words<NG / 2>(kd[i], head + page_size * (D / 2) + (slot0 + r + 8 * i) * (NG * 2));
+    }
+  }
+  XM_DEV void load_v(const uint8_t* head, int page_size, int slot0) {
+    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      ldg_words<NG / 2>(v[i], head + (slot0 + 2 * kq + (i & 1) + 8 * (i >> 1)) * (D / 2) + r * (NG * 2));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      ldg_words<NG / 2>(vd[i], head + page_size * (D / 2) + (slot0 + r + 8 * i) * (NG * 2));
+  }
+};
+template <int D>
+struct SubTile<XM_KV_F16, D> {
+  static constexpr int KC = D / 32, VC = D / 64;    // 16-byte pieces of a key (per lane) and of a value
+  uint32_t k[2][KC][4], v[4][VC][4];
+  XM_DEV void load_k(const uint8_t* head, int, int slot0) {
+    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) ldg_words<4>(k[i][c], head + (slot0 + r + 8 * i) * (D * 2) + c * 64 + kq * 16);
+  }
+  XM_DEV void load_v(const uint8_t* head, int, int slot0) {
+    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < VC; ++c)
+        ldg_words<4>(v[i][c], head + (slot0 + 2 * kq + (i & 1) + 8 * (i >> 1)) * (D * 2) + c * 128 + r * 16);
+  }
+};
+
+XM_DEV bool non_finite(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+
+struct DecArgs {
+  int chunk16;              // subtiles of a CTA
+  int nsplit;
+  float* part_o;            // [nsplit][T][Hq][D], where a row has more than one part
+  float2* part_ml;
+};
+
+template <typename QT_>
+XM_DEV void put_out4(QT_* p, bool vec, float4 v) {
+  uint2 w;
+  if constexpr (std::is_same<QT_, __half>::value) {
+    w = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = w;
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p);
+    q[0] = (uint16_t)w.x; q[1] = (uint16_t)(w.x >> 16); q[2] = (uint16_t)w.y; q[3] = (uint16_t)(w.y >> 16);
+  }
+}
+
+template <typename QT_, int D, int KV, int NT>
+__global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(const KvView kv, const AttnArgs a,
+                                                                               const DecArgs da) {
+  constexpr int R = 8 * NT, NG = D / 32, DP = D + 4;
+  constexpr int SUB = KV == XM_KV_Q4_0 ? 2 : 1;       // subtiles of a warp at a time
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ __align__(16) float o_s[kDecWarps][R][DP];
+  __shared__ float2 ml_s[kDecWarps][R];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, kq = lane & 3;
+  const int G = a.Hq / kv.Hk, hk = blockIdx.x % kv.Hk, split = blockIdx.y;
+  int rt, q_len;
+  int64_t t0;
+  const int s = find_tile<R>(kv, a.T, G, blockIdx.x / kv.Hk, rt, t0, q_len);
+  if (s < 0) return;
+  const TileSpan ts = tile_span<R>(kv, a, s, t0, q_len, rt, G);
+  if (ts.past_table && threadIdx.x == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+  const int parts = (ts.n16 + da.chunk16 - 1) / da.chunk16;
+  if (split > 0 && split >= parts) return;
+  const int v_lo = split * da.chunk16, v_hi = min(ts.n16, v_lo + da.chunk16);
+
+  // this lane's columns: rows 2 kq, 2 kq + 1 of every 8
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) pos[nt][c] = ts.p_first + min(ts.r0 + 8 * nt + 2 * kq + c, ts.r0 + ts.rows - 1) / G;
+
+  // q: row 8 nt + r, scaled by a power of two into fp16
+  uint32_t qb[NT][NG][2][2];
+  float q_f[NT][2];                                    // what turns a column's sum into a base-2 score
+  float q_off[NT][NG][2];                              // minus 8 sum of a block's q (4-bit)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int gr = ts.r0 + 8 * nt + r;
+    float x[NG][8];
+    float mx = 0.f;
+    if (8 * nt + r < ts.rows) {
+      const QT_* q = (const QT_*)a.q + (t0 + gr / G) * a.q_stride + (int64_t)(hk * G + gr % G) * D;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[g][i] = to_f32(q[32 * g + 8 * kq + i]);
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[g][i] = 0.f;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[g][i]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const int sh = fp16_row_shift(mx);
+    const float down = ldexpf(1.f, -sh);
+    const float f = ldexpf(a.scale * kLog2e, sh + (KV == XM_KV_Q4_0 ? 24 : 0));
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[g][i] = __half2float(__float2half_rn(x[g][i] * down));
+        sum += x[g][i];
+      }
+      if constexpr (KV == XM_KV_Q4_0) {
+        qb[nt][g][0][0] = half2_bits(x[g][0], x[g][4]);
+        qb[nt][g][0][1] = half2_bits(x[g][2], x[g][6]);
+        qb[nt][g][1][0] = half2_bits(x[g][1] * 0.0625f, x[g][5] * 0.0625f);
+        qb[nt][g][1][1] = half2_bits(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          q_off[nt][g][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * kq + c)) * (-8.f * 5.9604644775390625e-8f);
+      } else {
+        qb[nt][g][0][0] = half2_bits(x[g][0], x[g][1]);
+        qb[nt][g][0][1] = half2_bits(x[g][2], x[g][3]);
+        qb[nt][g][1][0] = half2_bits(x[g][4], x[g][5]);
+        qb[nt][g][1][1] = half2_bits(x[g][6], x[g][7]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) q_f[nt][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * kq + c));
+  }
+
+  float o[NT][D / 16][4], off[NT][4], R_[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    off[nt][0] = off[nt][1] = off[nt][2] = off[nt][3] = 0.f;
+    R_[nt][0] = R_[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
+
+  const int page_size = 1 << kv.page_shift, sub_shift = kv.page_shift - 4;
+  const int* table = kv.table + (int64_t)s * kv.table_stride;
+  const uint8_t* pool = kv.pool + (int64_t)hk * kv.head_bytes;
+  const int64_t page_bytes = kv.head_bytes * kv.Hk;
+  SubTile<KV, D> tile[SUB];
+  int page[SUB], next_page[SUB];
+  auto fetch_pages = [&](int v, int (&p)[SUB]) {
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) p[j] = __ldg(table + (ts.subtile(min(v + j, v_hi - 1)) >> sub_shift));
+  };
+  // the head's bytes in the page (page 0's where the page is bad: its keys are masked)
+  auto head_of = [&](int p) { return pool + ((unsigned)p < (uint64_t)kv.pages ? p : 0) * page_bytes; };
+  auto slot_of = [&](int v) { return (ts.subtile(min(v, v_hi - 1)) << 4) & (page_size - 1); };
+
+  constexpr int kStep = SUB * kDecWarps;
+  int v = v_lo + SUB * warp;
+  if (v < v_hi) {
+    fetch_pages(v, page);
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) tile[j].load_k(head_of(page[j]), page_size, slot_of(v + j));
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) tile[j].load_v(head_of(page[j]) + kv.head_bytes / 2, page_size, slot_of(v + j));
+    if (v + kStep < v_hi) fetch_pages(v + kStep, next_page);
+  }
+  for (; v < v_hi; v += kStep) {
+    const bool more = v + kStep < v_hi;
+    // which of this step's keys every row sees
+    bool full[SUB], bad[SUB];
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) {
+      const int key0 = ts.subtile(min(v + j, v_hi - 1)) << 4;
+      bad[j] = (unsigned)page[j] >= (uint64_t)kv.pages;
+      if (bad[j] && lane == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+      full[j] = v + j < v_hi && !bad[j] && key0 + 15 <= ts.pmin &&
+                (a.window == 0 || (int64_t)key0 > (int64_t)ts.pmax - a.window || key0 + 16 <= a.sinks);
+    }
+    // scores
+    float sc[NT][SUB][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) sc[nt][j][0] = sc[nt][j][1] = sc[nt][j][2] = sc[nt][j][3] = 0.f;
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) {
+      if constexpr (KV == XM_KV_Q4_0) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t wa = tile[j].k[0][g], wb = tile[j].k[1][g], xa = wa >> 8, xb = wb >> 8;
+          const float da_ = half_of(tile[j].kd[0][g / 2], g & 1), db_ = half_of(tile[j].kd[1][g / 2], g & 1);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float t[4] = {q_off[nt][g][0], q_off[nt][g][1], q_off[nt][g][0], q_off[nt][g][1]};
+            mma_16816(t, wa & 0x000f000fu, wb & 0x000f000fu, xa & 0x000f000fu, xb & 0x000f000fu, qb[nt][g][0][0],
+                      qb[nt][g][0][1]);
+            mma_16816(t, wa & 0x00f000f0u, wb & 0x00f000f0u, xa & 0x00f000f0u, xb & 0x00f000f0u, qb[nt][g][1][0],
+                      qb[nt][g][1][1]);
+            sc[nt][j][0] = fmaf(da_, t[0], sc[nt][j][0]);
+            sc[nt][j][1] = fmaf(da_, t[1], sc[nt][j][1]);
+            sc[nt][j][2] = fmaf(db_, t[2], sc[nt][j][2]);
+            sc[nt][j][3] = fmaf(db_, t[3], sc[nt][j][3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816(sc[nt][j], tile[j].k[0][c][2 * h], tile[j].k[1][c][2 * h], tile[j].k[0][c][2 * h + 1],
+                        tile[j].k[1][c][2 * h + 1], qb[nt][c][h][0], qb[nt][c][h][1]);
+      }
+    }
+    if (more) {                                        // the next keys load while these are used
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) tile[j].load_k(head_of(next_page[j]), page_size, slot_of(v + kStep + j));
+    }
+    // mask, running reference, weights
+    int e = 0;                                         // |d| < 2^e for every block scale of the step
+    if constexpr (KV == XM_KV_Q4_0) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < SUB; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = (ts.subtile(min(v + j, v_hi - 1)) << 4) + r + 8 * i;
+          const bool any = full[j] || (v + j < v_hi && !bad[j] && key <= ts.pmax &&
+                                       (a.window == 0 || (int64_t)key > (int64_t)ts.pmin - a.window || key < a.sinks));
+#pragma unroll
+          for (int w = 0; w < NG / 2; ++w) {
+            const uint32_t x = any ? tile[j].vd[i][w] & 0x7fff7fffu : 0u;
+            m = max(m, max(x & 0xffffu, x >> 16));
+          }
+        }
+      e = (int)(__reduce_max_sync(0xffffffffu, m) >> 10) - 14;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < SUB; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[nt][j][i] *= q_f[nt][i & 1];
+          if (!full[j]) {
+            const int key = (ts.subtile(min(v + j, v_hi - 1)) << 4) + r + 8 * (i >> 1);
+            if (v + j >= v_hi || bad[j] || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
+          }
+        }
+      float al[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float m = fmaxf(sc[nt][0][c], sc[nt][0][c + 2]);
+#pragma unroll
+        for (int j = 1; j < SUB; ++j) m = fmaxf(m, fmaxf(sc[nt][j][c], sc[nt][j][c + 2]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        // weights stay below 2^15: the reference moves only when they would pass it
+        const float want = m + (float)(e - 13);
+        const float was = R_[nt][c];
+        if (want > was + 2.f) R_[nt][c] = want;
+        const float ref = R_[nt][c] == -INFINITY ? 0.f : R_[nt][c];
+        al[c] = was == R_[nt][c] ? 1.f : ex2(was - ref);
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+          sc[nt][j][c] = ex2(sc[nt][j][c] - ref);
+          sc[nt][j][c + 2] = ex2(sc[nt][j][c + 2] - ref);
+        }
+      }
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          o[nt][i][0] *= al[0]; o[nt][i][1] *= al[1]; o[nt][i][2] *= al[0]; o[nt][i][3] *= al[1];
+        }
+        off[nt][0] *= al[0]; off[nt][1] *= al[1];
+        l[nt][0] *= al[0]; l[nt][1] *= al[1];
+      }
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) {
+        l[nt][0] += sc[nt][j][0] + sc[nt][j][2];
+        l[nt][1] += sc[nt][j][1] + sc[nt][j][3];
+      }
+    }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) {
+      if constexpr (KV == XM_KV_Q4_0) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float da_ = half_of(tile[j].vd[0][g / 2], g & 1), db_ = half_of(tile[j].vd[1][g / 2], g & 1);
+          const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
+          const uint32_t x = __byte_perm(tile[j].v[0][g / 2], tile[j].v[1][g / 2], sel);
+          const uint32_t y = __byte_perm(tile[j].v[2][g / 2], tile[j].v[3][g / 2], sel);
+          const uint32_t xs = x >> 8, ys = y >> 8;
+          const uint32_t eight = r / (8 / NG) == g ? 0x00080008u : 0u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float p0 = sc[nt][j][0] * da_, p1 = sc[nt][j][1] * da_, p2 = sc[nt][j][2] * db_, p3 = sc[nt][j][3] * db_;
+            if (!full[j]) {                            // a masked key's scale may be anything
+              p0 = sc[nt][j][0] == 0.f ? 0.f : p0;
+              p1 = sc[nt][j][1] == 0.f ? 0.f : p1;
+              p2 = sc[nt][j][2] == 0.f ? 0.f : p2;
+              p3 = sc[nt][j][3] == 0.f ? 0.f : p3;
+            }
+            const uint32_t b0 = transpose_8x8(half2_bits(p0, p1)), b1 = transpose_8x8(half2_bits(p2, p3));
+            mma_16816(o[nt][2 * g], x & 0x000f000fu, xs & 0x000f000fu, y & 0x000f000fu, ys & 0x000f000fu, b0, b1);
+            mma_16816(o[nt][2 * g + 1], x & 0x00f000f0u, xs & 0x00f000f0u, y & 0x00f000f0u, ys & 0x00f000f0u, b0, b1);
+            mma_16816(off[nt], eight, 0u, eight, 0u, b0, b1);
+          }
+        }
+      } else {
+        if (!full[j]) {
+          // values behind every row's mask become zeros; a non-finite value that only some rows see is
+          // taken out of the product and added to those rows one by one
+          const int key0 = ts.subtile(min(v + j, v_hi - 1)) << 4;
+          unsigned odd = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 2 * kq + (i & 1) + 8 * (i >> 1), key = key0 + at;
+            const bool any = v + j < v_hi && !bad[j] && key <= ts.pmax &&
+                             (a.window == 0 || (int64_t)key > (int64_t)ts.pmin - a.window || key < a.sinks);
+            bool nf = false;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                if (!any) tile[j].v[i][c][w] = 0u;
+                nf |= non_finite(tile[j].v[i][c][w]);
+              }
+            if (nf) odd |= 1u << at;
+          }
+          odd = ts.pmin == ts.pmax ? 0u : __reduce_or_sync(0xffffffffu, odd);
+          if (odd) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (odd >> (2 * kq + (i & 1) + 8 * (i >> 1)) & 1u)
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                  for (int w = 0; w < 4; ++w) tile[j].v[i][c][w] = 0u;
+            const uint8_t* vh = head_of(page[j]) + kv.head_bytes / 2;
+            for (unsigned left = odd; left; left &= left - 1) {
+              const int at = __ffs(left) - 1;
+              const __half* row = reinterpret_cast<const __half*>(vh + (slot_of(v + j) + at) * (D * 2));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const int from = (at & 7) * 4 + kq;
+                const float a0 = __shfl_sync(0xffffffffu, sc[nt][j][0], from), a1 = __shfl_sync(0xffffffffu, sc[nt][j][1], from);
+                const float a2 = __shfl_sync(0xffffffffu, sc[nt][j][2], from), a3 = __shfl_sync(0xffffffffu, sc[nt][j][3], from);
+                const float pc[2] = {at < 8 ? a0 : a2, at < 8 ? a1 : a3};
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                  if (sees(a, pos[nt][c], key0 + at))
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                      const int dim = 64 * (i / 4) + 8 * r + 2 * (i % 4);
+                      o[nt][i][c] = fmaf(pc[c], __half2float(row[dim]), o[nt][i][c]);
+                      o[nt][i][c + 2] = fmaf(pc[c], __half2float(row[dim + 1]), o[nt][i][c + 2]);
+                    }
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t b0 = transpose_8x8(half2_bits(sc[nt][j][0], sc[nt][j][1]));
+          const uint32_t b1 = transpose_8x8(half2_bits(sc[nt][j][2], sc[nt][j][3]));
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              mma_16816(o[nt][4 * c + w], __byte_perm(tile[j].v[0][c][w], tile[j].v[1][c][w], 0x5410u),
+                        __byte_perm(tile[j].v[0][c][w], tile[j].v[1][c][w], 0x7632u),
+                        __byte_perm(tile[j].v[2][c][w], tile[j].v[3][c][w], 0x5410u),
+                        __byte_perm(tile[j].v[2][c][w], tile[j].v[3][c][w], 0x7632u), b0, b1);
+        }
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int j = 0; j < SUB; ++j)
+        tile[j].load_v(head_of(next_page[j]) + kv.head_bytes / 2, page_size, slot_of(v + kStep + j));
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) page[j] = next_page[j];
+      if (v + 2 * kStep < v_hi) fetch_pages(v + 2 * kStep, next_page);
+    }
+  }
+
+  // the warps' parts meet in shared memory
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float x = l[nt][c];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (r == 0) ml_s[warp][8 * nt + 2 * kq + c] = make_float2(R_[nt][c], x);
+      float* row = &o_s[warp][8 * nt + 2 * kq + c][0];
+      if constexpr (KV == XM_KV_Q4_0) {
+        constexpr float k24 = 16777216.f, k20 = 1048576.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float f = __shfl_sync(0xffffffffu, off[nt][c], 4 * (g * (8 / NG)) + kq);
+          *reinterpret_cast<float4*>(row + 32 * g + 4 * r) =
+              make_float4(k24 * (o[nt][2 * g][c] - f), k20 * (o[nt][2 * g + 1][c] - 16.f * f),
+                          k24 * (o[nt][2 * g][c + 2] - f), k20 * (o[nt][2 * g + 1][c + 2] - 16.f * f));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2)
+          *reinterpret_cast<float4*>(row + 64 * (i / 4) + 8 * r + 2 * (i % 4)) =
+              make_float4(o[nt][i][c], o[nt][i][c + 2], o[nt][i + 1][c], o[nt][i + 1][c + 2]);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ts.rows * (D / 4); i += 32 * kDecWarps) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, ml_s[w][row].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float2 ml = ml_s[w][row];
+      const float f = ex2(ml.x - ref);
+      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][row][d]);
+      sum = fmaf(ml.y, f, sum);
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+    const int gr = ts.r0 + row;
+    const int64_t t = t0 + gr / G;
+    const int h = hk * G + gr % G;
+    if (parts <= 1) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      put_out4<QT_>((QT_*)a.out + t * a.out_stride + (int64_t)h * D + d, a.out_vec,
+                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    } else {
+      const int64_t cell = ((int64_t)split * a.T + t) * a.Hq + h;
+      *reinterpret_cast<float4*>(da.part_o + cell * D + d) = acc;
+      if (d == 0) da.part_ml[cell] = make_float2(m, sum);
+    }
+  }
+}
+
+// Joins the parts of the rows whose keys were split: one warp per (row, query head), in part order.
+template <typename QT_, int D, int R>
+__global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArgs a, const DecArgs da) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, G = a.Hq / kv.Hk;
+  const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (cell >= a.T * a.Hq) return;
+  const int64_t t = cell / a.Hq;
+  const int h = (int)(cell % a.Hq);
+  const int s = kv_sequence(kv, t);
+  if (s < 0) return;
+  int64_t t0;
+  int q_len;
+  sequence_rows(kv, a.T, s, t0, q_len);
+  const int gr = (int)(t - t0) * G + h % G;
+  const TileSpan ts = tile_span<R>(kv, a, s, t0, q_len, gr / R, G);
+  const int parts = (ts.n16 + da.chunk16 - 1) / da.chunk16;
+  if (parts <= 1) return;
+  float m = -INFINITY;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&da.part_ml[(int64_t)p * a.T * a.Hq + cell]).x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int d = lane * 4;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const int64_t at = (int64_t)p * a.T * a.Hq + cell;
+    const float2 ml = __ldcg(&da.part_ml[at]);
+    const float f = ex2(ml.x - ref);
+    sum = fmaf(ml.y, f, sum);
+    if (d < D) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(da.part_o + at * D + d));
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+  }
+  if (d >= D) return;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  put_out4<QT_>((QT_*)a.out + t * a.out_stride + (int64_t)h * D + d, a.out_vec,
+                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+}
+
+struct DecPlan {
+  int nt;               // groups of 8 rows per CTA; 0: the prompt kernel
+  int64_t tiles;        // row tiles, at most
+  int chunk16, nsplit;
+  int64_t ws_bytes;
+};
+
+DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, bool ragged) {
+  DecPlan p{};
+  const int G = Hq / Hk;
+  if (T * G > 16 * B && T > B) return p;
+  p.nt = T * G <= 8 * B ? 1 : 2;
+  const int R = 8 * p.nt;
+  p.tiles = ragged ? T * G / R + B : B * ((G + R - 1) / R);
+  // enough CTAs for three on each of the 148 SMs twice over, at least a step per warp each, and no
+  // more parts than keep the workspace small
+  const int64_t want = p.tiles * Hk * max_keys / (2 * 3 * 148);
+  int64_t chunk = std::max<int64_t>(128, std::min<int64_t>(2048, want));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (1 << 17) / std::max<int64_t>(1, T * Hq)));
+  chunk = std::max<int64_t>(chunk, (max_keys + most - 1) / most);
+  p.chunk16 = (int)((chunk + 127) / 128 * 8);
+  p.nsplit = (int)((max_keys + 16 * p.chunk16 - 1) / (16 * p.chunk16));
+  p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * T * Hq * (D * 4 + 8) : 0;
+  return p;
+}
+
+template <typename... KArgs, typename... Args>
+int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return xm_check_launch(what);
+}
+
+template <typename QT_, int D, int KV>
+int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* ws, cudaStream_t st) {
+  DecArgs da{p.chunk16, p.nsplit, (float*)ws, (float2*)((float*)ws + (int64_t)p.nsplit * a.T * a.Hq * D)};
+  const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)((a.T * a.Hq + 3) / 4));
+  int rc = p.nt == 1 ? kv_launch("kv attention", k_kv_decode<QT_, D, KV, 1>, grid, 32 * kDecWarps, st, kv, a, da)
+                     : kv_launch("kv attention", k_kv_decode<QT_, D, KV, 2>, grid, 32 * kDecWarps, st, kv, a, da);
+  if (rc || p.nsplit <= 1) return rc;
+  return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8>, mgrid, 128, st, kv, a, da)
+                   : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16>, mgrid, 128, st, kv, a, da);
+}
+
 template <typename QT_, int D, int KV>
 int attn_launch(const KvView& kv, const AttnArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
@@ -123,7 +865,15 @@ int attn_launch(const KvView& kv, const AttnArgs& a, cudaStream_t st) {
 }
 
 template <typename QT_>
-int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, cudaStream_t st) {
+int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, void* ws, cudaStream_t st) {
+  const DecPlan p = dec_plan(a.T, kv.B, a.Hq, kv.Hk, head_dim, (int64_t)kv.table_width << kv.page_shift, kv.cu != nullptr);
+  if (p.nt) {
+    if (head_dim == 128)
+      return kv_type == XM_KV_F16 ? decode_launch<QT_, 128, XM_KV_F16>(kv, a, p, ws, st)
+                                  : decode_launch<QT_, 128, XM_KV_Q4_0>(kv, a, p, ws, st);
+    return kv_type == XM_KV_F16 ? decode_launch<QT_, 64, XM_KV_F16>(kv, a, p, ws, st)
+                                : decode_launch<QT_, 64, XM_KV_Q4_0>(kv, a, p, ws, st);
+  }
   if (head_dim == 128)
     return kv_type == XM_KV_F16 ? attn_launch<QT_, 128, XM_KV_F16>(kv, a, st) : attn_launch<QT_, 128, XM_KV_Q4_0>(kv, a, st);
   return kv_type == XM_KV_F16 ? attn_launch<QT_, 64, XM_KV_F16>(kv, a, st) : attn_launch<QT_, 64, XM_KV_Q4_0>(kv, a, st);
@@ -134,8 +884,9 @@ int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, c
 extern "C" {
 
 int64_t xm_kv_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hk, int head_dim, int64_t max_keys) {
-  (void)T; (void)B; (void)Hq; (void)Hk; (void)head_dim; (void)max_keys;
-  return 16;
+  if (T < 1 || B < 1 || Hq < 1 || Hk < 1 || Hq % Hk || max_keys < 1) return 16;
+  return std::max<int64_t>(16, std::max(dec_plan(T, B, Hq, Hk, head_dim, max_keys, true).ws_bytes,
+                                        dec_plan(T, B, Hq, Hk, head_dim, max_keys, false).ws_bytes));
 }
 
 int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, int Hq, int Hk, int head_dim,
@@ -158,12 +909,14 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
   if (!d_q || !d_out) return xm_set_error(XM_ERR_INVALID, "kv_attention: null pointer");
   if (q_stride < (int64_t)Hq * head_dim || out_stride < (int64_t)Hq * head_dim || (((uintptr_t)d_q | (uintptr_t)d_out) & 1))
     return xm_set_error(XM_ERR_INVALID, "kv_attention: bad row pitch or alignment");
-  if (ws_bytes < xm_kv_attention_workspace_size(T, B, Hq, Hk, head_dim, table_width * page_size) || !d_ws)
-    return xm_set_error(XM_ERR_INVALID, "kv_attention: workspace too small");
-  AttnArgs a{d_q, T, q_stride, Hq, scale, window, sinks, d_out, out_stride};
+  if (ws_bytes < xm_kv_attention_workspace_size(T, B, Hq, Hk, head_dim, table_width * page_size) || !d_ws ||
+      ((uintptr_t)d_ws & 15))
+    return xm_set_error(XM_ERR_INVALID, "kv_attention: workspace too small or unaligned");
+  AttnArgs a{d_q, T, q_stride, Hq, scale, window, sinks, d_out, out_stride,
+             out_stride % 4 == 0 && ((uintptr_t)d_out & 7) == 0};
   cudaStream_t st = (cudaStream_t)stream;
-  return q_dtype == XM_DT_F16 ? attn_typed<__half>(kv, a, kv_type, head_dim, st)
-                              : attn_typed<__nv_bfloat16>(kv, a, kv_type, head_dim, st);
+  return q_dtype == XM_DT_F16 ? attn_typed<__half>(kv, a, kv_type, head_dim, d_ws, st)
+                              : attn_typed<__nv_bfloat16>(kv, a, kv_type, head_dim, d_ws, st);
 }
 
 }  // extern "C"

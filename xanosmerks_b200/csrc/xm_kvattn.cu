@@ -22,7 +22,7 @@ struct AttnArgs {
   int64_t T, q_stride;
   int Hq;
   float scale;
-  int64_t window, sinks;
+  int window, sinks;       // at most 2^30, the largest context
   void* out;
   int64_t out_stride;
   bool out_vec;          // rows of out allow stores of four values
@@ -153,6 +153,13 @@ XM_DEV void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+XM_DEV void mma_16816_from(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                           uint32_t b0, uint32_t b1) {   // d = a b + (c0, c1) in both halves of the rows
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 // transposes an 8 x 8 matrix of 16-bit values held two per lane (row lane / 4, columns 2 (lane % 4), + 1)
 XM_DEV uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
@@ -160,35 +167,36 @@ XM_DEV uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 template <int W>
-XM_DEV void ldg_words(uint32_t (&w)[W], const uint8_t* p) {
-  if constexpr (W == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (W == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+XM_DEV void lds_words(uint32_t (&w)[W], uint32_t at) {
+  if constexpr (W == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+  else if constexpr (W == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+}
+// 16 bytes from global to shared memory, asynchronously
+XM_DEV void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 XM_DEV float half_of(uint32_t w, int hi) {
   return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
 }
 
 // Rows [r0, r0 + R) of (token, query head) pairs of one sequence, and the keys that any of them sees:
-// subtiles of 16 keys, first the ones that hold sinks, then a run up to the last row's position.
+// units of UK keys, first the ones that hold sinks, then a run up to the last row's position.
 struct TileSpan {
   int s, rows;            // sequence; valid rows
   int64_t t0;             // row of the sequence's first new token
   int r0;
   int p_first;            // position of the sequence's first new token
   int pmin, pmax;         // positions of the tile's first and last token
-  int ns, a0, n16;        // sink subtiles; first subtile of the run; subtiles in all
+  int ns, a0, n;          // sink units; first unit of the run; units in all
   bool past_table;        // positions past the page table were asked for
-  XM_DEV int subtile(int v) const { return v < ns ? v : v - ns + a0; }
+  XM_DEV int unit(int v) const { return v < ns ? v : v - ns + a0; }
 };
 
-template <int R>
+template <int R, int UK>
 XM_DEV TileSpan tile_span(const KvView& kv, const AttnArgs& a, int s, int64_t t0, int q_len, int rt, int G) {
   TileSpan x;
   x.s = s;
@@ -204,17 +212,17 @@ XM_DEV TileSpan tile_span(const KvView& kv, const AttnArgs& a, int s, int64_t t0
   const int kend = (int)min((int64_t)x.pmax + 1, cap);
   int lo = 0, se = 0;
   if (a.window > 0) {
-    lo = (int)max((int64_t)0, (int64_t)x.pmin - a.window + 1);
-    se = (int)min(a.sinks, (int64_t)lo);
+    lo = max(0, x.pmin - a.window + 1);
+    se = min(a.sinks, lo);
   }
-  x.a0 = lo >> 4;
-  x.ns = min((se + 15) >> 4, x.a0);
-  x.n16 = kend > 0 ? x.ns + max(0, ((kend + 15) >> 4) - x.a0) : 0;
+  x.a0 = lo / UK;
+  x.ns = min((se + UK - 1) / UK, x.a0);
+  x.n = kend > 0 ? x.ns + max(0, (kend + UK - 1) / UK - x.a0) : 0;
   return x;
 }
 
 XM_DEV bool sees(const AttnArgs& a, int pos, int key) {
-  return key <= pos && (a.window == 0 || (int64_t)key > (int64_t)pos - a.window || key < a.sinks);
+  return key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
 }
 
 // The rows of sequence s among the call's T, [t0, t0 + q_len) (none of them outside the call, whatever
@@ -269,56 +277,86 @@ XM_DEV int find_tile(const KvView& kv, int64_t T, int G, int x, int& rt, int64_t
   return -1;
 }
 
-// One subtile's bytes as they come from the cache.
+// One subtile (16 keys) in a warp's part of shared memory: copied there 16 bytes at a time, and read
+// from there as fragments without bank conflicts.  Matrix row i of the keys, and inner index i of the
+// values' product, is key key_of(i) of the subtile, so that the four keys that a quarter of the lanes
+// reads together are four neighbours, whose pieces a small permutation spreads over the banks.
+XM_DEV int key_of(int i) { return (i & 8) | (i & 1) << 2 | (i & 6) >> 1; }
+
 template <int KV, int D>
 struct SubTile;
 template <int D>
 struct SubTile<XM_KV_Q4_0, D> {
-  static constexpr int NG = D / 32;
-  uint32_t k[2][NG], v[4][NG / 2], kd[2][NG / 2], vd[2][NG / 2];
-  XM_DEV void load_k(const uint8_t* head, int page_size, int slot0) {
-    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+  static constexpr int NG = D / 32, ROW = D / 2, P = ROW / 16;     // bytes and 16-byte pieces of a row of codes
+  static constexpr int kVAt = 16 * ROW, kKd = 2 * kVAt, kVd = kKd + 32 * NG, kBytes = kVd + 32 * NG;
+  uint32_t k[2][NG], v[4][NG / 2], kd[2][NG / 2], kx[2], vd[2][NG / 2];
+  // `to`: the subtile in shared memory; `from`: its first key row; `scales`: its first key's scales
+  static XM_DEV void copy(uint32_t to, const uint8_t* from, const uint8_t* scales, int64_t v_part, int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      ldg_words<NG>(k[i], head + (slot0 + r + 8 * i) * (D / 2) + kq * (NG * 4));
-      ldg_words<NG / 2>(kd[i], head + page_size * (D / 2) + (slot0 + r + 8 * i) * (NG * 2));
+    for (int i = 0; i < P / 2; ++i) {
+      const int c = lane + 32 * i, key = c / P, piece = c % P;
+      const int row = (key & 8) | (key & 3) << 1 | (key >> 2 & 1);               // key_of(row) = key
+      copy16(to + row * ROW + piece * 16, from + c * 16);
+      copy16(to + kVAt + key * ROW + (P == 4 ? piece ^ (key & 2) : piece) * 16, from + v_part + c * 16);
+    }
+    if (lane < 4 * NG) {
+      const int c = lane % (2 * NG), vals = lane / (2 * NG);
+      copy16(to + kKd + vals * 32 * NG + c * 16, scales + vals * v_part + c * 16);
     }
   }
-  XM_DEV void load_v(const uint8_t* head, int page_size, int slot0) {
-    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+  XM_DEV void read_k(uint32_t at, int r, int kq) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      ldg_words<NG / 2>(v[i], head + (slot0 + 2 * kq + (i & 1) + 8 * (i >> 1)) * (D / 2) + r * (NG * 2));
+    for (int i = 0; i < 2; ++i) {
+      lds_words<NG>(k[i], at + r * ROW + kq * (NG * 4) + 8 * i * ROW);
+      lds_words<NG / 2>(kd[i], at + kKd + key_of(r) * (2 * NG) + 8 * i * (2 * NG));
+      uint32_t x[1] = {0u};                            // the scales of blocks 2 kq, 2 kq + 1
+      if (kq < NG / 2) lds_words<1>(x, at + kKd + key_of(r) * (2 * NG) + kq * 4 + 8 * i * (2 * NG));
+      kx[i] = x[0];
+    }
+  }
+  XM_DEV void read_v(uint32_t at, int r, int kq) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      ldg_words<NG / 2>(vd[i], head + page_size * (D / 2) + (slot0 + r + 8 * i) * (NG * 2));
+    for (int i = 0; i < 4; ++i)     // keys kq, kq + 4, kq + 8, kq + 12
+      lds_words<NG / 2>(v[i], at + kVAt + kq * ROW + (P == 4 ? (r * 8) ^ (kq & 2) << 4 : r * 4) + 4 * i * ROW);
+  }
+  XM_DEV void read_vd(uint32_t at, int r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) lds_words<NG / 2>(vd[i], at + kVd + key_of(r) * (2 * NG) + 8 * i * (2 * NG));
   }
 };
 template <int D>
 struct SubTile<XM_KV_F16, D> {
-  static constexpr int KC = D / 32, VC = D / 64;    // 16-byte pieces of a key (per lane) and of a value
+  static constexpr int ROW = 2 * D, P = ROW / 16;                  // 16-byte pieces of a row
+  static constexpr int KC = D / 32, VC = D / 64;                   // pieces of a key (per lane) and of a value
+  static constexpr int kVAt = 16 * ROW, kBytes = 2 * kVAt;
   uint32_t k[2][KC][4], v[4][VC][4];
-  XM_DEV void load_k(const uint8_t* head, int, int slot0) {
-    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+  static XM_DEV void copy(uint32_t to, const uint8_t* from, const uint8_t*, int64_t v_part, int lane) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const int c = lane + 32 * i, key = c / P, piece = c % P;
+      copy16(to + key * ROW + (piece ^ (key & 4)) * 16, from + c * 16);
+      copy16(to + kVAt + key * ROW + (piece ^ (key & 3) << 1) * 16, from + v_part + c * 16);
+    }
+  }
+  XM_DEV void read_k(uint32_t at, int r, int kq) {
+    const int key = key_of(r);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) ldg_words<4>(k[i][c], head + (slot0 + r + 8 * i) * (D * 2) + c * 64 + kq * 16);
+      for (int c = 0; c < KC; ++c) lds_words<4>(k[i][c], at + (key + 8 * i) * ROW + ((4 * c + kq) ^ (key & 4)) * 16);
   }
-  XM_DEV void load_v(const uint8_t* head, int, int slot0) {
-    const int r = (threadIdx.x & 31) >> 2, kq = threadIdx.x & 3;
+  XM_DEV void read_v(uint32_t at, int r, int kq) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int c = 0; c < VC; ++c)
-        ldg_words<4>(v[i][c], head + (slot0 + 2 * kq + (i & 1) + 8 * (i >> 1)) * (D * 2) + c * 128 + r * 16);
+      for (int c = 0; c < VC; ++c) lds_words<4>(v[i][c], at + kVAt + (kq + 4 * i) * ROW + (8 * c + (r ^ kq << 1)) * 16);
   }
 };
 
 XM_DEV bool non_finite(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
 
 struct DecArgs {
-  int chunk16;              // subtiles of a CTA
+  int chunk;                // units of a CTA
   int nsplit;
   float* part_o;            // [nsplit][T][Hq][D], where a row has more than one part
   float2* part_ml;
@@ -341,14 +379,26 @@ XM_DEV void put_out4(QT_* p, bool vec, float4 v) {
   }
 }
 
+// Subtiles of a warp at a time, and such steps in a warp's ring (copies for the next ones are in flight
+// while one is used).
+template <int KV, int D, int NT>
+struct DecShape {
+  static constexpr int SUB = KV == XM_KV_Q4_0 ? 2 : 1, STAGES = 3;
+  static constexpr int kRing = STAGES * SUB * SubTile<KV, D>::kBytes;                       // bytes of a warp
+  static constexpr int kJoin = kDecWarps * 8 * NT * ((D + 4) * 4 + 8);                      // reuses the ring
+  static constexpr int kSmem = kDecWarps * kRing > kJoin ? kDecWarps * kRing : kJoin;
+  static constexpr int kCtas = NT > 1 ? 2 : KV == XM_KV_Q4_0 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2;   // of an SM
+};
+
 template <typename QT_, int D, int KV, int NT>
-__global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(const KvView kv, const AttnArgs a,
-                                                                               const DecArgs da) {
-  constexpr int R = 8 * NT, NG = D / 32, DP = D + 4;
-  constexpr int SUB = KV == XM_KV_Q4_0 ? 2 : 1;       // subtiles of a warp at a time
+__global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_kv_decode(const KvView kv,
+                                                                                          const AttnArgs a,
+                                                                                          const DecArgs da) {
+  using Sub = SubTile<KV, D>;
+  using Shape = DecShape<KV, D, NT>;
+  constexpr int R = 8 * NT, NG = D / 32, DP = D + 4, SUB = Shape::SUB, STAGES = Shape::STAGES, UK = 16 * SUB;
   constexpr float kLog2e = 1.4426950408889634f;
-  __shared__ __align__(16) float o_s[kDecWarps][R][DP];
-  __shared__ float2 ml_s[kDecWarps][R];
+  extern __shared__ __align__(16) uint8_t dec_smem[];
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, kq = lane & 3;
@@ -357,11 +407,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
   int64_t t0;
   const int s = find_tile<R>(kv, a.T, G, blockIdx.x / kv.Hk, rt, t0, q_len);
   if (s < 0) return;
-  const TileSpan ts = tile_span<R>(kv, a, s, t0, q_len, rt, G);
+  const TileSpan ts = tile_span<R, UK>(kv, a, s, t0, q_len, rt, G);
   if (ts.past_table && threadIdx.x == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-  const int parts = (ts.n16 + da.chunk16 - 1) / da.chunk16;
+  const int parts = (ts.n + da.chunk - 1) / da.chunk;
   if (split > 0 && split >= parts) return;
-  const int v_lo = split * da.chunk16, v_hi = min(ts.n16, v_lo + da.chunk16);
+  const int v_lo = split * da.chunk, v_hi = min(ts.n, v_lo + da.chunk);
 
   // this lane's columns: rows 2 kq, 2 kq + 1 of every 8
   int pos[NT][2];
@@ -373,7 +423,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
   // q: row 8 nt + r, scaled by a power of two into fp16
   uint32_t qb[NT][NG][2][2];
   float q_f[NT][2];                                    // what turns a column's sum into a base-2 score
-  float q_off[NT][NG][2];                              // minus 8 sum of a block's q (4-bit)
+  uint32_t q_off[NT][2];                               // 4-bit: -8 sum of a block's q, as high and low halves
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int gr = ts.r0 + 8 * nt + r;
@@ -398,8 +448,9 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int sh = fp16_row_shift(mx);
-    const float down = ldexpf(1.f, -sh);
-    const float f = ldexpf(a.scale * kLog2e, sh + (KV == XM_KV_Q4_0 ? 24 : 0));
+    const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
+    const float f = ldexpf(fabsf(a.scale) * kLog2e, sh + (KV == XM_KV_Q4_0 ? 24 : 0));
+    float block[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float sum = 0.f;
@@ -415,9 +466,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
         qb[nt][g][1][1] = half2_bits(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          q_off[nt][g][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * kq + c)) * (-8.f * 5.9604644775390625e-8f);
+        block[g] = sum * (-8.f * 5.9604644775390625e-8f);
       } else {
         qb[nt][g][0][0] = half2_bits(x[g][0], x[g][1]);
         qb[nt][g][0][1] = half2_bits(x[g][2], x[g][3]);
@@ -425,80 +474,103 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
         qb[nt][g][1][1] = half2_bits(x[g][6], x[g][7]);
       }
     }
+    if constexpr (KV == XM_KV_Q4_0) {                  // inner index 2 kq, 2 kq + 1 is a block; the others are zeros
+      float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; g += 2)
+        if (kq == g / 2) {
+          x0 = block[g];
+          x1 = block[g + 1];
+        }
+      q_off[nt][0] = half2_bits(x0, x1);
+      q_off[nt][1] = half2_bits(x0 - half_of(q_off[nt][0], 0), x1 - half_of(q_off[nt][0], 1));
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) q_f[nt][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * kq + c));
   }
 
-  float o[NT][D / 16][4], off[NT][4], R_[NT][2], l[NT][2];
+  float o[NT][D / 16][4], off[NT][NG][4], R_[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-    off[nt][0] = off[nt][1] = off[nt][2] = off[nt][3] = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) off[nt][g][0] = off[nt][g][1] = off[nt][g][2] = off[nt][g][3] = 0.f;
     R_[nt][0] = R_[nt][1] = -INFINITY;
     l[nt][0] = l[nt][1] = 0.f;
   }
 
-  const int page_size = 1 << kv.page_shift, sub_shift = kv.page_shift - 4;
+  const int page_mask = (1 << kv.page_shift) - 1;
+  const bool one_page = UK == 16 || kv.page_shift >= 5;   // a unit lies in one page (or in two of 16 tokens)
   const int* table = kv.table + (int64_t)s * kv.table_stride;
   const uint8_t* pool = kv.pool + (int64_t)hk * kv.head_bytes;
-  const int64_t page_bytes = kv.head_bytes * kv.Hk;
-  SubTile<KV, D> tile[SUB];
-  int page[SUB], next_page[SUB];
-  auto fetch_pages = [&](int v, int (&p)[SUB]) {
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) p[j] = __ldg(table + (ts.subtile(min(v + j, v_hi - 1)) >> sub_shift));
-  };
-  // the head's bytes in the page (page 0's where the page is bad: its keys are masked)
-  auto head_of = [&](int p) { return pool + ((unsigned)p < (uint64_t)kv.pages ? p : 0) * page_bytes; };
-  auto slot_of = [&](int v) { return (ts.subtile(min(v, v_hi - 1)) << 4) & (page_size - 1); };
+  const int64_t page_bytes = kv.head_bytes * kv.Hk, v_part = kv.head_bytes / 2;
+  const int codes = D / 2 << kv.page_shift;            // 4-bit: bytes of codes in front of the scales
+  const int steps = max(0, (v_hi - v_lo - warp + kDecWarps - 1) / kDecWarps);
+  const uint32_t ring = smem_u32(dec_smem) + warp * Shape::kRing;
 
-  constexpr int kStep = SUB * kDecWarps;
-  int v = v_lo + SUB * warp;
-  if (v < v_hi) {
-    fetch_pages(v, page);
+  // the warp's units are v_lo + warp + 4 i; lane l holds the page(s) of i = 32 b + l
+  auto page_of = [&](int i, int j) {
+    if (i >= steps) return 0;
+    const int at = ts.unit(v_lo + warp + i * kDecWarps) * UK + 16 * j >> kv.page_shift;
+    return at < kv.table_width ? __ldg(table + at) : -1;
+  };
+  int pages = page_of(lane, 0), pages_next = steps > 32 ? page_of(32 + lane, 0) : 0;
+  unsigned bad_steps = 0;                              // bit i: the step i % 32 has a page outside the pool
+  auto fetch = [&](int i) {                            // starts the copies of step i
+    if (i < steps) {
+      if (i > 0 && (i & 31) == 0) {
+        pages = pages_next;
+        pages_next = page_of(i + 32 + lane, 0);
+      }
+      const int key0 = ts.unit(v_lo + warp + i * kDecWarps) * UK;
+      bad_steps &= ~(1u << (i & 31));
+      const uint8_t* head;
+      const uint32_t to = ring + i % STAGES * (SUB * Sub::kBytes);
 #pragma unroll
-    for (int j = 0; j < SUB; ++j) tile[j].load_k(head_of(page[j]), page_size, slot_of(v + j));
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) tile[j].load_v(head_of(page[j]) + kv.head_bytes / 2, page_size, slot_of(v + j));
-    if (v + kStep < v_hi) fetch_pages(v + kStep, next_page);
-  }
-  for (; v < v_hi; v += kStep) {
-    const bool more = v + kStep < v_hi;
-    // which of this step's keys every row sees
-    bool full[SUB], bad[SUB];
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) {
-      const int key0 = ts.subtile(min(v + j, v_hi - 1)) << 4;
-      bad[j] = (unsigned)page[j] >= (uint64_t)kv.pages;
-      if (bad[j] && lane == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-      full[j] = v + j < v_hi && !bad[j] && key0 + 15 <= ts.pmin &&
-                (a.window == 0 || (int64_t)key0 > (int64_t)ts.pmax - a.window || key0 + 16 <= a.sinks);
+      for (int j = 0; j < SUB; ++j) {
+        if (j == 0 || !one_page) {
+          int p = __shfl_sync(0xffffffffu, pages, i & 31);
+          if (j > 0) p = page_of(i, j);
+          const bool in = (unsigned)p < (unsigned)kv.pages;
+          if (!in && (j == 0 || key0 + 16 * j <= ts.pmax)) bad_steps |= 1u << (i & 31);
+          head = pool + (in ? p : 0) * page_bytes;
+        }
+        const int slot = key0 + 16 * j & page_mask;
+        Sub::copy(to + j * Sub::kBytes, head + slot * Sub::ROW, head + codes + slot * (2 * NG), v_part, lane);
+      }
     }
-    // scores
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  // One step of UK keys from key0 on.  FULL: every row sees every one of them.
+  auto step = [&](auto full_, int key0, uint32_t at, bool hidden) {
+    constexpr bool FULL = decltype(full_)::value;
+    Sub tile[SUB];
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) tile[j].read_k(at + j * Sub::kBytes, r, kq);
     float sc[NT][SUB][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < SUB; ++j) sc[nt][j][0] = sc[nt][j][1] = sc[nt][j][2] = sc[nt][j][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < SUB; ++j) {
       if constexpr (KV == XM_KV_Q4_0) {
+        // the blocks' offsets first: sum of d (-8 sum q)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_16816_from(sc[nt][j], 0.f, 0.f, tile[j].kx[0], tile[j].kx[1], tile[j].kx[0], tile[j].kx[1], q_off[nt][0],
+                         q_off[nt][1]);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const uint32_t wa = tile[j].k[0][g], wb = tile[j].k[1][g], xa = wa >> 8, xb = wb >> 8;
           const float da_ = half_of(tile[j].kd[0][g / 2], g & 1), db_ = half_of(tile[j].kd[1][g / 2], g & 1);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float t[4] = {q_off[nt][g][0], q_off[nt][g][1], q_off[nt][g][0], q_off[nt][g][1]};
-            mma_16816(t, wa & 0x000f000fu, wb & 0x000f000fu, xa & 0x000f000fu, xb & 0x000f000fu, qb[nt][g][0][0],
-                      qb[nt][g][0][1]);
+            float t[4];
+            mma_16816_from(t, 0.f, 0.f, wa & 0x000f000fu, wb & 0x000f000fu, xa & 0x000f000fu, xb & 0x000f000fu,
+                           qb[nt][g][0][0], qb[nt][g][0][1]);
             mma_16816(t, wa & 0x00f000f0u, wb & 0x00f000f0u, xa & 0x00f000f0u, xb & 0x00f000f0u, qb[nt][g][1][0],
                       qb[nt][g][1][1]);
-            sc[nt][j][0] = fmaf(da_, t[0], sc[nt][j][0]);
-            sc[nt][j][1] = fmaf(da_, t[1], sc[nt][j][1]);
-            sc[nt][j][2] = fmaf(db_, t[2], sc[nt][j][2]);
-            sc[nt][j][3] = fmaf(db_, t[3], sc[nt][j][3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[nt][j][i] = fmaf(i < 2 ? da_ : db_, t[i], sc[nt][j][i]);
           }
         }
       } else {
@@ -507,16 +579,27 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_16816(sc[nt][j], tile[j].k[0][c][2 * h], tile[j].k[1][c][2 * h], tile[j].k[0][c][2 * h + 1],
-                        tile[j].k[1][c][2 * h + 1], qb[nt][c][h][0], qb[nt][c][h][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (c + h == 0)
+                mma_16816_from(sc[nt][j], 0.f, 0.f, tile[j].k[0][c][0], tile[j].k[1][c][0], tile[j].k[0][c][1],
+                               tile[j].k[1][c][1], qb[nt][c][0][0], qb[nt][c][0][1]);
+              else
+                mma_16816(sc[nt][j], tile[j].k[0][c][2 * h], tile[j].k[1][c][2 * h], tile[j].k[0][c][2 * h + 1],
+                          tile[j].k[1][c][2 * h + 1], qb[nt][c][h][0], qb[nt][c][h][1]);
+            }
       }
     }
-    if (more) {                                        // the next keys load while these are used
 #pragma unroll
-      for (int j = 0; j < SUB; ++j) tile[j].load_k(head_of(next_page[j]), page_size, slot_of(v + kStep + j));
+    for (int j = 0; j < SUB; ++j) {
+      tile[j].read_v(at + j * Sub::kBytes, r, kq);
+      if constexpr (KV == XM_KV_Q4_0) tile[j].read_vd(at + j * Sub::kBytes, r);
     }
-    // mask, running reference, weights
+    // whether any row sees key `at` of subtile j
+    auto any_sees = [&](int j, int row) {
+      if (FULL) return true;
+      const int key = key0 + 16 * j + row;
+      return !hidden && key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
+    };
     int e = 0;                                         // |d| < 2^e for every block scale of the step
     if constexpr (KV == XM_KV_Q4_0) {
       uint32_t m = 0;
@@ -524,30 +607,24 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
       for (int j = 0; j < SUB; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int key = (ts.subtile(min(v + j, v_hi - 1)) << 4) + r + 8 * i;
-          const bool any = full[j] || (v + j < v_hi && !bad[j] && key <= ts.pmax &&
-                                       (a.window == 0 || (int64_t)key > (int64_t)ts.pmin - a.window || key < a.sinks));
+          const bool any = any_sees(j, key_of(r) + 8 * i);
 #pragma unroll
-          for (int w = 0; w < NG / 2; ++w) {
-            const uint32_t x = any ? tile[j].vd[i][w] & 0x7fff7fffu : 0u;
-            m = max(m, max(x & 0xffffu, x >> 16));
-          }
+          for (int w = 0; w < NG / 2; ++w) m = __vmaxu2(m, any ? tile[j].vd[i][w] & 0x7fff7fffu : 0u);
         }
-      e = (int)(__reduce_max_sync(0xffffffffu, m) >> 10) - 14;
+      e = (int)(__reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16)) >> 10) - 14;
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      if (!FULL) {
 #pragma unroll
-      for (int j = 0; j < SUB; ++j)
+        for (int j = 0; j < SUB; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[nt][j][i] *= q_f[nt][i & 1];
-          if (!full[j]) {
-            const int key = (ts.subtile(min(v + j, v_hi - 1)) << 4) + r + 8 * (i >> 1);
-            if (v + j >= v_hi || bad[j] || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * j + key_of(r) + 8 * (i >> 1);
+            if (hidden || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
           }
-        }
-      float al[2];
+      }
+      float want[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float m = fmaxf(sc[nt][0][c], sc[nt][0][c + 2]);
@@ -556,25 +633,39 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        // weights stay below 2^15: the reference moves only when they would pass it
-        const float want = m + (float)(e - 13);
-        const float was = R_[nt][c];
-        if (want > was + 2.f) R_[nt][c] = want;
-        const float ref = R_[nt][c] == -INFINITY ? 0.f : R_[nt][c];
-        al[c] = was == R_[nt][c] ? 1.f : ex2(was - ref);
-#pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-          sc[nt][j][c] = ex2(sc[nt][j][c] - ref);
-          sc[nt][j][c + 2] = ex2(sc[nt][j][c + 2] - ref);
-        }
+        want[c] = !FULL && m == -INFINITY ? m : fmaf(m, q_f[nt][c], (float)(e - 13));
       }
-      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+      // weights stay below 2^15: the reference moves only when they would pass it
+      if (__any_sync(0xffffffffu, want[0] > R_[nt][0] + 2.f || want[1] > R_[nt][1] + 2.f)) {
+        float al[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float was = R_[nt][c];
+          if (want[c] > was + 2.f) R_[nt][c] = want[c];
+          al[c] = was == R_[nt][c] ? 1.f : ex2(was - R_[nt][c]);
+        }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[nt][i][0] *= al[0]; o[nt][i][1] *= al[1]; o[nt][i][2] *= al[0]; o[nt][i][3] *= al[1];
         }
-        off[nt][0] *= al[0]; off[nt][1] *= al[1];
+        if constexpr (KV == XM_KV_Q4_0) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            off[nt][g][0] *= al[0]; off[nt][g][1] *= al[1];
+          }
+        }
         l[nt][0] *= al[0]; l[nt][1] *= al[1];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float ref = R_[nt][c] == -INFINITY ? 0.f : R_[nt][c];
+#pragma unroll
+        for (int j = 0; j < SUB; ++j)
+#pragma unroll
+          for (int h = 0; h < 4; h += 2) {
+            const float x = ex2(fmaf(sc[nt][j][c + h], q_f[nt][c], -ref));
+            sc[nt][j][c + h] = !FULL && sc[nt][j][c + h] == -INFINITY ? 0.f : x;   // (q_f may be 0)
+          }
       }
 #pragma unroll
       for (int j = 0; j < SUB; ++j) {
@@ -593,11 +684,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
           const uint32_t x = __byte_perm(tile[j].v[0][g / 2], tile[j].v[1][g / 2], sel);
           const uint32_t y = __byte_perm(tile[j].v[2][g / 2], tile[j].v[3][g / 2], sel);
           const uint32_t xs = x >> 8, ys = y >> 8;
-          const uint32_t eight = r / (8 / NG) == g ? 0x00080008u : 0u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float p0 = sc[nt][j][0] * da_, p1 = sc[nt][j][1] * da_, p2 = sc[nt][j][2] * db_, p3 = sc[nt][j][3] * db_;
-            if (!full[j]) {                            // a masked key's scale may be anything
+            if (!FULL) {                               // a masked key's scale may be anything
               p0 = sc[nt][j][0] == 0.f ? 0.f : p0;
               p1 = sc[nt][j][1] == 0.f ? 0.f : p1;
               p2 = sc[nt][j][2] == 0.f ? 0.f : p2;
@@ -606,20 +696,18 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
             const uint32_t b0 = transpose_8x8(half2_bits(p0, p1)), b1 = transpose_8x8(half2_bits(p2, p3));
             mma_16816(o[nt][2 * g], x & 0x000f000fu, xs & 0x000f000fu, y & 0x000f000fu, ys & 0x000f000fu, b0, b1);
             mma_16816(o[nt][2 * g + 1], x & 0x00f000f0u, xs & 0x00f000f0u, y & 0x00f000f0u, ys & 0x00f000f0u, b0, b1);
-            mma_16816(off[nt], eight, 0u, eight, 0u, b0, b1);
+            mma_16816(off[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
           }
         }
       } else {
-        if (!full[j]) {
+        if (!FULL) {
           // values behind every row's mask become zeros; a non-finite value that only some rows see is
           // taken out of the product and added to those rows one by one
-          const int key0 = ts.subtile(min(v + j, v_hi - 1)) << 4;
           unsigned odd = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int at = 2 * kq + (i & 1) + 8 * (i >> 1), key = key0 + at;
-            const bool any = v + j < v_hi && !bad[j] && key <= ts.pmax &&
-                             (a.window == 0 || (int64_t)key > (int64_t)ts.pmin - a.window || key < a.sinks);
+            const int row = kq + 4 * i;
+            const bool any = any_sees(j, row);
             bool nf = false;
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
@@ -628,35 +716,37 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
                 if (!any) tile[j].v[i][c][w] = 0u;
                 nf |= non_finite(tile[j].v[i][c][w]);
               }
-            if (nf) odd |= 1u << at;
+            if (nf) odd |= 1u << row;
           }
           odd = ts.pmin == ts.pmax ? 0u : __reduce_or_sync(0xffffffffu, odd);
           if (odd) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (odd >> (2 * kq + (i & 1) + 8 * (i >> 1)) & 1u)
+              if (odd >> (kq + 4 * i) & 1u)
 #pragma unroll
                 for (int c = 0; c < D / 64; ++c)
 #pragma unroll
                   for (int w = 0; w < 4; ++w) tile[j].v[i][c][w] = 0u;
-            const uint8_t* vh = head_of(page[j]) + kv.head_bytes / 2;
             for (unsigned left = odd; left; left &= left - 1) {
-              const int at = __ffs(left) - 1;
-              const __half* row = reinterpret_cast<const __half*>(vh + (slot_of(v + j) + at) * (D * 2));
+              const int key = __ffs(left) - 1;
+              // this lane's values of the key: 16-byte piece 8 c + r of its row
+              uint32_t vw[D / 64][4];
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c)
+                lds_words<4>(vw[c], at + Sub::kVAt + key * Sub::ROW + (8 * c + (r ^ (key & 3) << 1)) * 16);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                const int from = (at & 7) * 4 + kq;
+                const int from = ((key & 3) << 1 | (key >> 2 & 1)) * 4 + kq;
                 const float a0 = __shfl_sync(0xffffffffu, sc[nt][j][0], from), a1 = __shfl_sync(0xffffffffu, sc[nt][j][1], from);
                 const float a2 = __shfl_sync(0xffffffffu, sc[nt][j][2], from), a3 = __shfl_sync(0xffffffffu, sc[nt][j][3], from);
-                const float pc[2] = {at < 8 ? a0 : a2, at < 8 ? a1 : a3};
+                const float pc[2] = {key < 8 ? a0 : a2, key < 8 ? a1 : a3};
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  if (sees(a, pos[nt][c], key0 + at))
+                  if (sees(a, pos[nt][c], key0 + key))
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
-                      const int dim = 64 * (i / 4) + 8 * r + 2 * (i % 4);
-                      o[nt][i][c] = fmaf(pc[c], __half2float(row[dim]), o[nt][i][c]);
-                      o[nt][i][c + 2] = fmaf(pc[c], __half2float(row[dim + 1]), o[nt][i][c + 2]);
+                      o[nt][i][c] = fmaf(pc[c], half_of(vw[i / 4][i % 4], 0), o[nt][i][c]);
+                      o[nt][i][c + 2] = fmaf(pc[c], half_of(vw[i / 4][i % 4], 1), o[nt][i][c + 2]);
                     }
               }
             }
@@ -677,17 +767,31 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
         }
       }
     }
-    if (more) {
+  };
+
+  // units [fa, fb) of the run, and the first fs, are seen whole by every row
+  const int fs = a.window > 0 ? min(ts.ns, a.sinks / UK) : 0;
+  const int fa = ts.ns + (a.window > 0 ? max(0, (ts.pmax - a.window + UK) / UK - ts.a0) : 0);
+  const int fb = ts.ns + (ts.pmin + 1) / UK - ts.a0;
 #pragma unroll
-      for (int j = 0; j < SUB; ++j)
-        tile[j].load_v(head_of(next_page[j]) + kv.head_bytes / 2, page_size, slot_of(v + kStep + j));
-#pragma unroll
-      for (int j = 0; j < SUB; ++j) page[j] = next_page[j];
-      if (v + 2 * kStep < v_hi) fetch_pages(v + 2 * kStep, next_page);
-    }
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+  for (int i = 0; i < steps; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();                                      // step i has landed, and every lane is done with step i - 1
+    const bool hidden = bad_steps >> (i & 31) & 1u;
+    fetch(i + STAGES - 1);
+    const int v = v_lo + warp + i * kDecWarps, key0 = ts.unit(v) * UK;
+    const uint32_t at = ring + i % STAGES * (SUB * Sub::kBytes);
+    if (hidden && lane == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+    if (!hidden && ((v >= fa && v < fb) || v < fs)) step(std::true_type{}, key0, at, false);
+    else step(std::false_type{}, key0, at, hidden);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();                                     // the ring's memory is free
 
   // the warps' parts meet in shared memory
+  float(*o_s)[R][DP] = reinterpret_cast<float(*)[R][DP]>(dec_smem);
+  float2(*ml_s)[R] = reinterpret_cast<float2(*)[R]>(dec_smem + kDecWarps * R * DP * 4);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -702,7 +806,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
         constexpr float k24 = 16777216.f, k20 = 1048576.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float f = __shfl_sync(0xffffffffu, off[nt][c], 4 * (g * (8 / NG)) + kq);
+          const float f = off[nt][g][c];
           *reinterpret_cast<float4*>(row + 32 * g + 4 * r) =
               make_float4(k24 * (o[nt][2 * g][c] - f), k20 * (o[nt][2 * g + 1][c] - 16.f * f),
                           k24 * (o[nt][2 * g][c + 2] - f), k20 * (o[nt][2 * g + 1][c + 2] - 16.f * f));
@@ -751,7 +855,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 3 : 2) k_kv_decode(c
 }
 
 // Joins the parts of the rows whose keys were split: one warp per (row, query head), in part order.
-template <typename QT_, int D, int R>
+template <typename QT_, int D, int R, int UK>
 __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArgs a, const DecArgs da) {
   grid_dep_wait();
   grid_dep_launch();
@@ -766,8 +870,8 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
   int q_len;
   sequence_rows(kv, a.T, s, t0, q_len);
   const int gr = (int)(t - t0) * G + h % G;
-  const TileSpan ts = tile_span<R>(kv, a, s, t0, q_len, gr / R, G);
-  const int parts = (ts.n16 + da.chunk16 - 1) / da.chunk16;
+  const TileSpan ts = tile_span<R, UK>(kv, a, s, t0, q_len, gr / R, G);
+  const int parts = (ts.n + da.chunk - 1) / da.chunk;
   if (parts <= 1) return;
   float m = -INFINITY;
   for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&da.part_ml[(int64_t)p * a.T * a.Hq + cell]).x);
@@ -798,7 +902,7 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
 struct DecPlan {
   int nt;               // groups of 8 rows per CTA; 0: the prompt kernel
   int64_t tiles;        // row tiles, at most
-  int chunk16, nsplit;
+  int chunk, nsplit;      // keys of a part; parts, at most
   int64_t ws_bytes;
 };
 
@@ -809,21 +913,25 @@ DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, 
   p.nt = T * G <= 8 * B ? 1 : 2;
   const int R = 8 * p.nt;
   p.tiles = ragged ? T * G / R + B : B * ((G + R - 1) / R);
-  // enough CTAs for three on each of the 148 SMs twice over, at least a step per warp each, and no
-  // more parts than keep the workspace small
-  const int64_t want = p.tiles * Hk * max_keys / (2 * 3 * 148);
-  int64_t chunk = std::max<int64_t>(128, std::min<int64_t>(2048, want));
+  // few tiles: one wave of four CTAs on each of the 148 SMs; many: chunks of 1024 keys, so that the
+  // sequences' different lengths even out.  At least a step for each warp, and no more parts than keep
+  // the workspace small
+  const int64_t base = p.tiles * Hk, slots = 3 * 148;
+  int64_t chunk = 2 * base <= slots ? (max_keys + slots / base - 1) / (slots / base) : 1024;
+  chunk = std::max<int64_t>(chunk, 128);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (1 << 17) / std::max<int64_t>(1, T * Hq)));
   chunk = std::max<int64_t>(chunk, (max_keys + most - 1) / most);
-  p.chunk16 = (int)((chunk + 127) / 128 * 8);
-  p.nsplit = (int)((max_keys + 16 * p.chunk16 - 1) / (16 * p.chunk16));
+  p.chunk = (int)((chunk + 127) / 128 * 128);
+  p.nsplit = (int)((max_keys + p.chunk - 1) / p.chunk);
   p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * T * Hq * (D * 4 + 8) : 0;
   return p;
 }
 
 template <typename... KArgs, typename... Args>
-int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t st,
+              Args... args) {
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.stream = st;
@@ -837,15 +945,30 @@ int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads
   return xm_check_launch(what);
 }
 
+template <typename QT_, int D, int KV, int NT>
+int decode_kernel(const KvView& kv, const AttnArgs& a, const DecArgs& da, dim3 grid, cudaStream_t st) {
+  constexpr int smem = DecShape<KV, D, NT>::kSmem;
+  static bool done[64] = {};                           // the attribute is set once per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || !done[dev])) {
+    const cudaError_t e = cudaFuncSetAttribute(k_kv_decode<QT_, D, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return kv_launch("kv attention", k_kv_decode<QT_, D, KV, NT>, grid, 32 * kDecWarps, smem, st, kv, a, da);
+}
+
 template <typename QT_, int D, int KV>
 int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* ws, cudaStream_t st) {
-  DecArgs da{p.chunk16, p.nsplit, (float*)ws, (float2*)((float*)ws + (int64_t)p.nsplit * a.T * a.Hq * D)};
+  constexpr int UK = 16 * DecShape<KV, D, 1>::SUB;
+  DecArgs da{p.chunk / UK, p.nsplit, (float*)ws, (float2*)((float*)ws + (int64_t)p.nsplit * a.T * a.Hq * D)};
   const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)((a.T * a.Hq + 3) / 4));
-  int rc = p.nt == 1 ? kv_launch("kv attention", k_kv_decode<QT_, D, KV, 1>, grid, 32 * kDecWarps, st, kv, a, da)
-                     : kv_launch("kv attention", k_kv_decode<QT_, D, KV, 2>, grid, 32 * kDecWarps, st, kv, a, da);
+  const int rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1>(kv, a, da, grid, st)
+                           : decode_kernel<QT_, D, KV, 2>(kv, a, da, grid, st);
   if (rc || p.nsplit <= 1) return rc;
-  return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8>, mgrid, 128, st, kv, a, da)
-                   : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16>, mgrid, 128, st, kv, a, da);
+  return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8, UK>, mgrid, 128, 0, st, kv, a, da)
+                   : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16, UK>, mgrid, 128, 0, st, kv, a, da);
 }
 
 template <typename QT_, int D, int KV>
@@ -912,7 +1035,8 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
   if (ws_bytes < xm_kv_attention_workspace_size(T, B, Hq, Hk, head_dim, table_width * page_size) || !d_ws ||
       ((uintptr_t)d_ws & 15))
     return xm_set_error(XM_ERR_INVALID, "kv_attention: workspace too small or unaligned");
-  AttnArgs a{d_q, T, q_stride, Hq, scale, window, sinks, d_out, out_stride,
+  const int64_t most = 1 << 30;                      // as good as none
+  AttnArgs a{d_q, T, q_stride, Hq, scale, window < most ? (int)window : 0, (int)std::min(sinks, most), d_out, out_stride,
              out_stride % 4 == 0 && ((uintptr_t)d_out & 7) == 0};
   cudaStream_t st = (cudaStream_t)stream;
   return q_dtype == XM_DT_F16 ? attn_typed<__half>(kv, a, kv_type, head_dim, d_ws, st)

@@ -323,7 +323,7 @@ int kv_view(const char* who, void* pool, int64_t pages, int kv_type, int Hk, int
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
     return xm_set_error(XM_ERR_INVALID, "%s: page size %d (a power of two from 16 to 1024)", who, page_size);
   if (Hk < 1 || Hk > 65535 || pages < 1 || pages > INT32_MAX || B < 1 || B > INT32_MAX || table_width < 1 ||
-      table_width > INT32_MAX / page_size || table_stride < 0)
+      table_width > (1 << 30) / page_size || table_stride < 0)
     return xm_set_error(XM_ERR_INVALID, "%s: bad cache sizes", who);
   if (!pool || !table || !lens) return xm_set_error(XM_ERR_INVALID, "%s: null pointer", who);
   if ((uintptr_t)pool & 15) return xm_set_error(XM_ERR_INVALID, "%s: the pool must be 16-byte aligned", who);

@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps) k_kv_attn(const KvView kv, co
 //
 // 4-bit rows are never unpacked to values.  The nibbles 0 and 4 (for keys; 0 of two keys, paired by a
 // byte permute, for values) of a word are, after one mask, two fp16 subnormals c 2^-24, the nibbles
-// 1 and 5 are c 2^-20: exact, one instruction for two codes.  The block scale and the offset of the
+// 1 and 5 are c 2^-20: exact, one instruction for two codes.  For values whole bytes (c + 16 c') 2^-24 and
+// their high nibbles enter, one instruction less, and the low codes' sums are the difference at the end.  The block scale and the offset of the
 // codes stay outside the product:
 //   S  = sum over blocks b of d_kb (sum_i q_i c_i - 8 sum_i q_i)       (the offset is the product's
 //        initial accumulator),
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps) k_kv_attn(const KvView kv, co
 // ---------------------------------------------------------------------------
 
 constexpr int kDecWarps = 4;
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = 128;     // one per thread of the merge
 
 XM_DEV float ex2(float x) {
   float y;
@@ -180,7 +181,8 @@ XM_DEV void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 XM_DEV float half_of(uint32_t w, int hi) {
-  return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return hi ? __high2float(h) : __low2float(h);
 }
 
 // Rows [r0, r0 + R) of (token, query head) pairs of one sequence, and the keys that any of them sees:
@@ -383,11 +385,12 @@ XM_DEV void put_out4(QT_* p, bool vec, float4 v) {
 // while one is used).
 template <int KV, int D, int NT>
 struct DecShape {
-  static constexpr int SUB = KV == XM_KV_Q4_0 ? 2 : 1, STAGES = 3;
+  static constexpr int SUB = KV == XM_KV_Q4_0 ? 2 : 1, STAGES = KV == XM_KV_Q4_0 ? 2 : 3;
   static constexpr int kRing = STAGES * SUB * SubTile<KV, D>::kBytes;                       // bytes of a warp
   static constexpr int kJoin = kDecWarps * 8 * NT * ((D + 4) * 4 + 8);                      // reuses the ring
-  static constexpr int kSmem = kDecWarps * kRing > kJoin ? kDecWarps * kRing : kJoin;
-  static constexpr int kCtas = NT > 1 ? 2 : KV == XM_KV_Q4_0 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2;   // of an SM
+  static constexpr int kQ = NT * (D / 32 * 2 * 256 + 4 * 128);                              // q fragments, q_f, q_off
+  static constexpr int kSmem = kQ + (kDecWarps * kRing > kJoin ? kDecWarps * kRing : kJoin);
+  static constexpr int kCtas = NT > 1 ? 2 : KV == XM_KV_Q4_0 || D == 64 ? 3 : 2;          // of an SM
 };
 
 template <typename QT_, int D, int KV, int NT>
@@ -419,75 +422,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) pos[nt][c] = ts.p_first + min(ts.r0 + 8 * nt + 2 * kq + c, ts.r0 + ts.rows - 1) / G;
-
-  // q: row 8 nt + r, scaled by a power of two into fp16
-  uint32_t qb[NT][NG][2][2];
-  float q_f[NT][2];                                    // what turns a column's sum into a base-2 score
-  uint32_t q_off[NT][2];                               // 4-bit: -8 sum of a block's q, as high and low halves
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int gr = ts.r0 + 8 * nt + r;
-    float x[NG][8];
-    float mx = 0.f;
-    if (8 * nt + r < ts.rows) {
-      const QT_* q = (const QT_*)a.q + (t0 + gr / G) * a.q_stride + (int64_t)(hk * G + gr % G) * D;
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[g][i] = to_f32(q[32 * g + 8 * kq + i]);
-    } else {
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[g][i] = 0.f;
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[g][i]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const int sh = fp16_row_shift(mx);
-    const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
-    const float f = ldexpf(fabsf(a.scale) * kLog2e, sh + (KV == XM_KV_Q4_0 ? 24 : 0));
-    float block[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[g][i] = __half2float(__float2half_rn(x[g][i] * down));
-        sum += x[g][i];
-      }
-      if constexpr (KV == XM_KV_Q4_0) {
-        qb[nt][g][0][0] = half2_bits(x[g][0], x[g][4]);
-        qb[nt][g][0][1] = half2_bits(x[g][2], x[g][6]);
-        qb[nt][g][1][0] = half2_bits(x[g][1] * 0.0625f, x[g][5] * 0.0625f);
-        qb[nt][g][1][1] = half2_bits(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        block[g] = sum * (-8.f * 5.9604644775390625e-8f);
-      } else {
-        qb[nt][g][0][0] = half2_bits(x[g][0], x[g][1]);
-        qb[nt][g][0][1] = half2_bits(x[g][2], x[g][3]);
-        qb[nt][g][1][0] = half2_bits(x[g][4], x[g][5]);
-        qb[nt][g][1][1] = half2_bits(x[g][6], x[g][7]);
-      }
-    }
-    if constexpr (KV == XM_KV_Q4_0) {                  // inner index 2 kq, 2 kq + 1 is a block; the others are zeros
-      float x0 = 0.f, x1 = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; g += 2)
-        if (kq == g / 2) {
-          x0 = block[g];
-          x1 = block[g + 1];
-        }
-      q_off[nt][0] = half2_bits(x0, x1);
-      q_off[nt][1] = half2_bits(x0 - half_of(q_off[nt][0], 0), x1 - half_of(q_off[nt][0], 1));
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) q_f[nt][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * kq + c));
-  }
 
   float o[NT][D / 16][4], off[NT][NG][4], R_[NT][2], l[NT][2];
 #pragma unroll
@@ -543,15 +477,105 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+
+  // q, by warp nt for all of them: row 8 nt + r, scaled by a power of two into fp16
+  const uint32_t q_at = smem_u32(dec_smem) + kDecWarps * Shape::kRing;
+  const uint32_t qb_at = q_at + lane * 16, qx_at = q_at + NT * NG * 2 * 256 + lane * 16;
+  if (warp < NT) {
+    const int nt = warp;
+    uint32_t qb[NG][2][2], q_off[2] = {0u, 0u};        // 4-bit: -8 sum of a block's q, as high and low halves
+    float q_f[2];                                      // what turns a column's sum into a base-2 score
+    const int gr = ts.r0 + 8 * nt + r;
+    float x[NG][8];
+    float mx = 0.f;
+    if (8 * nt + r < ts.rows) {
+      const QT_* q = (const QT_*)a.q + (t0 + gr / G) * a.q_stride + (int64_t)(hk * G + gr % G) * D;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[g][i] = to_f32(q[32 * g + 8 * kq + i]);
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[g][i] = 0.f;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[g][i]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const int sh = fp16_row_shift(mx);
+    const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
+    const float f = ldexpf(fabsf(a.scale) * kLog2e, sh + (KV == XM_KV_Q4_0 ? 24 : 0));
+    float block[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[g][i] = __half2float(__float2half_rn(x[g][i] * down));
+        sum += x[g][i];
+      }
+      if constexpr (KV == XM_KV_Q4_0) {
+        qb[g][0][0] = half2_bits(x[g][0], x[g][4]);
+        qb[g][0][1] = half2_bits(x[g][2], x[g][6]);
+        qb[g][1][0] = half2_bits(x[g][1] * 0.0625f, x[g][5] * 0.0625f);
+        qb[g][1][1] = half2_bits(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        block[g] = sum * (-8.f * 5.9604644775390625e-8f);
+      } else {
+        qb[g][0][0] = half2_bits(x[g][0], x[g][1]);
+        qb[g][0][1] = half2_bits(x[g][2], x[g][3]);
+        qb[g][1][0] = half2_bits(x[g][4], x[g][5]);
+        qb[g][1][1] = half2_bits(x[g][6], x[g][7]);
+      }
+    }
+    if constexpr (KV == XM_KV_Q4_0) {                  // inner index 2 kq, 2 kq + 1 is a block; the others are zeros
+      float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; g += 2)
+        if (kq == g / 2) {
+          x0 = block[g];
+          x1 = block[g + 1];
+        }
+      q_off[0] = half2_bits(x0, x1);
+      q_off[1] = half2_bits(x0 - half_of(q_off[0], 0), x1 - half_of(q_off[0], 1));
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) q_f[c] = __shfl_sync(0xffffffffu, f, 4 * (2 * kq + c));
+  #pragma unroll
+    for (int g = 0; g < NG; ++g)
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qb_at + (nt * NG + g) * 512), "r"(qb[g][0][0]),
+                   "r"(qb[g][0][1]), "r"(qb[g][1][0]), "r"(qb[g][1][1]) : "memory");
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qx_at + nt * 512), "r"(__float_as_uint(q_f[0])),
+                 "r"(__float_as_uint(q_f[1])), "r"(q_off[0]), "r"(q_off[1]) : "memory");
+  }
+  __syncthreads();
+  float q_f[NT][2];
+  uint32_t q_off[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    uint32_t w[4];
+    lds_words<4>(w, qx_at + nt * 512);
+    q_f[nt][0] = __uint_as_float(w[0]);
+    q_f[nt][1] = __uint_as_float(w[1]);
+    q_off[nt][0] = w[2];
+    q_off[nt][1] = w[3];
+  }
+
   // One step of UK keys from key0 on.  FULL: every row sees every one of them.
   auto step = [&](auto full_, int key0, uint32_t at, bool hidden) {
     constexpr bool FULL = decltype(full_)::value;
     Sub tile[SUB];
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) tile[j].read_k(at + j * Sub::kBytes, r, kq);
     float sc[NT][SUB][4];
 #pragma unroll
     for (int j = 0; j < SUB; ++j) {
+      tile[j].read_k(at + j * Sub::kBytes, r, kq);
       if constexpr (KV == XM_KV_Q4_0) {
         // the blocks' offsets first: sum of d (-8 sum q)
 #pragma unroll
@@ -565,10 +589,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float t[4];
-            mma_16816_from(t, 0.f, 0.f, wa & 0x000f000fu, wb & 0x000f000fu, xa & 0x000f000fu, xb & 0x000f000fu,
-                           qb[nt][g][0][0], qb[nt][g][0][1]);
-            mma_16816(t, wa & 0x00f000f0u, wb & 0x00f000f0u, xa & 0x00f000f0u, xb & 0x00f000f0u, qb[nt][g][1][0],
-                      qb[nt][g][1][1]);
+            uint32_t q[4];
+            lds_words<4>(q, qb_at + (nt * NG + g) * 512);
+            mma_16816_from(t, 0.f, 0.f, wa & 0x000f000fu, wb & 0x000f000fu, xa & 0x000f000fu, xb & 0x000f000fu, q[0],
+                           q[1]);
+            mma_16816(t, wa & 0x00f000f0u, wb & 0x00f000f0u, xa & 0x00f000f0u, xb & 0x00f000f0u, q[2], q[3]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[nt][j][i] = fmaf(i < 2 ? da_ : db_, t[i], sc[nt][j][i]);
           }
@@ -577,22 +602,23 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (c + h == 0)
-                mma_16816_from(sc[nt][j], 0.f, 0.f, tile[j].k[0][c][0], tile[j].k[1][c][0], tile[j].k[0][c][1],
-                               tile[j].k[1][c][1], qb[nt][c][0][0], qb[nt][c][0][1]);
-              else
-                mma_16816(sc[nt][j], tile[j].k[0][c][2 * h], tile[j].k[1][c][2 * h], tile[j].k[0][c][2 * h + 1],
-                          tile[j].k[1][c][2 * h + 1], qb[nt][c][h][0], qb[nt][c][h][1]);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t q[4];
+            lds_words<4>(q, qb_at + (nt * NG + c) * 512);
+            if (c == 0)
+              mma_16816_from(sc[nt][j], 0.f, 0.f, tile[j].k[0][0][0], tile[j].k[1][0][0], tile[j].k[0][0][1],
+                             tile[j].k[1][0][1], q[0], q[1]);
+            else
+              mma_16816(sc[nt][j], tile[j].k[0][c][0], tile[j].k[1][c][0], tile[j].k[0][c][1], tile[j].k[1][c][1], q[0],
+                        q[1]);
+            mma_16816(sc[nt][j], tile[j].k[0][c][2], tile[j].k[1][c][2], tile[j].k[0][c][3], tile[j].k[1][c][3], q[2],
+                      q[3]);
+          }
       }
     }
+    if constexpr (KV == XM_KV_Q4_0) {
 #pragma unroll
-    for (int j = 0; j < SUB; ++j) {
-      tile[j].read_v(at + j * Sub::kBytes, r, kq);
-      if constexpr (KV == XM_KV_Q4_0) tile[j].read_vd(at + j * Sub::kBytes, r);
+      for (int j = 0; j < SUB; ++j) tile[j].read_vd(at + j * Sub::kBytes, r);
     }
     // whether any row sees key `at` of subtile j
     auto any_sees = [&](int j, int row) {
@@ -676,6 +702,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     // O^T += V^T P^T
 #pragma unroll
     for (int j = 0; j < SUB; ++j) {
+      tile[j].read_v(at + j * Sub::kBytes, r, kq);
       if constexpr (KV == XM_KV_Q4_0) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -683,7 +710,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
           const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
           const uint32_t x = __byte_perm(tile[j].v[0][g / 2], tile[j].v[1][g / 2], sel);
           const uint32_t y = __byte_perm(tile[j].v[2][g / 2], tile[j].v[3][g / 2], sel);
-          const uint32_t xs = x >> 8, ys = y >> 8;
+          const uint32_t xs = __byte_perm(x, 0u, 0x4341u), ys = __byte_perm(y, 0u, 0x4341u);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float p0 = sc[nt][j][0] * da_, p1 = sc[nt][j][1] * da_, p2 = sc[nt][j][2] * db_, p3 = sc[nt][j][3] * db_;
@@ -694,7 +721,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
               p3 = sc[nt][j][3] == 0.f ? 0.f : p3;
             }
             const uint32_t b0 = transpose_8x8(half2_bits(p0, p1)), b1 = transpose_8x8(half2_bits(p2, p3));
-            mma_16816(o[nt][2 * g], x & 0x000f000fu, xs & 0x000f000fu, y & 0x000f000fu, ys & 0x000f000fu, b0, b1);
+            mma_16816(o[nt][2 * g], x & 0x00ff00ffu, xs, y & 0x00ff00ffu, ys, b0, b1);
             mma_16816(o[nt][2 * g + 1], x & 0x00f000f0u, xs & 0x00f000f0u, y & 0x00f000f0u, ys & 0x00f000f0u, b0, b1);
             mma_16816(off[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
           }
@@ -773,8 +800,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   const int fs = a.window > 0 ? min(ts.ns, a.sinks / UK) : 0;
   const int fa = ts.ns + (a.window > 0 ? max(0, (ts.pmax - a.window + UK) / UK - ts.a0) : 0);
   const int fb = ts.ns + (ts.pmin + 1) / UK - ts.a0;
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
   for (int i = 0; i < steps; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                      // step i has landed, and every lane is done with step i - 1
@@ -807,9 +832,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float f = off[nt][g][c];
+          // o[2g]: whole bytes c + 16 c', o[2g + 1]: 16 c', off: 8, each times 2^-24
+          const float lo = o[nt][2 * g + 1][c], hi = o[nt][2 * g + 1][c + 2];
           *reinterpret_cast<float4*>(row + 32 * g + 4 * r) =
-              make_float4(k24 * (o[nt][2 * g][c] - f), k20 * (o[nt][2 * g + 1][c] - 16.f * f),
-                          k24 * (o[nt][2 * g][c + 2] - f), k20 * (o[nt][2 * g + 1][c + 2] - 16.f * f));
+              make_float4(k24 * (o[nt][2 * g][c] - lo - f), k20 * (lo - 16.f * f), k24 * (o[nt][2 * g][c + 2] - hi - f),
+                          k20 * (hi - 16.f * f));
         }
       } else {
 #pragma unroll
@@ -854,15 +881,17 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   }
 }
 
-// Joins the parts of the rows whose keys were split: one warp per (row, query head), in part order.
+// Joins the parts of the rows whose keys were split: one CTA per (row, query head), its warps take the
+// parts in turn and are summed in a fixed order.
 template <typename QT_, int D, int R, int UK>
 __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArgs a, const DecArgs da) {
+  __shared__ float f_s[kMaxSplits];
+  __shared__ float red[4];
+  __shared__ __align__(16) float o_s[4][D];
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, G = a.Hq / kv.Hk;
-  const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (cell >= a.T * a.Hq) return;
-  const int64_t t = cell / a.Hq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.Hq / kv.Hk;
+  const int64_t cell = blockIdx.x, cells = a.T * a.Hq, t = cell / a.Hq;
   const int h = (int)(cell % a.Hq);
   const int s = kv_sequence(kv, t);
   if (s < 0) return;
@@ -873,27 +902,43 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
   const TileSpan ts = tile_span<R, UK>(kv, a, s, t0, q_len, gr / R, G);
   const int parts = (ts.n + da.chunk - 1) / da.chunk;
   if (parts <= 1) return;
-  float m = -INFINITY;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&da.part_ml[(int64_t)p * a.T * a.Hq + cell]).x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
+  const float2 ml = tid < parts ? __ldcg(&da.part_ml[(int64_t)tid * cells + cell]) : make_float2(-INFINITY, 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int d = lane * 4;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const int64_t at = (int64_t)p * a.T * a.Hq + cell;
-    const float2 ml = __ldcg(&da.part_ml[at]);
-    const float f = ex2(ml.x - ref);
-    sum = fmaf(ml.y, f, sum);
-    if (d < D) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(da.part_o + at * D + d));
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
+  float m = ml.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float f = ex2(ml.x - (m == -INFINITY ? 0.f : m));
+  f_s[tid] = f;
+  float sum = warp_sum(ml.y * f);
+  __syncthreads();
+  if (lane == 0) red[warp] = sum;
+  if (d < D) {
+#pragma unroll 8
+    for (int p = warp; p < parts; p += 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(da.part_o + ((int64_t)p * cells + cell) * D + d));
+      const float w = f_s[p];
+      acc.x = fmaf(x.x, w, acc.x);
+      acc.y = fmaf(x.y, w, acc.y);
+      acc.z = fmaf(x.z, w, acc.z);
+      acc.w = fmaf(x.w, w, acc.w);
     }
+    *reinterpret_cast<float4*>(&o_s[warp][d]) = acc;
   }
-  if (d >= D) return;
+  __syncthreads();
+  if (warp > 0 || d >= D) return;
+  sum = (red[0] + red[1]) + (red[2] + red[3]);
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    const float4 x = *reinterpret_cast<const float4*>(&o_s[w][d]);
+    acc.x += x.x;
+    acc.y += x.y;
+    acc.z += x.z;
+    acc.w += x.w;
+  }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   put_out4<QT_>((QT_*)a.out + t * a.out_stride + (int64_t)h * D + d, a.out_vec,
                 make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
@@ -913,7 +958,7 @@ DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, 
   p.nt = T * G <= 8 * B ? 1 : 2;
   const int R = 8 * p.nt;
   p.tiles = ragged ? T * G / R + B : B * ((G + R - 1) / R);
-  // few tiles: one wave of four CTAs on each of the 148 SMs; many: chunks of 1024 keys, so that the
+  // few tiles: one wave of three CTAs on each of the 148 SMs; many: chunks of 1024 keys, so that the
   // sequences' different lengths even out.  At least a step for each warp, and no more parts than keep
   // the workspace small
   const int64_t base = p.tiles * Hk, slots = 3 * 148;
@@ -963,7 +1008,7 @@ template <typename QT_, int D, int KV>
 int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* ws, cudaStream_t st) {
   constexpr int UK = 16 * DecShape<KV, D, 1>::SUB;
   DecArgs da{p.chunk / UK, p.nsplit, (float*)ws, (float2*)((float*)ws + (int64_t)p.nsplit * a.T * a.Hq * D)};
-  const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)((a.T * a.Hq + 3) / 4));
+  const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)(a.T * a.Hq));
   const int rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1>(kv, a, da, grid, st)
                            : decode_kernel<QT_, D, KV, 2>(kv, a, da, grid, st);
   if (rc || p.nsplit <= 1) return rc;

@@ -25,7 +25,7 @@ struct AttnArgs {
   int window, sinks;       // at most 2^30, the largest context
   void* out;
   int64_t out_stride;
-  bool out_vec;          // rows of out allow stores of four values
+  bool q_vec, out_vec;    // rows of q allow loads of 16 bytes, rows of out stores of four values
 };
 
 constexpr int kAttnWarps = 8;
@@ -443,6 +443,24 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   const int steps = max(0, (v_hi - v_lo - warp + kDecWarps - 1) / kDecWarps);
   const uint32_t ring = smem_u32(dec_smem) + warp * Shape::kRing;
 
+  // q's bytes start on their way before anything else: warp nt takes row 8 nt + r, values 32 g + 8 kq ...
+  uint4 q_raw[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) q_raw[g] = make_uint4(0u, 0u, 0u, 0u);
+  if (warp < NT && 8 * warp + r < ts.rows) {
+    const int gr = ts.r0 + 8 * warp + r;
+    const QT_* q = (const QT_*)a.q + (t0 + gr / G) * a.q_stride + (int64_t)(hk * G + gr % G) * D + 8 * kq;
+    if (a.q_vec) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) q_raw[g] = __ldg(reinterpret_cast<const uint4*>(q + 32 * g));
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<QT_*>(&q_raw[g])[i] = q[32 * g + i];
+    }
+  }
+
   // the warp's units are v_lo + warp + 4 i; lane l holds the page(s) of i = 32 b + l
   auto page_of = [&](int i, int j) {
     if (i >= steps) return 0;
@@ -487,21 +505,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     const int nt = warp;
     uint32_t qb[NG][2][2], q_off[2] = {0u, 0u};        // 4-bit: -8 sum of a block's q, as high and low halves
     float q_f[2];                                      // what turns a column's sum into a base-2 score
-    const int gr = ts.r0 + 8 * nt + r;
     float x[NG][8];
     float mx = 0.f;
-    if (8 * nt + r < ts.rows) {
-      const QT_* q = (const QT_*)a.q + (t0 + gr / G) * a.q_stride + (int64_t)(hk * G + gr % G) * D;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[g][i] = to_f32(q[32 * g + 8 * kq + i]);
-    } else {
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[g][i] = 0.f;
-    }
+      for (int i = 0; i < 8; ++i) x[g][i] = to_f32(reinterpret_cast<const QT_*>(&q_raw[g])[i]);
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -567,6 +576,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     q_off[nt][0] = w[2];
     q_off[nt][1] = w[3];
   }
+
+  uint32_t eights[4];                                  // codes 8 (kept in registers: the compiler would remake them)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm volatile("mov.u32 %0, 0x00080008;" : "=r"(eights[i]));
 
   // One step of UK keys from key0 on.  FULL: every row sees every one of them.
   auto step = [&](auto full_, int key0, uint32_t at, bool hidden) {
@@ -723,7 +736,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
             const uint32_t b0 = transpose_8x8(half2_bits(p0, p1)), b1 = transpose_8x8(half2_bits(p2, p3));
             mma_16816(o[nt][2 * g], x & 0x00ff00ffu, xs, y & 0x00ff00ffu, ys, b0, b1);
             mma_16816(o[nt][2 * g + 1], x & 0x00f000f0u, xs & 0x00f000f0u, y & 0x00f000f0u, ys & 0x00f000f0u, b0, b1);
-            mma_16816(off[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
+            mma_16816(off[nt][g], eights[0], eights[1], eights[2], eights[3], b0, b1);
           }
         }
       } else {
@@ -958,11 +971,11 @@ DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, 
   p.nt = T * G <= 8 * B ? 1 : 2;
   const int R = 8 * p.nt;
   p.tiles = ragged ? T * G / R + B : B * ((G + R - 1) / R);
-  // few tiles: one wave of three CTAs on each of the 148 SMs; many: chunks of 1024 keys, so that the
+  // few tiles: one wave of three CTAs on each of the 148 SMs; many: chunks of 2048 keys, so that the
   // sequences' different lengths even out.  At least a step for each warp, and no more parts than keep
   // the workspace small
   const int64_t base = p.tiles * Hk, slots = 3 * 148;
-  int64_t chunk = 2 * base <= slots ? (max_keys + slots / base - 1) / (slots / base) : 1024;
+  int64_t chunk = 2 * base <= slots ? (max_keys + slots / base - 1) / (slots / base) : 2048;
   chunk = std::max<int64_t>(chunk, 128);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (1 << 17) / std::max<int64_t>(1, T * Hq)));
   chunk = std::max<int64_t>(chunk, (max_keys + most - 1) / most);
@@ -1082,7 +1095,7 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
     return xm_set_error(XM_ERR_INVALID, "kv_attention: workspace too small or unaligned");
   const int64_t most = 1 << 30;                      // as good as none
   AttnArgs a{d_q, T, q_stride, Hq, scale, window < most ? (int)window : 0, (int)std::min(sinks, most), d_out, out_stride,
-             out_stride % 4 == 0 && ((uintptr_t)d_out & 7) == 0};
+             q_stride % 8 == 0 && ((uintptr_t)d_q & 15) == 0, out_stride % 4 == 0 && ((uintptr_t)d_out & 7) == 0};
   cudaStream_t st = (cudaStream_t)stream;
   return q_dtype == XM_DT_F16 ? attn_typed<__half>(kv, a, kv_type, head_dim, d_ws, st)
                               : attn_typed<__nv_bfloat16>(kv, a, kv_type, head_dim, d_ws, st);

@@ -93,14 +93,15 @@ def visible(pos, n, window, sinks):
 
 
 def attention_row(q, k, v, seen, scale):
-    """(output, sum p |v| / sum p, largest sum |q||k| scale) of one query row, float64."""
+    """(output, sum p |v| / sum p, largest sum |q||k| scale, sum |v|) of one query row, float64."""
     if not seen.any():
-        return np.zeros(v.shape[-1]), np.zeros(v.shape[-1]), 0.0
+        return np.zeros(v.shape[-1]), np.zeros(v.shape[-1]), 0.0, 0.0
     k, v = k[seen], v[seen]
     s = k @ q.astype(np.float64) * scale
     p = np.exp(s - s.max())
     p /= p.sum()
-    return p @ v, p @ np.abs(v), float((np.abs(k) @ np.abs(q.astype(np.float64))).max() * abs(scale))
+    return (p @ v, p @ np.abs(v), float((np.abs(k) @ np.abs(q.astype(np.float64))).max() * abs(scale)),
+            np.abs(v).sum(0))
 
 
 def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):

@@ -4,8 +4,8 @@
 // p - w, and the first `sinks`); query head h reads KV head h / (Hq / Hk):
 //   out = sum_k softmax_k(q . K_k * scale) V_k,  zeros for a row that sees no key.
 //
-// k_kv_attn: one warp per (row, query head), one pass over the keys with a running maximum and sum;
-// lane l holds values 2l, 2l + 1 of each half of the head (one per half at D = 64).
+// Few rows per sequence (decode steps): k_kv_decode, bound by reading the cache.  Many (prompts): k_kv_prompt, bound by
+// the products and the exponentials.
 #include <algorithm>
 #include <type_traits>
 
@@ -27,86 +27,6 @@ struct AttnArgs {
   int64_t out_stride;
   bool q_vec, out_vec;    // rows of q allow loads of 16 bytes, rows of out stores of four values
 };
-
-constexpr int kAttnWarps = 8;
-
-// value i of half `half` of lane's values of a cached row
-template <int D, int KV>
-XM_DEV float kv_value(const uint8_t* part, int page_size, int slot, bool is_v, int half, int i) {
-  constexpr int VPL = D / 64, NG = D / 32;
-  const int lane = threadIdx.x & 31;
-  if constexpr (KV == XM_KV_F16) {
-    return __half2float(((const __half*)part)[(int64_t)slot * D + half * (D / 2) + VPL * lane + i]);
-  } else {
-    const int g = half * (NG / 2) + (VPL * lane + i) / 32, e = (VPL * lane + i) % 32;
-    const uint8_t* row = part + (int64_t)slot * (D / 2);
-    const uint32_t w = is_v ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[NG * (e / 4) + g] >> (4 * (e % 4))
-                            : reinterpret_cast<const uint32_t*>(row)[NG * (e / 8) + g] >> (4 * (e % 8));
-    const float d = __half2float(reinterpret_cast<const __half*>(part + (int64_t)page_size * (D / 2))[slot * NG + g]);
-    return d * (float)((int)(w & 15) - 8);
-  }
-}
-
-template <typename QT_, int D, int KV>
-__global__ void __launch_bounds__(32 * kAttnWarps) k_kv_attn(const KvView kv, const AttnArgs a) {
-  constexpr int VPL = D / 64;
-  grid_dep_wait();
-  grid_dep_launch();
-  const int lane = threadIdx.x & 31;
-  const int64_t t = blockIdx.x;
-  const int h = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
-  const int s = kv_sequence(kv, t);
-  if (s < 0 || h >= a.Hq) return;
-  const int64_t pos = kv_position(kv, s, t);
-  const int hk = h / (a.Hq / kv.Hk);
-  const int page_size = 1 << kv.page_shift;
-  const QT_* q = (const QT_*)a.q + t * a.q_stride + (int64_t)h * D;
-  float qv[2][VPL], o[2][VPL];
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      qv[half][i] = to_f32(q[half * (D / 2) + VPL * lane + i]) * a.scale;
-      o[half][i] = 0.f;
-    }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t key = 0; key <= pos; ++key) {
-    if (a.window > 0 && key <= pos - a.window && key >= a.sinks) {
-      key = pos - a.window;
-      continue;
-    }
-    const int64_t page = kv_page(kv, s, key);
-    if (page < 0) continue;
-    const uint8_t* part = kv.pool + (page * kv.Hk + hk) * kv.head_bytes;
-    const int slot = (int)(key & (page_size - 1));
-    float dot = 0.f;
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) dot = fmaf(qv[half][i], kv_value<D, KV>(part, page_size, slot, false, half, i), dot);
-    dot = warp_sum(dot);
-    const float n = fmaxf(m, dot);
-    const float f = m == n ? 1.f : expf(m - n), p = dot == n ? 1.f : expf(dot - n);
-    m = n;
-    l = fmaf(l, f, p);
-    const uint8_t* vpart = part + kv.head_bytes / 2;
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        o[half][i] = fmaf(o[half][i], f, p * kv_value<D, KV>(vpart, page_size, slot, true, half, i));
-  }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  QT_* out = (QT_*)a.out + t * a.out_stride + (int64_t)h * D;
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const float v = o[half][i] * inv;
-      if constexpr (std::is_same<QT_, __half>::value) out[half * (D / 2) + VPL * lane + i] = __float2half_rn(v);
-      else out[half * (D / 2) + VPL * lane + i] = __float2bfloat16_rn(v);
-    }
-}
 
 // ---------------------------------------------------------------------------
 // Decode: up to 8 NT rows (token, query head) of one KV head of one sequence per CTA; the keys are
@@ -1029,20 +949,660 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
                    : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16, UK>, mgrid, 128, 0, st, kv, a, da);
 }
 
+// ---------------------------------------------------------------------------
+// Prompts: R = 128 or 256 rows (token, query head) of one KV head of one sequence per CTA, on
+// tcgen05.  The cache is walked in units of 128 keys, read once for all of the CTA's rows.
+//
+//   warps 0-3, 4-7   softmax of row tile 0, 1 (a thread is a row = a lane of tensor memory)
+//   warps 8-11       loaders: bring a unit's keys and values into shared memory as fp16
+//   warp 12          allocates tensor memory and issues the products (one thread)
+//
+// S = Q K^T (M = 128 rows, N = 128 keys) goes to tensor memory, the softmax warps turn it into P (fp16)
+// in place, and O += P V takes P from tensor memory and V as it lies in the cache, dimensions
+// contiguous.  The two row tiles alternate, so that one's products run during the other's softmax.
+// Tensor memory: S0 S1 (P in their first halves) at columns 0 and 128, O0 O1 at 256 and 256 + D.
+//
+// 4-bit rows become fp16 here, d (c - 8) rounded once (2^-11): a product per code would need the scales
+// inside the tensor core's inner dimension.  The order of the eight values that a word of keys yields is
+// kept, and q's is changed to it; the order of a word of values is a permutation of O's columns, undone
+// when O is written.  A unit with a scale above 4096 (values past fp16's range) is scaled by 2^-4.
+//
+// The running reference of a row moves only when a score passes it by 8 (P <= 2^8), so O, which stays in
+// tensor memory, is rescaled seldom.
+//
+// Masked keys: their scores are replaced, their values are zeros where no row sees them; a value that is not
+// finite and that only some rows see is taken out of the product and added to those rows alone.
+//
+// Bound: the products (4 R 128 D flops a unit at the tensor peak) and, as much, the 128 R exponentials
+// (16 a clock); the loaders' and the softmax's other instructions fit beside them.
+// ---------------------------------------------------------------------------
+constexpr int kUnit = 128;                         // keys of a unit
+constexpr int kPromptThreads = 13 * 32;
+
+XM_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+XM_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+XM_DEV void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+XM_DEV void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+XM_DEV void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+XM_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+XM_DEV void tmem_ld1(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+}
+XM_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+               "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+XM_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+XM_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 128-byte swizzle descriptors: rows of 128 bytes, groups of 8 rows 1024 bytes apart.  Inner dimension
+// contiguous (Q, K): the start moves by 32 bytes for 16 values; outer dimension contiguous (V: 64 values a
+// row, rows along the inner dimension): blocks of 64 outer values `block` bytes apart, the start moves by
+// 2048 bytes for 16 rows.
+XM_DEV uint64_t desc_sw128(uint32_t addr, uint32_t block) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)((block >> 4) & 0x3fffu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// fp16 x fp16 -> fp32, M = 128, N = n; b_outer: B's outer dimension is contiguous
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_outer) {
+  return 1u << 4 | (b_outer ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+struct PromptInfo {           // of the unit in a stage, written by the loaders
+  uint32_t bad[4];            // keys on a page outside the pool
+  uint32_t odd[4];            // keys whose values are not finite, taken out of the product
+  int k_exp, v_exp;           // the unit's keys / values are scaled by 2^-exp
+};
+
+template <int D>
+struct PromptShape {
+  static constexpr int kTile = 128 * 2 * D;                        // bytes of 128 fp16 rows
+  static constexpr int kBlock = 128 * 128;                         // of 64 of their columns
+  static constexpr int kSmem = 1024 + 2 * kTile + 4 * kTile + 512;   // Q0 Q1 | K x 2 | V x 2 | barriers
+};
+
+struct PromptCtl {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drain;
+  PromptInfo info[2];
+  uint32_t tmem;
+};
+
+// eight codes of a word of keys as d (c - 8), in the order 0 4 1 5 2 6 3 7; of a word of values, whose halves
+// are two blocks (d = their scales), in the order 0 0' 1 1' 2 2' 3 3'
+XM_DEV uint4 decode_word(uint32_t w, __half2 d) {
+  const uint32_t x = w >> 8, magic = 0x64006400u;       // 1024 + c, 1024 + 16 c
+  const uint32_t a = (w & 0x000f000fu) | magic, b = (w & 0x00f000f0u) | magic;
+  const uint32_t c = (x & 0x000f000fu) | magic, e = (x & 0x00f000f0u) | magic;
+  auto h2 = [](uint32_t v) { return *reinterpret_cast<const __half2*>(&v); };
+  auto bits = [](__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); };
+  const __half2 off = __float2half2_rn(-1032.f), six = __float2half2_rn(0.0625f), off16 = __float2half2_rn(-72.f);
+  return make_uint4(bits(__hmul2(__hadd2(h2(a), off), d)), bits(__hmul2(__hfma2(h2(b), six, off16), d)),
+                    bits(__hmul2(__hadd2(h2(c), off), d)), bits(__hmul2(__hfma2(h2(e), six, off16), d)));
+}
+
+XM_DEV bool loader_any(bool p) {                       // over the 128 loader threads
+  uint32_t r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+               : "=r"(r) : "r"((uint32_t)p) : "memory");
+  return r != 0;
+}
+
+template <typename QT_, int D, int KV, int R>
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv, const AttnArgs a) {
+  using Shape = PromptShape<D>;
+  constexpr int NG = D / 32;
+  constexpr float kLog2e = 1.4426950408889634f;
+  extern __shared__ uint8_t prompt_smem[];
+  const uint32_t base = (smem_u32(prompt_smem) + 1023u) & ~1023u;
+  uint8_t* const base_p = prompt_smem + (base - smem_u32(prompt_smem));
+  const uint32_t s_q = base, s_k = s_q + 2 * Shape::kTile, s_v = s_k + 2 * Shape::kTile;
+  PromptCtl* ctl = reinterpret_cast<PromptCtl*>(base_p + 6 * Shape::kTile);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int G = a.Hq / kv.Hk, hk = blockIdx.x % kv.Hk;
+  int rt, q_len;
+  int64_t t0;
+  // the last tiles of a sequence see the most keys: they start first
+  const int s = find_tile<R>(kv, a.T, G, (int)((gridDim.x - 1 - blockIdx.x) / kv.Hk), rt, t0, q_len);
+  if (s < 0) return;
+  const TileSpan ts = tile_span<R, kUnit>(kv, a, s, t0, q_len, rt, G);
+  if (ts.past_table && tid == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+  const int tiles = ts.rows > 128 ? 2 : 1, n = ts.n;
+  const int* table = kv.table + (int64_t)s * kv.table_stride;
+  const uint8_t* pool = kv.pool + (int64_t)hk * kv.head_bytes;
+  const int64_t page_bytes = kv.head_bytes * kv.Hk, v_part = kv.head_bytes / 2;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->k_full[i], 128);
+      mbar_init(&ctl->v_full[i], 128);
+      mbar_init(&ctl->p_full[i], 128);
+      mbar_init(&ctl->k_empty[i], 1);
+      mbar_init(&ctl->v_empty[i], 1);
+      mbar_init(&ctl->s_full[i], 1);
+      mbar_init(&ctl->o_done[i], 1);
+    }
+    mbar_init(&ctl->drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // q: a softmax thread brings its row, scaled by a power of two, into the swizzled tile
+  float q_f = 0.f;
+  const int tile = warp >> 2, row = tid & 127, gr = ts.r0 + 128 * tile + row;
+  const bool live = warp < 8 && 128 * tile + row < ts.rows;
+  const int64_t my_t = t0 + gr / G;
+  const int my_h = hk * G + gr % G, pos = live ? ts.p_first + gr / G : ts.pmax;
+  if (warp < 8 && tile < tiles) {
+    uint4 raw[D / 8];
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) raw[c] = make_uint4(0u, 0u, 0u, 0u);
+    if (live) {
+      const QT_* q = (const QT_*)a.q + my_t * a.q_stride + (int64_t)my_h * D;
+      if (a.q_vec) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) raw[c] = __ldg(reinterpret_cast<const uint4*>(q) + c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) reinterpret_cast<QT_*>(&raw[c])[i] = q[8 * c + i];
+      }
+    }
+    float mx = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(to_f32(reinterpret_cast<const QT_*>(&raw[c])[i])));
+    const int sh = fp16_row_shift(mx);
+    const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
+    q_f = ldexpf(fabsf(a.scale) * kLog2e, sh);
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f32(reinterpret_cast<const QT_*>(&raw[c])[i]) * down;
+      uint4 w;
+      if constexpr (KV == XM_KV_Q4_0)
+        w = make_uint4(half2_bits(x[0], x[4]), half2_bits(x[1], x[5]), half2_bits(x[2], x[6]), half2_bits(x[3], x[7]));
+      else
+        w = make_uint4(half2_bits(x[0], x[1]), half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
+      *reinterpret_cast<uint4*>(base_p + tile * Shape::kTile + (c / 8) * Shape::kBlock + row * 128 +
+                                ((c & 7) ^ (row & 7)) * 16) = w;
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+
+  if (warp == 12) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(D, true);
+      bool ok = true;
+      auto issue_s = [&](int i, int k) {               // S_i = Q_i K^T of unit k
+        const uint64_t da = desc_sw128(s_q + i * Shape::kTile, 16), db = desc_sw128(s_k + (k & 1) * Shape::kTile, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t off = (uint64_t)(((kk >> 2) * Shape::kBlock + (kk & 3) * 32) >> 4);
+          tc_mma_ss(tmem + i * 128, da + off, db + off, id_s, kk > 0);
+        }
+        tc_commit(&ctl->s_full[i]);
+      };
+      ok = mbar_wait_bounded(&ctl->k_full[0], 0);
+      tc_fence_after();
+      for (int i = 0; i < tiles && ok; ++i) issue_s(i, 0);
+      tc_commit(&ctl->k_empty[0]);
+      for (int k = 0; k < n && ok; ++k) {
+        ok = mbar_wait_bounded(&ctl->v_full[k & 1], (k >> 1) & 1);
+        for (int i = 0; i < tiles && ok; ++i) {
+          ok = mbar_wait_bounded(&ctl->p_full[i], k & 1);
+          if (!ok) break;
+          tc_fence_after();
+          // (the first unit starts O, unless the softmax warps have put taken-out values there)
+          const uint32_t* odd = ctl->info[0].odd;
+          const bool start = k == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) == 0u;
+          const uint64_t dv = desc_sw128(s_v + (k & 1) * Shape::kTile, Shape::kBlock);
+#pragma unroll
+          for (int kk = 0; kk < kUnit / 16; ++kk)
+            tc_mma_ts(tmem + 256 + i * D, tmem + i * 128 + kk * 8, dv + (uint64_t)(kk * (2048 >> 4)), id_o,
+                      kk > 0 || !start);
+          tc_commit(&ctl->o_done[i]);
+          if (i == tiles - 1) tc_commit(&ctl->v_empty[k & 1]);
+          if (k + 1 < n) {
+            // S_i overwrites P_i, which the product above reads
+            ok = mbar_wait_bounded(&ctl->o_done[i], k & 1);
+            if (ok && i == 0) ok = mbar_wait_bounded(&ctl->k_full[(k + 1) & 1], ((k + 1) >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(i, k + 1);
+            if (i == tiles - 1) tc_commit(&ctl->k_empty[(k + 1) & 1]);
+          }
+        }
+      }
+      tc_commit(&ctl->drain);                          // nothing of the tensor core's is left in flight
+      mbar_wait_bounded(&ctl->drain, 0);
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    const int t = tid - 256;                           // key of a unit (4-bit)
+    bool ok = true;
+    auto any_sees = [&](int key) {
+      return key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
+    };
+    auto all_see = [&](int key) {
+      return key <= ts.pmin && (a.window == 0 || key > ts.pmax - a.window || key < a.sinks);
+    };
+    // where a position's head is in its page, and whether there is one
+    auto locate = [&](int key, bool& in) {
+      const int at = key >> kv.page_shift;
+      const int p = at < kv.table_width ? __ldg(table + at) : -1;
+      in = (unsigned)p < (unsigned)kv.pages;
+      return pool + (in ? p : 0) * page_bytes;
+    };
+    const int page_mask = (1 << kv.page_shift) - 1;
+    if constexpr (KV == XM_KV_Q4_0) {
+      uint32_t kw[D / 8], vw[D / 8], kd[NG / 2], vd[NG / 2];
+      const int codes = D / 2 << kv.page_shift;
+      const uint8_t* head = nullptr;
+      bool in = false;
+      int slot = 0;
+      auto load_k = [&](int k) {
+        const int key = ts.unit(k) * kUnit + t;
+        head = locate(key, in);
+        slot = key & page_mask;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(head + slot * (D / 2)) + i);
+          kw[4 * i] = v.x; kw[4 * i + 1] = v.y; kw[4 * i + 2] = v.z; kw[4 * i + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) kd[i] = __ldg(reinterpret_cast<const uint32_t*>(head + codes + slot * (2 * NG)) + i);
+      };
+      auto load_v = [&]() {                            // of the unit that load_k has located
+        const uint8_t* h = head + v_part;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(h + slot * (D / 2)) + i);
+          vw[4 * i] = v.x; vw[4 * i + 1] = v.y; vw[4 * i + 2] = v.z; vw[4 * i + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) vd[i] = __ldg(reinterpret_cast<const uint32_t*>(h + codes + slot * (2 * NG)) + i);
+      };
+      if (n > 0) {
+        load_k(0);
+        load_v();
+      }
+      for (int k = 0; k < n; ++k) {                    // (a wait that gives up is not repeated; the barriers go on)
+        const int st = k & 1, key = ts.unit(k) * kUnit + t;
+        const bool seen = in && any_sees(key), bad = !in && any_sees(key);
+        bool odd = false;
+        uint32_t mk = 0, mv = 0;
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+          if (!seen) kd[i] = vd[i] = 0u;
+          mk = __vmaxu2(mk, kd[i] & 0x7fff7fffu);
+          mv = __vmaxu2(mv, vd[i] & 0x7fff7fffu);
+        }
+        mk = max(mk & 0xffffu, mk >> 16);
+        mv = max(mv & 0xffffu, mv >> 16);
+        if (mv >= 0x7c00u && !all_see(key)) {
+          odd = true;
+          mv = 0;
+#pragma unroll
+          for (int i = 0; i < NG / 2; ++i) vd[i] = 0u;
+        }
+        const bool big_k = loader_any(mk > 0x6c00u), big_v = loader_any(mv > 0x6c00u);     // 4096
+        if (k >= 2 && ok) ok = mbar_wait_bounded(&ctl->k_empty[st], ((k >> 1) - 1) & 1);
+        {
+          const __half2 down = __float2half2_rn(big_k ? 0.0625f : 1.f);
+          uint8_t* to = base_p + (s_k - base) + st * Shape::kTile + t * 128;
+#pragma unroll
+          for (int p = 0; p < D / 8; ++p) {            // word p: chunk NG' of block p % NG, quarter p / NG
+            const int g = p % NG, c = 4 * g + p / NG;  // 16-byte chunk of the row: values 8 c ...
+            const uint32_t dw = kd[g / 2];
+            const __half2 d2 = __hmul2(g & 1 ? __high2half2(*reinterpret_cast<const __half2*>(&dw))
+                                             : __low2half2(*reinterpret_cast<const __half2*>(&dw)), down);
+            *reinterpret_cast<uint4*>(to + (c / 8) * Shape::kBlock + ((c & 7) ^ (t & 7)) * 16) = decode_word(kw[p], d2);
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&ctl->k_full[st]);
+        if (k + 1 < n) load_k(k + 1);                  // (in, head, slot: the next unit's from here on)
+        if (k >= 2 && ok) ok = mbar_wait_bounded(&ctl->v_empty[st], ((k >> 1) - 1) & 1);
+        {
+          const __half2 down = __float2half2_rn(big_v ? 0.0625f : 1.f);
+          uint8_t* to = base_p + (s_v - base) + st * Shape::kTile + t * 128;
+#pragma unroll
+          for (int p = 0; p < D / 8; ++p) {            // word p is chunk p: columns 8 p ...
+            const uint32_t dw = vd[p % (NG / 2)];
+            *reinterpret_cast<uint4*>(to + (p / 8) * Shape::kBlock + ((p & 7) ^ (t & 7)) * 16) =
+                decode_word(vw[p], __hmul2(*reinterpret_cast<const __half2*>(&dw), down));
+          }
+        }
+        const unsigned bad_w = __ballot_sync(0xffffffffu, bad), odd_w = __ballot_sync(0xffffffffu, odd);
+        if (lane == 0) {
+          ctl->info[st].bad[warp - 8] = bad_w;
+          ctl->info[st].odd[warp - 8] = odd_w;
+          if (bad_w) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+        }
+        if (t == 0) {
+          ctl->info[st].k_exp = big_k ? 4 : 0;
+          ctl->info[st].v_exp = big_v ? 4 : 0;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&ctl->v_full[st]);
+        if (k + 1 < n) load_v();
+      }
+    } else {
+      constexpr int P = D / 8;                         // 16-byte chunks of a row
+      constexpr int kRowsAtOnce = 128 / P, kIter = 128 / kRowsAtOnce;
+      const int c = t % P, r0 = t / P;
+      // the copies of one part of a unit: chunk c of rows r0, r0 + kRowsAtOnce, ...
+      auto copy = [&](int k, int64_t part, uint32_t to, uint32_t& bad) {
+        const int key0 = ts.unit(k) * kUnit;
+#pragma unroll 4
+        for (int i = 0; i < kIter; ++i) {
+          const int r = r0 + i * kRowsAtOnce, key = key0 + r;
+          bool in;
+          const uint8_t* head = locate(key, in);
+          if (!in && any_sees(key)) bad |= 1u << i;
+          const uint32_t dst = to + (c / 8) * Shape::kBlock + r * 128 + ((c & 7) ^ (r & 7)) * 16;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(dst), "l"(head + part + (key & page_mask) * (2 * D) + c * 16),
+                         "r"(in && any_sees(key) ? 16u : 0u) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      // each part of the next unit is requested as soon as its stage is free, K before V
+      uint32_t bad_next = 0, bad_now = 0, none = 0;
+      if (n > 0) {
+        copy(0, 0, s_k, bad_next);
+        copy(0, v_part, s_v, none);
+      }
+      for (int k = 0; k < n; ++k) {                    // (a wait that gives up is not repeated; the barriers go on)
+        const int st = k & 1;
+        bad_now = bad_next;
+        bad_next = 0;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");           // K(k)
+        fence_proxy_async_smem();
+        mbar_arrive(&ctl->k_full[st]);
+        if (k + 1 < n) {
+          if (k >= 1 && ok) ok = mbar_wait_bounded(&ctl->k_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
+          copy(k + 1, 0, s_k + (st ^ 1) * Shape::kTile, bad_next);
+          asm volatile("cp.async.wait_group 1;" ::: "memory");         // V(k)
+        } else {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        // partly seen units: values that are not finite leave the product
+        const int key0 = ts.unit(k) * kUnit;
+        const bool whole = key0 + kUnit - 1 <= ts.pmin &&
+                           (a.window == 0 || key0 > ts.pmax - a.window || key0 + kUnit <= a.sinks);
+        if (t < 4) ctl->info[st].bad[t] = ctl->info[st].odd[t] = 0u;
+        if (t == 0) ctl->info[st].k_exp = ctl->info[st].v_exp = 0;
+        if (loader_any(!whole || bad_now)) {           // (also the barrier behind the zeros above)
+          for (int i = 0; i < kIter; ++i) {
+            const int r = r0 + i * kRowsAtOnce;
+            if (bad_now >> i & 1u) atomicOr(&ctl->info[st].bad[r >> 5], 1u << (r & 31));
+            if (all_see(key0 + r)) continue;
+            uint4* at = reinterpret_cast<uint4*>(base_p + (s_v - base) + st * Shape::kTile + (c / 8) * Shape::kBlock + r * 128 +
+                                                 ((c & 7) ^ (r & 7)) * 16);
+            const uint4 v = *at;
+            if (non_finite(v.x) || non_finite(v.y) || non_finite(v.z) || non_finite(v.w))
+              atomicOr(&ctl->info[st].odd[r >> 5], 1u << (r & 31));
+          }
+          loader_any(false);
+          for (int i = 0; i < kIter; ++i) {
+            const int r = r0 + i * kRowsAtOnce;
+            if (ctl->info[st].odd[r >> 5] >> (r & 31) & 1u)
+              *reinterpret_cast<uint4*>(base_p + (s_v - base) + st * Shape::kTile + (c / 8) * Shape::kBlock + r * 128 +
+                                        ((c & 7) ^ (r & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (bad_now) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&ctl->v_full[st]);
+        if (k + 1 < n) {
+          if (k >= 1 && ok) ok = mbar_wait_bounded(&ctl->v_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
+          copy(k + 1, v_part, s_v + (st ^ 1) * Shape::kTile, none);
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+  } else if (tile < tiles) {
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;             // this warp's 32 lanes of tensor memory
+    const uint32_t t_s = tmem + tile * 128 + lanes, t_o = tmem + 256 + tile * D + lanes;
+    // the tile's own rows decide which units need a mask
+    const int last = min(ts.rows, 128 * tile + 128) - 1;
+    const int pmin = ts.p_first + (ts.r0 + 128 * tile) / G, pmax = ts.p_first + (ts.r0 + last) / G;
+    float ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int k = 0; k < n; ++k) {
+      const int st = k & 1, key0 = ts.unit(k) * kUnit;
+      ok = mbar_wait_bounded(&ctl->v_full[st], (k >> 1) & 1) && mbar_wait_bounded(&ctl->s_full[tile], k & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const PromptInfo& info = ctl->info[st];
+      const uint32_t any_bad = info.bad[0] | info.bad[1] | info.bad[2] | info.bad[3];
+      const uint32_t any_odd = info.odd[0] | info.odd[1] | info.odd[2] | info.odd[3];
+      const bool whole = !any_bad && key0 + kUnit - 1 <= pmin &&
+                         (a.window == 0 || key0 > pmax - a.window || key0 + kUnit <= a.sinks);
+      const float f = info.k_exp ? q_f * 16.f : q_f;
+      // columns hi .. and, with a window, sk .. lo are hidden from this row
+      const int hi = pos - key0, lo = a.window > 0 ? pos - a.window - key0 : -1, sk = a.window > 0 ? a.sinks - key0 : 0;
+      auto mask = [&](uint32_t (&v)[32], int c0) {
+        const uint32_t b = info.bad[c0 >> 5];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = c0 + i;
+          if (c > hi || (c <= lo && c >= sk) || (b >> i & 1u)) v[i] = 0xff800000u;
+        }
+      };
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int c0 = 0; c0 < kUnit; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(t_s + c0, v);
+        tmem_ld_wait();
+        if (!whole) mask(v, c0);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+      }
+      const float want = m == -INFINITY ? m : m * f;
+      const bool move = want > ref + 8.f;
+      const float was = ref;
+      if (move) ref = want;
+      const float al = was == ref ? 1.f : ex2(was - ref);
+      l *= al;
+      if (any_odd || (k > 0 && __any_sync(0xffffffffu, move))) {
+        if (k > 0) {
+          ok = mbar_wait_bounded(&ctl->o_done[tile], (k - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        const float at0 = ref == -INFINITY ? 0.f : ref;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          uint32_t v[16];
+          if (k > 0) {
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(t_o + c0));
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = k > 0 ? __float_as_uint(__uint_as_float(v[i]) * al) : 0u;
+          if (any_odd) {
+            for (int w = 0; w < 4; ++w)
+              for (uint32_t left = info.odd[w]; left; left &= left - 1) {
+                const int c = 32 * w + __ffs(left) - 1;
+                uint32_t x;
+                tmem_ld1(t_s + c, x);
+                tmem_ld_wait();
+                // (a row that does not see the key adds nothing, not zero times it)
+                const bool see = !(c > hi || (c <= lo && c >= sk));
+                const float p = ex2(fmaf(__uint_as_float(x), f, -at0));
+                const int key = key0 + c;
+                const uint8_t* head = pool + __ldg(table + (key >> kv.page_shift)) * page_bytes + v_part;
+                const int slot = key & ((1 << kv.page_shift) - 1);
+#pragma unroll 1
+                for (int i = 0; i < 16; ++i) {
+                  float val;
+                  if constexpr (KV == XM_KV_Q4_0) {    // column 8 q + 2 e + b is value e of block 2 (q % (NG / 2)) + b
+                    const int q = (c0 + i) >> 3, e = ((c0 + i) >> 1) & 3, b = i & 1;
+                    const int blk = 2 * (q % (NG / 2)) + b;
+                    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(head + slot * (D / 2)) + q);
+                    const int code = (word >> (16 * b + 4 * e)) & 15;
+                    const __half d = reinterpret_cast<const __half*>(head + (D / 2 << kv.page_shift))[slot * NG + blk];
+                    val = __half2float(d) * (float)(code - 8);
+                  } else {
+                    val = __half2float(reinterpret_cast<const __half*>(head)[slot * D + c0 + i]);
+                  }
+                  float acc = __uint_as_float(0u);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    if (j == i) acc = __uint_as_float(v[j]);
+                  if (see) acc = fmaf(p, val, acc);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    if (j == i) v[j] = __float_as_uint(acc);
+                }
+                __syncwarp();
+              }
+          }
+          tmem_st16(t_o + c0, v);
+        }
+        tmem_st_wait();
+      }
+      // P, in place of S; scaled up where the unit's values are scaled down
+      const float at = ref == -INFINITY ? 0.f : ref;
+      const float shift = info.v_exp ? 4.f - at : -at;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < kUnit; c0 += 32) {
+        uint32_t v[32], p[16];
+        tmem_ld32(t_s + c0, v);
+        tmem_ld_wait();
+        if (!whole) mask(v, c0);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float x = ex2(fmaf(__uint_as_float(v[i]), f, shift)), y = ex2(fmaf(__uint_as_float(v[i + 1]), f, shift));
+          if (!whole) {                                // (f may be 0)
+            if (v[i] == 0xff800000u) x = 0.f;
+            if (v[i + 1] == 0xff800000u) y = 0.f;
+          }
+          s0 += x;
+          s1 += y;
+          p[i >> 1] = half2_bits(x, y);
+        }
+        tmem_st16(t_s + (c0 >> 1), p);
+      }
+      l = fmaf(s0 + s1, info.v_exp ? 0.0625f : 1.f, l);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&ctl->p_full[tile]);
+    }
+    // O / l
+    if (n > 0 && ok) ok = mbar_wait_bounded(&ctl->o_done[tile], (n - 1) & 1);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    QT_* out = (QT_*)a.out + my_t * a.out_stride + (int64_t)my_h * D;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t v[32];
+      if (n > 0 && ok) {
+        tmem_ld32(t_o + c0, v);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0u;
+      }
+      // eight neighbouring values at a time
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float x[8];
+        int dim;
+        if constexpr (KV == XM_KV_Q4_0) {              // columns c0 ..: eighths c0 / 8 .. of every block
+          // words q = c0 / 8 + 0..3; with n = q / (NG / 2), halves b: block 2 (q % (NG / 2)) + b
+          constexpr int PER = NG / 2;                  // words of an eighth
+          constexpr int EI = 4 / PER;                  // eighths in 32 columns: values 4 n ... 4 n + 3 of each block
+          const int blk = EI == 2 ? b : b % NG, first = EI == 2 ? 0 : 2 * (b / NG);
+          dim = 32 * blk + 4 * (c0 / 8 / PER + first);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int word = (first + e / 4) * PER + blk / 2;
+            x[e] = __uint_as_float(v[8 * word + 2 * (e & 3) + (blk & 1)]) * inv;
+          }
+        } else {
+          dim = c0 + 8 * b;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v[8 * b + e]) * inv;
+        }
+        if (live) {
+          put_out4<QT_>(out + dim, a.out_vec, make_float4(x[0], x[1], x[2], x[3]));
+          put_out4<QT_>(out + dim + 4, a.out_vec, make_float4(x[4], x[5], x[6], x[7]));
+        }
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <typename QT_, int D, int KV, int R>
+int prompt_kernel(const KvView& kv, const AttnArgs& a, int64_t tiles, cudaStream_t st) {
+  constexpr int smem = PromptShape<D>::kSmem;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(k_kv_prompt<QT_, D, KV, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return kv_launch("kv attention", k_kv_prompt<QT_, D, KV, R>, dim3((unsigned)(tiles * kv.Hk)), kPromptThreads, smem, st, kv, a);
+}
+
 template <typename QT_, int D, int KV>
-int attn_launch(const KvView& kv, const AttnArgs& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.T, (unsigned)((a.Hq + kAttnWarps - 1) / kAttnWarps));
-  cfg.blockDim = dim3(32 * kAttnWarps);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv_attn<QT_, D, KV>, kv, a);
-  if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention launch: %s", cudaGetErrorString(e));
-  return xm_check_launch("kv attention");
+int prompt_launch(const KvView& kv, const AttnArgs& a, cudaStream_t st) {
+  // 256 rows per CTA, unless that leaves SMs without one
+  const int64_t rows = a.T * (a.Hq / kv.Hk);
+  if ((rows / 256 + kv.B) * kv.Hk >= 148) return prompt_kernel<QT_, D, KV, 256>(kv, a, rows / 256 + kv.B, st);
+  return prompt_kernel<QT_, D, KV, 128>(kv, a, rows / 128 + kv.B, st);
 }
 
 template <typename QT_>
@@ -1056,8 +1616,10 @@ int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, v
                                 : decode_launch<QT_, 64, XM_KV_Q4_0>(kv, a, p, ws, st);
   }
   if (head_dim == 128)
-    return kv_type == XM_KV_F16 ? attn_launch<QT_, 128, XM_KV_F16>(kv, a, st) : attn_launch<QT_, 128, XM_KV_Q4_0>(kv, a, st);
-  return kv_type == XM_KV_F16 ? attn_launch<QT_, 64, XM_KV_F16>(kv, a, st) : attn_launch<QT_, 64, XM_KV_Q4_0>(kv, a, st);
+    return kv_type == XM_KV_F16 ? prompt_launch<QT_, 128, XM_KV_F16>(kv, a, st)
+                                : prompt_launch<QT_, 128, XM_KV_Q4_0>(kv, a, st);
+  return kv_type == XM_KV_F16 ? prompt_launch<QT_, 64, XM_KV_F16>(kv, a, st)
+                              : prompt_launch<QT_, 64, XM_KV_Q4_0>(kv, a, st);
 }
 
 }  // namespace

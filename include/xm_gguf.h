@@ -370,8 +370,8 @@ int xm_argmax(const float* d_logits, int64_t B, int64_t V, int* d_out, void* str
  * table_width * page_size), 16-byte aligned, no initial contents; two calls
  * that may run at the same time need one each.
  *
- * xm_sample: one token per row of logits (F32 / F16 / BF16, row pitch stride)
- * (sampling.py:94-158).  Weights exp((x - max) / T); in descending order, equal
+ * xm_sample: one token per row of up to 2^20 logits (F32 / F16 / BF16, row pitch
+ * stride) (sampling.py:94-158).  Weights exp((x - max) / T); in descending order, equal
  * logits by ascending index, the first top_k tokens are kept (<= 0: all), of
  * those the ones before which less than top_p of their mass lies (>= 1: all),
  * of those the ones of weight >= min_p (the largest is 1); the first is always

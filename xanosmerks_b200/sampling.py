@@ -26,7 +26,7 @@ def _per_row(v, name, dtype, rows, dev):
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
            out: torch.Tensor | None = None):
-    """(ids int32 [B], logprobs fp32 [B]) of ``logits`` [B, V] (fp32, fp16 or bf16, on a CUDA device).
+    """(ids int32 [B], logprobs fp32 [B]) of ``logits`` [B, V] (fp32, fp16 or bf16, on a CUDA device; V <= 2^20).
 
     Tokens weigh exp((x - max) / temperature).  In descending order of x (equal logits by ascending index)
     the first ``top_k`` are kept (0: all), of those the ones before which less than ``top_p`` of their mass

@@ -367,8 +367,8 @@ int xm_argmax(const float* d_logits, int64_t B, int64_t V, int* d_out, void* str
  * sequence, p the row's own (with window > 0: positions above p - window and
  * the first `sinks` ones); Hq / Hk <= 64 query heads per KV head; a row that
  * sees no key is zeros.  d_ws: xm_kv_attention_workspace_size bytes (max_keys =
- * table_width * page_size), 16-byte aligned, no initial contents; two calls
- * that may run at the same time need one each.
+ * table_width * page_size; 0: null is fine), 16-byte aligned, no initial
+ * contents; two calls that may run at the same time need one each.
  *
  * xm_sample: one token per row of up to 2^20 logits (F32 / F16 / BF16, row pitch
  * stride) (sampling.py:94-158).  Weights exp((x - max) / T); in descending order, equal

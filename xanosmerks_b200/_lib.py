@@ -7,7 +7,6 @@ fails with ``ImportError`` when the shared library has not been built
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -106,13 +105,23 @@ def _load():
 
 lib = _load()
 
-_HERE = contextlib.nullcontext()
 
 
-def on_device(dev):
-    """A context in which `dev` (with an index) is the current device; free where it already is."""
+def call_on(dev, fn, *args) -> int:
+    """fn(*args, stream) with `dev` (a CUDA device with an index) current and its current stream."""
     import torch
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, _raw_stream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev.index))
+
+
+def _raw_stream(index):
+    """The current stream's handle (torch's own accessor where this build has it: a fifth of a microsecond
+    instead of two)."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def check_device(what: str = "") -> None:

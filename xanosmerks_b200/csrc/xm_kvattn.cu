@@ -6,6 +6,8 @@
 //
 // Few rows per sequence (decode steps): k_kv_decode, bound by reading the cache.  Many (prompts): k_kv_prompt, bound by
 // the products and the exponentials.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -14,6 +16,8 @@
 int kv_view(const char* who, void* pool, int64_t pages, int kv_type, int Hk, int head_dim, int page_size,
             const int* table, int64_t table_stride, int64_t table_width, const int* cu, const int* lens, int64_t B,
             KvView* out);
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -58,6 +62,7 @@ struct AttnArgs {
 
 constexpr int kDecWarps = 4;
 constexpr int kMaxSplits = 128;     // one per thread of the merge
+constexpr int kMaxJoined = 8;       // CTAs of a cluster
 
 XM_DEV float ex2(float x) {
   float y;
@@ -280,7 +285,7 @@ XM_DEV bool non_finite(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7
 struct DecArgs {
   int chunk;                // units of a CTA
   int nsplit;
-  float* part_o;            // [nsplit][T][Hq][D], where a row has more than one part
+  float* part_o;            // [nsplit][T][Hq][D], where a row has more than one part; null: joined in a cluster
   float2* part_ml;
 };
 
@@ -309,7 +314,7 @@ struct DecShape {
   static constexpr int kRing = STAGES * SUB * SubTile<KV, D>::kBytes;                       // bytes of a warp
   static constexpr int kJoin = kDecWarps * 8 * NT * ((D + 4) * 4 + 8);                      // reuses the ring
   static constexpr int kQ = NT * (D / 32 * 2 * 256 + 4 * 128);                              // q fragments, q_f, q_off
-  static constexpr int kSmem = kQ + (kDecWarps * kRing > kJoin ? kDecWarps * kRing : kJoin);
+  static constexpr int kSmem = kQ + (kDecWarps * kRing > kJoin ? kDecWarps * kRing : kJoin) + 8 * NT * 8;
   static constexpr int kCtas = NT > 1 ? 2 : KV == XM_KV_Q4_0 || D == 64 ? 3 : 2;          // of an SM
 };
 
@@ -329,12 +334,15 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   int rt, q_len;
   int64_t t0;
   const int s = find_tile<R>(kv, a.T, G, blockIdx.x / kv.Hk, rt, t0, q_len);
-  if (s < 0) return;
+  if (s < 0) return;                                   // (every CTA of a cluster)
   const TileSpan ts = tile_span<R, UK>(kv, a, s, t0, q_len, rt, G);
   if (ts.past_table && threadIdx.x == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-  const int parts = (ts.n + da.chunk - 1) / da.chunk;
-  if (split > 0 && split >= parts) return;
-  const int v_lo = split * da.chunk, v_hi = min(ts.n, v_lo + da.chunk);
+  // parts of da.chunk units that k_kv_merge joins; or, in a cluster, even shares joined through its shared memories
+  const bool joined = da.part_o == nullptr && da.nsplit > 1;
+  const int chunk = joined ? (ts.n + da.nsplit - 1) / da.nsplit : da.chunk;
+  const int parts = joined ? 1 : (ts.n + chunk - 1) / chunk;
+  if (!joined && split > 0 && split >= parts) return;
+  const int v_lo = min(ts.n, split * chunk), v_hi = min(ts.n, v_lo + chunk);
 
   // this lane's columns: rows 2 kq, 2 kq + 1 of every 8
   int pos[NT][2];
@@ -750,6 +758,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   // the warps' parts meet in shared memory
   float(*o_s)[R][DP] = reinterpret_cast<float(*)[R][DP]>(dec_smem);
   float2(*ml_s)[R] = reinterpret_cast<float2(*)[R]>(dec_smem + kDecWarps * R * DP * 4);
+  float2* joint_s = reinterpret_cast<float2*>(dec_smem + Shape::kSmem - R * 8);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -802,7 +811,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     const int gr = ts.r0 + row;
     const int64_t t = t0 + gr / G;
     const int h = hk * G + gr % G;
-    if (parts <= 1) {
+    if (joined) {                                      // kept where the warps' parts were: only this thread reads those
+      *reinterpret_cast<float4*>(&o_s[0][row][d]) = acc;
+      if (d == 0) joint_s[row] = make_float2(m, sum);
+    } else if (parts <= 1) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
       put_out4<QT_>((QT_*)a.out + t * a.out_stride + (int64_t)h * D + d, a.out_vec,
                     make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
@@ -812,6 +824,43 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
       if (d == 0) da.part_ml[cell] = make_float2(m, sum);
     }
   }
+  if (!joined) return;
+  // the cluster's parts, in order, each CTA a share of the output
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  for (int i = (int)threadIdx.x + 32 * kDecWarps * split; i < ts.rows * (D / 4); i += 32 * kDecWarps * da.nsplit) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float2 ml[kMaxJoined];
+    float4 x[kMaxJoined];
+    float m = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < kMaxJoined; ++p) {
+      ml[p] = make_float2(-INFINITY, 0.f);
+      x[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p < da.nsplit) {
+        ml[p] = *cl.map_shared_rank(&joint_s[row], p);
+        x[p] = *reinterpret_cast<const float4*>(cl.map_shared_rank(&o_s[0][row][d], p));
+        m = fmaxf(m, ml[p].x);
+      }
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < kMaxJoined; ++p) {
+      const float f = ex2(ml[p].x - ref);
+      sum = fmaf(ml[p].y, f, sum);
+      acc.x = fmaf(x[p].x, f, acc.x);
+      acc.y = fmaf(x[p].y, f, acc.y);
+      acc.z = fmaf(x[p].z, f, acc.z);
+      acc.w = fmaf(x[p].w, f, acc.w);
+    }
+    const int gr = ts.r0 + row;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    put_out4<QT_>((QT_*)a.out + (t0 + gr / G) * a.out_stride + (int64_t)(hk * G + gr % G) * D + d, a.out_vec,
+                  make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  }
+  cl.sync();                                           // no CTA leaves while its part is read
 }
 
 // Joins the parts of the rows whose keys were split: one CTA per (row, query head), its warps take the
@@ -901,23 +950,26 @@ DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, 
   chunk = std::max<int64_t>(chunk, (max_keys + most - 1) / most);
   p.chunk = (int)((chunk + 127) / 128 * 128);
   p.nsplit = (int)((max_keys + p.chunk - 1) / p.chunk);
-  p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * T * Hq * (D * 4 + 8) : 0;
+  p.ws_bytes = p.nsplit > kMaxJoined ? (int64_t)p.nsplit * T * Hq * (D * 4 + 8) : 0;
   return p;
 }
 
 template <typename... KArgs, typename... Args>
-int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t st,
+int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int cluster_y, int threads, int smem, cudaStream_t st,
               Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.y = (unsigned)cluster_y;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster_y > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return xm_check_launch(what);
@@ -934,19 +986,24 @@ int decode_kernel(const KvView& kv, const AttnArgs& a, const DecArgs& da, dim3 g
     if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return kv_launch("kv attention", k_kv_decode<QT_, D, KV, NT>, grid, 32 * kDecWarps, smem, st, kv, a, da);
+  return kv_launch("kv attention", k_kv_decode<QT_, D, KV, NT>, grid, da.part_o ? 1 : da.nsplit, 32 * kDecWarps, smem,
+                   st, kv, a, da);
 }
 
 template <typename QT_, int D, int KV>
 int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* ws, cudaStream_t st) {
   constexpr int UK = 16 * DecShape<KV, D, 1>::SUB;
-  DecArgs da{p.chunk / UK, p.nsplit, (float*)ws, (float2*)((float*)ws + (int64_t)p.nsplit * a.T * a.Hq * D)};
+  DecArgs da{p.chunk / UK, p.nsplit, nullptr, nullptr};
+  if (p.ws_bytes) {
+    da.part_o = (float*)ws;
+    da.part_ml = (float2*)(da.part_o + (int64_t)p.nsplit * a.T * a.Hq * D);
+  }
   const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)(a.T * a.Hq));
   const int rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1>(kv, a, da, grid, st)
                            : decode_kernel<QT_, D, KV, 2>(kv, a, da, grid, st);
-  if (rc || p.nsplit <= 1) return rc;
-  return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8, UK>, mgrid, 128, 0, st, kv, a, da)
-                   : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16, UK>, mgrid, 128, 0, st, kv, a, da);
+  if (rc || !p.ws_bytes) return rc;
+  return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8, UK>, mgrid, 1, 128, 0, st, kv, a, da)
+                   : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16, UK>, mgrid, 1, 128, 0, st, kv, a, da);
 }
 
 // ---------------------------------------------------------------------------
@@ -1594,7 +1651,8 @@ int prompt_kernel(const KvView& kv, const AttnArgs& a, int64_t tiles, cudaStream
     if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return kv_launch("kv attention", k_kv_prompt<QT_, D, KV, R>, dim3((unsigned)(tiles * kv.Hk)), kPromptThreads, smem, st, kv, a);
+  return kv_launch("kv attention", k_kv_prompt<QT_, D, KV, R>, dim3((unsigned)(tiles * kv.Hk)), 1, kPromptThreads, smem, st,
+                   kv, a);
 }
 
 template <typename QT_, int D, int KV>
@@ -1627,9 +1685,9 @@ int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, v
 extern "C" {
 
 int64_t xm_kv_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hk, int head_dim, int64_t max_keys) {
-  if (T < 1 || B < 1 || Hq < 1 || Hk < 1 || Hq % Hk || max_keys < 1) return 16;
-  return std::max<int64_t>(16, std::max(dec_plan(T, B, Hq, Hk, head_dim, max_keys, true).ws_bytes,
-                                        dec_plan(T, B, Hq, Hk, head_dim, max_keys, false).ws_bytes));
+  if (T < 1 || B < 1 || Hq < 1 || Hk < 1 || Hq % Hk || max_keys < 1) return 0;
+  return std::max(dec_plan(T, B, Hq, Hk, head_dim, max_keys, true).ws_bytes,
+                  dec_plan(T, B, Hq, Hk, head_dim, max_keys, false).ws_bytes);
 }
 
 int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, int Hq, int Hk, int head_dim,
@@ -1652,8 +1710,8 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
   if (!d_q || !d_out) return xm_set_error(XM_ERR_INVALID, "kv_attention: null pointer");
   if (q_stride < (int64_t)Hq * head_dim || out_stride < (int64_t)Hq * head_dim || (((uintptr_t)d_q | (uintptr_t)d_out) & 1))
     return xm_set_error(XM_ERR_INVALID, "kv_attention: bad row pitch or alignment");
-  if (ws_bytes < xm_kv_attention_workspace_size(T, B, Hq, Hk, head_dim, table_width * page_size) || !d_ws ||
-      ((uintptr_t)d_ws & 15))
+  const int64_t need = xm_kv_attention_workspace_size(T, B, Hq, Hk, head_dim, table_width * page_size);
+  if (need && (ws_bytes < need || !d_ws || ((uintptr_t)d_ws & 15)))
     return xm_set_error(XM_ERR_INVALID, "kv_attention: workspace too small or unaligned");
   const int64_t most = 1 << 30;                      // as good as none
   AttnArgs a{d_q, T, q_stride, Hq, scale, window < most ? (int)window : 0, (int)std::min(sinks, most), d_out, out_stride,

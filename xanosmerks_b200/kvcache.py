@@ -20,9 +20,11 @@ There is no CPU fallback; calls run on the current stream of the pool's device.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
-from ._lib import DT_BF16, DT_F16, DT_F32, KV, check, lib, on_device
+from ._lib import DT_BF16, DT_F16, DT_F32, KV, call_on, check, lib
 
 __all__ = ["PagedKVCache", "rope_table"]
 
@@ -46,7 +48,11 @@ def _ints(t, what, dim, dev):
         raise ValueError(f"{what} is on {t.device}, the cache on {dev}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{what} must have unit stride in its last dimension")
-    return t
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(*sizes) -> int:
+    return lib.xm_kv_attention_workspace_size(*sizes)
 
 
 class PagedKVCache:
@@ -84,39 +90,39 @@ class PagedKVCache:
     # -- helpers ------------------------------------------------------------
     def _rows(self, block_table, kv_lens, cu_seqlens, rows):
         """Checks the arguments that name the tokens; the C ABI's (table, stride, width, cu, lens, B)."""
-        _ints(block_table, "block_table", 2, self.device)
-        _ints(kv_lens, "kv_lens", 1, self.device)
+        dev = self.device
+        _ints(block_table, "block_table", 2, dev)
+        _ints(kv_lens, "kv_lens", 1, dev)
         b = kv_lens.shape[0]
-        if block_table.shape[0] != b or b < 1 or block_table.shape[1] < 1:
+        n, width = block_table.shape
+        if n != b or b < 1 or width < 1:
             raise ValueError(f"block_table {tuple(block_table.shape)} does not fit {b} sequences")
         cu = None
         if cu_seqlens is not None:
-            _ints(cu_seqlens, "cu_seqlens", 1, self.device)
+            _ints(cu_seqlens, "cu_seqlens", 1, dev)
             if cu_seqlens.shape[0] != b + 1:
                 raise ValueError(f"cu_seqlens has {cu_seqlens.shape[0]} entries, {b} sequences need {b + 1}")
             cu = cu_seqlens.data_ptr()
         elif rows != b:
             raise ValueError(f"{rows} rows for {b} sequences: give cu_seqlens")
-        return block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu, kv_lens.data_ptr(), b
+        return block_table.data_ptr(), block_table.stride(0), width, cu, kv_lens.data_ptr(), b
 
-    def _out(self, out, shape, dtype):
+    def _out(self, out, rows, heads, dtype):
+        """(out, its row pitch): a new tensor [rows, heads, head_dim], or the caller's, checked."""
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device:
-            raise ValueError(f"out must be {dtype} {tuple(shape)} on {self.device}, got {out.dtype} "
+            return torch.empty((rows, heads, self.head_dim), dtype=dtype, device=self.device), heads * self.head_dim
+        if tuple(out.shape) != (rows, heads, self.head_dim) or out.dtype != dtype or out.device != self.device:
+            raise ValueError(f"out must be {dtype} {(rows, heads, self.head_dim)} on {self.device}, got {out.dtype} "
                              f"{tuple(out.shape)} on {out.device}")
-        self._heads(out, "out")
-        return out
+        return out, self._pitch(out, "out")
 
-    def _heads(self, t, what):
-        """Rows [T, heads, D] whose heads lie one after another."""
-        if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != self.head_dim):
+    def _pitch(self, t, what):
+        """The row pitch of t [T, heads, head_dim], whose heads must lie one after another."""
+        rows, heads, d = t.shape
+        pitch, head, one = t.stride()
+        if one != 1 or (heads > 1 and head != d):
             raise ValueError(f"{what}: the heads of a row must be contiguous")
-        return t
-
-    @staticmethod
-    def _pitch(t, width):
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+        return pitch if rows > 1 else max(pitch, heads * d)
 
     # -- operators ------------------------------------------------------------
     def append(self, qkv: torch.Tensor, num_heads: int, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -128,39 +134,38 @@ class PagedKVCache:
 
         ``qkv`` [T, (num_heads + 2 kv heads) * head_dim], fp32, fp16 or bf16.  Returns the queries
         [T, num_heads, head_dim] in ``out_dtype`` (fp16 or bf16; default: qkv's type, fp16 for fp32)."""
-        d, dev = self.head_dim, self.device
-        if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2 or qkv.dtype not in _DT or qkv.device != dev:
+        d, dev, hk = self.head_dim, self.device, self.num_kv_heads
+        dt = _DT.get(qkv.dtype) if isinstance(qkv, torch.Tensor) else None
+        if dt is None or qkv.dim() != 2 or qkv.device != dev:
             raise ValueError(f"append: qkv must be a 2-D fp32, fp16 or bf16 tensor on {dev}")
-        width = (num_heads + 2 * self.num_kv_heads) * d
-        if num_heads < 1 or num_heads % self.num_kv_heads or qkv.shape[1] != width:
-            raise ValueError(f"append: qkv rows of {qkv.shape[1]} values for {num_heads} query and "
-                             f"{self.num_kv_heads} KV heads of {d}")
-        if qkv.stride(1) != 1:
+        rows, width = qkv.shape
+        if num_heads < 1 or num_heads % hk or width != (num_heads + 2 * hk) * d:
+            raise ValueError(f"append: qkv rows of {width} values for {num_heads} query and {hk} KV heads of {d}")
+        pitch, one = qkv.stride()
+        if one != 1:
             raise ValueError("append: qkv must have unit stride in its last dimension")
-        rows = qkv.shape[0]
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
-        if rope is not None and (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[0] < 1
-                                 or tuple(rope.shape[1:]) != (d // 2, 2) or not rope.is_contiguous()
-                                 or rope.device != dev):
-            raise ValueError(f"append: rope must be a contiguous fp32 tensor [positions, {d // 2}, 2] on {dev}")
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_contiguous()
-                                  or w.device != dev):
-                raise ValueError(f"append: {name} must be a contiguous fp32 tensor [{d}] on {dev}")
+        angles, positions = None, 0
+        if rope is not None:
+            if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[0] < 1 or rope.shape[1] != d // 2
+                    or rope.shape[2] != 2 or not rope.is_contiguous() or rope.device != dev):
+                raise ValueError(f"append: rope must be a contiguous fp32 tensor [positions, {d // 2}, 2] on {dev}")
+            angles, positions = rope.data_ptr(), rope.shape[0]
+        norms = [None, None]
+        for i, w in enumerate((q_norm, k_norm)):
+            if w is not None:
+                if (w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != d or not w.is_contiguous()
+                        or w.device != dev):
+                    raise ValueError(f"append: {'qk'[i]}_norm must be a contiguous fp32 tensor [{d}] on {dev}")
+                norms[i] = w.data_ptr()
         if out_dtype is None:
-            out_dtype = out.dtype if out is not None else torch.float16 if qkv.dtype == torch.float32 else qkv.dtype
-        if out_dtype not in (torch.float16, torch.bfloat16):
+            out_dtype = out.dtype if out is not None else torch.float16 if dt == DT_F32 else qkv.dtype
+        if out_dtype is not torch.float16 and out_dtype is not torch.bfloat16:
             raise ValueError(f"append: queries are fp16 or bf16, not {out_dtype}")
-        q = self._out(out, (rows, num_heads, d), out_dtype)
-        with on_device(dev):
-            check(lib.xm_kv_append(qkv.data_ptr(), _DT[qkv.dtype], rows, self._pitch(qkv, width), num_heads,
-                                   self.num_kv_heads, d, rope.data_ptr() if rope is not None else None,
-                                   rope.shape[0] if rope is not None else 0,
-                                   q_norm.data_ptr() if q_norm is not None else None,
-                                   k_norm.data_ptr() if k_norm is not None else None, eps, self.pool.data_ptr(),
-                                   self.num_pages, self._kv, self.page_size, *where, q.data_ptr(), _DT[out_dtype],
-                                   self._pitch(q, num_heads * d), torch.cuda.current_stream(dev).cuda_stream),
-                  "kv append")
+        q, q_pitch = self._out(out, rows, num_heads, out_dtype)
+        check(call_on(dev, lib.xm_kv_append, qkv.data_ptr(), dt, rows, pitch if rows > 1 else max(pitch, width),
+                      num_heads, hk, d, angles, positions, *norms, eps, self.pool.data_ptr(), self.num_pages, self._kv,
+                      self.page_size, *where, q.data_ptr(), _DT[out_dtype], q_pitch), "kv append")
         return q
 
     def read(self, block_table: torch.Tensor, kv_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
@@ -171,14 +176,11 @@ class PagedKVCache:
         if rows is None or rows < 0:
             raise ValueError("read: num_tokens (the number of rows) is needed with cu_seqlens")
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
-        shape = (rows, self.num_kv_heads, self.head_dim)
         # rows behind the last sequence stay zeros
         make = torch.empty if cu_seqlens is None else torch.zeros
-        k, v = (make(shape, dtype=torch.float16, device=self.device) for _ in range(2))
-        with on_device(self.device):
-            check(lib.xm_kv_read(self.pool.data_ptr(), self.num_pages, self._kv, self.num_kv_heads, self.head_dim,
-                                 self.page_size, *where, rows, k.data_ptr(), v.data_ptr(),
-                                 torch.cuda.current_stream(self.device).cuda_stream), "kv read")
+        k, v = make((2, rows, self.num_kv_heads, self.head_dim), dtype=torch.float16, device=self.device).unbind(0)
+        check(call_on(self.device, lib.xm_kv_read, self.pool.data_ptr(), self.num_pages, self._kv, self.num_kv_heads,
+                      self.head_dim, self.page_size, *where, rows, k.data_ptr(), v.data_ptr()), "kv read")
         return k, v
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -189,28 +191,25 @@ class PagedKVCache:
         position p to positions above p - window and the first ``sinks`` ones.  Query head h reads KV head
         h // (heads / kv heads).  ``scale`` defaults to 1 / sqrt(head_dim).  A row that sees no key is zeros.
         Without ``out``, rows behind the last sequence are not initialised."""
-        d, dev = self.head_dim, self.device
+        d, dev, hk = self.head_dim, self.device, self.num_kv_heads
         if (not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16)
                 or q.device != dev):
             raise ValueError(f"attend: q must be a 3-D fp16 or bf16 tensor on {dev}")
-        rows, heads = q.shape[0], q.shape[1]
-        if q.shape[2] != d or heads < 1 or heads % self.num_kv_heads:
-            raise ValueError(f"attend: q {tuple(q.shape)} for {self.num_kv_heads} KV heads of {d}")
+        rows, heads, width = q.shape
+        if width != d or heads < 1 or heads % hk:
+            raise ValueError(f"attend: q {tuple(q.shape)} for {hk} KV heads of {d}")
         if window < 0 or sinks < 0:
             raise ValueError("attend: window and sinks must not be negative")
-        self._heads(q, "attend: q")
+        pitch = self._pitch(q, "attend: q")
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
-        o = self._out(out, (rows, heads, d), q.dtype)
-        need = lib.xm_kv_attention_workspace_size(rows, where[5], heads, self.num_kv_heads, d,
-                                                  where[2] * self.page_size)
+        o, o_pitch = self._out(out, rows, heads, q.dtype)
+        need = _workspace_size(rows, where[5], heads, hk, d, where[2] * self.page_size)
         # a workspace for each call: two captured graphs, or two streams, never share one
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        with on_device(dev):
-            check(lib.xm_kv_attention(q.data_ptr(), _DT[q.dtype], rows, self._pitch(q, heads * d), heads,
-                                      self.num_kv_heads, d, d ** -0.5 if scale is None else scale, window, sinks,
-                                      self.pool.data_ptr(), self.num_pages, self._kv, self.page_size, *where,
-                                      o.data_ptr(), self._pitch(o, heads * d), ws.data_ptr(), need,
-                                      torch.cuda.current_stream(dev).cuda_stream), "kv attention")
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(call_on(dev, lib.xm_kv_attention, q.data_ptr(), _DT[q.dtype], rows, pitch, heads, hk, d,
+                      d ** -0.5 if scale is None else scale, window, sinks, self.pool.data_ptr(), self.num_pages,
+                      self._kv, self.page_size, *where, o.data_ptr(), o_pitch, None if ws is None else ws.data_ptr(),
+                      need), "kv attention")
         return o
 
     def __repr__(self):

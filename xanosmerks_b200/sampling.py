@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import DT_BF16, DT_F16, DT_F32, check, lib, on_device
+from ._lib import DT_BF16, DT_F16, DT_F32, call_on, check, lib
 
 __all__ = ["sample"]
 
@@ -19,7 +19,7 @@ def _per_row(v, name, dtype, rows, dev):
     """(scalar, device pointer or None) of a parameter given as a number or as a tensor with one entry per row."""
     if not isinstance(v, torch.Tensor):
         return v, None
-    if v.dtype != dtype or tuple(v.shape) != (rows,) or v.device != dev or not v.is_contiguous():
+    if v.dtype != dtype or v.dim() != 1 or v.shape[0] != rows or v.device != dev or not v.is_contiguous():
         raise ValueError(f"sample: {name} must be a number or a contiguous {dtype} tensor [{rows}] on {dev}")
     return 0, v.data_ptr()
 
@@ -37,27 +37,26 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 
     Each parameter is a number or a tensor with one entry per row (``top_k`` int32, the others fp32).
     ``out``: an int32 tensor [B] for the ids."""
-    if (not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DT or not logits.is_cuda
-            or logits.shape[1] < 1):
+    dt = _DT.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
+    if dt is None or logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1:
         raise ValueError("sample: logits must be a 2-D fp32, fp16 or bf16 CUDA tensor")
     b, v = logits.shape
     dev = logits.device
-    if v > 1 and logits.stride(1) != 1:
+    pitch, one = logits.stride()
+    if v > 1 and one != 1:
         raise ValueError("sample: logits must have unit stride in the last dimension")
-    if (not isinstance(u, torch.Tensor) or u.dtype != torch.float32 or tuple(u.shape) != (b,) or u.device != dev
-            or not u.is_contiguous()):
+    if not isinstance(u, torch.Tensor):
         raise ValueError(f"sample: u must be a contiguous fp32 tensor [{b}] on {dev}")
+    _, up = _per_row(u, "u", torch.float32, b, dev)
     t, tp = _per_row(temperature, "temperature", torch.float32, b, dev)
     k, kp = _per_row(top_k, "top_k", torch.int32, b, dev)
     p, pp = _per_row(top_p, "top_p", torch.float32, b, dev)
     m, mp = _per_row(min_p, "min_p", torch.float32, b, dev)
     if out is None:
         out = torch.empty(b, dtype=torch.int32, device=dev)
-    elif out.dtype != torch.int32 or tuple(out.shape) != (b,) or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"sample: out must be a contiguous int32 tensor [{b}] on {dev}")
+    else:
+        _per_row(out, "out", torch.int32, b, dev)
     logp = torch.empty(b, dtype=torch.float32, device=dev)
-    with on_device(dev):
-        check(lib.xm_sample(logits.data_ptr(), _DT[logits.dtype], b, v, logits.stride(0) if b > 1 else v,
-                            u.data_ptr(), t, tp, k, kp, p, pp, m, mp, out.data_ptr(), logp.data_ptr(),
-                            torch.cuda.current_stream(dev).cuda_stream), "sample")
+    check(call_on(dev, lib.xm_sample, logits.data_ptr(), dt, b, v, pitch if b > 1 else v, up, t, tp, k, kp, p, pp, m,
+                  mp, out.data_ptr(), logp.data_ptr()), "sample")
     return out, logp

@@ -42,21 +42,24 @@ __host__ __device__ inline int64_t kv_part_bytes(int kv_type, int D, int page_si
   return kv_type == XM_KV_F16 ? (int64_t)page_size * D * 2 : (int64_t)page_size * (D / 2 + D / 16);
 }
 
-// The sequence of row t, or -1 for a row behind the last sequence.
-XM_DEV int kv_sequence(const KvView& kv, int64_t t) {
-  if (!kv.cu) return t < kv.B ? (int)t : -1;
-  int lo = 0, hi = kv.B;                       // the first s in [0, B] with cu[s + 1] > t, B if there is none
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((int64_t)__ldg(kv.cu + mid + 1) > t) hi = mid; else lo = mid + 1;
+// The sequence and position of row t (position negative: the sequence holds fewer tokens than it has
+// rows; sequence -1: behind the last one).  Every lane of the warp calls it with the same t: the offsets are
+// compared 32 at a time, so that their loads do not wait for one another.
+struct KvPlace {
+  int seq;
+  int64_t pos;
+};
+XM_DEV KvPlace kv_place(const KvView& kv, int64_t t) {
+  if (!kv.cu) return t < kv.B ? KvPlace{(int)t, (int64_t)__ldg(kv.lens + t) - 1} : KvPlace{-1, -1};
+  const int lane = threadIdx.x & 31;
+  int seq = 0;
+#pragma unroll 4
+  for (int s0 = 0; s0 < kv.B; s0 += 32) {             // how many sequences end at or before t
+    const bool past = s0 + lane < kv.B && (int64_t)__ldg(kv.cu + s0 + lane + 1) <= t;
+    seq += __popc(__ballot_sync(0xffffffffu, past));
   }
-  return lo < kv.B && (int64_t)__ldg(kv.cu + lo) <= t ? lo : -1;
-}
-
-// The position of row t of sequence s (negative: the sequence holds fewer tokens than it has rows).
-XM_DEV int64_t kv_position(const KvView& kv, int s, int64_t t) {
-  const int64_t len = __ldg(kv.lens + s);
-  return kv.cu ? len - ((int64_t)__ldg(kv.cu + s + 1) - t) : len - 1;
+  if (seq >= kv.B || (int64_t)__ldg(kv.cu + seq) > t) return KvPlace{-1, -1};
+  return KvPlace{seq, (int64_t)__ldg(kv.lens + seq) - ((int64_t)__ldg(kv.cu + seq + 1) - t)};
 }
 
 // The page that holds position pos >= 0 of sequence s, or -1 (and the error bit) where the table or

@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.Hq / kv.Hk;
   const int64_t cell = blockIdx.x, cells = a.T * a.Hq, t = cell / a.Hq;
   const int h = (int)(cell % a.Hq);
-  const int s = kv_sequence(kv, t);
+  const int s = kv_place(kv, t).seq;
   if (s < 0) return;
   int64_t t0;
   int q_len;

@@ -1,6 +1,6 @@
 // Appending to and reading from the paged key/value cache (layout: xm_kv.cuh).
 //
-// k_kv_put: one warp per (row, head).  A query or key head x of D values is
+// k_kv_put: a query or key head x of D values is
 // optionally normalised, x' = x w / sqrt(mean(x^2) + eps), and rotated by the
 // angles of its position, y[i] = x'[i] cos_i - x'[i + D/2] sin_i and
 // y[i + D/2] = x'[i + D/2] cos_i + x'[i] sin_i with (cos, sin) from a table that
@@ -16,167 +16,160 @@
 // arithmetic runs at half the fp32 rate here and is off the critical path of
 // the memory traffic); everything else is fp32.
 //
-// Bound: memory.  Lane l holds values 2l, 2l + 1 of each half of the head (one
-// value per half at D = 64), so the rotation needs no exchange, a half-head is
-// one 256-byte load at fp32, and a group of 32 values is 16 lanes.
+// Bound: memory for prompts, latency for single tokens.  D / 8 lanes take a head, so a warp two heads
+// of 128 or four of 64: lane l of them holds the values 4 l .. 4 l + 3 of each half, so the rotation
+// needs no exchange, loads and stores are 8 or 16 bytes, and a block of 32 values is 8 lanes.  A
+// block's codes are words of 2 lanes (keys) or halfwords of one (values).
 #include <type_traits>
 
 #include "xm_kv.cuh"
 
 namespace {
 
-// Q4_0 of the groups of 32 values held VPL per lane by 32 / VPL consecutive lanes (VPL = 1 or 2,
-// values VPL l, VPL l + 1).  c: the codes; returns the group's d (as fp16).
-template <int VPL>
-XM_DEV __half q4_group(const float (&x)[VPL], int (&c)[VPL]) {
-  constexpr int W = 32 / VPL;                         // lanes of a group
+constexpr int kPutWarps = 8;
+constexpr unsigned kAll = 0xffffffffu;
+
+// Q4_0 of the block held four values a lane by 8 neighbouring lanes: the lane's four codes as a halfword, d.
+XM_DEV uint32_t q4_block(const float (&x)[4], __half& dh) {
   const int lane = threadIdx.x & 31;
   bool bad = false;
   float mag = 0.f;
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
+  for (int i = 0; i < 4; ++i) {
     bad |= !(fabsf(x[i]) < INFINITY);
     mag = fmaxf(mag, fabsf(x[i]));
   }
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
-  const unsigned group = VPL == 1 ? 0xffffffffu : 0xffffu << (lane & 16);
-  const bool spoilt = __ballot_sync(0xffffffffu, bad) & group;
-  bool mine = false;                                  // this lane holds a value of largest magnitude
+  for (int o = 4; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(kAll, mag, o));
+  const unsigned block = 0xffu << (lane & 24);
+  const bool spoilt = __ballot_sync(kAll, bad) & block;
+  bool mine = false;                                  // this lane holds a value of largest magnitude: its first
   float a = 0.f;
 #pragma unroll
-  for (int i = VPL - 1; i >= 0; --i)
+  for (int i = 3; i >= 0; --i)
     if (fabsf(x[i]) == mag) {
       mine = true;
       a = x[i];
     }
-  const unsigned who = __ballot_sync(0xffffffffu, mine) & group;
-  a = __shfl_sync(0xffffffffu, a, who ? __ffs(who) - 1 : lane);
-  // a non-finite value spoils its group: d = NaN, every value of the group reads as NaN
-  const __half dh = spoilt ? __ushort_as_half((unsigned short)0x7fff) : __float2half_rn(a * -0.125f);
+  const unsigned who = __ballot_sync(kAll, mine) & block;
+  a = __shfl_sync(kAll, a, who ? __ffs(who) - 1 : lane);
+  // a non-finite value spoils its block: d = NaN, every value of it reads as NaN
+  dh = spoilt ? __ushort_as_half((unsigned short)0x7fff) : __float2half_rn(a * -0.125f);
   const float d = __half2float(dh), ad = fabsf(d);
-  const bool blank = !(ad > 0.f && ad < INFINITY);
+  if (!(ad > 0.f && ad < INFINITY)) return 0x8888u;
   const float inv = 1.0f / d;
+  uint32_t codes = 0;
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    int q = 8;
-    if (!blank) {
-      const float y = d < 0.f ? -x[i] : x[i];
-      float e = floorf(fmaf(x[i], inv, 8.5f));
-      e = fminf(fmaxf(e, 0.f), 15.f);
-      if (e > 0.f && fmaf(8.5f - e, ad, y) < 0.f) e -= 1.f;
-      else if (e < 15.f && fmaf(7.5f - e, ad, y) >= 0.f) e += 1.f;
-      q = (int)e;
-    }
-    c[i] = q;
+  for (int i = 0; i < 4; ++i) {
+    const float y = d < 0.f ? -x[i] : x[i];
+    float e = floorf(fmaf(x[i], inv, 8.5f));
+    e = fminf(fmaxf(e, 0.f), 15.f);
+    if (e > 0.f && fmaf(8.5f - e, ad, y) < 0.f) e -= 1.f;
+    else if (e < 15.f && fmaf(7.5f - e, ad, y) >= 0.f) e += 1.f;
+    codes |= (uint32_t)(int)e << (4 * i);
   }
-  return dh;
+  return codes;
 }
 
-// Writes one half of a head (values VPL l + i + half D / 2 on lane l) as codes into row `slot` of a part.
-// VALUES: the values' order of the codes instead of the keys'.
-template <int D, bool VALUES>
-XM_DEV void put_half_q4(const float (&x)[D / 64], int half, uint8_t* part, int page_size, int slot) {
-  constexpr int VPL = D / 64, NG = D / 32;
-  const int lane = threadIdx.x & 31;
-  int c[VPL];
-  const __half d = q4_group<VPL>(x, c);
-  uint32_t w = 0;                                     // this lane's nibbles
+// Writes a head (lo, hi: this lane's values of its halves) as codes into row `slot` of a part, where `on`; every
+// lane of the warp calls it.  values: the values' order of the codes instead of the keys'.
+template <int D>
+XM_DEV void put_q4(const float (&lo)[4], const float (&hi)[4], bool values, bool on, uint8_t* part, int page_size,
+                   int slot) {
+  constexpr int LPH = D / 8, NG = D / 32;
+  const int l = threadIdx.x & (LPH - 1), n = l & 7;   // lane of the head; of its block
+  __half d[2];
+  uint32_t w[2] = {q4_block(lo, d[0]), q4_block(hi, d[1])};
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) w |= (uint32_t)c[i] << (4 * i);
-  const int g = half * (NG / 2) + (VPL * lane) / 32;  // group
-  const int e = (VPL * lane) % 32;                    // first value in the group
-  constexpr int PER = VALUES ? 4 : 8;                 // values of a word (halfword)
-  w <<= 4 * (e % PER);
-#pragma unroll
-  for (int o = 1; o < PER / VPL; o <<= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
+  for (int h = 0; h < 2; ++h) {                       // keys: a word is the halfwords of two lanes
+    const uint32_t o = __shfl_xor_sync(kAll, w[h], 1);
+    if (!values) w[h] = l & 1 ? o | w[h] << 16 : w[h] | o << 16;
+  }
+  uint32_t s0 = (uint32_t)__half_as_ushort(d[0]) | (uint32_t)__half_as_ushort(d[1]) << 16;
   uint8_t* row = part + (int64_t)slot * (D / 2);
-  if (e % PER == 0) {
-    if (VALUES)
-      reinterpret_cast<uint16_t*>(row)[NG * (e / 4) + g] = (uint16_t)w;
-    else
-      reinterpret_cast<uint32_t*>(row)[NG * (e / 8) + g] = w;
+  uint8_t* scales = part + (int64_t)page_size * (D / 2) + slot * (2 * NG);
+  if constexpr (NG == 4) {
+    // lanes 0-7 hold blocks 0 and 2, lanes 8-15 blocks 1 and 3: the former take both
+    const uint32_t o0 = __shfl_xor_sync(kAll, w[0], 8), o1 = __shfl_xor_sync(kAll, w[1], 8);
+    const uint32_t o2 = __shfl_xor_sync(kAll, s0, 8);
+    if (!on || l >= 8) return;
+    if (values)
+      *reinterpret_cast<uint2*>(row + 8 * n) = make_uint2(w[0] | o0 << 16, w[1] | o1 << 16);
+    else if (!(n & 1))
+      *reinterpret_cast<uint4*>(row + 8 * n) = make_uint4(w[0], o0, w[1], o1);
+    if (n == 0)
+      *reinterpret_cast<uint2*>(scales) = make_uint2((s0 & 0xffffu) | o2 << 16, s0 >> 16 | (o2 & 0xffff0000u));
+  } else {
+    if (!on) return;
+    if (values)
+      *reinterpret_cast<uint32_t*>(row + 4 * n) = w[0] | w[1] << 16;
+    else if (!(n & 1))
+      *reinterpret_cast<uint2*>(row + 4 * n) = make_uint2(w[0], w[1]);
+    if (n == 0) *reinterpret_cast<uint32_t*>(scales) = s0;
   }
-  if (e == 0) reinterpret_cast<__half*>(part + (int64_t)page_size * (D / 2))[slot * NG + g] = d;
 }
 
-template <typename XT, int VPL>
-XM_DEV void load_vals(const XT* p, bool pairs, float (&v)[VPL]) {
-  if constexpr (VPL == 2) {
-    if (pairs) {
-      if constexpr (sizeof(XT) == 4) {
-        const float2 f = *reinterpret_cast<const float2*>(p);
-        v[0] = f.x; v[1] = f.y;
-      } else {
-        XT t[2];
-        *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(p);
-        v[0] = to_f32(t[0]); v[1] = to_f32(t[1]);
-      }
-      return;
-    }
-  }
+// four neighbouring values; `wide`: the rows allow one load (store)
+template <typename XT>
+XM_DEV void load4(const XT* p, bool wide, float (&v)[4]) {
+  if (wide) {
+    ld4f<XT>(p, v);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) v[i] = to_f32(p[i]);
-}
-
-template <typename QT_, int VPL>
-XM_DEV void store_vals(QT_* p, bool pairs, const float (&v)[VPL]) {
-  if constexpr (VPL == 2) {
-    if (pairs) {
-      QT_ t[2];
-      if constexpr (sizeof(QT_) == 2 && std::is_same<QT_, __half>::value) {
-        t[0] = __float2half_rn(v[0]); t[1] = __float2half_rn(v[1]);
-      } else {
-        t[0] = __float2bfloat16_rn(v[0]); t[1] = __float2bfloat16_rn(v[1]);
-      }
-      *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(t);
-      return;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = to_f32(p[i]);
   }
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    if constexpr (std::is_same<QT_, __half>::value) p[i] = __float2half_rn(v[i]);
-    else p[i] = __float2bfloat16_rn(v[i]);
+}
+XM_DEV void store4(void* p, bool bf16, bool wide, const float (&v)[4]) {
+  uint2 w;
+  if (bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+  if (wide) {
+    *reinterpret_cast<uint2*>(p) = w;
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p);
+    q[0] = (uint16_t)w.x; q[1] = (uint16_t)(w.x >> 16); q[2] = (uint16_t)w.y; q[3] = (uint16_t)(w.y >> 16);
   }
 }
 
-XM_DEV double warp_sum_f64(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// One head in arithmetic of type F: normalise and rotate lo (first half) and hi (second half).
+// Heads in arithmetic of type F: normalise (w: this lane's weights of the halves, where `norm`) and rotate (cs:
+// (cos, sin) of the lane's four angles, where `turn`).  Every lane of the warp calls it.
 template <typename F, int D>
-XM_DEV void norm_rotate(float (&lo)[D / 64], float (&hi)[D / 64], const float* __restrict__ w, double eps,
-                        const float2* __restrict__ cs) {
-  constexpr int VPL = D / 64;
-  const int lane = threadIdx.x & 31;
-  F a[VPL], b[VPL];
+XM_DEV void norm_rotate(float (&lo)[4], float (&hi)[4], bool norm, const float4& wl, const float4& wh, double eps,
+                        bool turn, const float2 (&cs)[4]) {
+  F a[4], b[4];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
+  for (int i = 0; i < 4; ++i) {
     a[i] = (F)lo[i];
     b[i] = (F)hi[i];
   }
-  if (w) {
+  if (__any_sync(kAll, norm)) {
     F ss = 0;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) ss += a[i] * a[i] + b[i] * b[i];
-    F r;
-    if constexpr (sizeof(F) == 8) r = 1.0 / sqrt(warp_sum_f64(ss) / D + eps);
-    else r = 1.0f / sqrtf(warp_sum(ss) * (1.0f / D) + (float)eps);
+    for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      a[i] = a[i] * r * (F)__ldg(w + VPL * lane + i);
-      b[i] = b[i] * r * (F)__ldg(w + D / 2 + VPL * lane + i);
+    for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+    if (norm) {
+      F r;
+      if constexpr (sizeof(F) == 8) r = rsqrt(ss * (1.0 / D) + eps);
+      else r = rsqrtf(ss * (1.0f / D) + (float)eps);
+      const float l4[4] = {wl.x, wl.y, wl.z, wl.w}, h4[4] = {wh.x, wh.y, wh.z, wh.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[i] = a[i] * r * (F)l4[i];
+        b[i] = b[i] * r * (F)h4[i];
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    if (cs) {
-      const float2 t = __ldg(cs + VPL * lane + i);
-      lo[i] = (float)(a[i] * (F)t.x - b[i] * (F)t.y);
-      hi[i] = (float)(b[i] * (F)t.x + a[i] * (F)t.y);
+  for (int i = 0; i < 4; ++i) {
+    if (turn) {
+      lo[i] = (float)(a[i] * (F)cs[i].x - b[i] * (F)cs[i].y);
+      hi[i] = (float)(b[i] * (F)cs[i].x + a[i] * (F)cs[i].y);
     } else {
       lo[i] = (float)a[i];
       hi[i] = (float)b[i];
@@ -194,22 +187,32 @@ struct PutArgs {
   double eps;
   void* q;
   int64_t q_stride;
-  bool in_pairs, out_pairs;     // rows allow loads / stores of two values
-  int q_bf16;
+  bool in_wide, out_wide, norm_wide;      // rows allow loads / stores of four values
+  bool q_bf16;
+  int warps;                              // of a row (a power of two): a CTA takes kPutWarps / warps rows
 };
 
-constexpr int kPutWarps = 8;
-
 template <typename XT, int D, int KV>
-__global__ void __launch_bounds__(32 * kPutWarps) k_kv_put(const KvView kv, const PutArgs a) {
-  constexpr int VPL = D / 64;
+__global__ void __launch_bounds__(32 * kPutWarps, 3) k_kv_put(const KvView kv, const PutArgs a) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH;
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const int s = kv_sequence(kv, t);
-  if (s < 0) return;                                   // behind the last sequence: left as it is
-  const int64_t pos = kv_position(kv, s, t);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (LPH - 1);
+  const int64_t t = (int64_t)blockIdx.x * (kPutWarps / a.warps) + warp / a.warps;
+  if (t >= a.T) return;
+  const int part_of = blockIdx.y * a.warps + (warp & (a.warps - 1));
+  const int heads = a.Hq + 2 * kv.Hk, step = gridDim.y * a.warps * HPW;
+  int h = part_of * HPW + lane / LPH;
+  const XT* x = (const XT*)a.qkv + t * a.qkv_stride + 4 * l;
+  // the first head's values start on their way before the row's place is known
+  float lo[4] = {}, hi[4] = {};
+  if (h < heads) {
+    load4<XT>(x + (int64_t)h * D, a.in_wide, lo);
+    load4<XT>(x + (int64_t)h * D + D / 2, a.in_wide, hi);
+  }
+  const KvPlace at = kv_place(kv, t);
+  if (at.seq < 0) return;                              // behind the last sequence: left as it is
+  const int64_t pos = at.pos;
   bool ok = pos >= 0;
   int64_t page = -1;
   if (ok) {
@@ -217,95 +220,130 @@ __global__ void __launch_bounds__(32 * kPutWarps) k_kv_put(const KvView kv, cons
       atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
       ok = false;
     } else {
-      page = kv_page(kv, s, pos);
+      page = kv_page(kv, at.seq, pos);
       ok = page >= 0;
     }
   }
-  const float2* cs = a.rope && ok ? reinterpret_cast<const float2*>(a.rope) + pos * (D / 2) : nullptr;
+  float2 cs[4];
+  const bool turn = a.rope && ok;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    cs[i] = turn ? __ldg(reinterpret_cast<const float2*>(a.rope) + pos * (D / 2) + 4 * l + i) : make_float2(1.f, 0.f);
   const int page_size = 1 << kv.page_shift, slot = (int)(pos & (page_size - 1));
-  const int heads = a.Hq + 2 * kv.Hk;
-  for (int h = blockIdx.y * kPutWarps + warp; h < heads; h += gridDim.y * kPutWarps) {
-    const XT* x = (const XT*)a.qkv + t * a.qkv_stride + (int64_t)h * D;
-    float lo[VPL], hi[VPL];
-    load_vals<XT, VPL>(x + VPL * lane, a.in_pairs, lo);
-    load_vals<XT, VPL>(x + D / 2 + VPL * lane, a.in_pairs, hi);
-    if (h < a.Hq) {
-      norm_rotate<float, D>(lo, hi, a.q_norm, a.eps, cs);
+  for (int first = part_of * HPW; first < heads; first += step) {
+    float nlo[4] = {}, nhi[4] = {};                    // the next heads load while these are worked on
+    if (h + step < heads) {
+      load4<XT>(x + (int64_t)(h + step) * D, a.in_wide, nlo);
+      load4<XT>(x + (int64_t)(h + step) * D + D / 2, a.in_wide, nhi);
+    }
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + kv.Hk;
+    const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    float4 wl = make_float4(0.f, 0.f, 0.f, 0.f), wh = wl;
+    if (w) {
+      if (a.norm_wide) {
+        wl = __ldg(reinterpret_cast<const float4*>(w) + l);
+        wh = __ldg(reinterpret_cast<const float4*>(w + D / 2) + l);
+      } else {
+        wl = make_float4(w[4 * l], w[4 * l + 1], w[4 * l + 2], w[4 * l + 3]);
+        wh = make_float4(w[D / 2 + 4 * l], w[D / 2 + 4 * l + 1], w[D / 2 + 4 * l + 2], w[D / 2 + 4 * l + 3]);
+      }
+    }
+    const bool exact = KV == XM_KV_Q4_0 && !is_q && !is_v && h < heads;
+    if (!__any_sync(kAll, exact)) {
+      norm_rotate<float, D>(lo, hi, w != nullptr, wl, wh, a.eps, turn && !is_v, cs);
+    } else {
+      float l2[4] = {lo[0], lo[1], lo[2], lo[3]}, h2[4] = {hi[0], hi[1], hi[2], hi[3]};
+      norm_rotate<double, D>(l2, h2, exact && w != nullptr, wl, wh, a.eps, turn, cs);
+      // (a warp has heads of several kinds only where their counts are odd)
+      if (!__all_sync(kAll, exact)) norm_rotate<float, D>(lo, hi, !exact && w != nullptr, wl, wh, a.eps, turn && !is_v, cs);
+      if (exact) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = l2[i];
+          hi[i] = h2[i];
+        }
+      }
+    }
+    if (is_q) {
       if (!ok) {                                       // no position: a query of zeros
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) lo[i] = hi[i] = 0.f;
+        for (int i = 0; i < 4; ++i) lo[i] = hi[i] = 0.f;
       }
-      const int64_t o = t * a.q_stride + (int64_t)h * D + VPL * lane;
-      if (a.q_bf16) {
-        store_vals<__nv_bfloat16, VPL>((__nv_bfloat16*)a.q + o, a.out_pairs, lo);
-        store_vals<__nv_bfloat16, VPL>((__nv_bfloat16*)a.q + o + D / 2, a.out_pairs, hi);
-      } else {
-        store_vals<__half, VPL>((__half*)a.q + o, a.out_pairs, lo);
-        store_vals<__half, VPL>((__half*)a.q + o + D / 2, a.out_pairs, hi);
-      }
-      continue;
+      uint16_t* o = (uint16_t*)a.q + t * a.q_stride + (int64_t)h * D + 4 * l;
+      store4(o, a.q_bf16, a.out_wide, lo);
+      store4(o + D / 2, a.q_bf16, a.out_wide, hi);
     }
-    if (!ok) continue;
-    const bool is_v = h >= a.Hq + kv.Hk;
-    const int hk = h - a.Hq - (is_v ? kv.Hk : 0);
-    uint8_t* part = kv.pool + (page * kv.Hk + hk) * kv.head_bytes + (is_v ? kv.head_bytes / 2 : 0);
+    const bool store = !is_q && ok && h < heads;
+    const int hk = is_v ? h - a.Hq - kv.Hk : h - a.Hq;
+    uint8_t* part = kv.pool + (store ? (page * kv.Hk + hk) * kv.head_bytes + (is_v ? kv.head_bytes / 2 : 0) : 0);
     if constexpr (KV == XM_KV_F16) {
-      if (!is_v) norm_rotate<float, D>(lo, hi, a.k_norm, a.eps, cs);
-      __half* row = (__half*)part + (int64_t)slot * D + VPL * lane;
-      store_vals<__half, VPL>(row, true, lo);
-      store_vals<__half, VPL>(row + D / 2, true, hi);
-    } else {
-      if (is_v) {
-        put_half_q4<D, true>(lo, 0, part, page_size, slot);
-        put_half_q4<D, true>(hi, 1, part, page_size, slot);
-      } else {
-        norm_rotate<double, D>(lo, hi, a.k_norm, a.eps, cs);
-        put_half_q4<D, false>(lo, 0, part, page_size, slot);
-        put_half_q4<D, false>(hi, 1, part, page_size, slot);
+      if (store) {
+        __half* row = (__half*)part + (int64_t)slot * D + 4 * l;
+        store4(row, false, true, lo);
+        store4(row + D / 2, false, true, hi);
       }
+    } else {
+      if (__any_sync(kAll, store)) put_q4<D>(lo, hi, is_v, store, part, page_size, slot);
+    }
+    h += step;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = nlo[i];
+      hi[i] = nhi[i];
     }
   }
 }
 
-// Reads the cached keys and values of the rows back as fp16 values [T][Hk][D]: one warp per (row, KV
-// head, part); d (c - 8) is exact in fp32 and rounded once.
+// Reads the cached keys and values of the rows back as fp16 values [T][Hk][D]: a lane eight neighbouring values of
+// a head, one word of codes (keys) or two halfwords (values); d (c - 8) is exact in fp32 and rounded once.
 template <int D, int KV>
 __global__ void __launch_bounds__(32 * kPutWarps) k_kv_get(const KvView kv, __half* __restrict__ k,
-                                                           __half* __restrict__ v) {
-  constexpr int VPL = D / 64, NG = D / 32;
+                                                           __half* __restrict__ v, bool wide, int64_t T, int warps) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, NG = D / 32;
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const int s = kv_sequence(kv, t);
-  if (s < 0) return;
-  const int64_t pos = kv_position(kv, s, t);
-  const int64_t page = pos >= 0 ? kv_page(kv, s, pos) : -1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & (LPH - 1);
+  const int64_t t = (int64_t)blockIdx.x * (kPutWarps / warps) + warp / warps;
+  if (t >= T) return;
+  const KvPlace at = kv_place(kv, t);
+  if (at.seq < 0) return;
+  const int64_t pos = at.pos, page = pos >= 0 ? kv_page(kv, at.seq, pos) : -1;
   const int page_size = 1 << kv.page_shift, slot = (int)(pos & (page_size - 1));
-  for (int h = blockIdx.y * kPutWarps + warp; h < 2 * kv.Hk; h += gridDim.y * kPutWarps) {
+  const int g = c >> 2, e = c & 3;                     // block of the eight values, which eighths of it
+  for (int h = (blockIdx.y * warps + (warp & (warps - 1))) * HPW + lane / LPH; h < 2 * kv.Hk; h += gridDim.y * warps * HPW) {
     const bool is_v = h >= kv.Hk;
     const int hk = is_v ? h - kv.Hk : h;
-    __half* o = (is_v ? v : k) + (t * kv.Hk + hk) * D + VPL * lane;
-    const uint8_t* part = kv.pool + (page * kv.Hk + hk) * kv.head_bytes + (is_v ? kv.head_bytes / 2 : 0);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float x[VPL];
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) x[i] = 0.f;
-      if (page >= 0) {
-        if constexpr (KV == XM_KV_F16) {
-          load_vals<__half, VPL>((const __half*)part + (int64_t)slot * D + half * (D / 2) + VPL * lane, true, x);
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);
+    if (page >= 0) {
+      const uint8_t* part = kv.pool + (page * kv.Hk + hk) * kv.head_bytes + (is_v ? kv.head_bytes / 2 : 0);
+      if constexpr (KV == XM_KV_F16) {
+        o = __ldg(reinterpret_cast<const uint4*>(part + (int64_t)slot * (2 * D)) + c);
+      } else {
+        const uint8_t* row = part + (int64_t)slot * (D / 2);
+        uint32_t w;
+        if (is_v) {
+          const uint16_t* hw = reinterpret_cast<const uint16_t*>(row) + NG * (2 * e) + g;
+          w = (uint32_t)__ldg(hw) | (uint32_t)__ldg(hw + NG) << 16;
         } else {
-          const int g = half * (NG / 2) + (VPL * lane) / 32, e = (VPL * lane) % 32;
-          const uint8_t* row = part + (int64_t)slot * (D / 2);
-          const uint32_t w = is_v ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[NG * (e / 4) + g] >> (4 * (e % 4))
-                                  : reinterpret_cast<const uint32_t*>(row)[NG * (e / 8) + g] >> (4 * (e % 8));
-          const float d = __half2float(reinterpret_cast<const __half*>(part + (int64_t)page_size * (D / 2))[slot * NG + g]);
-#pragma unroll
-          for (int i = 0; i < VPL; ++i) x[i] = d * (float)((int)((w >> (4 * i)) & 15) - 8);
+          w = __ldg(reinterpret_cast<const uint32_t*>(row) + NG * e + g);
         }
+        const float d = __half2float(reinterpret_cast<const __half*>(part + (int64_t)page_size * (D / 2))[slot * NG + g]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = d * i2f_small((int)((w >> (4 * i)) & 15) - 8);
+        __half2 p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        o = *reinterpret_cast<const uint4*>(p);
       }
-      store_vals<__half, VPL>(o + half * (D / 2), true, x);
+    }
+    __half* to = (is_v ? v : k) + (t * kv.Hk + hk) * D + 8 * c;
+    if (wide) {
+      *reinterpret_cast<uint4*>(to) = o;
+    } else {
+      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(to)[i] = w[i];
     }
   }
 }
@@ -336,13 +374,22 @@ int kv_view(const char* who, void* pool, int64_t pages, int kv_type, int Hk, int
 
 namespace {
 
+// Warps of a row: few rows: as many as its heads need, over several CTAs (latency); many: two, so that finding a
+// row's place is paid for by half of its heads (8800 rows of 48 heads: see k_kv_put).
+struct RowGrid {
+  dim3 grid;
+  int warps;
+};
+RowGrid row_grid(int64_t T, int heads, int D) {
+  const int per_warp = 256 / D, need = (heads + per_warp - 1) / per_warp;
+  if (T >= 1024) return {dim3((unsigned)((T + kPutWarps / 2 - 1) / (kPutWarps / 2))), 2};
+  return {dim3((unsigned)T, (unsigned)((need + kPutWarps - 1) / kPutWarps)), kPutWarps};
+}
+
 template <typename... KArgs, typename... Args>
-int launch_rows(const char* what, void (*kernel)(KArgs...), int64_t T, int heads, cudaStream_t st, Args... args) {
+int launch_rows(const char* what, void (*kernel)(KArgs...), const RowGrid& g, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  // few rows: one head per warp (latency); many: a row per CTA, its warps loop over the heads and reuse the
-  // row's place and angles
-  const unsigned gy = T >= 1024 ? 1u : (unsigned)((heads + kPutWarps - 1) / kPutWarps);
-  cfg.gridDim = dim3((unsigned)T, gy);
+  cfg.gridDim = g.grid;
   cfg.blockDim = dim3(32 * kPutWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -356,13 +403,14 @@ int launch_rows(const char* what, void (*kernel)(KArgs...), int64_t T, int heads
 }
 
 template <typename XT>
-int put_typed(const KvView& kv, const PutArgs& a, int kv_type, int head_dim, cudaStream_t st) {
-  const int heads = a.Hq + 2 * kv.Hk;
+int put_typed(const KvView& kv, PutArgs a, int kv_type, int head_dim, cudaStream_t st) {
+  const RowGrid g = row_grid(a.T, a.Hq + 2 * kv.Hk, head_dim);
+  a.warps = g.warps;
   if (head_dim == 128)
-    return kv_type == XM_KV_F16 ? launch_rows("kv append", k_kv_put<XT, 128, XM_KV_F16>, a.T, heads, st, kv, a)
-                                : launch_rows("kv append", k_kv_put<XT, 128, XM_KV_Q4_0>, a.T, heads, st, kv, a);
-  return kv_type == XM_KV_F16 ? launch_rows("kv append", k_kv_put<XT, 64, XM_KV_F16>, a.T, heads, st, kv, a)
-                              : launch_rows("kv append", k_kv_put<XT, 64, XM_KV_Q4_0>, a.T, heads, st, kv, a);
+    return kv_type == XM_KV_F16 ? launch_rows("kv append", k_kv_put<XT, 128, XM_KV_F16>, g, st, kv, a)
+                                : launch_rows("kv append", k_kv_put<XT, 128, XM_KV_Q4_0>, g, st, kv, a);
+  return kv_type == XM_KV_F16 ? launch_rows("kv append", k_kv_put<XT, 64, XM_KV_F16>, g, st, kv, a)
+                              : launch_rows("kv append", k_kv_put<XT, 64, XM_KV_Q4_0>, g, st, kv, a);
 }
 
 }  // namespace
@@ -399,8 +447,9 @@ int xm_kv_append(const void* d_qkv, int x_dtype, int64_t T, int64_t qkv_stride, 
       (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) & 3))
     return xm_set_error(XM_ERR_INVALID, "kv_append: bad row pitch or alignment");
   PutArgs a{d_qkv, T, qkv_stride, Hq, d_rope, rope_rows, d_q_norm, d_k_norm, eps, d_q, q_stride,
-            qkv_stride % 2 == 0 && ((uintptr_t)d_qkv & (2 * sz - 1)) == 0,
-            q_stride % 2 == 0 && ((uintptr_t)d_q & 3) == 0, q_dtype == XM_DT_BF16};
+            qkv_stride % 4 == 0 && ((uintptr_t)d_qkv & (4 * sz - 1)) == 0,
+            q_stride % 4 == 0 && ((uintptr_t)d_q & 7) == 0, (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) & 15) == 0,
+            q_dtype == XM_DT_BF16, 0};
   cudaStream_t st = (cudaStream_t)stream;
   if (x_dtype == XM_DT_F32) return put_typed<float>(kv, a, kv_type, head_dim, st);
   if (x_dtype == XM_DT_F16) return put_typed<__half>(kv, a, kv_type, head_dim, st);
@@ -419,14 +468,16 @@ int xm_kv_read(const void* d_pool, int64_t pages, int kv_type, int Hk, int head_
   if (T == 0) return XM_OK;
   if (!d_k || !d_v || (((uintptr_t)d_k | (uintptr_t)d_v) & 3))
     return xm_set_error(XM_ERR_INVALID, "kv_read: null or unaligned output");
+  const RowGrid g = row_grid(T, 2 * Hk, head_dim);
+  const bool wide = (((uintptr_t)d_k | (uintptr_t)d_v) & 15) == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (head_dim == 128)
     return kv_type == XM_KV_F16
-               ? launch_rows("kv read", k_kv_get<128, XM_KV_F16>, T, 2 * Hk, st, kv, (__half*)d_k, (__half*)d_v)
-               : launch_rows("kv read", k_kv_get<128, XM_KV_Q4_0>, T, 2 * Hk, st, kv, (__half*)d_k, (__half*)d_v);
+               ? launch_rows("kv read", k_kv_get<128, XM_KV_F16>, g, st, kv, (__half*)d_k, (__half*)d_v, wide, T, g.warps)
+               : launch_rows("kv read", k_kv_get<128, XM_KV_Q4_0>, g, st, kv, (__half*)d_k, (__half*)d_v, wide, T, g.warps);
   return kv_type == XM_KV_F16
-             ? launch_rows("kv read", k_kv_get<64, XM_KV_F16>, T, 2 * Hk, st, kv, (__half*)d_k, (__half*)d_v)
-             : launch_rows("kv read", k_kv_get<64, XM_KV_Q4_0>, T, 2 * Hk, st, kv, (__half*)d_k, (__half*)d_v);
+             ? launch_rows("kv read", k_kv_get<64, XM_KV_F16>, g, st, kv, (__half*)d_k, (__half*)d_v, wide, T, g.warps)
+             : launch_rows("kv read", k_kv_get<64, XM_KV_Q4_0>, g, st, kv, (__half*)d_k, (__half*)d_v, wide, T, g.warps);
 }
 
 }  // extern "C"

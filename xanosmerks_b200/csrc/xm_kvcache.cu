@@ -57,17 +57,28 @@ XM_DEV uint32_t q4_block(const float (&x)[4], __half& dh) {
   dh = spoilt ? __ushort_as_half((unsigned short)0x7fff) : __float2half_rn(a * -0.125f);
   const float d = __half2float(dh), ad = fabsf(d);
   if (!(ad > 0.f && ad < INFINITY)) return 0x8888u;
-  const float inv = 1.0f / d;
-  uint32_t codes = 0;
+  // x / d + 8 to the nearest whole number, by an approximate reciprocal and the addition of 2^23; within 1e-4 of a
+  // border the exact comparisons decide
+  const float inv = __fdividef(1.0f, d), magic = 8388608.f;
+  float e[4];
+  bool near = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float y = d < 0.f ? -x[i] : x[i];
-    float e = floorf(fmaf(x[i], inv, 8.5f));
-    e = fminf(fmaxf(e, 0.f), 15.f);
-    if (e > 0.f && fmaf(8.5f - e, ad, y) < 0.f) e -= 1.f;
-    else if (e < 15.f && fmaf(7.5f - e, ad, y) >= 0.f) e += 1.f;
-    codes |= (uint32_t)(int)e << (4 * i);
+    const float z = fminf(fmaxf(fmaf(x[i], inv, 8.f), 0.f), 15.f), t = z + magic;
+    e[i] = t;
+    near |= fabsf(z - (t - magic)) > 0.4999f;
   }
+  if (__any_sync(__activemask(), near)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = d < 0.f ? -x[i] : x[i], c = e[i] - magic;
+      if (c > 0.f && fmaf(8.5f - c, ad, y) < 0.f) e[i] -= 1.f;
+      else if (c < 15.f && fmaf(7.5f - c, ad, y) >= 0.f) e[i] += 1.f;
+    }
+  }
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) codes |= (__float_as_uint(e[i]) & 15u) << (4 * i);
   return codes;
 }
 

@@ -65,6 +65,10 @@ class LlamaOracle:
         self.k = np.zeros((L, batch, Hk, max_ctx, D), dtype=np.float32)
         self.v = np.zeros_like(self.k)
 
+    def stored(self, x):
+        """What the cache keeps of keys or values."""
+        return x
+
     def _attn(self, layer, x, pos):
         """attention.py:39-115 (fused_qkv, RoPE, cache append, causal SDPA, o_proj)."""
         c, w = self.cfg, self.w["layers"][layer]
@@ -74,10 +78,12 @@ class LlamaOracle:
         k = (x @ w["wk"].T).reshape(B, S, Hk, D).transpose(0, 2, 1, 3)
         v = (x @ w["wv"].T).reshape(B, S, Hk, D).transpose(0, 2, 1, 3)
         positions = np.arange(pos, pos + S)
+        if "q_norm" in w:                                     # per-head norms in front of the rotation
+            q, k = rms_norm(q, w["q_norm"], c["norm_eps"]), rms_norm(k, w["k_norm"], c["norm_eps"])
         q = rope(q, positions, c["rope_theta"])
         k = rope(k, positions, c["rope_theta"])
-        self.k[layer, :, :, pos:pos + S] = k
-        self.v[layer, :, :, pos:pos + S] = v
+        self.k[layer, :, :, pos:pos + S] = self.stored(k)
+        self.v[layer, :, :, pos:pos + S] = self.stored(v)
         kv = pos + S
         kf, vf = self.k[layer, :, :, :kv], self.v[layer, :, :, :kv]
         r = Hq // Hk

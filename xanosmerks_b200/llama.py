@@ -11,7 +11,11 @@ attention with RoPE and the KV append fused in, argmax).  A decode step is 5-6
 launches per layer and is captured once into a CUDA graph.
 
 Layout: per layer the Q, K, V rows are concatenated into one GGUF tensor (one
-GEMV), and so are gate and up; the caches are fp16 ``[B][Hk][max_ctx][128]``.
+GEMV), and so are gate and up; the caches are fp16 ``[B][Hk][max_ctx][128]``,
+or, with ``kv_type``, a :class:`~xanosmerks_b200.kvcache.PagedKVCache` per layer
+(fp16 or 4-bit), which also takes models that normalise the heads of queries and
+keys.  The next token is the first maximum (greedy) or sampled
+(:meth:`LlamaDecoder.set_sampling`).
 
 Tensor parallelism (``world_size > 1``, one process per GPU): attention heads
 and FFN columns are split across ranks (QKV and gate/up column-parallel, O and
@@ -28,8 +32,10 @@ import numpy as np
 import torch
 
 from . import qtypes
-from ._lib import DT_F32, PRO_NONE, PRO_RMSNORM, PRO_SWIGLU, check, check_device, lib
+from ._lib import DT_F16, DT_F32, PRO_NONE, PRO_RMSNORM, PRO_SWIGLU, check, check_device, lib
+from .kvcache import PagedKVCache, rope_table
 from .ops import GGUFTensor, gemm_supported
+from .sampling import sample
 from .synth import make_weight_device
 
 __all__ = ["LlamaConfig", "LlamaWeights", "LlamaDecoder", "synth_llama_weights", "shard_rows", "shard_cols"]
@@ -55,6 +61,7 @@ class LlamaConfig:
     down_qtype: str = "Q6_K"
     output_qtype: str = "Q6_K"
     embed_qtype: str = "Q4_K"
+    qk_norm: bool = False                # RMSNorm of each query and key head before the rotation
 
     def reference_config(self) -> dict:
         """The keys the reference's model classes read (forward.py, attention.py)."""
@@ -109,7 +116,8 @@ class LlamaWeights:
     """One rank's weights.  ``layers[i]``: ``qkv`` [(Hq+2Hk)*128, D] (this rank's
     heads), ``o`` [D, Hq*128 / world], ``gate_up`` [2F / world, D] (gate rows then
     up rows), ``down`` [D, F / world], ``attn_norm`` / ``ffn_norm`` fp32 [D];
-    ``embed`` [V, D], ``norm`` fp32 [D], ``output`` [V, D]."""
+    ``embed`` [V, D], ``norm`` fp32 [D], ``output`` [V, D]; with ``cfg.qk_norm`` also
+    ``q_norm`` / ``k_norm`` fp32 [head_dim] per layer."""
 
     def __init__(self, cfg: LlamaConfig, embed, layers, norm, output, rank=0, world=1):
         self.cfg, self.embed, self.layers, self.norm, self.output = cfg, embed, layers, norm, output
@@ -118,7 +126,7 @@ class LlamaWeights:
     @classmethod
     def from_full(cls, cfg: LlamaConfig, full: dict, rank: int = 0, world: int = 1) -> "LlamaWeights":
         """Shard full per-layer tensors ``wq, wk, wv, wo, wg, wu, wd`` (GGUFTensor)
-        and ``n1, n2`` for ``rank`` of ``world``."""
+        and ``n1, n2`` (with ``cfg.qk_norm`` also ``qn, kn``) for ``rank`` of ``world``."""
         hq, hk, hd, F = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.intermediate_size
         if hq % world or hk % world or F % world:
             raise ValueError(f"heads {hq}/{hk} and FFN {F} must divide by the world size {world}")
@@ -134,6 +142,8 @@ class LlamaWeights:
             down = lw["wd"] if world == 1 else shard_cols(lw["wd"], rank * f_l, (rank + 1) * f_l)
             layers.append({"qkv": qkv, "o": o, "gate_up": gu, "down": down,
                            "attn_norm": lw["n1"], "ffn_norm": lw["n2"]})
+            if cfg.qk_norm:
+                layers[-1].update(q_norm=lw["qn"], k_norm=lw["kn"])
         return cls(cfg, full["embed"], layers, full["norm"], full["output"], rank, world)
 
 
@@ -149,8 +159,8 @@ def synth_llama_weights(cfg: LlamaConfig, seed: int = 0, device="cuda"):
         raw = make_weight_device(qt, n, k, seed=seed * 100003 + s, device=device, scale=_WEIGHT_SCALE.get(qt))
         return GGUFTensor(raw, qt, (n, k), device=device)
 
-    def norm_w():
-        return (1.0 + 0.05 * torch.randn(D, generator=g, device=device)).float()
+    def norm_w(n=D):
+        return (1.0 + 0.05 * torch.randn(n, generator=g, device=device)).float()
 
     layers = []
     for i in range(cfg.num_layers):
@@ -163,12 +173,14 @@ def synth_llama_weights(cfg: LlamaConfig, seed: int = 0, device="cuda"):
                        "wu": w(cfg.gate_up_qtype, F, D, b + 5),
                        "wd": w(cfg.down_qtype, D, F, b + 6),
                        "n1": norm_w(), "n2": norm_w()})
+        if cfg.qk_norm:
+            layers[-1].update(qn=norm_w(hd), kn=norm_w(hd))
     return {"embed": w(cfg.embed_qtype, V, D, 1), "layers": layers, "norm": norm_w(),
             "output": w(cfg.output_qtype, V, D, 2)}
 
 
 class LlamaDecoder:
-    """Greedy decoder for ``batch`` sequences of up to ``max_ctx`` tokens.
+    """Decoder for ``batch`` sequences of up to ``max_ctx`` tokens, greedy unless ``set_sampling`` says otherwise.
 
     ``prefill(ids)`` runs the prompt (ids [B, S]) through the layers, 8 tokens
     per sequence at a time, and returns the next token of each sequence;
@@ -181,14 +193,19 @@ class LlamaDecoder:
     all-reduce over NVLink peer memory of ``xm_allreduce_add``, buffers shared
     through CUDA IPC) or ``"nccl"`` (``torch.distributed.all_reduce``).  Call
     ``close()`` on every rank before tearing the process group down.
+
+    ``kv_type``: None keeps contiguous fp16 caches; ``"F16"`` or ``"Q4_0"`` keep the keys and values in a
+    ``PagedKVCache`` per layer (pages of ``page_size`` tokens), in 16 or 4 bits; ``cfg.qk_norm`` needs one.
     """
 
     LQ_MAX = 8
     COMM_CTAS = 16
 
     def __init__(self, weights: LlamaWeights, batch: int, max_ctx: int, device=None, process_group=None,
-                 collective: str = "p2p"):
+                 collective: str = "p2p", kv_type: str | None = None, page_size: int = 64):
         cfg = weights.cfg
+        if cfg.qk_norm and kv_type is None:
+            raise NotImplementedError("LlamaDecoder: normalised query and key heads need a paged cache (kv_type)")
         self.cfg, self.w, self.B, self.max_ctx = cfg, weights, int(batch), int(max_ctx)
         self.world = weights.world
         self.pg = process_group
@@ -214,10 +231,22 @@ class LlamaDecoder:
         self.ids = torch.zeros(rows, **i32)               # token ids of the rows being processed
         self.next_ids = torch.zeros(self.B, **i32)
         self.pos0 = torch.zeros(self.B, **i32)            # tokens already in the cache per sequence
-        self.kc = torch.zeros(cfg.num_layers, self.B, self.hk, self.max_ctx, hd, dtype=torch.float16, device=dev)
-        self.vc = torch.zeros_like(self.kc)
-        aws = lib.xm_attention_workspace_size(self.B, self.hk, self.max_ctx)
-        self.attn_ws = torch.zeros(aws, dtype=torch.uint8, device=dev)
+        self.kv_type = kv_type
+        if kv_type is None:
+            self.kc = torch.zeros(cfg.num_layers, self.B, self.hk, self.max_ctx, hd, dtype=torch.float16, device=dev)
+            self.vc = torch.zeros_like(self.kc)
+            aws = lib.xm_attention_workspace_size(self.B, self.hk, self.max_ctx)
+            self.attn_ws = torch.zeros(aws, dtype=torch.uint8, device=dev)
+        else:
+            width = -(-self.max_ctx // page_size)
+            self.caches = [PagedKVCache(self.B * width, self.hk, hd, page_size, kv_type, device=dev)
+                           for _ in range(cfg.num_layers)]
+            self.block_table = torch.arange(self.B * width, **i32).view(self.B, width)
+            self.kv_lens = torch.zeros(self.B, **i32)      # tokens per sequence with the ones being processed
+            self.rope = rope_table(self.max_ctx, hd, cfg.rope_theta, device=dev)
+            self.cu = {}                                   # row offsets by new tokens per sequence
+        self.sampling = None
+        self.u = torch.zeros(self.B, **f32)                # the step's random numbers
         kmax = max(D, cfg.intermediate_size, self.hq * hd)
         self.gemv_ws = torch.zeros(lib.xm_qgemv_workspace_size(kmax, 8) + 4096, dtype=torch.uint8, device=dev)
         self.graph = None
@@ -293,7 +322,8 @@ class LlamaDecoder:
         for r0 in range(0, rows, 8):
             m = min(8, rows - r0)
             check(lib.xm_qgemv_ex(wt.qtype.type_id, wt.data.data_ptr(), wt.nbytes, n, k, x[r0:r0 + m].data_ptr(),
-                                  DT_F32, m, x.stride(0), prologue, norm.data_ptr() if norm is not None else None,
+                                  DT_F16 if x.dtype == torch.float16 else DT_F32, m, x.stride(0), prologue,
+                                  norm.data_ptr() if norm is not None else None,
                                   self.cfg.norm_eps, None, y[r0:r0 + m].data_ptr(), 1 if accumulate else 0,
                                   self.gemv_ws.data_ptr(), self.gemv_ws.numel(), self._stream()), "qgemv_ex")
 
@@ -309,22 +339,40 @@ class LlamaDecoder:
         dist.all_reduce(p, group=self.pg)
         self.h[:rows].add_(p)
 
+    def _paged_attention(self, li: int, lw, qkv: torch.Tensor, lq: int) -> torch.Tensor:
+        """Normalise, rotate and store the rows of layer li's QKV projection, then attend: fp16 [rows, Hq * head_dim]."""
+        cu = None
+        if lq > 1:
+            cu = self.cu.get(lq)
+            if cu is None:
+                cu = self.cu[lq] = torch.arange(0, (self.B + 1) * lq, lq, dtype=torch.int32, device=self.dev)
+        cache = self.caches[li]
+        q = cache.append(qkv, self.hq, self.block_table, self.kv_lens, cu, rope=self.rope, q_norm=lw.get("q_norm"),
+                         k_norm=lw.get("k_norm"), eps=self.cfg.norm_eps)
+        return cache.attend(q, self.block_table, self.kv_lens, cu).flatten(1)
+
     def _layers(self, lq: int):
         cfg, B = self.cfg, self.B
         rows = B * lq
         st = self._stream()
+        if self.kv_type is not None:
+            torch.add(self.pos0, lq, out=self.kv_lens)
         for li, lw in enumerate(self.w.layers):
             # attention block (forward.py:107-111)
             self._proj(lw["qkv"], self.h, rows, self.qkv, PRO_RMSNORM, lw["attn_norm"])
-            check(lib.xm_attention(self.qkv.data_ptr(), self.qkv_dim, self.kc[li].data_ptr(),
-                                   self.vc[li].data_ptr(), self.pos0.data_ptr(), B, lq, self.hq, self.hk,
-                                   cfg.head_dim, cfg.rope_theta, self.max_ctx, self.attn.data_ptr(),
-                                   self.hq * cfg.head_dim, self.attn_ws.data_ptr(), self.attn_ws.numel(), st),
-                  "attention")
-            if self.world == 1:
-                self._proj(lw["o"], self.attn, rows, self.h, accumulate=True)
+            attn = self.attn
+            if self.kv_type is not None:
+                attn = self._paged_attention(li, lw, self.qkv[:rows], lq)
             else:
-                self._proj(lw["o"], self.attn, rows, self.part)
+                check(lib.xm_attention(self.qkv.data_ptr(), self.qkv_dim, self.kc[li].data_ptr(),
+                                       self.vc[li].data_ptr(), self.pos0.data_ptr(), B, lq, self.hq, self.hk,
+                                       cfg.head_dim, cfg.rope_theta, self.max_ctx, self.attn.data_ptr(),
+                                       self.hq * cfg.head_dim, self.attn_ws.data_ptr(), self.attn_ws.numel(), st),
+                      "attention")
+            if self.world == 1:
+                self._proj(lw["o"], attn, rows, self.h, accumulate=True)
+            else:
+                self._proj(lw["o"], attn, rows, self.part)
                 self._allreduce_add(rows)
             # MLP block (forward.py:113-116)
             self._proj(lw["gate_up"], self.h, rows, self.gu, PRO_RMSNORM, lw["ffn_norm"])
@@ -335,14 +383,13 @@ class LlamaDecoder:
                 self._allreduce_add(rows)
 
     def _head(self, lq: int):
-        """Final RMSNorm + output projection of each sequence's last row, then argmax."""
+        """Final RMSNorm + output projection of each sequence's last row, then the next tokens."""
         D = self.cfg.hidden_size
         ow = self.w.output
         if self.B >= self.GEMM_DECODE_ROWS and ow.qtype.name != "Q4_K" and gemm_supported(ow.qtype, ow.shape[1]):
             last = self.h[:self.B * lq].view(self.B, lq, D)[:, lq - 1]     # each sequence's last row
             self._gemm(ow, last, self.B, self.logits, PRO_RMSNORM, self.w.norm, ws=self.dec_gemm_ws)
-            check(lib.xm_argmax(self.logits.data_ptr(), self.B, self.cfg.vocab_size, self.next_ids.data_ptr(),
-                                self._stream()), "argmax")
+            self._choose()
             return
         for b0 in range(0, self.B, 8):
             m = min(8, self.B - b0)
@@ -351,8 +398,20 @@ class LlamaDecoder:
                                   DT_F32, m, lq * D, PRO_RMSNORM, self.w.norm.data_ptr(), self.cfg.norm_eps, None,
                                   self.logits[b0:b0 + m].data_ptr(), 0, self.gemv_ws.data_ptr(),
                                   self.gemv_ws.numel(), self._stream()), "output head")
+        self._choose()
+
+    def _choose(self):
+        """next_ids from the logits: the first maximum, or sampled with the numbers in ``u``."""
+        if self.sampling is not None:
+            sample(self.logits, self.u, out=self.next_ids, **self.sampling)
+            return
         check(lib.xm_argmax(self.logits.data_ptr(), self.B, self.cfg.vocab_size, self.next_ids.data_ptr(),
                             self._stream()), "argmax")
+
+    def _draw(self):
+        """New random numbers for the next step (before it, not in it: a captured step reads them from ``u``)."""
+        if self.sampling is not None:
+            torch.rand(self.B, generator=self.generator, out=self.u)
 
     def _embed(self, rows, ids):
         e = self.w.embed
@@ -364,6 +423,18 @@ class LlamaDecoder:
         self.pos0.zero_()
         self.length = 0
         self.graph = None
+
+    def set_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0):
+        """Sample the next tokens (see :func:`~xanosmerks_b200.sampling.sample`; numbers, or tensors with one entry
+        per sequence) with random numbers from a generator seeded with ``seed``; ``temperature=None``: greedy again.
+        A captured step is dropped."""
+        self.graph = None
+        if temperature is None:
+            self.sampling = None
+            return
+        self.generator = torch.Generator(device=self.dev)
+        self.generator.manual_seed(seed)
+        self.sampling = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     def forward_tokens(self, ids: torch.Tensor) -> torch.Tensor:
         """Run ids [B, lq] (lq <= 8) at the current positions; returns the next token per sequence."""
@@ -377,6 +448,7 @@ class LlamaDecoder:
         if lo < 0 or hi >= self.cfg.vocab_size:
             raise ValueError(f"token ids must lie in [0, {self.cfg.vocab_size}), got [{lo}, {hi}]")
         self.ids[:rows].copy_(ids.reshape(-1).to(self.dev, torch.int32))
+        self._draw()
         self._embed(rows, self.ids)
         self._layers(lq)
         self._head(lq)
@@ -420,14 +492,15 @@ class LlamaDecoder:
                 self._gemm_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
             ws = self._gemm_ws
         norm_p = norm.data_ptr() if norm is not None else None
+        dt = DT_F16 if x.dtype == torch.float16 else DT_F32
         if pitched is not None:
             pad, pitch = pitched
             check(lib.xm_qgemm_ex_pitched(wt.qtype.type_id, pad.data_ptr(), pitch, pad.numel(), n, k, x.data_ptr(),
-                                          DT_F32, rows, x.stride(0), prologue, norm_p, self.cfg.norm_eps, None,
+                                          dt, rows, x.stride(0), prologue, norm_p, self.cfg.norm_eps, None,
                                           y.data_ptr(), 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
                                           self._stream()), "qgemm_ex_pitched")
             return
-        check(lib.xm_qgemm_ex(wt.qtype.type_id, wt.data.data_ptr(), wt.nbytes, n, k, x.data_ptr(), DT_F32, rows,
+        check(lib.xm_qgemm_ex(wt.qtype.type_id, wt.data.data_ptr(), wt.nbytes, n, k, x.data_ptr(), dt, rows,
                               x.stride(0), prologue, norm_p, self.cfg.norm_eps, None, y.data_ptr(),
                               1 if accumulate else 0, ws.data_ptr(), ws.numel(), self._stream()), "qgemm_ex")
 
@@ -471,11 +544,16 @@ class LlamaDecoder:
         check(lib.xm_embed(e.qtype.type_id, e.data.data_ptr(), e.nbytes, e.shape[0], e.shape[1], idv.data_ptr(),
                            rows, h.data_ptr(), st), "embed")
         # 16 or more tokens: one attention call over all sequences (the tensor-core prefill path)
-        whole = S >= 16
+        whole = S >= 16 or self.kv_type is not None
+        if self.kv_type is not None:
+            self.kv_lens.fill_(S)
+        self._draw()
         zeros_b = torch.zeros(B, dtype=torch.int32, device=self.dev)
         for li, lw in enumerate(self.w.layers):
             self._gemm(lw["qkv"], h, rows, qkv, PRO_RMSNORM, lw["attn_norm"])
-            if whole:
+            if self.kv_type is not None:
+                attn = self._paged_attention(li, lw, qkv, S)
+            elif whole:
                 check(lib.xm_attention(qkv.data_ptr(), self.qkv_dim, self.kc[li].data_ptr(), self.vc[li].data_ptr(),
                                        zeros_b.data_ptr(), B, S, self.hq, self.hk, hd, cfg.rope_theta,
                                        self.max_ctx, attn.data_ptr(), self.hq * hd, self.attn_ws.data_ptr(),
@@ -515,7 +593,11 @@ class LlamaDecoder:
         h.add_(part)
 
     def decode_step(self):
-        """One greedy step from device state: the token in next_ids enters at pos0."""
+        """One step from device state: the token in next_ids enters at pos0."""
+        self._draw()
+        self._step()
+
+    def _step(self):
         B = self.B
         self._embed(B, self.next_ids)
         self._layers(1)
@@ -529,7 +611,7 @@ class LlamaDecoder:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.stream(s):
             with torch.cuda.graph(g, stream=s):
-                self.decode_step()
+                self._step()
         torch.cuda.current_stream(self.dev).wait_stream(s)
         self.graph = g
         return g
@@ -539,6 +621,7 @@ class LlamaDecoder:
         if self.length + n > self.max_ctx:
             raise ValueError("context overflow")
         for _ in range(n):
+            self._draw()
             self.graph.replay()
         self.length += n
 
@@ -550,7 +633,7 @@ class LlamaDecoder:
             check_device("LlamaDecoder")
 
     def generate(self, prompt, max_new_tokens: int, use_graph: bool = True) -> np.ndarray:
-        """Greedy generation: prompt [B, S] -> generated ids [B, max_new_tokens]."""
+        """Generation, greedy or as ``set_sampling`` says: prompt [B, S] -> generated ids [B, max_new_tokens]."""
         self.reset()
         out = np.zeros((self.B, max_new_tokens), dtype=np.int64)
         nxt = self.prefill(prompt)

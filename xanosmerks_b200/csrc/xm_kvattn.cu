@@ -1012,12 +1012,18 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 //
 //   warps 0-3, 4-7   softmax of row tile 0, 1 (a thread is a row = a lane of tensor memory)
 //   warps 8-11       loaders: bring a unit's keys and values into shared memory as fp16
-//   warp 12          allocates tensor memory and issues the products (one thread)
+//   warps 12, 13     issue the products of row tile 0, 1 (one thread each); warp 12 allocates tensor memory
 //
-// S = Q K^T (M = 128 rows, N = 128 keys) goes to tensor memory, the softmax warps turn it into P (fp16)
-// in place, and O += P V takes P from tensor memory and V as it lies in the cache, dimensions
-// contiguous.  The two row tiles alternate, so that one's products run during the other's softmax.
-// Tensor memory: S0 S1 (P in their first halves) at columns 0 and 128, O0 O1 at 256 and 256 + D.
+// S = Q K^T (M = 128 rows, N = 64 keys, a half unit) goes to tensor memory, the softmax warps turn it into P (fp16) in
+// place, and O += P V takes P from tensor memory and V as it lies in the cache, dimensions contiguous.  S
+// has two buffers per row tile, so the next half's S is computed while this one's softmax runs, and that
+// is never held up by the product that reads its P.  Tensor memory: S of tile i, half h at column 128 i + 64 h,
+// O of tile i at 256 + D i.
+//
+// What decides the speed is the chain of one row tile: a row of S is read once, 64 columns into registers (a
+// tcgen05.wait::ld waits for every load, and costs some 300 clocks), its maximum taken, P computed.  With
+// units of 128 keys and P over a single S the chain of a unit was 6100 clocks (PV and S follow one another in it);
+// a 8192-token prompt took 790 us.
 //
 // 4-bit rows become fp16 here, d (c - 8) rounded once (2^-11): a product per code would need the scales
 // inside the tensor core's inner dimension.  The order of the eight values that a word of keys yields is
@@ -1034,20 +1040,63 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // (16 a clock); the loaders' and the softmax's other instructions fit beside them.
 // ---------------------------------------------------------------------------
 constexpr int kUnit = 128;                         // keys of a unit
-constexpr int kPromptThreads = 13 * 32;
+constexpr int kPromptThreads = 14 * 32;
 
 XM_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 XM_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 XM_DEV void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-XM_DEV void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// The products of a unit from one asm block each: the issuing thread shares its scheduler with busy warps, so every
+// instruction between two products counts.  Descriptors are {low, high} words; only the start (low) moves.
+// d = A B^T over 16 K values, K = {4, 8}, blocks of 64 values 16 KB apart
+template <int K>
+XM_DEV void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc) {
+  if constexpr (K == 8)
+  asm volatile("{\n .reg .pred p0, p1;\n .reg .b64 da, db;\n .reg .b32 x, y;\n"
+               " setp.eq.b32 p0, 0, 0;\n setp.ne.b32 p1, 0, 0;\n"
+               " mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p1;\n"
+               " add.u32 x, %1, 2;\n add.u32 y, %2, 2;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 4;\n add.u32 y, %2, 4;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 6;\n add.u32 y, %2, 6;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 1024;\n add.u32 y, %2, 1024;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 1026;\n add.u32 y, %2, 1026;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 1028;\n add.u32 y, %2, 1028;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 1030;\n add.u32 y, %2, 1030;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               "}"
+               ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc) : "memory");
+  else
+  asm volatile("{\n .reg .pred p0, p1;\n .reg .b64 da, db;\n .reg .b32 x, y;\n"
+               " setp.eq.b32 p0, 0, 0;\n setp.ne.b32 p1, 0, 0;\n"
+               " mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p1;\n"
+               " add.u32 x, %1, 2;\n add.u32 y, %2, 2;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 4;\n add.u32 y, %2, 4;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               " add.u32 x, %1, 6;\n add.u32 y, %2, 6;\n mov.b64 da, {x, %3};\n mov.b64 db, {y, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p0;\n"
+               "}"
+               ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc) : "memory");
 }
-XM_DEV void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// d (+)= A B over 64 values, A in tensor memory
+XM_DEV void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p0, p1;\n .reg .b64 db;\n .reg .b32 x, y;\n"
+               " setp.eq.b32 p0, 0, 0;\n setp.ne.b32 p1, %5, 0;\n"
+               " mov.b64 db, {%2, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p1;\n"
+               " add.u32 x, %1, 8;\n add.u32 y, %2, 128;\n mov.b64 db, {y, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p0;\n"
+               " add.u32 x, %1, 16;\n add.u32 y, %2, 256;\n mov.b64 db, {y, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p0;\n"
+               " add.u32 x, %1, 24;\n add.u32 y, %2, 384;\n mov.b64 db, {y, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p0;\n"
+               "}"
+               ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate) : "memory");
 }
 XM_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -1059,13 +1108,21 @@ XM_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+XM_DEV void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 XM_DEV void tmem_ld1(uint32_t taddr, uint32_t& r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
 }
-XM_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-               "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+XM_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+XM_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 XM_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 XM_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -1097,7 +1154,7 @@ struct PromptShape {
 };
 
 struct PromptCtl {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drain;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], drain[2];
   PromptInfo info[2];
   uint32_t tmem;
 };
@@ -1113,6 +1170,14 @@ XM_DEV uint4 decode_word(uint32_t w, __half2 d) {
   const __half2 off = __float2half2_rn(-1032.f), six = __float2half2_rn(0.0625f), off16 = __float2half2_rn(-72.f);
   return make_uint4(bits(__hmul2(__hadd2(h2(a), off), d)), bits(__hmul2(__hfma2(h2(b), six, off16), d)),
                     bits(__hmul2(__hadd2(h2(c), off), d)), bits(__hmul2(__hfma2(h2(e), six, off16), d)));
+}
+
+// A wait that tests once before it suspends (on a phase that is over that is half the time).
+XM_DEV bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok || mbar_wait_bounded(bar, parity);
 }
 
 XM_DEV bool loader_any(bool p) {                       // over the 128 loader threads
@@ -1152,13 +1217,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->k_full[i], 128);
       mbar_init(&ctl->v_full[i], 128);
-      mbar_init(&ctl->p_full[i], 128);
-      mbar_init(&ctl->k_empty[i], 1);
-      mbar_init(&ctl->v_empty[i], 1);
-      mbar_init(&ctl->s_full[i], 1);
-      mbar_init(&ctl->o_done[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&ctl->s_full[i][h], 1);
+        mbar_init(&ctl->p_full[i][h], 128);
+        mbar_init(&ctl->o_done[i][h], 1);
+      }
+      mbar_init(&ctl->k_empty[i], tiles);
+      mbar_init(&ctl->v_empty[i], tiles);
     }
-    mbar_init(&ctl->drain, 1);
+    mbar_init(&ctl->drain[0], 1);
+    mbar_init(&ctl->drain[1], 1);
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -1172,41 +1240,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
   const int64_t my_t = t0 + gr / G;
   const int my_h = hk * G + gr % G, pos = live ? ts.p_first + gr / G : ts.pmax;
   if (warp < 8 && tile < tiles) {
-    uint4 raw[D / 8];
+    // 64 values at a time; twice, for the largest magnitude and for the tile (the second time from L1)
+    const QT_* q = (const QT_*)a.q + my_t * a.q_stride + (int64_t)my_h * D;
+    uint4 raw[8];
+    auto read = [&](int c0) {
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) raw[c] = make_uint4(0u, 0u, 0u, 0u);
-    if (live) {
-      const QT_* q = (const QT_*)a.q + my_t * a.q_stride + (int64_t)my_h * D;
-      if (a.q_vec) {
+      for (int c = 0; c < 8; ++c) {
+        raw[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (live) {
+          if (a.q_vec) {
+            raw[c] = __ldg(reinterpret_cast<const uint4*>(q) + c0 + c);
+          } else {
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) raw[c] = __ldg(reinterpret_cast<const uint4*>(q) + c);
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) reinterpret_cast<QT_*>(&raw[c])[i] = q[8 * c + i];
+            for (int i = 0; i < 8; ++i) reinterpret_cast<QT_*>(&raw[c])[i] = q[8 * (c0 + c) + i];
+          }
+        }
       }
-    }
+    };
     float mx = 0.f;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D / 8; c0 += 8) {
+      read(c0);
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c)
+      for (int c = 0; c < 8; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(to_f32(reinterpret_cast<const QT_*>(&raw[c])[i])));
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(to_f32(reinterpret_cast<const QT_*>(&raw[c])[i])));
+    }
     const int sh = fp16_row_shift(mx);
     const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
     q_f = ldexpf(fabsf(a.scale) * kLog2e, sh);
+#pragma unroll 1
+    for (int c0 = 0; c0 < D / 8; c0 += 8) {
+      if (D > 64) read(c0);
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      float x[8];
+      for (int c = 0; c < 8; ++c) {
+        float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32(reinterpret_cast<const QT_*>(&raw[c])[i]) * down;
-      uint4 w;
-      if constexpr (KV == XM_KV_Q4_0)
-        w = make_uint4(half2_bits(x[0], x[4]), half2_bits(x[1], x[5]), half2_bits(x[2], x[6]), half2_bits(x[3], x[7]));
-      else
-        w = make_uint4(half2_bits(x[0], x[1]), half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
-      *reinterpret_cast<uint4*>(base_p + tile * Shape::kTile + (c / 8) * Shape::kBlock + row * 128 +
-                                ((c & 7) ^ (row & 7)) * 16) = w;
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(reinterpret_cast<const QT_*>(&raw[c])[i]) * down;
+        uint4 w;
+        if constexpr (KV == XM_KV_Q4_0)
+          w = make_uint4(half2_bits(x[0], x[4]), half2_bits(x[1], x[5]), half2_bits(x[2], x[6]), half2_bits(x[3], x[7]));
+        else
+          w = make_uint4(half2_bits(x[0], x[1]), half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
+        *reinterpret_cast<uint4*>(base_p + tile * Shape::kTile + (c0 / 8) * Shape::kBlock + row * 128 +
+                                  (c ^ (row & 7)) * 16) = w;
+      }
     }
     fence_proxy_async_smem();
   }
@@ -1215,52 +1293,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
 
-  if (warp == 12) {
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(D, true);
+  if (warp >= 12) {
+    const int i = warp - 12;                           // the row tile whose products this thread issues
+    if (lane == 0 && i < tiles && n > 0) {
+      constexpr uint32_t id_s = idesc_f16(64, false), id_o = idesc_f16(D, true), kHalf = 64 * 128 >> 4;
+      const uint32_t high = (uint32_t)(desc_sw128(0, 16) >> 32);
+      const uint32_t lo_q = (uint32_t)desc_sw128(s_q + i * Shape::kTile, 16), lo_k = (uint32_t)desc_sw128(s_k, 16);
+      const uint32_t lo_v = (uint32_t)desc_sw128(s_v, Shape::kBlock);
+      const uint32_t t_s = tmem + i * 128, t_o = tmem + 256 + i * D;
       bool ok = true;
-      auto issue_s = [&](int i, int k) {               // S_i = Q_i K^T of unit k
-        const uint64_t da = desc_sw128(s_q + i * Shape::kTile, 16), db = desc_sw128(s_k + (k & 1) * Shape::kTile, 16);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t off = (uint64_t)(((kk >> 2) * Shape::kBlock + (kk & 3) * 32) >> 4);
-          tc_mma_ss(tmem + i * 128, da + off, db + off, id_s, kk > 0);
-        }
-        tc_commit(&ctl->s_full[i]);
+      auto issue_s = [&](int u) {                      // S = Q K^T of half unit u
+        const int k = u >> 1, h = u & 1;
+        if (h == 0) ok = mbar_wait_soon(&ctl->k_full[k & 1], (k >> 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        tc_mma_ss<D / 16>(t_s + 64 * h, lo_q, lo_k + (k & 1) * (Shape::kTile >> 4) + h * kHalf, high, id_s);
+        tc_commit(&ctl->s_full[i][h]);
+        if (h == 1) tc_commit(&ctl->k_empty[k & 1]);
       };
-      ok = mbar_wait_bounded(&ctl->k_full[0], 0);
-      tc_fence_after();
-      for (int i = 0; i < tiles && ok; ++i) issue_s(i, 0);
-      tc_commit(&ctl->k_empty[0]);
-      for (int k = 0; k < n && ok; ++k) {
-        ok = mbar_wait_bounded(&ctl->v_full[k & 1], (k >> 1) & 1);
-        for (int i = 0; i < tiles && ok; ++i) {
-          ok = mbar_wait_bounded(&ctl->p_full[i], k & 1);
-          if (!ok) break;
-          tc_fence_after();
-          // (the first unit starts O, unless the softmax warps have put taken-out values there)
-          const uint32_t* odd = ctl->info[0].odd;
-          const bool start = k == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) == 0u;
-          const uint64_t dv = desc_sw128(s_v + (k & 1) * Shape::kTile, Shape::kBlock);
-#pragma unroll
-          for (int kk = 0; kk < kUnit / 16; ++kk)
-            tc_mma_ts(tmem + 256 + i * D, tmem + i * 128 + kk * 8, dv + (uint64_t)(kk * (2048 >> 4)), id_o,
-                      kk > 0 || !start);
-          tc_commit(&ctl->o_done[i]);
-          if (i == tiles - 1) tc_commit(&ctl->v_empty[k & 1]);
-          if (k + 1 < n) {
-            // S_i overwrites P_i, which the product above reads
-            ok = mbar_wait_bounded(&ctl->o_done[i], k & 1);
-            if (ok && i == 0) ok = mbar_wait_bounded(&ctl->k_full[(k + 1) & 1], ((k + 1) >> 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(i, k + 1);
-            if (i == tiles - 1) tc_commit(&ctl->k_empty[(k + 1) & 1]);
-          }
+      issue_s(0);
+      for (int u = 0; u < 2 * n && ok; ++u) {
+        const int k = u >> 1, h = u & 1;
+        if (u + 1 < 2 * n) {
+          // the other buffer's P has been read when the last product is done
+          if (u > 0) ok = mbar_wait_soon(&ctl->o_done[i][h ^ 1], ((u - 1) >> 1) & 1);
+          if (ok) issue_s(u + 1);
         }
+        if (ok && h == 0) ok = mbar_wait_soon(&ctl->v_full[k & 1], (k >> 1) & 1);
+        // (the first half starts O, unless the softmax warps have put taken-out values there)
+        const uint32_t* odd = ctl->info[0].odd;
+        const bool start = u == 0 && (odd[0] | odd[1]) == 0u;
+        if (ok) ok = mbar_wait_soon(&ctl->p_full[i][h], k & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tc_mma_ts(t_o, t_s + 64 * h, lo_v + (k & 1) * (Shape::kTile >> 4) + h * kHalf, high, id_o, !start);
+        tc_commit(&ctl->o_done[i][h]);
+        if (h == 1) tc_commit(&ctl->v_empty[k & 1]);
       }
-      tc_commit(&ctl->drain);                          // nothing of the tensor core's is left in flight
-      mbar_wait_bounded(&ctl->drain, 0);
+      tc_commit(&ctl->drain[i]);                       // nothing of the tensor core's is left in flight
+      mbar_wait_bounded(&ctl->drain[i], 0);
     }
     __syncwarp();
   } else if (warp >= 8) {
@@ -1272,56 +1343,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     auto all_see = [&](int key) {
       return key <= ts.pmin && (a.window == 0 || key > ts.pmax - a.window || key < a.sinks);
     };
-    // where a position's head is in its page, and whether there is one
-    auto locate = [&](int key, bool& in) {
+    auto page_of = [&](int key) {
       const int at = key >> kv.page_shift;
-      const int p = at < kv.table_width ? __ldg(table + at) : -1;
-      in = (unsigned)p < (unsigned)kv.pages;
-      return pool + (in ? p : 0) * page_bytes;
+      return at < kv.table_width ? __ldg(table + at) : -1;
     };
+    auto in_pool = [&](int p) { return (unsigned)p < (unsigned)kv.pages; };
     const int page_mask = (1 << kv.page_shift) - 1;
     if constexpr (KV == XM_KV_Q4_0) {
-      uint32_t kw[D / 8], vw[D / 8], kd[NG / 2], vd[NG / 2];
+      // a thread is a key; its page is requested two units ahead, its bytes one (each part when the last is decoded)
+      struct Raw {
+        uint32_t kw[D / 8], vw[D / 8], kd[NG / 2], vd[NG / 2];
+      };
       const int codes = D / 2 << kv.page_shift;
-      const uint8_t* head = nullptr;
+      auto key_of_unit = [&](int k) { return ts.unit(min(k, n - 1)) * kUnit + t; };
+      auto request = [&](const uint8_t* q, int slot, uint32_t (&w)[D / 8], uint32_t (&d)[NG / 2]) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(q + slot * (D / 2)) + i);
+          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) d[i] = __ldg(reinterpret_cast<const uint32_t*>(q + codes + slot * (2 * NG)) + i);
+      };
+      int next_page = n > 0 ? page_of(key_of_unit(0)) : -1, slot = 0;
       bool in = false;
-      int slot = 0;
-      auto load_k = [&](int k) {
-        const int key = ts.unit(k) * kUnit + t;
-        head = locate(key, in);
-        slot = key & page_mask;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(head + slot * (D / 2)) + i);
-          kw[4 * i] = v.x; kw[4 * i + 1] = v.y; kw[4 * i + 2] = v.z; kw[4 * i + 3] = v.w;
-        }
-#pragma unroll
-        for (int i = 0; i < NG / 2; ++i) kd[i] = __ldg(reinterpret_cast<const uint32_t*>(head + codes + slot * (2 * NG)) + i);
+      const uint8_t* head = nullptr;
+      auto place = [&](int k) {                        // of unit k, whose page has arrived
+        in = in_pool(next_page);
+        head = pool + (in ? next_page : 0) * page_bytes;
+        slot = key_of_unit(k) & page_mask;
+        next_page = page_of(key_of_unit(k + 1));
       };
-      auto load_v = [&]() {                            // of the unit that load_k has located
-        const uint8_t* h = head + v_part;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(h + slot * (D / 2)) + i);
-          vw[4 * i] = v.x; vw[4 * i + 1] = v.y; vw[4 * i + 2] = v.z; vw[4 * i + 3] = v.w;
-        }
-#pragma unroll
-        for (int i = 0; i < NG / 2; ++i) vd[i] = __ldg(reinterpret_cast<const uint32_t*>(h + codes + slot * (2 * NG)) + i);
-      };
+      Raw x;
       if (n > 0) {
-        load_k(0);
-        load_v();
+        place(0);
+        request(head, slot, x.kw, x.kd);
+        request(head + v_part, slot, x.vw, x.vd);
       }
       for (int k = 0; k < n; ++k) {                    // (a wait that gives up is not repeated; the barriers go on)
-        const int st = k & 1, key = ts.unit(k) * kUnit + t;
+        const int st = k & 1, key = key_of_unit(k);
         const bool seen = in && any_sees(key), bad = !in && any_sees(key);
         bool odd = false;
         uint32_t mk = 0, mv = 0;
 #pragma unroll
         for (int i = 0; i < NG / 2; ++i) {
-          if (!seen) kd[i] = vd[i] = 0u;
-          mk = __vmaxu2(mk, kd[i] & 0x7fff7fffu);
-          mv = __vmaxu2(mv, vd[i] & 0x7fff7fffu);
+          if (!seen) x.kd[i] = x.vd[i] = 0u;
+          mk = __vmaxu2(mk, x.kd[i] & 0x7fff7fffu);
+          mv = __vmaxu2(mv, x.vd[i] & 0x7fff7fffu);
         }
         mk = max(mk & 0xffffu, mk >> 16);
         mv = max(mv & 0xffffu, mv >> 16);
@@ -1329,35 +1397,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
           odd = true;
           mv = 0;
 #pragma unroll
-          for (int i = 0; i < NG / 2; ++i) vd[i] = 0u;
+          for (int i = 0; i < NG / 2; ++i) x.vd[i] = 0u;
         }
         const bool big_k = loader_any(mk > 0x6c00u), big_v = loader_any(mv > 0x6c00u);     // 4096
-        if (k >= 2 && ok) ok = mbar_wait_bounded(&ctl->k_empty[st], ((k >> 1) - 1) & 1);
-        {
-          const __half2 down = __float2half2_rn(big_k ? 0.0625f : 1.f);
-          uint8_t* to = base_p + (s_k - base) + st * Shape::kTile + t * 128;
+        if (k >= 2 && ok) ok = mbar_wait_soon(&ctl->k_empty[st], ((k >> 1) - 1) & 1);
+        const __half2 down_k = __float2half2_rn(big_k ? 0.0625f : 1.f), down_v = __float2half2_rn(big_v ? 0.0625f : 1.f);
+        uint8_t* to = base_p + (s_k - base) + st * Shape::kTile + t * 128;
 #pragma unroll
-          for (int p = 0; p < D / 8; ++p) {            // word p: chunk NG' of block p % NG, quarter p / NG
-            const int g = p % NG, c = 4 * g + p / NG;  // 16-byte chunk of the row: values 8 c ...
-            const uint32_t dw = kd[g / 2];
-            const __half2 d2 = __hmul2(g & 1 ? __high2half2(*reinterpret_cast<const __half2*>(&dw))
-                                             : __low2half2(*reinterpret_cast<const __half2*>(&dw)), down);
-            *reinterpret_cast<uint4*>(to + (c / 8) * Shape::kBlock + ((c & 7) ^ (t & 7)) * 16) = decode_word(kw[p], d2);
-          }
+        for (int p = 0; p < D / 8; ++p) {              // word p: block p % NG, quarter p / NG
+          const int g = p % NG, c = 4 * g + p / NG;    // 16-byte chunk of the row: values 8 c ...
+          const __half2 dw = *reinterpret_cast<const __half2*>(&x.kd[g / 2]);
+          const __half2 d2 = __hmul2(g & 1 ? __high2half2(dw) : __low2half2(dw), down_k);
+          *reinterpret_cast<uint4*>(to + (c / 8) * Shape::kBlock + ((c & 7) ^ (t & 7)) * 16) = decode_word(x.kw[p], d2);
         }
         fence_proxy_async_smem();
         mbar_arrive(&ctl->k_full[st]);
-        if (k + 1 < n) load_k(k + 1);                  // (in, head, slot: the next unit's from here on)
-        if (k >= 2 && ok) ok = mbar_wait_bounded(&ctl->v_empty[st], ((k >> 1) - 1) & 1);
-        {
-          const __half2 down = __float2half2_rn(big_v ? 0.0625f : 1.f);
-          uint8_t* to = base_p + (s_v - base) + st * Shape::kTile + t * 128;
+        uint32_t vd[NG / 2];
 #pragma unroll
-          for (int p = 0; p < D / 8; ++p) {            // word p is chunk p: columns 8 p ...
-            const uint32_t dw = vd[p % (NG / 2)];
-            *reinterpret_cast<uint4*>(to + (p / 8) * Shape::kBlock + ((p & 7) ^ (t & 7)) * 16) =
-                decode_word(vw[p], __hmul2(*reinterpret_cast<const __half2*>(&dw), down));
-          }
+        for (int i = 0; i < NG / 2; ++i) vd[i] = x.vd[i];
+        if (k + 1 < n) {
+          place(k + 1);
+          request(head, slot, x.kw, x.kd);
+        }
+        if (k >= 2 && ok) ok = mbar_wait_soon(&ctl->v_empty[st], ((k >> 1) - 1) & 1);
+        to = base_p + (s_v - base) + st * Shape::kTile + t * 128;
+#pragma unroll
+        for (int p = 0; p < D / 8; ++p) {              // word p is chunk p: columns 8 p ...
+          const __half2 dw = *reinterpret_cast<const __half2*>(&vd[p % (NG / 2)]);
+          *reinterpret_cast<uint4*>(to + (p / 8) * Shape::kBlock + ((p & 7) ^ (t & 7)) * 16) =
+              decode_word(x.vw[p], __hmul2(dw, down_v));
         }
         const unsigned bad_w = __ballot_sync(0xffffffffu, bad), odd_w = __ballot_sync(0xffffffffu, odd);
         if (lane == 0) {
@@ -1371,33 +1439,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
         }
         fence_proxy_async_smem();
         mbar_arrive(&ctl->v_full[st]);
-        if (k + 1 < n) load_v();
+        if (k + 1 < n) request(head + v_part, slot, x.vw, x.vd);
       }
     } else {
       constexpr int P = D / 8;                         // 16-byte chunks of a row
       constexpr int kRowsAtOnce = 128 / P, kIter = 128 / kRowsAtOnce;
       const int c = t % P, r0 = t / P;
+      // lane j of a warp holds the page of the unit's keys 16 j ...
+      auto pages_of = [&](int k) { return lane < 8 ? page_of(ts.unit(min(k, n - 1)) * kUnit + 16 * lane) : -1; };
       // the copies of one part of a unit: chunk c of rows r0, r0 + kRowsAtOnce, ...
-      auto copy = [&](int k, int64_t part, uint32_t to, uint32_t& bad) {
+      auto copy = [&](int k, int pages, int64_t part, uint32_t to, uint32_t& bad) {
         const int key0 = ts.unit(k) * kUnit;
-#pragma unroll 4
+#pragma unroll
         for (int i = 0; i < kIter; ++i) {
           const int r = r0 + i * kRowsAtOnce, key = key0 + r;
-          bool in;
-          const uint8_t* head = locate(key, in);
-          if (!in && any_sees(key)) bad |= 1u << i;
+          const int p = __shfl_sync(0xffffffffu, pages, r >> 4);
+          const bool in = in_pool(p), seen = any_sees(key);
+          if (!in && seen) bad |= 1u << i;
           const uint32_t dst = to + (c / 8) * Shape::kBlock + r * 128 + ((c & 7) ^ (r & 7)) * 16;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                       ::"r"(dst), "l"(head + part + (key & page_mask) * (2 * D) + c * 16),
-                         "r"(in && any_sees(key) ? 16u : 0u) : "memory");
+                       ::"r"(dst), "l"(pool + (in ? p : 0) * page_bytes + part + (key & page_mask) * (2 * D) + c * 16),
+                         "r"(in && seen ? 16u : 0u) : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       // each part of the next unit is requested as soon as its stage is free, K before V
       uint32_t bad_next = 0, bad_now = 0, none = 0;
+      int pages = -1;                                  // of the next unit
       if (n > 0) {
-        copy(0, 0, s_k, bad_next);
-        copy(0, v_part, s_v, none);
+        pages = pages_of(0);
+        copy(0, pages, 0, s_k, bad_next);
+        copy(0, pages, v_part, s_v, none);
+        pages = pages_of(1);
       }
       for (int k = 0; k < n; ++k) {                    // (a wait that gives up is not repeated; the barriers go on)
         const int st = k & 1;
@@ -1407,8 +1480,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
         fence_proxy_async_smem();
         mbar_arrive(&ctl->k_full[st]);
         if (k + 1 < n) {
-          if (k >= 1 && ok) ok = mbar_wait_bounded(&ctl->k_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
-          copy(k + 1, 0, s_k + (st ^ 1) * Shape::kTile, bad_next);
+          if (k >= 1 && ok) ok = mbar_wait_soon(&ctl->k_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
+          copy(k + 1, pages, 0, s_k + (st ^ 1) * Shape::kTile, bad_next);
           asm volatile("cp.async.wait_group 1;" ::: "memory");         // V(k)
         } else {
           asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1442,8 +1515,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
         fence_proxy_async_smem();
         mbar_arrive(&ctl->v_full[st]);
         if (k + 1 < n) {
-          if (k >= 1 && ok) ok = mbar_wait_bounded(&ctl->v_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
-          copy(k + 1, v_part, s_v + (st ^ 1) * Shape::kTile, none);
+          if (k >= 1 && ok) ok = mbar_wait_soon(&ctl->v_empty[st ^ 1], (((k + 1) >> 1) - 1) & 1);
+          copy(k + 1, pages, v_part, s_v + (st ^ 1) * Shape::kTile, none);
+          pages = pages_of(k + 2);
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1456,49 +1530,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     const int pmin = ts.p_first + (ts.r0 + 128 * tile) / G, pmax = ts.p_first + (ts.r0 + last) / G;
     float ref = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int k = 0; k < n; ++k) {
-      const int st = k & 1, key0 = ts.unit(k) * kUnit;
-      ok = mbar_wait_bounded(&ctl->v_full[st], (k >> 1) & 1) && mbar_wait_bounded(&ctl->s_full[tile], k & 1);
+    for (int u = 0; u < 2 * n; ++u) {
+      const int k = u >> 1, h = u & 1, st = k & 1, key0 = ts.unit(k) * kUnit + 64 * h;
+      ok = (h == 1 || mbar_wait_soon(&ctl->v_full[st], (k >> 1) & 1)) && mbar_wait_soon(&ctl->s_full[tile][h], k & 1);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      uint32_t v[64];
+      {
+        uint32_t(&va)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
+        uint32_t(&vb)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[32]);
+        tmem_ld32(t_s + 64 * h, va);
+        tmem_ld32(t_s + 64 * h + 32, vb);
+      }
       const PromptInfo& info = ctl->info[st];
-      const uint32_t any_bad = info.bad[0] | info.bad[1] | info.bad[2] | info.bad[3];
-      const uint32_t any_odd = info.odd[0] | info.odd[1] | info.odd[2] | info.odd[3];
-      const bool whole = !any_bad && key0 + kUnit - 1 <= pmin &&
-                         (a.window == 0 || key0 > pmax - a.window || key0 + kUnit <= a.sinks);
+      const uint32_t bad0 = info.bad[2 * h], bad1 = info.bad[2 * h + 1], any_odd = info.odd[2 * h] | info.odd[2 * h + 1];
+      const bool whole = !(bad0 | bad1) && key0 + 63 <= pmin &&
+                         (a.window == 0 || key0 > pmax - a.window || key0 + 64 <= a.sinks);
       const float f = info.k_exp ? q_f * 16.f : q_f;
       // columns hi .. and, with a window, sk .. lo are hidden from this row
       const int hi = pos - key0, lo = a.window > 0 ? pos - a.window - key0 : -1, sk = a.window > 0 ? a.sinks - key0 : 0;
-      auto mask = [&](uint32_t (&v)[32], int c0) {
-        const uint32_t b = info.bad[c0 >> 5];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = c0 + i;
-          if (c > hi || (c <= lo && c >= sk) || (b >> i & 1u)) v[i] = 0xff800000u;
-        }
-      };
+      tmem_ld_wait();
       float m = -INFINITY;
-#pragma unroll 1
-      for (int c0 = 0; c0 < kUnit; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(t_s + c0, v);
-        tmem_ld_wait();
-        if (!whole) mask(v, c0);
+      if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+        for (int c = 0; c < 64; ++c)
+          if (c > hi || (c <= lo && c >= sk) || ((c < 32 ? bad0 : bad1) >> (c & 31) & 1u)) v[c] = 0xff800000u;
       }
+#pragma unroll
+      for (int i = 0; i < 64; i += 2) m = fmaxf(m, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
       const float want = m == -INFINITY ? m : m * f;
       const bool move = want > ref + 8.f;
       const float was = ref;
       if (move) ref = want;
       const float al = was == ref ? 1.f : ex2(was - ref);
       l *= al;
-      if (any_odd || (k > 0 && __any_sync(0xffffffffu, move))) {
-        if (k > 0) {
-          ok = mbar_wait_bounded(&ctl->o_done[tile], (k - 1) & 1);
+      if (any_odd || (u > 0 && __any_sync(0xffffffffu, move))) {
+        if (u > 0) {
+          ok = mbar_wait_soon(&ctl->o_done[tile][h ^ 1], ((u - 1) >> 1) & 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -1507,24 +1578,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
         }
         const float at0 = ref == -INFINITY ? 0.f : ref;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 16) {
-          uint32_t v[16];
-          if (k > 0) {
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                : "r"(t_o + c0));
+        for (int c0 = 0; c0 < D; c0 += 8) {
+          uint32_t o[8];
+          if (u > 0) {
+            tmem_ld8(t_o + c0, o);
             tmem_ld_wait();
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = k > 0 ? __float_as_uint(__uint_as_float(v[i]) * al) : 0u;
+          for (int i = 0; i < 8; ++i) o[i] = u > 0 ? __float_as_uint(__uint_as_float(o[i]) * al) : 0u;
           if (any_odd) {
-            for (int w = 0; w < 4; ++w)
-              for (uint32_t left = info.odd[w]; left; left &= left - 1) {
+            for (int w = 0; w < 2; ++w)
+              for (uint32_t left = info.odd[2 * h + w]; left; left &= left - 1) {
                 const int c = 32 * w + __ffs(left) - 1;
                 uint32_t x;
-                tmem_ld1(t_s + c, x);
+                tmem_ld1(t_s + 64 * h + c, x);
                 tmem_ld_wait();
                 // (a row that does not see the key adds nothing, not zero times it)
                 const bool see = !(c > hi || (c <= lo && c >= sk));
@@ -1533,7 +1600,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
                 const uint8_t* head = pool + __ldg(table + (key >> kv.page_shift)) * page_bytes + v_part;
                 const int slot = key & ((1 << kv.page_shift) - 1);
 #pragma unroll 1
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 8; ++i) {
                   float val;
                   if constexpr (KV == XM_KV_Q4_0) {    // column 8 q + 2 e + b is value e of block 2 (q % (NG / 2)) + b
                     const int q = (c0 + i) >> 3, e = ((c0 + i) >> 1) & 3, b = i & 1;
@@ -1545,52 +1612,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
                   } else {
                     val = __half2float(reinterpret_cast<const __half*>(head)[slot * D + c0 + i]);
                   }
-                  float acc = __uint_as_float(0u);
 #pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    if (j == i) acc = __uint_as_float(v[j]);
-                  if (see) acc = fmaf(p, val, acc);
-#pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    if (j == i) v[j] = __float_as_uint(acc);
+                  for (int j = 0; j < 8; ++j)
+                    if (j == i && see) o[j] = __float_as_uint(fmaf(p, val, __uint_as_float(o[j])));
                 }
                 __syncwarp();
               }
           }
-          tmem_st16(t_o + c0, v);
+          tmem_st8(t_o + c0, o);
         }
         tmem_st_wait();
       }
-      // P, in place of S; scaled up where the unit's values are scaled down
-      const float at = ref == -INFINITY ? 0.f : ref;
-      const float shift = info.v_exp ? 4.f - at : -at;
-      float s0 = 0.f, s1 = 0.f;
-#pragma unroll 1
-      for (int c0 = 0; c0 < kUnit; c0 += 32) {
-        uint32_t v[32], p[16];
-        tmem_ld32(t_s + c0, v);
-        tmem_ld_wait();
-        if (!whole) mask(v, c0);
+      // P in place of S; scaled up where the values are scaled down
+      const float at = ref == -INFINITY ? 0.f : ref, down = info.v_exp ? 4.f - at : -at;
+      const float2 ff = make_float2(f, f), sh = make_float2(down, down);
+      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+      auto weights = [&](auto whole_) {
+        constexpr bool kWhole = decltype(whole_)::value;
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float x = ex2(fmaf(__uint_as_float(v[i]), f, shift)), y = ex2(fmaf(__uint_as_float(v[i + 1]), f, shift));
-          if (!whole) {                                // (f may be 0)
-            if (v[i] == 0xff800000u) x = 0.f;
-            if (v[i + 1] == 0xff800000u) y = 0.f;
+        for (int i = 0; i < 64; i += 2) {
+          const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), ff, sh);
+          float2 z = make_float2(ex2(y.x), ex2(y.y));
+          if constexpr (!kWhole) {                     // (f may be 0)
+            if (v[i] == 0xff800000u) z.x = 0.f;
+            if (v[i + 1] == 0xff800000u) z.y = 0.f;
           }
-          s0 += x;
-          s1 += y;
-          p[i >> 1] = half2_bits(x, y);
+          if (i & 2) s1 = __fadd2_rn(s1, z); else s0 = __fadd2_rn(s0, z);
+          v[i >> 1] = half2_bits(z.x, z.y);
         }
-        tmem_st16(t_s + (c0 >> 1), p);
-      }
-      l = fmaf(s0 + s1, info.v_exp ? 0.0625f : 1.f, l);
+      };
+      if (whole) weights(std::true_type{}); else weights(std::false_type{});
+      tmem_st32(t_s + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+      l = fmaf((s0.x + s0.y) + (s1.x + s1.y), info.v_exp ? 0.0625f : 1.f, l);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&ctl->p_full[tile]);
+      mbar_arrive(&ctl->p_full[tile][h]);
     }
     // O / l
-    if (n > 0 && ok) ok = mbar_wait_bounded(&ctl->o_done[tile], (n - 1) & 1);
+    if (n > 0 && ok) ok = mbar_wait_soon(&ctl->o_done[tile][1], (n - 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     const float inv = l == 0.f ? 0.f : 1.0f / l;

@@ -48,35 +48,40 @@ struct SampleArgs {
 };
 
 // ---------------------------------------------------------------------------
-// A cut through the descending order (top-k: k tokens above it, top-p: a mass) is found by a histogram:
-// the logits between the largest and the smallest fall into kBins bins by a monotone function, and the
-// cut lies in the bin in which the count or the mass passes the limit.  Where no more than kList tokens lie
-// in the bins up to it, or up to the one that min_p ends in (128000 normal logits: some 250 in the fullest of 2048
-// bins), they are gathered by one CTA, sorted, cut and drawn from there.  Otherwise the bin becomes the
-// next interval until it holds at most kList tokens, which are sorted; an interval of one value is cut
-// by index; and the token is drawn by a pass over the row.
+// A cut through the descending order (top-k: k tokens above it, top-p: a mass).  Up to kList tokens that hold
+// everything that can be kept are gathered by one CTA, sorted, cut and drawn from there:
+// * top_k: every thread has the maxima of four groups of its logits from the pass that loads them.  The top_k-th
+//   largest of these has top_k tokens at or above it, so the top_k largest tokens lie in its bin of a histogram of the
+//   maxima or above (128000 normal logits, top_k 300: some 305 tokens in 2048 bins).
+// * top_p: the cut lies in the bin of a histogram of masses in which the mass passes the limit; min_p bounds the
+//   bins that count.
+// Where more tokens than that lie above, the bin becomes the next interval of a histogram of all tokens until it
+// holds at most kList tokens, which are sorted; an interval of one value is cut by index; and the token is drawn by
+// a pass over the row.
 //
 // Weights: 2^y with y = (x - max) log2(e) / T in 64 bits, by a table of 2^(j / 256) and a polynomial of
 // degree 3 on the rest (table-driven exponential after Tang, 1989): 2e-13 of the value, less than the
 // rounding to a whole multiple of 2^-F.
 //
 // Bound: latency for few rows (passes over shared memory and three to eight exchanges across a cluster); for many
-// the instructions of the weights, some 25 a logit, ten of them in 64 bits.
+// the instructions of the weights, some 25 a logit, ten of them in 64 bits, and with top_p alone the atomic adds to
+// shared memory (about one lane a clock on an SM: that is why a bin's mass is two words, of which the
+// upper one takes carries and weights above 2^-12 only, and why top_k counts maxima and not logits).
 // ---------------------------------------------------------------------------
 constexpr int kSampleThreads = 512, kBins = 2048, kList = 512, kTable = 256;
 static_assert(kList == kSampleThreads, "the list is sorted with one entry a thread");
 typedef unsigned long long u64;
 
 struct alignas(16) SampleSmem {
-  unsigned cnt[kBins], mass[3][kBins];  // a bin's mass as sums of three 15-bit digits (a CTA has up to 2^17 logits)
+  unsigned low[kBins], high[kBins];     // a bin's mass (or count, in low)
   u64 list[kList];
   double table[kTable];
-  u64 xch[2][8][4];                     // exchange slots: buffer, rank, value
+  u64 xch[2][8][2];                     // exchange slots: buffer, rank, value
   u64 warp_sum[32], warp_cnt[32];
-  u64 red[32][4];
+  u64 red[16][2];                       // four 32-bit values of each warp
   unsigned list_n;
   int found_bin;
-  u64 found_cnt, found_before, found_upto;
+  u64 found_before;
   unsigned tau;
   int cut;
 };
@@ -154,42 +159,55 @@ struct Sampler {
     return (u64)__double_as_longlong(t + 4503599627370496.0) & 0xfffffffffffffull;   // + 2^52
   }
 
-  // sums (op 0) or maxima (op 1) of up to 4 values over the cluster, the same in every thread
-  template <int N>
-  XM_DEV void all(u64 (&v)[N], const int (&op)[N]) {
+  // sums (op 0) or maxima (op 1) of four 32-bit values over the cluster, the same in every thread
+  XM_DEV void all(unsigned (&v)[4], const int (&op)[4]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const u64 u = __shfl_xor_sync(0xffffffffu, v[i], o);
-        v[i] = op[i] ? max(v[i], u) : v[i] + u;
-      }
-      if (lane == 0) sm.red[warp][i] = v[i];
-    }
+    for (int i = 0; i < 4; ++i) v[i] = op[i] ? __reduce_max_sync(0xffffffffu, v[i]) : __reduce_add_sync(0xffffffffu, v[i]);
+    if (lane == 0) *reinterpret_cast<uint4*>(sm.red[warp]) = make_uint4(v[0], v[1], v[2], v[3]);
     __syncthreads();
     if (warp == 0) {
+      uint4 t = make_uint4(0u, 0u, 0u, 0u);
+      if (lane < NT / 32) t = *reinterpret_cast<const uint4*>(sm.red[lane]);
+      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        u64 u = lane < NT / 32 ? sm.red[lane][i] : 0ull;
-#pragma unroll
-        for (int o = NT / 64; o > 0; o >>= 1) {
-          const u64 t = __shfl_xor_sync(0xffffffffu, u, o);
-          u = op[i] ? max(u, t) : u + t;
-        }
-        u = __shfl_sync(0xffffffffu, u, 0);
-        if (lane < C) cl.map_shared_rank(&sm, lane)->xch[turn][rank][i] = u;
-      }
+      for (int i = 0; i < 4; ++i)
+        v[i] = op[i] ? __reduce_max_sync(0xffffffffu, v[i]) : __reduce_add_sync(0xffffffffu, v[i]);
+      if (lane < C)
+        *reinterpret_cast<uint4*>(cl.map_shared_rank(&sm, lane)->xch[turn][rank]) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     sync();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = 0ull;
-      for (int r = 0; r < C; ++r) {
-        const u64 u = sm.xch[turn][r][i];
-        v[i] = op[i] ? max(v[i], u) : v[i] + u;
-      }
+    for (int i = 0; i < 4; ++i) v[i] = 0u;
+    for (int r = 0; r < C; ++r) {
+      const uint4 t = *reinterpret_cast<const uint4*>(sm.xch[turn][r]);
+      v[0] = op[0] ? max(v[0], t.x) : v[0] + t.x;
+      v[1] = op[1] ? max(v[1], t.y) : v[1] + t.y;
+      v[2] = op[2] ? max(v[2], t.z) : v[2] + t.z;
+      v[3] = op[3] ? max(v[3], t.w) : v[3] + t.w;
     }
     turn ^= 1;
+  }
+  // the sum of v over the cluster's threads
+  XM_DEV u64 sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) sm.warp_sum[warp] = v;
+    __syncthreads();
+    u64 cta = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) cta += sm.warp_sum[w];
+    return over_ranks(cta, C);
+  }
+  // the sum of v, the same in every thread of a CTA, over the first n ranks
+  XM_DEV u64 over_ranks(u64 v, int n) {
+    if (C == 1) return n ? v : 0ull;
+    if (tid < C) cl.map_shared_rank(&sm, tid)->xch[turn][rank][0] = v;
+    sync();
+    v = 0ull;
+    for (int r = 0; r < n; ++r) v += sm.xch[turn][r][0];
+    turn ^= 1;
+    return v;
   }
   XM_DEV void sync() {
     if (C > 1) cl.sync(); else __syncthreads();
@@ -294,130 +312,139 @@ struct Sampler {
     return r;
   }
 
-  // The CTA's list in descending order (key, then lowest index), one entry a thread: (key, ~index), 0 behind the
-  // last.  Strides of a warp go by shuffles, the others through shared memory.
-  XM_DEV u64 sorted(u64 v) {
-#pragma unroll 1
-    for (int k = 2; k <= NT; k <<= 1) {
-#pragma unroll 1
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        u64 o;
-        if (j >= 32) {
-          __syncthreads();
-          sm.list[tid] = v;
-          __syncthreads();
-          o = sm.list[tid ^ j];
-        } else {
-          o = __shfl_xor_sync(0xffffffffu, v, j);
-        }
-        const bool first_half = (tid & j) == 0, down = (tid & k) == 0;      // down: the larger one to the first half
-        v = first_half == down ? max(v, o) : min(v, o);
+  // n entries, one a thread (0 behind the last, all different), in descending order: each goes to the place that the
+  // number of the larger ones gives (of 320 entries a third of the time of a bitonic network).
+  XM_DEV u64 sorted(u64 v, int n) {
+    __syncthreads();
+    sm.list[tid] = v;
+    __syncthreads();
+    int at = 0;
+    if (tid < n) {
+#pragma unroll 4
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(sm.list + j);
+        at += (int)(t.x > v) + (int)(t.y > v);
       }
     }
-    return v;
+    __syncthreads();
+    if (tid < n) sm.list[at] = v;
+    __syncthreads();
+    return tid < n ? sm.list[tid] : 0ull;
   }
-  // rank 0's list from what in(logit, index) names; the caller is behind a sync() that follows list_n = 0
-  template <typename IN>
-  XM_DEV void gather(IN in) {
-    SampleSmem* to = cl.map_shared_rank(&sm, 0);
-    each([&](float v, int i) {
-      if (in(v, i)) to->list[atomicAdd(&to->list_n, 1u)] = (u64)order_key(v) << 32 | (unsigned)~i;
-    });
+  // List of this CTA: cleared (a __syncthreads() has to follow), filled, and rank 0's view of all of them, one entry
+  // a thread, behind a sync() that follows the last push and where they are kList at most.
+  XM_DEV void clear_list() {
+    if (tid == 0) sm.list_n = 0;
+  }
+  XM_DEV void push(float v, int i) {
+    if (*(volatile unsigned*)&sm.list_n > kList) return;          // more than can be used
+    const unsigned at = atomicAdd(&sm.list_n, 1u);
+    if (at < kList) sm.list[at] = (u64)order_key(v) << 32 | (unsigned)~i;
+  }
+  XM_DEV u64 pull() {
+    u64 e = 0;
+    if (rank == 0) {
+      unsigned c[8], at = tid;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) c[r] = r < C ? cl.map_shared_rank(&sm, r)->list_n : 0u;
+      int from = -1;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (from < 0) {
+          if (at < c[r]) from = r; else at -= c[r];
+        }
+      if (from >= 0) e = cl.map_shared_rank(&sm, from)->list[at];
+    }
     sync();
+    return e;
   }
-  XM_DEV u64 entry() const { return (unsigned)tid < sm.list_n ? sm.list[tid] : 0ull; }
 
-  // Histogram of the logits that in(logit, index) names between lo and hi, by the function of bin(); then the bin in
-  // which the count (or the mass) that starts at `base` reaches `limit`, or limit(total) of it.
   struct Bins {
     float hi, lo, top, half, scale;
-    // a monotone function (to the nearest whole number, by adding 2^23); the ends have bins of their own, so a
-    // step leaves at least one of them out
+    // a monotone function (to the nearest whole number, by adding 2^23) that takes what is below lo to the last bin;
+    // the ends have bins of their own, so a step leaves at least one of them out
     XM_DEV Bins(float h, float l) : hi(h), lo(l) {
       half = hi - lo < INFINITY ? 1.f : 0.5f;
-      top = hi * half;
+      top = fminf(hi, 3.402823466e38f) * half;
       scale = (kBins - 1) / (top - lo * half);
     }
     XM_DEV int operator()(float v) const {
       const float t = fminf(fmaxf((top - v * half) * scale, 0.f), (float)(kBins - 1)) + 8388608.f;
-      return v == hi ? 0 : v == lo ? kBins - 1 : __float_as_int(t) & (kBins - 1);
+      return v == hi ? 0 : v <= lo ? kBins - 1 : __float_as_int(t) & (kBins - 1);
     }
   };
-  template <bool MASS, typename IN, typename LIMIT>
-  XM_DEV void histogram(const Bins& bin, IN in, u64 base, LIMIT limit_of, int last_bin) {
-    for (int b = tid; b < kBins; b += NT) {
-      sm.cnt[b] = 0u;
-      if (MASS) sm.mass[0][b] = sm.mass[1][b] = sm.mass[2][b] = 0u;
-    }
-    if (tid == 0) sm.list_n = 0;
+  XM_DEV void clear_bins() {
+    for (int b = tid; b < kBins; b += NT) sm.low[b] = sm.high[b] = 0u;
     __syncthreads();
-    each([&](float v, int i) {
-      if (v <= bin.hi && v >= bin.lo && in(v, i)) {
-        const int b = bin(v);
-        atomicAdd(&sm.cnt[b], 1u);
-        if (MASS) {
-          const u64 w = weight(v);
-          if (w) {
-            atomicAdd(&sm.mass[0][b], (unsigned)w & 0x7fffu);
-            atomicAdd(&sm.mass[1][b], (unsigned)(w >> 15) & 0x7fffu);
-            atomicAdd(&sm.mass[2][b], (unsigned)(w >> 30));
-          }
+  }
+  // (the carries out of the lower words are the same in every order of the additions)
+  XM_DEV void add_mass(int b, u64 w) {
+    if (!w) return;
+    const unsigned l = (unsigned)w, old = atomicAdd(&sm.low[b], l), h = (unsigned)(w >> 32) + (old + l < l);
+    if (h) atomicAdd(&sm.high[b], h);
+  }
+  // The bin of the cluster's histograms, behind a sync(), in which the sum that starts at `base` reaches `limit`, -1
+  // where none does, and the sum before it.  Each CTA adds up its share of the bins over the cluster.
+  XM_DEV void find(u64 base, u64 limit) {
+    static_assert(kBins / 4 <= NT, "a thread's bins are one 16-byte load");
+    const int share = kBins / C;
+    u64 ds[4] = {}, mine = 0;
+    if (4 * tid < share) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < C) {
+          const SampleSmem* p = cl.map_shared_rank(&sm, r);
+          const uint4 t = reinterpret_cast<const uint4*>(p->low + rank * share)[tid];
+          const uint4 h = reinterpret_cast<const uint4*>(p->high + rank * share)[tid];
+          ds[0] += (u64)h.x << 32 | t.x; ds[1] += (u64)h.y << 32 | t.y;
+          ds[2] += (u64)h.z << 32 | t.z; ds[3] += (u64)h.w << 32 | t.w;
         }
-      }
-    });
-    sync();
-    // every CTA sums all bins over the cluster
-    constexpr int PER = kBins / NT;
-    static_assert(PER == 4, "a thread's bins are one 16-byte load");
-    unsigned cs[PER] = {};
-    u64 ds[PER] = {}, mine = 0, count = 0;
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < C) {
-        const SampleSmem* p = cl.map_shared_rank(&sm, r);
-        const uint4 t = reinterpret_cast<const uint4*>(p->cnt)[tid];
-        cs[0] += t.x; cs[1] += t.y; cs[2] += t.z; cs[3] += t.w;
-        if (MASS) {
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const uint4 m = reinterpret_cast<const uint4*>(p->mass[k])[tid];
-            ds[0] += (u64)m.x << 15 * k; ds[1] += (u64)m.y << 15 * k;
-            ds[2] += (u64)m.z << 15 * k; ds[3] += (u64)m.w << 15 * k;
-          }
-        }
-      }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (!MASS) ds[j] = cs[j];
-      mine += ds[j];
-      count += cs[j];
     }
-    u64 total, counted;
-    u64 before = scan(mine, sm.warp_sum, total) - mine + base, upto = scan(count, sm.warp_cnt, counted) - count;
-    const u64 limit = limit_of(total);
-    if (tid == 0) sm.found_upto = 0;
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      upto += cs[j];
-      if (before < limit && before + ds[j] >= limit) {
-        sm.found_bin = tid * PER + j;
-        sm.found_cnt = cs[j];
-        sm.found_before = before;
-        sm.found_upto = upto;
-      }
+    for (int j = 0; j < 4; ++j) mine += ds[j];
+    if (tid == 0) sm.found_bin = -1;
+    u64 total, before = scan(mine, sm.warp_sum, total) - mine + base;        // (holds __syncthreads())
+    before += over_ranks(total, rank);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (before < limit && before + ds[j] >= limit)
+        for (int r = 0; r < C; ++r) {
+          SampleSmem* p = cl.map_shared_rank(&sm, r);
+          p->found_bin = rank * share + 4 * tid + j;
+          p->found_before = before;
+        }
       before += ds[j];
     }
+    sync();
+  }
+  // Puts what lies in the bins up to `upto` on the lists and returns their number; the logits of bin b, which hold
+  // every one between their extremes, become the next interval.
+  template <typename IN>
+  XM_DEV u64 collect(const Bins& bin, IN in, int upto, int b, u64& n, float& hi, float& lo) {
+    clear_list();
     __syncthreads();
-    // tokens in the bins up to last_bin, where that comes first
-    if (last_bin < sm.found_bin && last_bin / PER == tid) {
-      u64 n = upto;
-#pragma unroll
-      for (int j = PER - 1; j >= 0; --j)
-        if (tid * PER + j > last_bin) n -= cs[j];
-      sm.found_upto = n;
-    }
-    __syncthreads();
+    float h = -INFINITY, g = INFINITY;
+    unsigned v[4] = {};
+    each([&](float x, int i) {
+      if (!(x <= bin.hi && x > -INFINITY) || !in(x, i)) return;
+      const int at = bin(x);
+      if (at <= upto) {
+        ++v[3];
+        push(x, i);
+      }
+      if (at == b && x >= bin.lo) {
+        h = fmaxf(h, x);
+        g = fminf(g, x);
+        ++v[2];
+      }
+    });
+    v[0] = order_key(h);
+    v[1] = g < INFINITY ? ~order_key(g) : 0u;
+    all(v, {1, 1, 0, 0});
+    hi = from_key(v[0]);
+    lo = from_key(~v[1]);
+    n = v[2];
+    return v[3];
   }
 
   // Cuts the descending order of the logits that in(logit, index) names, between lo and hi, n of them, before which
@@ -427,11 +454,16 @@ struct Sampler {
   XM_DEV void select(IN in, u64 n, float hi, float lo, u64 base, u64 limit, uint32_t& tau, int& cut) {
     for (;;) {
       if (n <= kList) {
-        if (tid == 0) sm.list_n = 0;
+        clear_list();
+        __syncthreads();
+        each([&](float v, int i) {
+          if (v <= hi && v >= lo && in(v, i)) push(v, i);
+        });
         sync();
-        gather([&](float v, int i) { return v <= hi && v >= lo && in(v, i); });
+        u64 e = pull();
         if (rank == 0) {
-          const u64 e = sorted(entry()), w = !e ? 0ull : MASS ? weight(from_key((uint32_t)(e >> 32))) : 1ull;
+          e = sorted(e, (int)n);
+          const u64 w = !e ? 0ull : MASS ? weight(from_key((uint32_t)(e >> 32))) : 1ull;
           u64 sum;
           const u64 upto = base + scan(w, sm.warp_sum, sum);
           if (upto - w < limit && upto >= limit)
@@ -454,27 +486,17 @@ struct Sampler {
         return;
       }
       const Bins bin(hi, lo);
-      histogram<MASS>(bin, in, base, [&](u64) { return limit; }, kBins);
-      narrow(bin, in, n, hi, lo, base);
+      clear_bins();
+      each([&](float v, int i) {
+        if (v <= hi && v >= lo && in(v, i)) {
+          if (MASS) add_mass(bin(v), weight(v)); else atomicAdd(&sm.low[bin(v)], 1u);
+        }
+      });
+      sync();
+      find(base, limit);
+      base = sm.found_before;
+      collect(bin, in, -1, sm.found_bin, n, hi, lo);
     }
-  }
-  // The found bin's own extremes are the next interval (the bin holds all of the logits between them).
-  template <typename IN>
-  XM_DEV void narrow(const Bins& bin, IN in, u64& n, float& hi, float& lo, u64& base) {
-    const int b = sm.found_bin;
-    n = sm.found_cnt;
-    base = sm.found_before;
-    float h = -INFINITY, g = INFINITY;
-    each([&](float v, int i) {
-      if (v <= bin.hi && v >= bin.lo && bin(v) == b && in(v, i)) {
-        h = fmaxf(h, v);
-        g = fminf(g, v);
-      }
-    });
-    u64 v[2] = {order_key(h), g < INFINITY ? (u64)(~order_key(g)) : 0ull};
-    all(v, {1, 1});                                               // (and the histograms have been read)
-    hi = from_key((uint32_t)v[0]);
-    lo = from_key(~(uint32_t)v[1]);
   }
 };
 
@@ -493,7 +515,9 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
   const bool greedy = !(T > 0.f), cuts = !greedy && ((top_k > 0 && top_k < a.V) || top_p < 1.f);
 
   if (tid < kTable) sm.table[tid] = exp2((double)tid / kTable);
-  float mx = -INFINITY, mn = INFINITY;
+  float group[4], mn = INFINITY;                                   // maxima of a quarter of this thread's logits each
+#pragma unroll
+  for (int e = 0; e < 4; ++e) group[e] = -INFINITY;
   unsigned real = 0;
 #pragma unroll 4
   for (int j = 0; j < s.pieces; ++j) {
@@ -507,15 +531,21 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x = to_f32(v[e]);
-      mx = fmaxf(mx, x);                                          // (a NaN loses)
+      group[e] = fmaxf(group[e], x);                              // (a NaN loses)
       if (cuts && x > -INFINITY) {
         mn = fminf(mn, x);
         ++real;
       }
     }
   }
-  u64 st[3] = {order_key(mx), mn < INFINITY ? (u64)(~order_key(mn)) : 0ull, real};
-  s.all(st, {1, 1, 0});
+  float least = INFINITY, mx = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    mx = fmaxf(mx, group[e]);
+    if (group[e] > -INFINITY) least = fminf(least, group[e]);
+  }
+  unsigned st[4] = {order_key(mx), mn < INFINITY ? ~order_key(mn) : 0u, real, least < INFINITY ? ~order_key(least) : 0u};
+  s.all(st, {1, 1, 0, 1});
   if (st[0] == 0) {                                               // nothing to choose from (the whole cluster)
     if (s.rank == 0 && tid == 0) {
       a.ids[b] = 0;
@@ -524,7 +554,7 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
     return;
   }
   const u64 n = st[2];
-  s.mx = from_key((uint32_t)st[0]);
+  s.mx = from_key(st[0]);
   s.frac = a.frac_bits;
   s.one = (double)(1ull << a.frac_bits);
   s.c_y = greedy ? 0.0 : 1.4426950408889634 * kTable / (double)T;
@@ -554,64 +584,114 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
     return key > tau || (key == tau && i <= cut);
   };
   if (by_count || by_mass) {
-    float hi = s.mx, lo = from_key(~(uint32_t)st[1]);
-    auto every = [](float, int) { return true; };
-    const typename Sampler<XT, NT, RES>::Bins bin(hi, lo);
+    typedef typename Sampler<XT, NT, RES>::Bins Bins;
+    float hi = s.mx, lo = from_key(~st[1]);
+    auto every = [](float v, int) { return v > -INFINITY; };
     // the bin that min_p ends in, behind the roundings of its logit and of bin()
     const float below = T * logf(fminf(min_p, 1.f));
     const float v_min = wmin ? s.mx + below - 4e-7f * (fabsf(s.mx) + fabsf(below)) : -INFINITY;
-    const int last = hi == lo || !(v_min >= lo) ? kBins : min(kBins - 1, bin(v_min) + 1);
-    u64 zt = 0, limit = (u64)top_k, left = n, base = 0;
-    bool fits = n <= kList;
-    if (fits) {
-      if (tid == 0) sm.list_n = 0;
+    u64 zt = 0, limit = (u64)top_k, left = n, base = 0, listed = ~0ull;
+    bool whole = n <= kList, uncut = false;                       // uncut: min_p leaves out what top_p would
+    if (whole) {
+      s.clear_list();
+      __syncthreads();
+      s.each([&](float v, int i) {
+        if (v > -INFINITY) s.push(v, i);
+      });
       s.sync();
-    } else if (hi < lo || hi > lo) {
-      if (by_count) s.template histogram<false>(bin, every, 0ull, [&](u64) { return limit; }, last);
-      else s.template histogram<true>(bin, every, 0ull, [&](u64 z) { zt = z; return limit = mass_limit(z); }, last);
-      fits = sm.found_upto <= kList;
+      listed = n;
+    } else if (by_count && top_k <= kList) {
+      const Bins bin(hi, from_key(~st[3]));
+      if (bin.hi > bin.lo) {
+        s.clear_bins();
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (group[e] > -INFINITY) atomicAdd(&sm.low[bin(group[e])], 1u);
+        s.sync();
+        s.find(0, limit);
+        float h, l;
+        u64 m;
+        listed = s.collect(bin, every, sm.found_bin, -1, m, h, l);
+        if (sm.found_bin < 0) listed = ~0ull;
+      }
+    } else if (by_count && !by_mass && v_min >= lo && hi > lo) {
+      const Bins bin(hi, lo);
+      float h, l;
+      u64 m;
+      listed = s.collect(bin, every, min(kBins - 1, bin(v_min) + 1), -1, m, h, l);
+    } else if (!by_count && hi > lo) {
+      const Bins bin(hi, lo);
+      const int last = v_min >= lo ? min(kBins - 1, bin(v_min) + 1) : kBins - 1;
+      s.clear_bins();
+      s.each([&](float v, int) {
+        if (!(v > -INFINITY)) return;
+        const u64 w = s.weight(v);
+        const int at = bin(v);
+        zt += w;
+        if (at <= last) s.add_mass(at, w);
+      });
+      zt = s.sum(zt);
+      limit = mass_limit(zt);
+      s.find(0, limit);
+      const int found = sm.found_bin;
+      uncut = found < 0;
+      base = sm.found_before;
+      listed = s.collect(bin, every, uncut ? last : found, found, left, hi, lo);
     }
-    if (fits && !(by_count && n > kList && last < sm.found_bin && by_mass)) {
-      // everything that can be kept is in one CTA's list
-      const int upto = n <= kList ? kBins : min(sm.found_bin, last);
-      s.gather([&](float v, int) { return v > -INFINITY && (n <= kList || bin(v) <= upto); });
+    if (listed <= kList) {
+      // everything that can be kept is on the lists
+      const u64 all = s.pull();
       if (s.rank != 0) return;
-      const u64 e = s.sorted(s.entry());
+      const u64 e = s.sorted(all, (int)listed);
       const bool in = e && (!by_count || tid < top_k);
       const float v = from_key((uint32_t)(e >> 32));
       const u64 w = in ? s.weight(v) : 0ull;
       u64 sum, z;
       const u64 incl = s.scan(w, sm.warp_sum, sum);
-      // (the mass of the top_k, or of all, where the list holds less)
-      const u64 p = by_mass ? mass_limit(by_count || n <= kList ? sum : zt) : ~0ull;
+      // (the mass of the top_k, or of all, where the list may hold less)
+      const u64 p = by_mass ? mass_limit(by_count || whole ? sum : zt) : ~0ull;
       const bool keep = in && incl - w < p && w >= wmin;
-      // in index order
-      u64 f = s.sorted(keep ? (u64)(unsigned)e << 32 | (uint32_t)(e >> 32) : 0ull);       // (~index, key), descending
-      const float vf = from_key((uint32_t)f);
-      const u64 wf = f ? s.weight(vf) : 0ull;
-      const u64 inf = s.scan(wf, sm.warp_sum, z), tgt = s.target(u, z);
-      if (inf - wf <= tgt && inf > tgt) done((int)~(unsigned)(f >> 32), vf, z);
+      // each kept one adds up those of lower index (the bins hold the indices)
+      const unsigned id = keep ? ~(unsigned)e : ~0u;
+      const u64 wk = keep ? w : 0ull;
+      sm.list[tid] = wk;
+      sm.low[tid] = id;
+      s.scan(wk, sm.warp_cnt, z);
+      const u64 tgt = s.target(u, z);
+      const int m = __syncthreads_count(keep);                    // (the first m)
+      if (keep) {
+        u64 at = 0;
+#pragma unroll 2
+        for (int j = 0; j < m; j += 4) {
+          const uint4 t = *reinterpret_cast<const uint4*>(sm.low + j);
+          const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(sm.list + j);
+          const ulonglong2 w1 = *reinterpret_cast<const ulonglong2*>(sm.list + j + 2);
+          if (t.x < id) at += w0.x;
+          if (t.y < id) at += w0.y;
+          if (t.z < id) at += w1.x;
+          if (t.w < id) at += w1.y;
+        }
+        if (at <= tgt && at + wk > tgt) done((int)id, v, z);
+      }
       return;
     }
     if (by_count) {
-      if (n > kList && hi > lo) s.narrow(bin, every, left, hi, lo, base);
       s.template select<false>(every, left, hi, lo, base, limit, tau, cut);
       cut_any = true;
       if (by_mass) {
-        u64 z[1] = {0ull};
+        u64 z = 0;
         s.each([&](float v, int i) {
-          if (above(v, i)) z[0] += s.weight(v);
+          if (above(v, i)) z += s.weight(v);
         });
-        s.all(z, {0});
+        z = s.sum(z);
         uint32_t t;
         int c;
-        s.template select<true>(above, limit, s.mx, from_key(tau), 0ull, mass_limit(z[0]), t, c);
+        s.template select<true>(above, limit, s.mx, from_key(tau), 0ull, mass_limit(z), t, c);
         tau = t;
         cut = c;
       }
-    } else {
-      if (hi > lo) s.narrow(bin, every, left, hi, lo, base);
-      else limit = mass_limit(n << s.frac);
+    } else if (!uncut) {
+      if (hi == lo && left == n) limit = mass_limit(n << s.frac);
       s.template select<true>(every, left, hi, lo, base, limit, tau, cut);
       cut_any = true;
     }

@@ -137,7 +137,7 @@ struct Sampler {
   // f(logit, index) for every logit of this thread (NaN and -inf among them)
   template <typename F>
   XM_DEV void each(F f) const {
-#pragma unroll 2
+#pragma unroll 1
     for (int j = 0; j < pieces; ++j) {
       float v[4];
       get(xs, first - lane * 4, 128 * j + lane * 4, v);

@@ -1180,6 +1180,14 @@ XM_DEV bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
   return ok || mbar_wait_bounded(bar, parity);
 }
 
+// One lane of the warp, so that the compiler knows that it is one: what only a uniform register can give an instruction
+// (the descriptors of a product) is otherwise brought there by a loop over the active lanes.
+XM_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+
 XM_DEV bool loader_any(bool p) {                       // over the 128 loader threads
   uint32_t r;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
@@ -1295,7 +1303,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
 
   if (warp >= 12) {
     const int i = warp - 12;                           // the row tile whose products this thread issues
-    if (lane == 0 && i < tiles && n > 0) {
+    if (i < tiles && n > 0 && elect_one()) {
       constexpr uint32_t id_s = idesc_f16(64, false), id_o = idesc_f16(D, true), kHalf = 64 * 128 >> 4;
       const uint32_t high = (uint32_t)(desc_sw128(0, 16) >> 32);
       const uint32_t lo_q = (uint32_t)desc_sw128(s_q + i * Shape::kTile, 16), lo_k = (uint32_t)desc_sw128(s_k, 16);

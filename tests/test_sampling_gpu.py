@@ -156,3 +156,38 @@ def test_the_share_of_each_token():
     count = torch.bincount(ids.cpu().long(), minlength=v).double()
     assert count[2] == 0 and count[5] == 0
     assert ((count[[0, 1, 3, 4, 6]] - n * p).abs() <= 2).all()               # evenly spread numbers: at most one off at each end
+
+
+@pytest.mark.parametrize("v", [9001, 40000])
+def test_more_tokens_than_a_list_holds_above_the_cut(v):
+    g = torch.Generator().manual_seed(v)
+    u = torch.rand(12, generator=g).cuda()
+    two = torch.where(torch.rand(12, v, generator=g) < 0.5, 0.0, -2.0).cuda()          # two values only
+    near = (torch.randn(12, v, generator=g) * 1e-3).cuda()
+    steps = (-torch.logspace(-6, 6, v)[torch.randperm(v, generator=g)]).repeat(12, 1).cuda()   # evenly spaced in the exponent
+    for x in (two, near, steps):
+        compare(x, u, top_k=10)
+        compare(x, u, top_k=512, top_p=0.6)
+        compare(x, u, top_k=513, min_p=0.3)
+        compare(x, u, top_k=v - 1, top_p=0.5, min_p=0.2)
+        compare(x, u, top_p=0.99, min_p=0.5)           # min_p leaves out what top_p would, and more than 512 are left
+        compare(x, u, top_p=0.2, min_p=0.5)
+        compare(x, u, top_p=0.99999)
+
+
+@pytest.mark.parametrize("count", [1, 3, 700])
+def test_infinite_logits_among_many(count):
+    """All of the mass lies on the infinite ones, evenly."""
+    v, rows = 30000, 6
+    x, u = make(rows, v, seed=77)
+    at = torch.randperm(v, generator=torch.Generator().manual_seed(78))[:count].sort().values
+    x[:, at.cuda()] = float("inf")
+    at = at.numpy()
+    un = u.cpu().numpy().astype(np.float64)
+    for kw, share in ((dict(), 1.0), (dict(top_p=0.9), 0.9), (dict(top_k=2000, top_p=0.5), 0.5), (dict(top_k=400), None),
+                      (dict(top_p=0.5, min_p=0.1), 0.5)):
+        kept = min(count, 400) if share is None else max(1, int(np.ceil(np.float64(np.float32(share)) * count)))
+        ids, logp = sample(x, u, **kw)
+        want = at[np.minimum(np.floor(un * kept).astype(int), kept - 1)]
+        assert (ids.cpu().numpy() == want).all(), kw
+        assert (logp.cpu() + np.log(kept)).abs().max() <= 1e-6

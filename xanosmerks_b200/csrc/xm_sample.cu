@@ -439,7 +439,7 @@ struct Sampler {
       }
     });
     v[0] = order_key(h);
-    v[1] = g < INFINITY ? ~order_key(g) : 0u;
+    v[1] = v[2] ? ~order_key(g) : 0u;
     all(v, {1, 1, 0, 0});
     hi = from_key(v[0]);
     lo = from_key(~v[1]);
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
     mx = fmaxf(mx, group[e]);
     if (group[e] > -INFINITY) least = fminf(least, group[e]);
   }
-  unsigned st[4] = {order_key(mx), mn < INFINITY ? ~order_key(mn) : 0u, real, least < INFINITY ? ~order_key(least) : 0u};
+  unsigned st[4] = {order_key(mx), real ? ~order_key(mn) : 0u, real, mx > -INFINITY ? ~order_key(least) : 0u};
   s.all(st, {1, 1, 0, 1});
   if (st[0] == 0) {                                               // nothing to choose from (the whole cluster)
     if (s.rank == 0 && tid == 0) {

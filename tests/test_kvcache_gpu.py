@@ -379,6 +379,26 @@ def test_nan_in_a_visible_key_spoils_the_rows_that_see_it(kv):
     assert torch.isnan(one).all()
 
 
+@pytest.mark.parametrize("kv", ["Q4_0", "F16"])
+def test_nan_in_any_column_of_a_prompt(kv):
+    """A key that every later row sees whole: the rows in front of it keep their values, the others are NaN."""
+    n, page = 300, 16
+    table, lens, cu, pages = layout([n], [n], page, seed=54)
+    c, pool = filled_cache(pages, 1, 128, page, kv, seed=55)
+    q = torch.randn(n, 2, 128, generator=torch.Generator().manual_seed(56)).half().cuda()
+    want = c.attend(q, dev(table), dev(lens), dev(cu))
+    at = 0 if kv == "F16" else page * 64
+    width = 256 if kv == "F16" else 8
+    for p in (0, 1, 6, 7, 13, 62, 70, 127):
+        before = c.pool.clone()
+        o = at + (p % page) * width
+        c.pool[int(table[0, p // page]), 0, o:o + width] = torch.tensor([0xff, 0x7f] * (width // 2), dtype=torch.uint8,
+                                                                       device="cuda")
+        out = c.attend(q, dev(table), dev(lens), dev(cu))
+        assert torch.equal(out[:p], want[:p]) and torch.isnan(out[p:]).all(), p
+        c.pool.copy_(before)
+
+
 def test_attention_strides_and_scale():
     """Queries and outputs inside wider tensors at an odd pitch; a scale of one's own."""
     table, lens, cu, pages = layout([1, 35], [40, 50], 16, seed=61)

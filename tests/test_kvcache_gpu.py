@@ -283,6 +283,30 @@ def test_attention(kv, d, dtype, hq, hk, page, window, sinks, ql, kl):
     check_attention(c, pool, q, out, table, qls, kl, window, sinks)
 
 
+@pytest.mark.parametrize("kv,d,dtype,hq,hk,page,window,sinks,ql,kl", [
+    ("Q4_0", 128, "float16", 4, 1, 64, 0, 0, [17], [3001]),
+    ("F16", 128, "bfloat16", 8, 2, 16, 0, 0, [40, 0, 3, 20], [2600, 0, 513, 20]),       # parts of their own number
+    ("Q4_0", 64, "bfloat16", 7, 1, 32, 0, 0, [33, 5], [1025, 4000]),
+    ("F16", 64, "float16", 5, 1, 32, 700, 4, [30, 9], [4000, 3100]),
+    ("Q4_0", 128, "float16", 3, 3, 16, 2000, 70, [20, 90], [30, 4001]),                 # fewer tokens than rows: nothing to see
+])
+def test_few_rows_behind_long_contexts(kv, d, dtype, hq, hk, page, window, sinks, ql, kl):
+    """More rows than a decode step and fewer than fill the device: the keys are split."""
+    kl = [max(k, 0) for k in kl]
+    assert _lib.lib.xm_kv_attention_workspace_size(sum(ql), len(ql), hq, hk, d, max(kl)) > 0
+    dt = getattr(torch, dtype)
+    table, lens, cu, pages = layout(ql, kl, page, seed=14)
+    c, pool = filled_cache(pages, hk, d, page, kv, seed=15)
+    q = (torch.randn(sum(ql) + 2, hq, d, generator=torch.Generator().manual_seed(16)) * 2).to(dt).cuda()
+    out = torch.full_like(q, 7.0)
+    c.attend(q, dev(table), dev(lens), dev(cu), window=window, sinks=sinks, out=out)
+    assert (out[sum(ql):] == 7).all()
+    check_attention(c, pool, q[:-2], out[:-2], table, ql, kl, window, sinks)
+    again = torch.full_like(q, 7.0)
+    c.attend(q, dev(table), dev(lens), dev(cu), window=window, sinks=sinks, out=again)
+    assert torch.equal(out, again) and _lib.lib.xm_device_status(0) == 0
+
+
 @pytest.mark.parametrize("kv", ["Q4_0", "F16"])
 @pytest.mark.parametrize("qscale,kscale", [(1e-4, 1e-3), (30.0, 1.0), (200.0, 50.0), (1.0, 3e-6)])
 def test_attention_magnitudes(kv, qscale, kscale):

@@ -283,10 +283,12 @@ struct SubTile<XM_KV_F16, D> {
 XM_DEV bool non_finite(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
 
 struct DecArgs {
-  int chunk;                // units of a CTA
+  int chunk;                // units of a part, at least
   int nsplit;
   float* part_o;            // [nsplit][T][Hq][D], where a row has more than one part; null: joined in a cluster
   float2* part_ml;
+  // units of each part of n: at least `chunk`, and as many as leave no more than nsplit parts
+  XM_DEV int part_units(int n) const { return max(chunk, (n + nsplit - 1) / nsplit); }
 };
 
 template <typename QT_>
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   if (ts.past_table && threadIdx.x == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
   // parts of da.chunk units that k_kv_merge joins; or, in a cluster, even shares joined through its shared memories
   const bool joined = da.part_o == nullptr && da.nsplit > 1;
-  const int chunk = joined ? (ts.n + da.nsplit - 1) / da.nsplit : da.chunk;
+  const int chunk = joined ? (ts.n + da.nsplit - 1) / da.nsplit : da.part_units(ts.n);
   const int parts = joined ? 1 : (ts.n + chunk - 1) / chunk;
   if (!joined && split > 0 && split >= parts) return;
   const int v_lo = min(ts.n, split * chunk), v_hi = min(ts.n, v_lo + chunk);
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
   sequence_rows(kv, a.T, s, t0, q_len);
   const int gr = (int)(t - t0) * G + h % G;
   const TileSpan ts = tile_span<R, UK>(kv, a, s, t0, q_len, gr / R, G);
-  const int parts = (ts.n + da.chunk - 1) / da.chunk;
+  const int chunk = da.part_units(ts.n), parts = (ts.n + chunk - 1) / chunk;
   if (parts <= 1) return;
   const float2 ml = tid < parts ? __ldcg(&da.part_ml[(int64_t)tid * cells + cell]) : make_float2(-INFINITY, 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -928,15 +930,25 @@ __global__ void __launch_bounds__(128) k_kv_merge(const KvView kv, const AttnArg
 
 struct DecPlan {
   int nt;               // groups of 8 rows per CTA; 0: the prompt kernel
+  int rows;             // of a CTA of the prompt kernel
   int64_t tiles;        // row tiles, at most
-  int chunk, nsplit;      // keys of a part; parts, at most
+  int chunk, nsplit;      // keys of a part (the prompt kernel: at least); parts, at most
   int64_t ws_bytes;
 };
 
 DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, bool ragged) {
   DecPlan p{};
   const int G = Hq / Hk;
-  if (T * G > 16 * B && T > B) return p;
+  if (T * G > 16 * B && T > B) {
+    // 256 rows per CTA, unless that leaves SMs without one; and where half of the SMs have none all the same, the keys
+    // are split (16 rows behind 131071 keys, 8 KV heads, Q4_0: 18 parts take 159 us, one 2289)
+    p.rows = (T * G / 256 + B) * Hk >= 148 ? 256 : 128;
+    p.tiles = T * G / p.rows + B;
+    p.chunk = 512;
+    p.nsplit = (int)std::max<int64_t>(1, std::min({148 / (p.tiles * Hk), (max_keys + 511) / 512, (int64_t)kMaxSplits}));
+    p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * T * Hq * (D * 4 + 8) : 0;
+    return p;
+  }
   p.nt = T * G <= 8 * B ? 1 : 2;
   const int R = 8 * p.nt;
   p.tiles = ragged ? T * G / R + B : B * ((G + R - 1) / R);
@@ -1213,7 +1225,7 @@ XM_DEV bool loader_any(bool p) {                       // over the 128 loader th
 }
 
 template <typename QT_, int D, int KV, int R>
-__global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv, const AttnArgs a) {
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv, const AttnArgs a, const DecArgs da) {
   using Shape = PromptShape<D>;
   constexpr int NG = D / 32;
   constexpr float kLog2e = 1.4426950408889634f;
@@ -1233,7 +1245,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
   if (s < 0) return;
   const TileSpan ts = tile_span<R, kUnit>(kv, a, s, t0, q_len, rt, G);
   if (ts.past_table && tid == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-  const int tiles = ts.rows > 128 ? 2 : 1, n = ts.n;
+  // this CTA's part of the units (a plan of one part takes them all)
+  const int chunk = da.part_units(ts.n), parts = (ts.n + chunk - 1) / chunk, split = blockIdx.y;
+  if (split > 0 && split >= parts) return;
+  const int v_lo = split * chunk, n = min(ts.n, v_lo + chunk) - v_lo;
+  const int tiles = ts.rows > 128 ? 2 : 1;
   const int* table = kv.table + (int64_t)s * kv.table_stride;
   const uint8_t* pool = kv.pool + (int64_t)hk * kv.head_bytes;
   const int64_t page_bytes = kv.head_bytes * kv.Hk, v_part = kv.head_bytes / 2;
@@ -1380,7 +1396,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
         uint32_t kw[D / 8], vw[D / 8], kd[NG / 2], vd[NG / 2];
       };
       const int codes = D / 2 << kv.page_shift;
-      auto key_of_unit = [&](int k) { return ts.unit(min(k, n - 1)) * kUnit + t; };
+      auto key_of_unit = [&](int k) { return ts.unit(v_lo + min(k, n - 1)) * kUnit + t; };
       auto request = [&](const uint8_t* q, int slot, uint32_t (&w)[D / 8], uint32_t (&d)[NG / 2]) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -1471,10 +1487,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
       constexpr int kRowsAtOnce = 128 / P, kIter = 128 / kRowsAtOnce;
       const int c = t % P, r0 = t / P;
       // lane j of a warp holds the page of the unit's keys 16 j ...
-      auto pages_of = [&](int k) { return lane < 8 ? page_of(ts.unit(min(k, n - 1)) * kUnit + 16 * lane) : -1; };
+      auto pages_of = [&](int k) { return lane < 8 ? page_of(ts.unit(v_lo + min(k, n - 1)) * kUnit + 16 * lane) : -1; };
       // the copies of one part of a unit: chunk c of rows r0, r0 + kRowsAtOnce, ...
       auto copy = [&](int k, int pages, int64_t part, uint32_t to, uint32_t& bad) {
-        const int key0 = ts.unit(k) * kUnit;
+        const int key0 = ts.unit(v_lo + k) * kUnit;
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {
           const int r = r0 + i * kRowsAtOnce, key = key0 + r;
@@ -1512,7 +1528,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
           asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         // partly seen units: values that are not finite leave the product
-        const int key0 = ts.unit(k) * kUnit;
+        const int key0 = ts.unit(v_lo + k) * kUnit;
         const bool whole = key0 + kUnit - 1 <= ts.pmin &&
                            (a.window == 0 || key0 > ts.pmax - a.window || key0 + kUnit <= a.sinks);
         if (t < 4) ctl->info[st].bad[t] = ctl->info[st].odd[t] = 0u;
@@ -1556,7 +1572,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     float ref = -INFINITY, l = 0.f;
     bool ok = true;
     for (int u = 0; u < 2 * n; ++u) {
-      const int k = u >> 1, h = u & 1, st = k & 1, key0 = ts.unit(k) * kUnit + 64 * h;
+      const int k = u >> 1, h = u & 1, st = k & 1, key0 = ts.unit(v_lo + k) * kUnit + 64 * h;
       ok = (h == 1 || mbar_wait_soon(&ctl->v_full[st], (k >> 1) & 1)) && mbar_wait_soon(&ctl->s_full[tile][h], k & 1);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -1682,7 +1698,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     if (n > 0 && ok) ok = mbar_wait_soon(&ctl->o_done[tile][1], (n - 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = parts > 1 ? 1.f : l == 0.f ? 0.f : 1.0f / l;
+    if (live && parts > 1) da.part_ml[((int64_t)split * a.T + my_t) * a.Hq + my_h] = make_float2(ref, l);
     QT_* out = (QT_*)a.out + my_t * a.out_stride + (int64_t)my_h * D;
 #pragma unroll 1
     for (int c0 = 0; c0 < D; c0 += 32) {
@@ -1715,7 +1732,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v[8 * b + e]) * inv;
         }
-        if (live) {
+        if (live && parts > 1) {
+          float* const part = da.part_o + (((int64_t)split * a.T + my_t) * a.Hq + my_h) * D + dim;
+          *reinterpret_cast<float4*>(part) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(part + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else if (live) {
           put_out4<QT_>(out + dim, a.out_vec, make_float4(x[0], x[1], x[2], x[3]));
           put_out4<QT_>(out + dim + 4, a.out_vec, make_float4(x[4], x[5], x[6], x[7]));
         }
@@ -1730,7 +1751,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
 }
 
 template <typename QT_, int D, int KV, int R>
-int prompt_kernel(const KvView& kv, const AttnArgs& a, int64_t tiles, cudaStream_t st) {
+int prompt_kernel(const KvView& kv, const AttnArgs& a, const DecArgs& da, int64_t tiles, cudaStream_t st) {
   constexpr int smem = PromptShape<D>::kSmem;
   static bool done[64] = {};
   int dev = 0;
@@ -1740,16 +1761,21 @@ int prompt_kernel(const KvView& kv, const AttnArgs& a, int64_t tiles, cudaStream
     if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return kv_launch("kv attention", k_kv_prompt<QT_, D, KV, R>, dim3((unsigned)(tiles * kv.Hk)), 1, kPromptThreads, smem, st,
-                   kv, a);
+  return kv_launch("kv attention", k_kv_prompt<QT_, D, KV, R>, dim3((unsigned)(tiles * kv.Hk), (unsigned)da.nsplit), 1, kPromptThreads,
+                   smem, st, kv, a, da);
 }
 
 template <typename QT_, int D, int KV>
-int prompt_launch(const KvView& kv, const AttnArgs& a, cudaStream_t st) {
-  // 256 rows per CTA, unless that leaves SMs without one
-  const int64_t rows = a.T * (a.Hq / kv.Hk);
-  if ((rows / 256 + kv.B) * kv.Hk >= 148) return prompt_kernel<QT_, D, KV, 256>(kv, a, rows / 256 + kv.B, st);
-  return prompt_kernel<QT_, D, KV, 128>(kv, a, rows / 128 + kv.B, st);
+int prompt_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* ws, cudaStream_t st) {
+  DecArgs da{p.chunk / kUnit, p.nsplit, nullptr, nullptr};
+  if (p.rows == 256) return prompt_kernel<QT_, D, KV, 256>(kv, a, da, p.tiles, st);
+  if (p.ws_bytes) {
+    da.part_o = (float*)ws;
+    da.part_ml = (float2*)(da.part_o + (int64_t)p.nsplit * a.T * a.Hq * D);
+  }
+  const int rc = prompt_kernel<QT_, D, KV, 128>(kv, a, da, p.tiles, st);
+  if (rc || p.nsplit == 1) return rc;
+  return kv_launch("kv attention merge", k_kv_merge<QT_, D, 128, kUnit>, dim3((unsigned)(a.T * a.Hq)), 1, 128, 0, st, kv, a, da);
 }
 
 template <typename QT_>
@@ -1763,10 +1789,10 @@ int attn_typed(const KvView& kv, const AttnArgs& a, int kv_type, int head_dim, v
                                 : decode_launch<QT_, 64, XM_KV_Q4_0>(kv, a, p, ws, st);
   }
   if (head_dim == 128)
-    return kv_type == XM_KV_F16 ? prompt_launch<QT_, 128, XM_KV_F16>(kv, a, st)
-                                : prompt_launch<QT_, 128, XM_KV_Q4_0>(kv, a, st);
-  return kv_type == XM_KV_F16 ? prompt_launch<QT_, 64, XM_KV_F16>(kv, a, st)
-                              : prompt_launch<QT_, 64, XM_KV_Q4_0>(kv, a, st);
+    return kv_type == XM_KV_F16 ? prompt_launch<QT_, 128, XM_KV_F16>(kv, a, p, ws, st)
+                                : prompt_launch<QT_, 128, XM_KV_Q4_0>(kv, a, p, ws, st);
+  return kv_type == XM_KV_F16 ? prompt_launch<QT_, 64, XM_KV_F16>(kv, a, p, ws, st)
+                              : prompt_launch<QT_, 64, XM_KV_Q4_0>(kv, a, p, ws, st);
 }
 
 }  // namespace

@@ -335,7 +335,7 @@ def test_attention_blocks_of_very_different_scales():
 
 
 @pytest.mark.parametrize("kv", ["Q4_0", "F16"])
-@pytest.mark.parametrize("ql", [None, [3, 2, 0, 40]])
+@pytest.mark.parametrize("ql", [None, [3, 2, 0, 40], [3, 2, 0, 200]])
 def test_rows_that_see_nothing_and_empty_sequences(kv, ql):
     """Empty sequences, and sequences with fewer tokens than rows, give zeros; rows behind the last are left."""
     kl = [0, 1, 70, 5]

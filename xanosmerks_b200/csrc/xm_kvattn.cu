@@ -939,7 +939,10 @@ struct DecPlan {
 DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, bool ragged) {
   DecPlan p{};
   const int G = Hq / Hk;
-  if (T * G > 16 * B && T > B) {
+  // Up to 32 rows (token, query head) of each KV head a sequence: the decode kernel (32 rows of 8 sequences of 8192 keys, 8 KV
+  // heads: 66 us, with the prompt kernel 148; of one sequence 21 and 27).  Above: the prompt kernel (64 rows: 135 and 147,
+  // 33 and 28; behind 131072 keys 313 and 159).
+  if (T * G > 32 * B && T > B) {
     // 256 rows per CTA, unless that leaves SMs without one; and where half of the SMs have none all the same, the keys
     // are split (16 rows behind 131071 keys, 8 KV heads, Q4_0: 18 parts take 159 us, one 2289)
     p.rows = (T * G / 256 + B) * Hk >= 148 ? 256 : 128;

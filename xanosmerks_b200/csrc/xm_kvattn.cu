@@ -37,18 +37,21 @@ struct AttnArgs {
 // split over the warps of a CTA, and over CTAs in chunks of `chunk` keys whose partial softmaxes
 // k_kv_merge joins.
 //
-// Bound: memory (the cache is read once); the work per byte decides whether that is reached.  A warp
+// Bound: memory (the cache is read once); the work per byte decides whether that is reached.  8 sequences of up to
+// 4096 keys in fp16 (8 KV heads): 24.6 us, 0.59 of the copy bandwidth; 64 sequences of up to 8192 in 4 bits: 118 us, 0.52
+// of it, about 340 instructions per 16 keys and head and three CTAs an SM (168 registers a thread; four spill and
+// are slower).  A warp
 // takes 16 keys at a time on mma.sync m16n8k16 (fp16 operands, fp32 sums) with the keys, or the
 // values' dimensions, as the 16 matrix rows and the query rows as the 8 columns:
 //   S^T [16 keys x 8 rows] = K q^T,   O^T [D x 8 rows] += V^T P^T.
-// Operands come from global memory straight into the fragments: the order of the products' inner
-// dimension is free, and the cache's layout was chosen for it.
+// The rows pass through a ring of each warp in shared memory (cp.async) and are read from there as fragments as
+// they lie: the order of the products' inner dimension is free, and the cache's layout was chosen for it.
 //
 // 4-bit rows are never unpacked to values.  The nibbles 0 and 4 (for keys; 0 of two keys, paired by a
 // byte permute, for values) of a word are, after one mask, two fp16 subnormals c 2^-24, the nibbles
 // 1 and 5 are c 2^-20: exact, one instruction for two codes.  For values whole bytes (c + 16 c') 2^-24 and
-// their high nibbles enter, one instruction less, and the low codes' sums are the difference at the end.  The block scale and the offset of the
-// codes stay outside the product:
+// their high nibbles enter, one instruction less, and the low codes' sums are the difference at the end.
+// The block scale and the offset of the codes stay outside the product:
 //   S  = sum over blocks b of d_kb (sum_i q_i c_i - 8 sum_i q_i)       (the offset is the product's
 //        initial accumulator),
 //   O  = sum_k c_k (p_k d_kb) - 8 sum_k p_k d_kb                       (one more product with constants).
@@ -939,12 +942,12 @@ struct DecPlan {
 DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, bool ragged) {
   DecPlan p{};
   const int G = Hq / Hk;
-  // Up to 32 rows (token, query head) of each KV head a sequence: the decode kernel (32 rows of 8 sequences of 8192 keys, 8 KV
-  // heads: 66 us, with the prompt kernel 148; of one sequence 21 and 27).  Above: the prompt kernel (64 rows: 135 and 147,
-  // 33 and 28; behind 131072 keys 313 and 159).
+  // Up to 32 rows (token, query head) of each KV head a sequence: the decode kernel (32 rows each of 8 sequences of
+  // 8192 keys, 8 KV heads: 66 us, with the prompt kernel 148; of one sequence 21 and 27).  Above: the prompt kernel
+  // (64 rows each: decode 135, prompt 147; of one sequence 33 and 28, behind 131072 keys 313 and 159).
   if (T * G > 32 * B && T > B) {
-    // 256 rows per CTA, unless that leaves SMs without one; and where half of the SMs have none all the same, the keys
-    // are split (16 rows behind 131071 keys, 8 KV heads, Q4_0: 18 parts take 159 us, one 2289)
+    // 256 rows per CTA, unless that leaves SMs without one; and where half of the SMs have none all the same, the
+    // keys are split (64 rows of each of 8 KV heads behind 131072 keys, Q4_0: 18 parts take 159 us, one 2289)
     p.rows = (T * G / 256 + B) * Hk >= 148 ? 256 : 128;
     p.tiles = T * G / p.rows + B;
     p.chunk = 512;
@@ -1036,14 +1039,17 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // O of tile i at 256 + D i.
 //
 // What decides the speed is the chain of one row tile: a row of S is read once, 64 columns into registers (a
-// tcgen05.wait::ld waits for every load, and costs some 300 clocks), its maximum taken, P computed.  With
-// units of 128 keys and P over a single S the chain of a unit was 6100 clocks (PV and S follow one another in it);
-// a 8192-token prompt took 790 us.
+// tcgen05.wait::ld waits for every load, and costs some 300 clocks), its maximum taken, P computed.  A prompt of
+// 8192 tokens (32 query and 8 KV heads of 128, 4 bits) took 790 us with units of 128 keys and one S per row tile
+// (PV and S follow one another in the chain: 6100 clocks a unit), 779 with half units and two S, 760 with the products
+// issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma): 738 TFLOP/s.
 //
 // 4-bit rows become fp16 here, d (c - 8) rounded once (2^-11): a product per code would need the scales
 // inside the tensor core's inner dimension.  The order of the eight values that a word of keys yields is
 // kept, and q's is changed to it; the order of a word of values is a permutation of O's columns, undone
 // when O is written.  A unit with a scale above 4096 (values past fp16's range) is scaled by 2^-4.
+// Norm-wise, over thousands of normal keys, the roundings to fp16 put the outputs off by 1.8e-4 (keys), 1.6e-4 (values)
+// and 2.1e-4 (P), 3.3e-4 together; the rounding of an fp16 output alone is 2.0e-4.
 //
 // The running reference of a row moves only when a score passes it by 8 (P <= 2^8), so O, which stays in
 // tensor memory, is rescaled seldom.
@@ -1051,8 +1057,9 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // Masked keys: their scores are replaced, their values are zeros where no row sees them; a value that is not
 // finite and that only some rows see is taken out of the product and added to those rows alone.
 //
-// Bound: the products (4 R 128 D flops a unit at the tensor peak) and, as much, the 128 R exponentials
-// (16 a clock); the loaders' and the softmax's other instructions fit beside them.
+// Bound: the products (4 R 128 D flops a unit at the tensor peak: 2048 clocks a unit of R = 256, D = 128) and, as much, the 128 R exponentials (16 a clock: 2048 clocks a unit); neither is reached, since a
+// row tile's chain (some 5000 clocks a unit: waits 800, maximum 1200, exponentials and rounding 2200, loads and stores of
+// tensor memory 700) is only halved by the other's.
 // ---------------------------------------------------------------------------
 constexpr int kUnit = 128;                         // keys of a unit
 constexpr int kPromptThreads = 14 * 32;

@@ -110,7 +110,7 @@ class PagedKVCache:
     def _out(self, out, rows, heads, dtype):
         """(out, its row pitch): a new tensor [rows, heads, head_dim], or the caller's, checked."""
         if out is None:
-            return torch.empty((rows, heads, self.head_dim), dtype=dtype, device=self.device), heads * self.head_dim
+            return self.pool.new_empty((rows, heads, self.head_dim), dtype=dtype), heads * self.head_dim
         if tuple(out.shape) != (rows, heads, self.head_dim) or out.dtype != dtype or out.device != self.device:
             raise ValueError(f"out must be {dtype} {(rows, heads, self.head_dim)} on {self.device}, got {out.dtype} "
                              f"{tuple(out.shape)} on {out.device}")
@@ -177,8 +177,8 @@ class PagedKVCache:
             raise ValueError("read: num_tokens (the number of rows) is needed with cu_seqlens")
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
         # rows behind the last sequence stay zeros
-        make = torch.empty if cu_seqlens is None else torch.zeros
-        k, v = make((2, rows, self.num_kv_heads, self.head_dim), dtype=torch.float16, device=self.device).unbind(0)
+        make = self.pool.new_empty if cu_seqlens is None else self.pool.new_zeros
+        k, v = make((2, rows, self.num_kv_heads, self.head_dim), dtype=torch.float16).unbind(0)
         check(call_on(self.device, lib.xm_kv_read, self.pool.data_ptr(), self.num_pages, self._kv, self.num_kv_heads,
                       self.head_dim, self.page_size, *where, rows, k.data_ptr(), v.data_ptr()), "kv read")
         return k, v
@@ -202,7 +202,10 @@ class PagedKVCache:
             raise ValueError("attend: window and sinks must not be negative")
         pitch = self._pitch(q, "attend: q")
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
-        o, o_pitch = self._out(out, rows, heads, q.dtype)
+        if out is None and q.is_contiguous():
+            o, o_pitch = torch.empty_like(q), heads * d
+        else:
+            o, o_pitch = self._out(out, rows, heads, q.dtype)
         need = _workspace_size(rows, where[5], heads, hk, d, where[2] * self.page_size)
         # a workspace for each call: two captured graphs, or two streams, never share one
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

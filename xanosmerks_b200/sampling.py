@@ -53,10 +53,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     p, pp = _per_row(top_p, "top_p", torch.float32, b, dev)
     m, mp = _per_row(min_p, "min_p", torch.float32, b, dev)
     if out is None:
-        out = torch.empty(b, dtype=torch.int32, device=dev)
+        out = u.new_empty(b, dtype=torch.int32)
     else:
         _per_row(out, "out", torch.int32, b, dev)
-    logp = torch.empty(b, dtype=torch.float32, device=dev)
+    logp = torch.empty_like(u)
     check(call_on(dev, lib.xm_sample, logits.data_ptr(), dt, b, v, pitch if b > 1 else v, up, t, tp, k, kp, p, pp, m,
                   mp, out.data_ptr(), logp.data_ptr()), "sample")
     return out, logp

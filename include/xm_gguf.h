@@ -363,7 +363,7 @@ int xm_argmax(const float* d_logits, int64_t B, int64_t V, int* d_out, void* str
  * xm_kv_read: the cached keys and values of the rows as fp16 [T][Hk][D].
  *
  * xm_kv_attention: out row t (type and head layout of q) =
- * softmax(q K^T scale) V per query head over the positions 0 .. p of its
+ * softmax(q K^T scale) V (scale finite) per query head over the positions 0 .. p of its
  * sequence, p the row's own (with window > 0: positions above p - window and
  * the first `sinks` ones); Hq / Hk <= 64 query heads per KV head; a row that
  * sees no key is zeros.  d_ws: xm_kv_attention_workspace_size bytes (max_keys =

@@ -70,7 +70,8 @@ def test_append_arguments_are_refused(kw):
 
 @pytest.mark.parametrize("kw", [dict(hq=31), dict(hq=0), dict(hq=520), dict(dt=0), dict(stride=4095), dict(ostride=4095), dict(q=None),
                                 dict(out=None), dict(window=-1), dict(sinks=-1), dict(ws=None, width=4096), dict(wsb=4096, width=4096),
-                                dict(ws=P + 8, width=4096), dict(q=P + 1)])
+                                dict(ws=P + 8, width=4096), dict(q=P + 1),
+                                dict(scale=float("nan")), dict(scale=float("inf"))])
 def test_attention_arguments_are_refused(kw):
     assert attend(**kw) == _lib.XM_ERR_INVALID, kw
 

@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "xm_kv.cuh"
@@ -944,10 +945,10 @@ DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, 
   const int G = Hq / Hk;
   // Up to 32 rows (token, query head) of each KV head a sequence: the decode kernel (32 rows each of 8 sequences of
   // 8192 keys, 8 KV heads: 66 us, with the prompt kernel 148; of one sequence 21 and 27).  Above: the prompt kernel
-  // (64 rows each: decode 135, prompt 147; of one sequence 33 and 28, behind 131072 keys 313 and 159).
+  // (64 rows each: decode 135, prompt 140; of one sequence 33 and 28, behind 131072 keys 313 and 142).
   if (T * G > 32 * B && T > B) {
     // 256 rows per CTA, unless that leaves SMs without one; and where half of the SMs have none all the same, the
-    // keys are split (64 rows of each of 8 KV heads behind 131072 keys, Q4_0: 18 parts take 159 us, one 2289)
+    // keys are split (64 rows of each of 8 KV heads behind 131072 keys, Q4_0: 18 parts take 142 us, one 2289)
     p.rows = (T * G / 256 + B) * Hk >= 148 ? 256 : 128;
     p.tiles = T * G / p.rows + B;
     p.chunk = 512;
@@ -1042,7 +1043,10 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // tcgen05.wait::ld waits for every load, and costs some 300 clocks), its maximum taken, P computed.  A prompt of
 // 8192 tokens (32 query and 8 KV heads of 128, 4 bits) took 790 us with units of 128 keys and one S per row tile
 // (PV and S follow one another in the chain: 6100 clocks a unit), 779 with half units and two S, 760 with the products
-// issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma): 738 TFLOP/s.
+// issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma), 730 with one body
+// for masked and whole units (no spills): 753 TFLOP/s.  Four chunks of up to 1000 tokens behind up to 5000, window 1024,
+// sinks, fp16, 28 query and 4 KV heads of 64: 92 us with two to five instructions a column for the mask, 76 with a
+// word of its bits.
 //
 // 4-bit rows become fp16 here, d (c - 8) rounded once (2^-11): a product per code would need the scales
 // inside the tensor core's inner dimension.  The order of the eight values that a word of keys yields is
@@ -1212,7 +1216,8 @@ XM_DEV bool elect_one() {
 
 // 2^y on the multipliers: y = k + r, |r| <= 1/2, Taylor's polynomial of degree 5 (2.4e-6 of the value; the weights are
 // rounded to fp16).  A quarter of a unit's weights this way takes 5% off the kernel (8192 tokens, 736 -> 705 us); with
-// a half it is slower than with none.  NaN stays NaN; below 2^-126 it is 2^-126.
+// a half it is slower than with none.  NaN stays NaN; below 2^-126 it is 2^-126 (a weight of 0 in fp16, and nothing in
+// a sum whose largest term is at least 2^-8).
 XM_DEV float2 ex2_fma(float2 y) {
   auto both = [](float v) { return make_float2(v, v); };
   asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n max.NaN.f32 %1, %1, 0fC2FC0000;" : "+f"(y.x), "+f"(y.y));
@@ -1226,6 +1231,9 @@ XM_DEV float2 ex2_fma(float2 y) {
   return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(k.x) << 23) + 0x3f800000u),
                                    __uint_as_float((__float_as_uint(k.y) << 23) + 0x3f800000u)));
 }
+
+// the lowest n of 64 bits (any n)
+XM_DEV uint64_t below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 XM_DEV bool loader_any(bool p) {                       // over the 128 loader threads
   uint32_t r;
@@ -1319,7 +1327,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     }
     const int sh = fp16_row_shift(mx);
     const float down = a.scale < 0.f ? -ldexpf(1.f, -sh) : ldexpf(1.f, -sh);
-    q_f = ldexpf(fabsf(a.scale) * kLog2e, sh);
+    q_f = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, sh), 1.1754944e-38f);
 #pragma unroll 1
     for (int c0 = 0; c0 < D / 8; c0 += 8) {
       if (D > 64) read(c0);
@@ -1600,15 +1608,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
       const uint32_t bad0 = info.bad[2 * h], bad1 = info.bad[2 * h + 1], any_odd = info.odd[2 * h] | info.odd[2 * h + 1];
       const bool whole = !(bad0 | bad1) && key0 + 63 <= pmin &&
                          (a.window == 0 || key0 > pmax - a.window || key0 + 64 <= a.sinks);
-      const float f = info.k_exp ? q_f * 16.f : q_f;
+      const float f = info.k_exp ? q_f * 16.f : q_f;    // never 0: hidden scores stay -inf
       // columns hi .. and, with a window, sk .. lo are hidden from this row
       const int hi = pos - key0, lo = a.window > 0 ? pos - a.window - key0 : -1, sk = a.window > 0 ? a.sinks - key0 : 0;
       tmem_ld_wait();
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (!whole) {
+        // a bit for each column that this row sees: two instructions a column
+        const uint64_t seen = below(hi + 1) & ~(below(lo + 1) & ~below(sk)) & ~((uint64_t)bad1 << 32 | bad0);
+        const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
         for (int c = 0; c < 64; ++c)
-          if (c > hi || (c <= lo && c >= sk) || ((c < 32 ? bad0 : bad1) >> (c & 31) & 1u)) v[c] = 0xff800000u;
+          if (!((c < 32 ? s0 : s1) & 1u << (c & 31))) v[c] = 0xff800000u;
       }
 #pragma unroll
       for (int i = 0; i < 64; i += 8)
@@ -1682,22 +1693,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
       const float at = ref == -INFINITY ? 0.f : ref, down = info.v_exp ? 4.f - at : -at;
       const float2 ff = make_float2(f, f), sh = make_float2(down, down);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-      auto weights = [&](auto whole_) {
-        constexpr bool kWhole = decltype(whole_)::value;
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), ff, sh);
-          float2 z;                                    // one pair of four without the function unit
-          if (kWhole && i % 8 == 6) z = ex2_fma(y); else z = make_float2(ex2(y.x), ex2(y.y));
-          if constexpr (!kWhole) {                     // (f may be 0)
-            if (v[i] == 0xff800000u) z.x = 0.f;
-            if (v[i + 1] == 0xff800000u) z.y = 0.f;
-          }
-          if (i & 2) s1 = __fadd2_rn(s1, z); else s0 = __fadd2_rn(s0, z);
-          v[i >> 1] = half2_bits(z.x, z.y);
-        }
-      };
-      if (whole) weights(std::true_type{}); else weights(std::false_type{});
+      for (int i = 0; i < 64; i += 2) {
+        const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), ff, sh);
+        // one pair of four without the function unit
+        const float2 z = i % 8 == 6 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
+        if (i & 2) s1 = __fadd2_rn(s1, z); else s0 = __fadd2_rn(s0, z);
+        v[i >> 1] = half2_bits(z.x, z.y);
+      }
       tmem_st32(t_s + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
       l = fmaf((s0.x + s0.y) + (s1.x + s1.y), info.v_exp ? 0.0625f : 1.f, l);
       tmem_st_wait();
@@ -1708,7 +1711,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
     if (n > 0 && ok) ok = mbar_wait_soon(&ctl->o_done[tile][1], (n - 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    const float inv = parts > 1 ? 1.f : l == 0.f ? 0.f : 1.0f / l;
+    const float inv = parts > 1 ? 1.f : ref == -INFINITY ? 0.f : 1.0f / l;
     if (live && parts > 1) da.part_ml[((int64_t)split * a.T + my_t) * a.Hq + my_h] = make_float2(ref, l);
     QT_* out = (QT_*)a.out + my_t * a.out_stride + (int64_t)my_h * D;
 #pragma unroll 1
@@ -1831,6 +1834,7 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
   if (q_dtype != XM_DT_F16 && q_dtype != XM_DT_BF16)
     return xm_set_error(XM_ERR_INVALID, "kv_attention: queries are fp16 or bf16, not type %d", q_dtype);
   if (window < 0 || sinks < 0) return xm_set_error(XM_ERR_INVALID, "kv_attention: negative window or sinks");
+  if (!std::isfinite(scale)) return xm_set_error(XM_ERR_INVALID, "kv_attention: the scale is not finite");
   if (T == 0) return XM_OK;
   if (!d_q || !d_out) return xm_set_error(XM_ERR_INVALID, "kv_attention: null pointer");
   if (q_stride < (int64_t)Hq * head_dim || out_stride < (int64_t)Hq * head_dim || (((uintptr_t)d_q | (uintptr_t)d_out) & 1))

@@ -17,7 +17,7 @@
 // the memory traffic); everything else is fp32.
 //
 // Bound: memory for prompts by the bytes, instructions in fact (normalisation and rotation of keys in 64 bits, the exact
-// decisions of codes: eight prompts of up to 2048 tokens, normalised heads, 4 bits: 91 us, nearly twice what the bytes take, with four CTAs an SM, 94 with three; the
+// decisions of codes: eight prompts of up to 2048 tokens, normalised heads, 4 bits: 90 us, nearly twice what the bytes take, with four CTAs an SM, 94 with three; the
 // read 19), latency for single tokens.  D / 8 lanes take a head, so a warp two heads
 // of 128 or four of 64: lane l of them holds the values 4 l .. 4 l + 3 of each half, so the rotation
 // needs no exchange, loads and stores are 8 or 16 bytes, and a block of 32 values is 8 lanes.  A

@@ -1044,7 +1044,7 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // 8192 tokens (32 query and 8 KV heads of 128, 4 bits) took 790 us with units of 128 keys and one S per row tile
 // (PV and S follow one another in the chain: 6100 clocks a unit), 779 with half units and two S, 760 with the products
 // issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma), 730 with one body
-// for masked and whole units (no spills): 753 TFLOP/s.  Four chunks of up to 1000 tokens behind up to 5000, window 1024,
+// for masked and whole units (no spills), 727 with an eighth of them there: 756 TFLOP/s.  Four chunks of up to 1000 tokens behind up to 5000, window 1024,
 // sinks, fp16, 28 query and 4 KV heads of 64: 92 us with two to five instructions a column for the mask, 76 with a
 // word of its bits.
 //
@@ -1215,8 +1215,8 @@ XM_DEV bool elect_one() {
 }
 
 // 2^y on the multipliers: y = k + r, |r| <= 1/2, Taylor's polynomial of degree 5 (2.4e-6 of the value; the weights are
-// rounded to fp16).  A quarter of a unit's weights this way takes 5% off the kernel (8192 tokens, 736 -> 705 us); with
-// a half it is slower than with none.  NaN stays NaN; below 2^-126 it is 2^-126 (a weight of 0 in fp16, and nothing in
+// rounded to fp16).  With an eighth of the weights this way 8192 tokens take 677 us, with none 692, a quarter 688, three
+// eighths 678.  NaN stays NaN; below 2^-126 it is 2^-126 (a weight of 0 in fp16, and nothing in
 // a sum whose largest term is at least 2^-8).
 XM_DEV float2 ex2_fma(float2 y) {
   auto both = [](float v) { return make_float2(v, v); };
@@ -1696,8 +1696,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(const KvView kv
 #pragma unroll
       for (int i = 0; i < 64; i += 2) {
         const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), ff, sh);
-        // one pair of four without the function unit
-        const float2 z = i % 8 == 6 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
+        // one pair of eight without the function unit
+        const float2 z = i % 16 == 6 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
         if (i & 2) s1 = __fadd2_rn(s1, z); else s0 = __fadd2_rn(s0, z);
         v[i >> 1] = half2_bits(z.x, z.y);
       }

@@ -527,6 +527,43 @@ def test_two_streams_and_a_captured_graph():
         assert torch.equal(graphs[0][1], want[0]) and torch.equal(graphs[1][1], want[1])
 
 
+def test_split_prompts_on_two_streams_and_in_graphs():
+    """More rows than a step, keys in parts: each call has its own workspace, in graphs too, and a replay follows the
+    lengths on the device."""
+    ql, kl = [40, 30], [3000, 1500]
+    table, lens, cu, pages = layout(ql, kl, 64, seed=94)
+    tb, ln, co = dev(table), dev(lens), dev(cu)
+    c, _ = filled_cache(pages, 1, 128, 64, "Q4_0", seed=95)
+    assert _lib.lib.xm_kv_attention_workspace_size(70, 2, 4, 1, 128, table.shape[1] * 64) > 0
+    qa = torch.randn(70, 4, 128, generator=torch.Generator().manual_seed(96)).half().cuda()
+    qb = (qa * 0.5).contiguous()
+    want = c.attend(qa, tb, ln, co), c.attend(qb, tb, ln, co)
+    torch.cuda.synchronize()
+    streams, got = (torch.cuda.Stream(), torch.cuda.Stream()), []
+    for _ in range(5):
+        for st, q, w in zip(streams, (qa, qb), want):
+            with torch.cuda.stream(st):
+                got.append((c.attend(q, tb, ln, co), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for x, w in got)
+    graphs = []
+    for st, q in zip(streams, (qa, qb)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            graphs.append((g, c.attend(q, tb, ln, co)))
+    shorter = c.attend(qa, tb, ln - 700, co)
+    for less, expect in ((0, want[0]), (700, shorter)):
+        ln.copy_(dev(lens) - less)
+        torch.cuda.synchronize()
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], expect)
+        if not less:
+            assert torch.equal(graphs[1][1], want[1])
+
+
 @pytest.mark.parametrize("kv,norm", [("Q4_0", True), ("F16", False)])
 def test_prompt_then_steps_as_a_decoder_uses_them(kv, norm):
     """Append a prompt, attend, then append and attend token by token: the same rows as attending everything

@@ -191,3 +191,27 @@ def test_infinite_logits_among_many(count):
         want = at[np.minimum(np.floor(un * kept).astype(int), kept - 1)]
         assert (ids.cpu().numpy() == want).all(), kw
         assert (logp.cpu() + np.log(kept)).abs().max() <= 1e-6
+
+
+def test_two_streams_and_a_captured_call():
+    x, u = make(20, 33000, seed=101)
+    kw = dict(temperature=0.9, top_p=0.95)
+    want = sample(x, u, **kw), sample(x, u, top_k=40, **kw)
+    streams, got = (torch.cuda.Stream(), torch.cuda.Stream()), []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, w, k in zip(streams, want, (0, 40)):
+            with torch.cuda.stream(st):
+                got.append((sample(x, u, top_k=k, **kw), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in got for a, b in zip(g, w))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=streams[0]):
+        ids, logp = sample(x, u, **kw)
+    y, un = make(20, 33000, seed=102)
+    x.copy_(y), u.copy_(un)
+    g.replay()
+    torch.cuda.synchronize()
+    now = sample(x, u, **kw)
+    assert torch.equal(ids, now[0]) and torch.equal(logp, now[1])
+    compare(x, u, **kw)

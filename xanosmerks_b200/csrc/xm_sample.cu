@@ -214,6 +214,14 @@ struct Sampler {
   XM_DEV void sync() {
     if (C > 1) cl.sync(); else __syncthreads();
   }
+  // A CTA's shared memory may be accessed by the others of its cluster once it has started: every CTA says so first,
+  // and waits for the others in front of the first exchange (the load of the row lies between).
+  XM_DEV void started() const {
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;");
+  }
+  XM_DEV void wait_started() const {
+    if (C > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+  }
 
   // inclusive sum of v over the CTA's threads; sum: over all of them
   XM_DEV u64 scan(u64 v, u64* per_warp, u64& sum) {
@@ -509,6 +517,7 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
   grid_dep_wait();
   grid_dep_launch();
   Sampler<XT, NT, RES> s(a, sm, reinterpret_cast<XT*>(sample_smem + sizeof(SampleSmem)));
+  s.started();
   const int b = (int)(blockIdx.x / s.C), tid = threadIdx.x;
   const float T = a.d_temperature ? a.d_temperature[b] : a.temperature;
   const int top_k = a.d_top_k ? a.d_top_k[b] : a.top_k;
@@ -547,6 +556,7 @@ __global__ void __launch_bounds__(NT, 2) k_sample(const SampleArgs a) {
     if (group[e] > -INFINITY) least = fminf(least, group[e]);
   }
   unsigned st[4] = {order_key(mx), real ? ~order_key(mn) : 0u, real, mx > -INFINITY ? ~order_key(least) : 0u};
+  s.wait_started();
   s.all(st, {1, 1, 0, 1});
   if (st[0] == 0) {                                               // nothing to choose from (the whole cluster)
     if (s.rank == 0 && tid == 0) {

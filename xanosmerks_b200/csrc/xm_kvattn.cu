@@ -402,7 +402,13 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     return at < kv.table_width ? __ldg(table + at) : -1;
   };
   int pages = page_of(lane, 0), pages_next = steps > 32 ? page_of(32 + lane, 0) : 0;
-  unsigned bad_steps = 0;                              // bit i: the step i % 32 has a page outside the pool
+  // Bits SUB i + j (mod 32): subtile j of step i lies on a page outside the pool that some row needs.  (A page whose keys no
+  // row sees, behind a window, may be gone: its bytes are masked like those of any other hidden key.)
+  unsigned bad_tiles = 0;
+  constexpr unsigned kTiles = (1u << SUB) - 1;
+  auto needed = [&](int key, int keys) {               // whether any row sees one of the keys from `key` on
+    return key <= ts.pmax && (a.window == 0 || key + keys - 1 > ts.pmin - a.window || key < a.sinks);
+  };
   auto fetch = [&](int i) {                            // starts the copies of step i
     if (i < steps) {
       if (i > 0 && (i & 31) == 0) {
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
         pages_next = page_of(i + 32 + lane, 0);
       }
       const int key0 = ts.unit(v_lo + warp + i * kDecWarps) * UK;
-      bad_steps &= ~(1u << (i & 31));
+      bad_tiles &= ~(kTiles << (SUB * i & 31));
       const uint8_t* head;
       const uint32_t to = ring + i % STAGES * (SUB * Sub::kBytes);
 #pragma unroll
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
           int p = __shfl_sync(0xffffffffu, pages, i & 31);
           if (j > 0) p = page_of(i, j);
           const bool in = (unsigned)p < (unsigned)kv.pages;
-          if (!in && (j == 0 || key0 + 16 * j <= ts.pmax)) bad_steps |= 1u << (i & 31);
+          if (!in && needed(key0 + 16 * j, one_page ? UK : 16)) bad_tiles |= (one_page ? kTiles : 1u << j) << (SUB * i & 31);
           head = pool + (in ? p : 0) * page_bytes;
         }
         const int slot = key0 + 16 * j & page_mask;
@@ -515,8 +521,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
   for (int i = 0; i < 4; ++i) asm volatile("mov.u32 %0, 0x00080008;" : "=r"(eights[i]));
 
-  // One step of UK keys from key0 on.  FULL: every row sees every one of them.
-  auto step = [&](auto full_, int key0, uint32_t at, bool hidden) {
+  // One step of UK keys from key0 on.  FULL: every row sees every one of them; hidden: a bit for each subtile without a page.
+  auto step = [&](auto full_, int key0, uint32_t at, unsigned hidden) {
     constexpr bool FULL = decltype(full_)::value;
     Sub tile[SUB];
     float sc[NT][SUB][4];
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     auto any_sees = [&](int j, int row) {
       if (FULL) return true;
       const int key = key0 + 16 * j + row;
-      return !hidden && key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
+      return !(hidden >> j & 1u) && key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
     };
     int e = 0;                                         // |d| < 2^e for every block scale of the step
     if constexpr (KV == XM_KV_Q4_0) {
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = key0 + 16 * j + key_of(r) + 8 * (i >> 1);
-            if (hidden || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
+            if ((hidden >> j & 1u) || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
           }
       }
       float want[2];
@@ -750,12 +756,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   for (int i = 0; i < steps; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                      // step i has landed, and every lane is done with step i - 1
-    const bool hidden = bad_steps >> (i & 31) & 1u;
+    const unsigned hidden = bad_tiles >> (SUB * i & 31) & kTiles;
     fetch(i + STAGES - 1);
     const int v = v_lo + warp + i * kDecWarps, key0 = ts.unit(v) * UK;
     const uint32_t at = ring + i % STAGES * (SUB * Sub::kBytes);
     if (hidden && lane == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-    if (!hidden && ((v >= fa && v < fb) || v < fs)) step(std::true_type{}, key0, at, false);
+    if (!hidden && ((v >= fa && v < fb) || v < fs)) step(std::true_type{}, key0, at, 0u);
     else step(std::false_type{}, key0, at, hidden);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -324,7 +324,9 @@ struct DecShape {
   static constexpr int kCtas = NT > 1 ? 2 : KV == XM_KV_Q4_0 || D == 64 ? 3 : 2;          // of an SM
 };
 
-template <typename QT_, int D, int KV, int NT>
+// ONE_PAGE: a step's unit lies in one page (else in two of 16 tokens, and each is looked up; chosen at run time that costs
+// the other page sizes 2 to 4 %: 64 sequences of up to 8192 tokens in 4 bits 121 to 123 us, this way 117).
+template <typename QT_, int D, int KV, int NT, bool ONE_PAGE>
 __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_kv_decode(const KvView kv,
                                                                                           const AttnArgs a,
                                                                                           const DecArgs da) {
@@ -369,7 +371,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   }
 
   const int page_mask = (1 << kv.page_shift) - 1;
-  const bool one_page = UK == 16 || kv.page_shift >= 5;   // a unit lies in one page (or in two of 16 tokens)
   const int* table = kv.table + (int64_t)s * kv.table_stride;
   const uint8_t* pool = kv.pool + (int64_t)hk * kv.head_bytes;
   const int64_t page_bytes = kv.head_bytes * kv.Hk, v_part = kv.head_bytes / 2;
@@ -402,12 +403,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     return at < kv.table_width ? __ldg(table + at) : -1;
   };
   int pages = page_of(lane, 0), pages_next = steps > 32 ? page_of(32 + lane, 0) : 0;
-  // Bits SUB i + j (mod 32): subtile j of step i lies on a page outside the pool that some row needs.  (A page whose keys no
-  // row sees, behind a window, may be gone: its bytes are masked like those of any other hidden key.)
-  unsigned bad_tiles = 0;
-  constexpr unsigned kTiles = (1u << SUB) - 1;
-  auto needed = [&](int key, int keys) {               // whether any row sees one of the keys from `key` on
-    return key <= ts.pmax && (a.window == 0 || key + keys - 1 > ts.pmin - a.window || key < a.sinks);
+  // Bit i: step i % 32 lies on a page outside the pool (the second of its pages: in bad_second), unless no row sees a key
+  // of that page.  (Such a page, behind a window, may be gone: its bytes are masked like those of any hidden key.)
+  unsigned bad = 0, bad_second = 0;
+  auto needed = [&](int key) {                         // whether any row sees one of 16 keys (a whole unit has one)
+    return ONE_PAGE || (key <= ts.pmax && (a.window == 0 || key + 15 > ts.pmin - a.window || key < a.sinks));
   };
   auto fetch = [&](int i) {                            // starts the copies of step i
     if (i < steps) {
@@ -416,16 +416,17 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
         pages_next = page_of(i + 32 + lane, 0);
       }
       const int key0 = ts.unit(v_lo + warp + i * kDecWarps) * UK;
-      bad_tiles &= ~(kTiles << (SUB * i & 31));
+      bad &= ~(1u << (i & 31));
+      if (!ONE_PAGE) bad_second &= ~(1u << (i & 31));
       const uint8_t* head;
       const uint32_t to = ring + i % STAGES * (SUB * Sub::kBytes);
 #pragma unroll
       for (int j = 0; j < SUB; ++j) {
-        if (j == 0 || !one_page) {
+        if (j == 0 || !ONE_PAGE) {
           int p = __shfl_sync(0xffffffffu, pages, i & 31);
           if (j > 0) p = page_of(i, j);
           const bool in = (unsigned)p < (unsigned)kv.pages;
-          if (!in && needed(key0 + 16 * j, one_page ? UK : 16)) bad_tiles |= (one_page ? kTiles : 1u << j) << (SUB * i & 31);
+          if (!in && needed(key0 + 16 * j)) (j ? bad_second : bad) |= 1u << (i & 31);
           head = pool + (in ? p : 0) * page_bytes;
         }
         const int slot = key0 + 16 * j & page_mask;
@@ -521,8 +522,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
   for (int i = 0; i < 4; ++i) asm volatile("mov.u32 %0, 0x00080008;" : "=r"(eights[i]));
 
-  // One step of UK keys from key0 on.  FULL: every row sees every one of them; hidden: a bit for each subtile without a page.
-  auto step = [&](auto full_, int key0, uint32_t at, unsigned hidden) {
+  // One step of UK keys, its subtiles' from first.x and first.y on (kNoKeys: without a page).  FULL: every row sees every
+  // one of them.
+  constexpr int kNoKeys = 0x7fffffff - 64;             // behind every position
+  auto step = [&](auto full_, int2 first, uint32_t at) {
+    const int keys[2] = {first.x, first.y};
     constexpr bool FULL = decltype(full_)::value;
     Sub tile[SUB];
     float sc[NT][SUB][4];
@@ -576,8 +580,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
     // whether any row sees key `at` of subtile j
     auto any_sees = [&](int j, int row) {
       if (FULL) return true;
-      const int key = key0 + 16 * j + row;
-      return !(hidden >> j & 1u) && key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
+      const int key = keys[j] + row;
+      return key <= ts.pmax && (a.window == 0 || key > ts.pmin - a.window || key < a.sinks);
     };
     int e = 0;                                         // |d| < 2^e for every block scale of the step
     if constexpr (KV == XM_KV_Q4_0) {
@@ -599,8 +603,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
         for (int j = 0; j < SUB; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * j + key_of(r) + 8 * (i >> 1);
-            if ((hidden >> j & 1u) || !sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
+            const int key = keys[j] + key_of(r) + 8 * (i >> 1);
+            if (!sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
           }
       }
       float want[2];
@@ -722,7 +726,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
                 const float pc[2] = {key < 8 ? a0 : a2, key < 8 ? a1 : a3};
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  if (sees(a, pos[nt][c], key0 + key))
+                  if (sees(a, pos[nt][c], keys[j] + key))
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                       o[nt][i][c] = fmaf(pc[c], half_of(vw[i / 4][i % 4], 0), o[nt][i][c]);
@@ -756,13 +760,15 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
   for (int i = 0; i < steps; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                      // step i has landed, and every lane is done with step i - 1
-    const unsigned hidden = bad_tiles >> (SUB * i & 31) & kTiles;
-    fetch(i + STAGES - 1);
     const int v = v_lo + warp + i * kDecWarps, key0 = ts.unit(v) * UK;
-    const uint32_t at = ring + i % STAGES * (SUB * Sub::kBytes);
+    const bool hide_x = bad >> (i & 31) & 1u, hide_y = ONE_PAGE ? hide_x : bad_second >> (i & 31) & 1u;
+    const bool hidden = hide_x || hide_y;
+    const int2 first = make_int2(hide_x ? kNoKeys : key0, hide_y ? kNoKeys : key0 + 16);
     if (hidden && lane == 0) atomicOr(&g_xm_device_error, XM_DEVERR_PAGE);
-    if (!hidden && ((v >= fa && v < fb) || v < fs)) step(std::true_type{}, key0, at, 0u);
-    else step(std::false_type{}, key0, at, hidden);
+    fetch(i + STAGES - 1);
+    const uint32_t at = ring + i % STAGES * (SUB * Sub::kBytes);
+    if (!hidden && ((v >= fa && v < fb) || v < fs)) step(std::true_type{}, first, at);
+    else step(std::false_type{}, first, at);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();                                     // the ring's memory is free
@@ -1000,18 +1006,18 @@ int kv_launch(const char* what, void (*kernel)(KArgs...), dim3 grid, int cluster
   return xm_check_launch(what);
 }
 
-template <typename QT_, int D, int KV, int NT>
+template <typename QT_, int D, int KV, int NT, bool ONE_PAGE>
 int decode_kernel(const KvView& kv, const AttnArgs& a, const DecArgs& da, dim3 grid, cudaStream_t st) {
   constexpr int smem = DecShape<KV, D, NT>::kSmem;
   static bool done[64] = {};                           // the attribute is set once per device
   int dev = 0;
   cudaGetDevice(&dev);
   if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || !done[dev])) {
-    const cudaError_t e = cudaFuncSetAttribute(k_kv_decode<QT_, D, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(k_kv_decode<QT_, D, KV, NT, ONE_PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "kv attention: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return kv_launch("kv attention", k_kv_decode<QT_, D, KV, NT>, grid, da.part_o ? 1 : da.nsplit, 32 * kDecWarps, smem,
+  return kv_launch("kv attention", k_kv_decode<QT_, D, KV, NT, ONE_PAGE>, grid, da.part_o ? 1 : da.nsplit, 32 * kDecWarps, smem,
                    st, kv, a, da);
 }
 
@@ -1024,8 +1030,13 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
     da.part_ml = (float2*)(da.part_o + (int64_t)p.nsplit * a.T * a.Hq * D);
   }
   const dim3 grid((unsigned)(p.tiles * kv.Hk), (unsigned)p.nsplit), mgrid((unsigned)(a.T * a.Hq));
-  const int rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1>(kv, a, da, grid, st)
-                           : decode_kernel<QT_, D, KV, 2>(kv, a, da, grid, st);
+  int rc;
+  if (UK == 32 && kv.page_shift == 4)
+    rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1, UK == 16>(kv, a, da, grid, st)
+                   : decode_kernel<QT_, D, KV, 2, UK == 16>(kv, a, da, grid, st);
+  else
+    rc = p.nt == 1 ? decode_kernel<QT_, D, KV, 1, true>(kv, a, da, grid, st)
+                   : decode_kernel<QT_, D, KV, 2, true>(kv, a, da, grid, st);
   if (rc || !p.ws_bytes) return rc;
   return p.nt == 1 ? kv_launch("kv attention merge", k_kv_merge<QT_, D, 8, UK>, mgrid, 1, 128, 0, st, kv, a, da)
                    : kv_launch("kv attention merge", k_kv_merge<QT_, D, 16, UK>, mgrid, 1, 128, 0, st, kv, a, da);

@@ -1,0 +1,36 @@
+"""GPU: attention over the paged cache at the edges of what it allows."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_kvcache_gpu import dev, filled_cache, layout
+from xanosmerks_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kv", ["Q4_0", "F16"])
+@pytest.mark.parametrize("n", [96, 102, 80])            # of the spoilt key's unit all is seen, all but for the first rows, a part
+@pytest.mark.parametrize("rows", [1, 2, 60])
+def test_a_spoilt_value_of_a_key_of_vanishing_weight(kv, n, rows):
+    """A visible key takes part with a positive weight, however small: its NaN is every row's that sees it."""
+    d, page, kl = 128, 32, [n]
+    table, lens, cu, pages = layout([rows], kl, page, seed=221)
+    c, _ = filled_cache(pages, 1, d, page, kv, seed=222, scale=0.25)
+    q = torch.ones(rows, 2, d, dtype=torch.float16, device="cuda")
+    p = 66                                               # the key: -4 in every dimension, scores some 2000 below the others
+    row = torch.full((1, 3 * d), -4.0, device="cuda")
+    at = dev(np.array([p + 1], np.int32))
+    c.append(row, 1, dev(table), at)
+    page_at, half = int(table[0, p // page]), c.pool.shape[2] // 2
+    lo, width = (half, 2 * d) if kv == "F16" else (half + page * d // 2, d // 16)
+    lo += (p % page) * width
+    want = c.attend(q, dev(table), dev(lens), dev(cu), scale=4.0)
+    assert torch.isfinite(want).all()
+    c.pool[page_at, :, lo:lo + width] = torch.tensor([0xff, 0x7f] * (width // 2), dtype=torch.uint8, device="cuda")
+    out = c.attend(q, dev(table), dev(lens), dev(cu), scale=4.0)
+    first = max(0, p - (kl[0] - rows))                   # the first row that sees the key
+    assert torch.equal(out[:first], want[:first])
+    assert torch.isnan(out[first:]).all()
+    assert _lib.lib.xm_device_status(0) == 0

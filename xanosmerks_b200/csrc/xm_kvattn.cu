@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
         }
       e = (int)(__reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16)) >> 10) - 14;
     }
+    unsigned hidden[NT] = {};                          // bit 4 j + i: sc[nt][j][i] is of a key that its row does not see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (!FULL) {
@@ -604,7 +605,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = keys[j] + key_of(r) + 8 * (i >> 1);
-            if (!sees(a, pos[nt][i & 1], key)) sc[nt][j][i] = -INFINITY;
+            if (!sees(a, pos[nt][i & 1], key)) {
+              sc[nt][j][i] = -INFINITY;
+              hidden[nt] |= 1u << (4 * j + i);
+            }
           }
       }
       float want[2];
@@ -647,7 +651,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {
             const float x = ex2(fmaf(sc[nt][j][c + h], q_f[nt][c], -ref));
-            sc[nt][j][c + h] = !FULL && sc[nt][j][c + h] == -INFINITY ? 0.f : x;   // (q_f may be 0)
+            sc[nt][j][c + h] = !FULL && hidden[nt] >> (4 * j + c + h) & 1u ? 0.f : x;
           }
       }
 #pragma unroll
@@ -671,11 +675,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float p0 = sc[nt][j][0] * da_, p1 = sc[nt][j][1] * da_, p2 = sc[nt][j][2] * db_, p3 = sc[nt][j][3] * db_;
-            if (!FULL) {                               // a masked key's scale may be anything
-              p0 = sc[nt][j][0] == 0.f ? 0.f : p0;
-              p1 = sc[nt][j][1] == 0.f ? 0.f : p1;
-              p2 = sc[nt][j][2] == 0.f ? 0.f : p2;
-              p3 = sc[nt][j][3] == 0.f ? 0.f : p3;
+            if (!FULL) {                               // a hidden key's scale may be anything (a seen one's counts,
+              const unsigned hide = hidden[nt] >> 4 * j;   // however small its weight)
+              p0 = hide & 1u ? 0.f : p0;
+              p1 = hide & 2u ? 0.f : p1;
+              p2 = hide & 4u ? 0.f : p2;
+              p3 = hide & 8u ? 0.f : p3;
             }
             const uint32_t b0 = transpose_8x8(half2_bits(p0, p1)), b1 = transpose_8x8(half2_bits(p2, p3));
             mma_16816(o[nt][2 * g], x & 0x00ff00ffu, xs, y & 0x00ff00ffu, ys, b0, b1);

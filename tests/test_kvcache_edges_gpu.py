@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_kvcache_gpu import dev, filled_cache, layout
+from tests.test_kvcache_gpu import check_attention, dev, filled_cache, layout
 from xanosmerks_b200 import _lib
+from xanosmerks_b200.kvcache import PagedKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -33,4 +34,26 @@ def test_a_spoilt_value_of_a_key_of_vanishing_weight(kv, n, rows):
     first = max(0, p - (kl[0] - rows))                   # the first row that sees the key
     assert torch.equal(out[:first], want[:first])
     assert torch.isnan(out[first:]).all()
+    assert _lib.lib.xm_device_status(0) == 0
+
+
+@pytest.mark.parametrize("kv", ["Q4_0", "F16"])
+@pytest.mark.parametrize("ql,kl,less", [([3, 5], [40, 50], 2), ([3, 5], [40, 700], 4), ([3, 5], [40, 50], 6),
+                                        ([20, 200], [90, 300], 37), ([20, 200], [90, 300], 205), ([3, 70], [9, 4000], 11)])
+def test_fewer_rows_than_the_offsets_name(kv, ql, kl, less):
+    """The first rows of a step: each keeps the position that the offsets and lengths give it."""
+    page, n = 16, sum(ql)
+    table, lens, cu, pages = layout(ql, kl, page, seed=231)
+    c, pool = filled_cache(pages, 2, 64, page, kv, seed=232)
+    q = torch.randn(n, 4, 64, generator=torch.Generator().manual_seed(233)).half().cuda()
+    whole = c.attend(q, dev(table), dev(lens), dev(cu))
+    check_attention(c, pool, q, whole, table, ql, kl, 0, 0)
+    got = c.attend(q[:n - less], dev(table), dev(lens), dev(cu)).double()
+    # another number of rows may take other parts of the keys: both within the bounds of a row (see check_attention),
+    # values of order 1
+    assert (got - whole[:n - less].double()).abs().max() <= 2 * (2.0 ** -11 * 2 + 2.0 ** -10)
+    a, b = (PagedKVCache(pages, 2, 64, page, kv) for _ in range(2))
+    qkv = torch.randn(n, 8 * 64, generator=torch.Generator().manual_seed(234)).cuda()
+    qa, qb = (x.append(r, 4, dev(table), dev(lens), dev(cu)) for x, r in ((a, qkv), (b, qkv[:n - less])))
+    assert torch.equal(qa[:n - less], qb)
     assert _lib.lib.xm_device_status(0) == 0

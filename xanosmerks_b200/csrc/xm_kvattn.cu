@@ -134,8 +134,8 @@ XM_DEV TileSpan tile_span(const KvView& kv, const AttnArgs& a, int s, int64_t t0
   x.t0 = t0;
   x.r0 = rt * R;
   x.rows = min(R, q_len * G - x.r0);
-  const int len = __ldg(kv.lens + s);
-  x.p_first = len - q_len;
+  // (the offsets count, not q_len: rows that they name behind the call's last are of the sequence all the same)
+  x.p_first = __ldg(kv.lens + s) - (kv.cu ? __ldg(kv.cu + s + 1) - (int)t0 : 1);
   x.pmin = x.p_first + x.r0 / G;
   x.pmax = x.p_first + (x.r0 + x.rows - 1) / G;
   const int64_t cap = (int64_t)kv.table_width << kv.page_shift;

@@ -57,3 +57,18 @@ def test_fewer_rows_than_the_offsets_name(kv, ql, kl, less):
     qa, qb = (x.append(r, 4, dev(table), dev(lens), dev(cu)) for x, r in ((a, qkv), (b, qkv[:n - less])))
     assert torch.equal(qa[:n - less], qb)
     assert _lib.lib.xm_device_status(0) == 0
+
+
+@pytest.mark.parametrize("kv", ["Q4_0", "F16"])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_queries_near_the_smallest_numbers(kv, rows):
+    """bf16 reaches far below fp16 and, with its subnormals, below 2^-126: all scores are nearly 0, no row is spoilt."""
+    table, lens, cu, pages = layout([rows], [90], 16, seed=241)
+    c, pool = filled_cache(pages, 1, 128, 16, kv, seed=242)
+    q = torch.randn(rows, 4, 128, generator=torch.Generator().manual_seed(243))
+    q *= torch.tensor([1e-30, 1e-35, 3e-38, 5e-40])[None, :, None]
+    q[:, :, ::5] = 0.0
+    q = q.to(torch.bfloat16).cuda()
+    assert (q[0, 3] != 0).any()
+    out = c.attend(q, dev(table), dev(lens), dev(cu))
+    check_attention(c, pool, q, out, table, [rows], [90], 0, 0)

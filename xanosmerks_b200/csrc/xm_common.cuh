@@ -200,13 +200,14 @@ XM_DEV float xm_act(int act, float x) {
   return x;
 }
 
-// The power-of-two exponent s with amax / 2^s in [2^14, 2^15) (0 for zero or non-finite rows).
+// The power-of-two exponent s with amax / 2^s in [2^14, 2^15) (0 for zero or non-finite rows).  Not below -126: 2^-s has
+// to be a number of fp32 (of a row below 2^-112 it leaves less than 2^14).
 XM_DEV int fp16_row_shift(float amax) {
   int s = 0;
   if (amax > 0.f && amax < INFINITY) {
     int e;
     frexpf(amax, &e);           // amax = f * 2^e, f in [0.5, 1): amax in [2^(e-1), 2^e)
-    s = (e - 1) - 14;
+    s = max((e - 1) - 14, -126);
   }
   return s;
 }

@@ -200,6 +200,7 @@ class PagedKVCache:
             raise ValueError(f"attend: q {tuple(q.shape)} for {hk} KV heads of {d}")
         if window < 0 or sinks < 0:
             raise ValueError("attend: window and sinks must not be negative")
+        window, sinks = min(window, 1 << 31), min(sinks, 1 << 31)      # (longer than any context; numbers that C can hold)
         pitch = self._pitch(q, "attend: q")
         where = self._rows(block_table, kv_lens, cu_seqlens, rows)
         if out is None and q.is_contiguous():

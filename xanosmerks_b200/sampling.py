@@ -50,6 +50,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     _, up = _per_row(u, "u", torch.float32, b, dev)
     t, tp = _per_row(temperature, "temperature", torch.float32, b, dev)
     k, kp = _per_row(top_k, "top_k", torch.int32, b, dev)
+    if kp is None:
+        k = min(max(k, 0), v)                            # (a number that C's int need not hold)
     p, pp = _per_row(top_p, "top_p", torch.float32, b, dev)
     m, mp = _per_row(min_p, "min_p", torch.float32, b, dev)
     if out is None:

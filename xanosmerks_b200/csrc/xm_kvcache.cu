@@ -378,6 +378,8 @@ int kv_view(const char* who, void* pool, int64_t pages, int kv_type, int Hk, int
     return xm_set_error(XM_ERR_INVALID, "%s: bad cache sizes", who);
   if (!pool || !table || !lens) return xm_set_error(XM_ERR_INVALID, "%s: null pointer", who);
   if ((uintptr_t)pool & 15) return xm_set_error(XM_ERR_INVALID, "%s: the pool must be 16-byte aligned", who);
+  if (((uintptr_t)table | (uintptr_t)cu | (uintptr_t)lens) & 3)
+    return xm_set_error(XM_ERR_INVALID, "%s: unaligned page table, offsets or lengths", who);
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
   *out = KvView{(uint8_t*)pool, pages, 2 * kv_part_bytes(kv_type, head_dim, page_size), table, table_stride,

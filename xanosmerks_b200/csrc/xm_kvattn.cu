@@ -51,7 +51,8 @@ struct AttnArgs {
 // 4-bit rows are never unpacked to values.  The nibbles 0 and 4 (for keys; 0 of two keys, paired by a
 // byte permute, for values) of a word are, after one mask, two fp16 subnormals c 2^-24, the nibbles
 // 1 and 5 are c 2^-20: exact, one instruction for two codes.  For values whole bytes (c + 16 c') 2^-24 and
-// their high nibbles enter, one instruction less, and the low codes' sums are the difference at the end.
+// their high nibbles enter, one instruction less, and the low codes' sums are the difference at the end (of sums of up to
+// 255 p d in fp32: some 2^-18 of a block's largest value, where p d itself is rounded to 2^-11).
 // The block scale and the offset of the codes stay outside the product:
 //   S  = sum over blocks b of d_kb (sum_i q_i c_i - 8 sum_i q_i)       (the offset is the product's
 //        initial accumulator),

@@ -348,7 +348,9 @@ int xm_argmax(const float* d_logits, int64_t B, int64_t V, int* d_out, void* str
  * table_width entries.  Rows behind cu[B] are left alone.  A row at a negative
  * position (more rows than tokens) is not stored and yields zeros.  A position
  * past the table or the rotation table, or a page outside the pool, is treated
- * the same and sets XM_DEVERR_PAGE in xm_device_status.
+ * the same and sets XM_DEVERR_PAGE in xm_device_status; the attention leaves such
+ * keys out.  Entries of pages that no row of the call sees, behind a window, may
+ * be anything.
  *
  * xm_kv_append: qkv row t = [q | k | v] (Hq, Hk, Hk heads of D, F32 / F16 /
  * BF16, row pitch qkv_stride elements).  Each query and key head x is normalised

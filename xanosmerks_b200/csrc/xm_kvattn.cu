@@ -40,8 +40,8 @@ struct AttnArgs {
 //
 // Bound: memory (the cache is read once); the work per byte decides whether that is reached.  8 sequences of up to
 // 4096 keys in fp16 (8 KV heads): 24.6 us, 0.59 of the copy bandwidth; 64 sequences of up to 8192 in 4 bits: 118 us, 0.52
-// of it, about 340 instructions per 16 keys and head and three CTAs an SM (168 registers a thread; four spill and
-// are slower).  A warp
+// of it.  At three CTAs an SM (168 registers a thread; four spill and are slower) latency is the limit: 17 % of the warps
+// active, issue slots 54 %, about 340 instructions per 16 keys and head, DRAM 41 %.  A warp
 // takes 16 keys at a time on mma.sync m16n8k16 (fp16 operands, fp32 sums) with the keys, or the
 // values' dimensions, as the 16 matrix rows and the query rows as the 8 columns:
 //   S^T [16 keys x 8 rows] = K q^T,   O^T [D x 8 rows] += V^T P^T.
@@ -961,6 +961,9 @@ struct DecPlan {
 DecPlan dec_plan(int64_t T, int64_t B, int Hq, int Hk, int D, int64_t max_keys, bool ragged) {
   DecPlan p{};
   const int G = Hq / Hk;
+  // One kernel for the call, by the mean: a call that mixes steps and prompts is slower than two (63 steps behind up to 8192
+  // keys 113 us, a chunk of 450 tokens behind 4096 83, both in one call 438).  Parts come from max_keys, the width of the
+  // table: the lengths are on the device (640 keys in a table of 640: 5.4 us, of 131072: 9.4).
   // Up to 32 rows (token, query head) of each KV head a sequence: the decode kernel (32 rows each of 8 sequences of
   // 8192 keys, 8 KV heads: 66 us, with the prompt kernel 148; of one sequence 21 and 27).  Above: the prompt kernel
   // (64 rows each: decode 135, prompt 140; of one sequence 33 and 28, behind 131072 keys 313 and 142).
@@ -1064,12 +1067,13 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 //
 // What decides the speed is the chain of one row tile: a row of S is read once, 64 columns into registers (a
 // tcgen05.wait::ld waits for every load, and costs some 300 clocks), its maximum taken, P computed.  A prompt of
-// 8192 tokens (32 query and 8 KV heads of 128, 4 bits) took 790 us with units of 128 keys and one S per row tile
-// (PV and S follow one another in the chain: 6100 clocks a unit), 779 with half units and two S, 760 with the products
-// issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma), 730 with one body
-// for masked and whole units (no spills), 727 with an eighth of them there: 756 TFLOP/s.  Four chunks of up to 1000 tokens behind up to 5000, window 1024,
-// sinks, fp16, 28 query and 4 KV heads of 64: 92 us with two to five instructions a column for the mask, 76 with a
-// word of its bits.
+// 8192 tokens (32 query and 8 KV heads of 128, 4 bits; calls from Python on changing inputs) took 790 us with units of 128
+// keys and one S per row tile (PV and S follow one another in the chain: 6100 clocks a unit), 779 with half units and two S,
+// 760 with the products issued by an elected lane, 745 with a quarter of the exponentials on the multipliers (ex2_fma), 730
+// with one body for masked and whole units, 717 with an eighth of them there: 766 TFLOP/s (in a graph on the same inputs
+// 664; fp16 827).  The 4-bit instances spill 16 to 24 bytes at 128 registers, the most that 14 warps leave.  Four chunks of up to
+// 1000 tokens behind up to 5000, window 1024, sinks, fp16, 28 query and 4 KV heads of 64: 92 us with two to five
+// instructions a column for the mask, 75 with a word of its bits.
 //
 // 4-bit rows become fp16 here, d (c - 8) rounded once (2^-11): a product per code would need the scales
 // inside the tensor core's inner dimension.  The order of the eight values that a word of keys yields is
@@ -1084,9 +1088,10 @@ int decode_launch(const KvView& kv, const AttnArgs& a, const DecPlan& p, void* w
 // Masked keys: their scores are replaced, their values are zeros where no row sees them; a value that is not
 // finite and that only some rows see is taken out of the product and added to those rows alone.
 //
-// Bound: the products (4 R 128 D flops a unit at the tensor peak: 2048 clocks a unit of R = 256, D = 128) and, as much, the 128 R exponentials (16 a clock: 2048 clocks a unit); neither is reached, since a
-// row tile's chain (some 5000 clocks a unit: waits 800, maximum 1200, exponentials and rounding 2200, loads and stores of
-// tensor memory 700) is only halved by the other's.
+// Bound: the products (4 R 128 D flops a unit at the tensor peak: 2048 clocks a unit of R = 256, D = 128) and, as much, the
+// 128 R exponentials (16 a clock: 2048 clocks a unit); neither is reached, since a row tile's chain (some 5000 clocks a unit:
+// waits 800, maximum 1200, exponentials and rounding 2200, loads and stores of tensor memory 700) is only halved by the
+// other's.
 // ---------------------------------------------------------------------------
 constexpr int kUnit = 128;                         // keys of a unit
 constexpr int kPromptThreads = 14 * 32;
@@ -1238,8 +1243,8 @@ XM_DEV bool elect_one() {
 }
 
 // 2^y on the multipliers: y = k + r, |r| <= 1/2, Taylor's polynomial of degree 5 (2.4e-6 of the value; the weights are
-// rounded to fp16).  With an eighth of the weights this way 8192 tokens take 677 us, with none 692, a quarter 688, three
-// eighths 678.  NaN stays NaN; below 2^-126 it is 2^-126 (a weight of 0 in fp16, and nothing in
+// rounded to fp16).  A prompt of 8192 tokens in a captured graph, 4 bits (fp16): with none of the weights this way 684 us
+// (797), an eighth 664 (827), a quarter 679 (856), three eighths 675 (895).  NaN stays NaN; below 2^-126 it is 2^-126 (a weight of 0 in fp16, and nothing in
 // a sum whose largest term is at least 2^-8).
 XM_DEV float2 ex2_fma(float2 y) {
   auto both = [](float v) { return make_float2(v, v); };

@@ -16,9 +16,10 @@
 // arithmetic runs at half the fp32 rate here and is off the critical path of
 // the memory traffic); everything else is fp32.
 //
-// Bound: memory for prompts by the bytes, instructions in fact (normalisation and rotation of keys in 64 bits, the exact
-// decisions of codes: eight prompts of up to 2048 tokens, normalised heads, 4 bits: 90 us, nearly twice what the bytes take, with four CTAs an SM, 94 with three; the
-// read 19), latency for single tokens.  D / 8 lanes take a head, so a warp two heads
+// Bound: memory by the bytes for prompts, but eight prompts of up to 2048 tokens take 89 us (normalised heads, 4 bits; four
+// CTAs an SM, 94 with three), nearly twice what the bytes do: issue slots 68 %, 35 % of the warps active, each with one head in
+// flight.  Norms and rotations of keys in 64 bits and exact codes are a part of it: 76 without norms, 64 with an fp16 cache, 59
+// with neither.  The read takes 19.  Single tokens: latency.  D / 8 lanes take a head, so a warp two heads
 // of 128 or four of 64: lane l of them holds the values 4 l .. 4 l + 3 of each half, so the rotation
 // needs no exchange, loads and stores are 8 or 16 bytes, and a block of 32 values is 8 lanes.  A
 // block's codes are words of 2 lanes (keys) or halfwords of one (values).

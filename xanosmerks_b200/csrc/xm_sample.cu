@@ -6,13 +6,13 @@
 // them is always kept.  The result is the first token i, in index order, at which the kept mass of
 // 0 .. i exceeds u times the kept mass.
 //
-// Masses are whole numbers: w_i is rounded to 2^-F (F = 44, less for more than 2^18 tokens), and sums
+// Masses are whole numbers: w_i is rounded to 2^-F (F = 44, less for rows of 2^19 logits and more), and sums
 // of whole numbers do not depend on their order, so a call gives the same token whatever the launch
 // shape.  With 2^17 kept tokens the borders are off by about 1e-11 of the mass.
 //
 // A cluster of C CTAs per row, each warp a contiguous piece of it; the logits stay in shared memory, so the row is
-// read once (RES; rows that do not fit, of more than 300000 fp32 logits, are read again from L2 for each
-// pass).  What the CTAs have to tell one another (maxima, totals, histograms) goes through their shared
+// read once (RES; rows that do not fit, of more than 294912 fp32 or 589824 16-bit logits, are read again from L2 for
+// each pass).  What the CTAs have to tell one another (maxima, totals, histograms) goes through their shared
 // memories.
 #include <cooperative_groups.h>
 
@@ -63,12 +63,13 @@ struct SampleArgs {
 // degree 3 on the rest (table-driven exponential after Tang, 1989): 2e-13 of the value, less than the
 // rounding to a whole multiple of 2^-F.
 //
-// One row of 32000 fp32 logits: 14 us with temperature alone, 22 with top_k and top_p, 39 with top_p alone; 64 rows of
-// 128000: 49, 67 and 121 (a cluster of 8 CTAs a row, two CTAs an SM: 1.7 waves).
-// Bound: latency for few rows (passes over shared memory and three to eight exchanges across a cluster); for many
-// the instructions of the weights, some 25 a logit, ten of them in 64 bits, and with top_p alone the atomic adds to
-// shared memory (about one lane a clock on an SM: that is why a bin's mass is two words, of which the
-// upper one takes carries and weights above 2^-12 only, and why top_k counts maxima and not logits).
+// Temperature alone, top_k 50, top_p 0.9 alone, in a captured graph with L2 flushed: one row of 32000 fp32 logits 14, 21 and
+// 41 us (L2 warm 8, 13, 23); 64 rows of 128000 49, 55 and 121 (a cluster of 8 CTAs a row, two CTAs an SM: 1.7 waves).
+// Bound: latency.  For few rows of passes over shared memory and three to eight exchanges across a cluster; for many of the
+// weights' chains (some 25 instructions a logit, ten of them in 64 bits, at 64 registers with some 170 bytes of spills: issue
+// slots 43 %, DRAM 5 %).  With top_p alone the atomic adds to shared memory come on top (about one lane a clock on an SM:
+// that is why a bin's mass is two words, of which the upper one takes carries and weights above 2^-12 only, and why top_k
+// counts maxima and not logits).
 // ---------------------------------------------------------------------------
 constexpr int kSampleThreads = 512, kBins = 2048, kList = 512, kTable = 256;
 static_assert(kList == kSampleThreads, "the list is sorted with one entry a thread");

@@ -12,8 +12,9 @@ b), ``kv_lens`` (int32 [B]) the tokens of each sequence *with* its new ones, and
 ``block_table`` (int32 [B, W]) the pages of each sequence in order; everything
 lives on the device, so that a step can be captured into a CUDA graph.  Rows
 behind ``cu_seqlens[-1]`` are left alone; a row before position 0 is not stored
-and yields zeros; a position without a page does too and shows up in
-``_lib.check_device``.
+and yields zeros; a position without a page does too (as a key it is left out of
+the attention) and shows up in ``_lib.check_device``.  Entries of pages that no
+row sees, behind a window, may be anything: those pages can go back to the pool.
 
 There is no CPU fallback; calls run on the current stream of the pool's device.
 """

@@ -427,7 +427,7 @@ class LlamaDecoder:
     def set_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0):
         """Sample the next tokens (see :func:`~xanosmerks_b200.sampling.sample`; numbers, or tensors with one entry
         per sequence) with random numbers from a generator seeded with ``seed``; ``temperature=None``: greedy again.
-        A captured step is dropped."""
+        A captured step is dropped.  Under tensor parallelism every rank makes the same call (all of them hold all logits)."""
         self.graph = None
         if temperature is None:
             self.sampling = None

@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, DecShape<KV, D, NT>::kCtas) k_
 
   // One step of UK keys, its subtiles' from first.x and first.y on (kNoKeys: without a page).  FULL: every row sees every
   // one of them.
-  constexpr int kNoKeys = 0x7fffffff - 64;             // behind every position
+  constexpr int kNoKeys = 0x7fffffff - 15;             // behind every position that a table reaches, with the 15 keys after it
   auto step = [&](auto full_, int2 first, uint32_t at) {
     const int keys[2] = {first.x, first.y};
     constexpr bool FULL = decltype(full_)::value;

@@ -223,6 +223,24 @@ int xm_rmsnorm(const void* d_x, int x_dtype, int64_t m, int64_t k, int64_t x_str
                const float* d_norm_w, float eps, float* d_out, void* stream);
 
 /*
+ * What stands between two blocks, in one pass over m rows of D <= 32768 values
+ * (row pitches in elements; F32 / F16 / BF16 each):
+ *   v = y, or y post_w / sqrt(mean(y^2) + eps) where d_post_w (fp32 [D]) is given
+ *   h' = h + scale * gate * v                          -> d_out (type of h; may be h)
+ *   next = h' pre_w / sqrt(mean(h'^2) + eps)           -> d_next, where d_pre_w (fp32 [D]) is given
+ * gate (may be null): row r takes gate row r / rows_per_gate, `gate_pitch`
+ * elements apart, one value a column (gate_wide) or one for the row.  All in
+ * fp32, each output rounded once (next comes from the unrounded h').
+ *
+ * Replaces the residual adds and norms around the blocks of forward.py:104-116.
+ */
+int xm_residual_norm(const void* d_h, int h_type, int64_t h_pitch, const void* d_y, int y_type, int64_t y_pitch,
+                     int64_t rows, int64_t D, const float* d_post_w, const void* d_gate, int gate_type,
+                     int64_t gate_pitch, int gate_wide, int64_t rows_per_gate, float scale, const float* d_pre_w,
+                     float eps, void* d_out, int64_t out_pitch, void* d_next, int next_type, int64_t next_pitch,
+                     void* stream);
+
+/*
  * Sparse mixture-of-experts block (Mixtral-style gated experts):
  *   out[t] = sum over the k experts e chosen for token t (ascending e) of
  *            w[t][e] * ((act(x_t @ W1_e.T) * (x_t @ W3_e.T)) @ W2_e.T)
@@ -276,6 +294,32 @@ int xm_moe_experts(const void* d_rows, int x_dtype, int64_t P, int64_t H, int64_
                    int64_t workspace_bytes, void* stream);
 int xm_moe_combine(const float* d_rows, int64_t T, int64_t H, int E, int k, int64_t F, const void* d_workspace,
                    float* d_out, void* stream);
+
+/*
+ * The MoE block of xm_moe_forward for a few tokens (a decode step; T <= 64),
+ * with the norm before it and the residual add behind it:
+ *   v = x, or x w / sqrt(mean(x^2) + eps) where d_norm_w (fp32 [H]) is given
+ *   out[t] = residual[t] + sum over the k experts e chosen for token t
+ *            (ascending e) of w[t][e] * ((act(v_t @ W1_e.T) * (v_t @ W3_e.T)) @ W2_e.T)
+ * x [T][H] of x_dtype, residual (fp32, may be null) and out (fp32) with row
+ * pitches in elements; out may be x or the residual.  Routing as in
+ * xm_moe_forward, with the logits summed in 64 bits and equal ones decided for
+ * the lower expert.  d_w1 / d_w3 / d_w2 are DEVICE arrays of E device pointers
+ * (16-byte aligned) to GGUF blocks of `qtype`, any block type; weights of Q4_K,
+ * Q5_K, Q6_K and Q8_0 enter with the block's own value, those of the other
+ * types rounded to fp16 as dequantisation rounds them; activations keep 22 bits.
+ * E <= 256, k <= 16; H (<= 16384) and F multiples of 256.  d_workspace (256-byte
+ * aligned, xm_moe_step_workspace_size bytes, no initial contents): one for each
+ * call that may run at the same time.  Three launches, no host synchronisation;
+ * the same result for every launch.
+ *
+ * Replaces moe.py:54-115 with the norm and the residual add of forward.py:113-116.
+ */
+int64_t xm_moe_step_workspace_size(int64_t T, int64_t H, int64_t F, int E, int k, int qtype);
+int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_stride, const float* d_norm_w, float eps,
+                const float* d_gate, int E, int k, int64_t F, const void* const* d_w1, const void* const* d_w3,
+                const void* const* d_w2, int qtype, int activation, const float* d_residual, int64_t residual_stride,
+                float* d_out, int64_t out_stride, void* d_workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * xm_qgemv without a workspace argument, for callers that cannot allocate
@@ -403,6 +447,23 @@ int xm_kv_attention(const void* d_q, int q_dtype, int64_t T, int64_t q_stride, i
 int xm_sample(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t stride, const float* d_u,
               float temperature, const float* d_temperature, int top_k, const int* d_top_k, float top_p,
               const float* d_top_p, float min_p, const float* d_min_p, int* d_ids, float* d_logprob, void* stream);
+
+/*
+ * Log-probabilities of given tokens, one per row of up to 2^20 logits (F32 /
+ * F16 / BF16, row pitch stride), under softmax(x / T): logprob[b] of tokens[b]
+ * (int32 or int64, by token_bytes), entropy[b] of the row in nats, rank[b] = how
+ * many tokens have a larger logit or the same one at a lower index; and the
+ * `top` (<= 64, <= V) largest logits, equal ones by ascending index:
+ * top_ids[b][top], top_logprobs[b][top].  A token outside 0 .. V - 1 gives NaN
+ * and rank -1.  NaN logits count as -inf (log-probability -inf); a row of
+ * nothing else has entropy 0.  Logits of +inf share the mass.  T <= 0: the first
+ * maximum has log-probability 0, the others -inf.  T is per row where
+ * d_temperature is given.  Same result for any launch.  (The log-probability
+ * that sampling.py:94-158 draws from, before its filters.)
+ */
+int xm_logprobs(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t stride, const void* d_tokens,
+                int token_bytes, float temperature, const float* d_temperature, int top, float* d_logprob,
+                float* d_entropy, int* d_rank, int* d_top_ids, float* d_top_logprobs, void* stream);
 
 /*
  * Tensor-parallel exchange over NVLink peer memory (one process per GPU of a

@@ -81,6 +81,12 @@ SIGNATURES = {
     "xm_kv_attention": (_int, [_vp, _int, _i64, _i64, _int, _int, _int, _f32, _i64, _i64, _vp, _i64, _int, _int, _vp,
                                _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "xm_sample": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _int, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp]),
+    "xm_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _f32, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "xm_residual_norm": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _i64, _int, _i64, _f32, _vp,
+                                _f32, _vp, _i64, _vp, _int, _i64, _vp]),
+    "xm_moe_step_workspace_size": (_i64, [_i64, _i64, _i64, _int, _int, _int]),
+    "xm_moe_step": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _int, _int, _i64, _vp, _vp, _vp, _int, _int, _vp,
+                           _i64, _vp, _i64, _vp, _i64, _vp]),
     "xm_comm_destroy": (_int, [_vp]),
     "xm_allreduce_add": (_int, [_vp, _vp, _vp, _i64, _vp]),
 }

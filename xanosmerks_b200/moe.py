@@ -10,19 +10,27 @@ reference are raised.  The forward pass runs entirely on the GPU
 (``xm_moe_forward``): routing, stable sort by expert, grouped tensor-core
 GEMMs, the gated activation (``hidden_act``: silu/swish, gelu, relu or
 identity, as the reference's ``apply_activation``) and the ordered combine.
+For a few tokens, ``MoELayer.step`` (``xm_moe_step``) reads only the experts that
+they chose, with the norm before the layer and the residual add behind it.
 """
 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
 
-from ._lib import ACT, DT_BF16, DT_F16, DT_F32, XMError, check, lib
+from ._lib import ACT, DT_BF16, DT_F16, DT_F32, XMError, call_on, check, lib
 from .ops import GGUFTensor, _workspace
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_workspace(*sizes) -> int:
+    return lib.xm_moe_step_workspace_size(*sizes)
 
 
 class MoELayer:
@@ -66,6 +74,51 @@ class MoELayer:
         self._p3 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w3])
         self._p2 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w2])
         self._is_dense = self.num_experts_per_tok == self.num_experts
+        # the same pointers on the device, for step(): w1, w3, w2
+        self._table = torch.tensor([[w.data.data_ptr() for w in ws] for ws in (self.w1, self.w3, self.w2)],
+                                   dtype=torch.int64, device=self.device) if self.device.type == "cuda" else None
+
+    STEP_TOKENS = 64   # tokens of a step at most
+
+    def step(self, x: torch.Tensor, norm_weight: torch.Tensor | None = None, eps: float = 1e-5,
+             residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer for a few tokens (a decode step): fp32 [T, H] =
+        residual + sum of the chosen experts' results on x, or on x norm_weight / sqrt(mean(x^2) + eps).
+
+        ``x`` [T, H], T <= 64, fp32, fp16 or bf16 on the weights' device; ``norm_weight`` fp32 [H]; ``residual`` and
+        ``out`` fp32 [T, H] (``out`` may be ``x`` or ``residual``: the step of a residual stream in place).  Only the blocks of
+        the experts that some token chose are read.  Up to 256 experts, 16 of them a token.  More tokens, and
+        differences to :meth:`forward_device`: that one multiplies weights rounded to fp16 with fp16 activations, this one the
+        blocks' own values (of Q4_K, Q5_K, Q6_K and Q8_0) with activations of 22 bits."""
+        H, F, E, k, dev = self.hidden, self.intermediate, self.num_experts, self.num_experts_per_tok, self.device
+        dt = _DT.get(x.dtype) if isinstance(x, torch.Tensor) else None
+        if dt is None or x.dim() != 2 or x.shape[1] != H or x.device != dev or (x.stride(1) != 1 and H > 1):
+            raise ValueError(f"step: x must be an fp32, fp16 or bf16 tensor [tokens, {H}] on {dev} with unit stride in its last "
+                             f"dimension")
+        T = x.shape[0]
+        if T > self.STEP_TOKENS:
+            raise ValueError(f"step: {T} tokens (up to {self.STEP_TOKENS}; forward_device takes more)")
+        if norm_weight is not None and (norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (H,)
+                                        or not norm_weight.is_contiguous() or norm_weight.device != dev):
+            raise ValueError(f"step: norm_weight must be a contiguous fp32 tensor [{H}] on {dev}")
+        for name, t in (("residual", residual), ("out", out)):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (T, H) or t.device != dev or t.stride(1) != 1):
+                raise ValueError(f"step: {name} must be an fp32 tensor [{T}, {H}] on {dev} with unit stride in its last dimension")
+        if out is None:
+            out = torch.empty((T, H), dtype=torch.float32, device=dev)
+        if T == 0:
+            return out
+        pitch = [t.stride(0) if t is not None and T > 1 else H for t in (x, residual, out)]
+        # a workspace for each call: two captured graphs, or two streams, never share one
+        need = _step_workspace(T, H, F, E, k, self.qtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        table = self._table.data_ptr()
+        check(call_on(dev, lib.xm_moe_step, x.data_ptr(), dt, T, H, pitch[0],
+                      None if norm_weight is None else norm_weight.data_ptr(), eps, self.gate.data_ptr(), E, k, F, table,
+                      table + 8 * E, table + 16 * E, self.qtype, ACT[self.activation],
+                      None if residual is None else residual.data_ptr(), pitch[1], out.data_ptr(), pitch[2], ws.data_ptr(),
+                      need), "moe step")
+        return out
 
     def forward_device(self, x: torch.Tensor) -> torch.Tensor:
         """x: CUDA tensor (..., H) -> fp32 CUDA tensor of the same shape."""

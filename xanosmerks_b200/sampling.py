@@ -1,26 +1,33 @@
-"""Sampling tokens from logits (the reference's ``sample``, sampling.py:94-158) from given random numbers.
+"""Sampling tokens from logits (the reference's ``sample``, sampling.py:94-158) from given random numbers, and
+the log-probabilities of given tokens.
 
 ``sample(logits, u, ...)`` chooses one token per row by temperature, top-k, top-p and min-p; the random
 numbers are an input (one uniform number in [0, 1) per row), so that the same call gives the same tokens.
+``logprobs(logits, tokens, ...)`` scores tokens: their log-probability and rank, the entropy of each row and
+its largest alternatives.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
 from ._lib import DT_BF16, DT_F16, DT_F32, call_on, check, lib
 
-__all__ = ["sample"]
+__all__ = ["sample", "logprobs", "TokenLogprobs", "MAX_TOP"]
+
+MAX_TOP = 64   # alternatives of a row
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 
 
-def _per_row(v, name, dtype, rows, dev):
+def _per_row(v, name, dtype, rows, dev, what="sample"):
     """(scalar, device pointer or None) of a parameter given as a number or as a tensor with one entry per row."""
     if not isinstance(v, torch.Tensor):
         return v, None
     if v.dtype != dtype or v.dim() != 1 or v.shape[0] != rows or v.device != dev or not v.is_contiguous():
-        raise ValueError(f"sample: {name} must be a number or a contiguous {dtype} tensor [{rows}] on {dev}")
+        raise ValueError(f"{what}: {name} must be a number or a contiguous {dtype} tensor [{rows}] on {dev}")
     return 0, v.data_ptr()
 
 
@@ -62,3 +69,48 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     check(call_on(dev, lib.xm_sample, logits.data_ptr(), dt, b, v, pitch if b > 1 else v, up, t, tp, k, kp, p, pp, m,
                   mp, out.data_ptr(), logp.data_ptr()), "sample")
     return out, logp
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`logprobs` gives of B rows (on the logits' device)."""
+
+    logprob: torch.Tensor                    # fp32 [B]: of the given tokens
+    entropy: torch.Tensor                    # fp32 [B], in nats
+    rank: torch.Tensor                       # int32 [B]: tokens before the given one in descending order
+    top_ids: torch.Tensor | None             # int32 [B, top], in descending order
+    top_logprobs: torch.Tensor | None        # fp32 [B, top]
+
+
+def logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature=1.0, top: int = 0) -> TokenLogprobs:
+    """Log-probabilities of ``tokens`` [B] (int32 or int64) under softmax(``logits`` / temperature), ``logits`` [B, V]
+    (fp32, fp16 or bf16, on a CUDA device; V <= 2^20), with the entropy of each row, the rank of each token (how many
+    have a larger logit, or the same one at a lower index) and the ``top`` (up to 64) largest logits (equal ones by
+    ascending index).
+
+    ``temperature``: a number, or an fp32 tensor [B]; 0: the first maximum has log-probability 0, the others -inf.  A token
+    outside the vocabulary (-1 for padding, say) gives NaN and rank -1.  NaN logits count as -inf, which have
+    log-probability -inf; a row of nothing else has entropy 0.  Logits of +inf share the mass."""
+    dt = _DT.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
+    if dt is None or logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1:
+        raise ValueError("logprobs: logits must be a 2-D fp32, fp16 or bf16 CUDA tensor")
+    b, v = logits.shape
+    dev = logits.device
+    pitch, one = logits.stride()
+    if v > 1 and one != 1:
+        raise ValueError("logprobs: logits must have unit stride in the last dimension")
+    if (not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1
+            or tokens.shape[0] != b or tokens.device != dev or not tokens.is_contiguous()):
+        raise ValueError(f"logprobs: tokens must be a contiguous int32 or int64 tensor [{b}] on {dev}")
+    if not 0 <= top <= min(MAX_TOP, v):
+        raise ValueError(f"logprobs: {top} alternatives (0 to {min(MAX_TOP, v)})")
+    t, tp = _per_row(temperature, "temperature", torch.float32, b, dev, "logprobs")
+    # (one allocation: three values a row, then the alternatives)
+    some = torch.empty((3 + 2 * top) * b, dtype=torch.float32, device=dev)
+    lp, ent, rank = some[:b], some[b:2 * b], some[2 * b:3 * b].view(torch.int32)
+    ids = tops = None
+    if top:
+        ids, tops = some[3 * b:(3 + top) * b].view(torch.int32).view(b, top), some[(3 + top) * b:].view(b, top)
+    check(call_on(dev, lib.xm_logprobs, logits.data_ptr(), dt, b, v, pitch if b > 1 else v, tokens.data_ptr(),
+                  tokens.element_size(), t, tp, top, lp.data_ptr(), ent.data_ptr(), rank.data_ptr(),
+                  ids.data_ptr() if top else None, tops.data_ptr() if top else None), "logprobs")
+    return TokenLogprobs(lp, ent, rank, ids, tops)

@@ -3,21 +3,26 @@
 //   v = x, or x w / sqrt(mean x^2 + eps);  l = gate v;  the k largest l, p = softmax over them;
 //   out = residual + sum over the k experts e, ascending, of p_e W2_e (act(W1_e v) * (W3_e v))
 //
-// Bound: HBM, the blocks of the experts that some token chose (each read once for up to 4 NT tokens of an expert).
+// Bound: HBM, the blocks of the experts that some token chose (each read once for up to M = 4 or 8 tokens of an expert).
 //
 // Three launches, each starting while the one before it ends:
 //   k_moe_step_route   a cluster a token: norm, logits in 64 bits (a near tie of two experts goes one way), top k, softmax
 //   k_moe_step<UP>     a = act(W1 v) * (W3 v) of every (token, expert) pair
 //   k_moe_step<DOWN>   W2 a; whoever writes the last partial result of some output rows adds them up
 //
-// The products run on mma.sync (m16n8k16, fp16 with fp32 sums): sixteen weight rows by eight columns, a column pair per
-// token: x = 2^s (hi + 2^-11 lo), both fp16, so that an activation keeps some 22 bits.  A tile of UP is eight rows of W1 and
-// the same eight of W3, so that one thread holds the gate and the up value of a feature.
+// The products run on mma.sync (m16n8k16, fp16 with fp32 sums): sixteen weight rows by eight columns.  An activation is
+// 2^s (hi + lo), both fp16, which keeps some 22 bits: up to 4 tokens have a column for each part, up to 8 tokens a column each
+// and two products.  A tile of UP is eight rows of W1 and the same eight of W3, so that one thread holds the gate and the up
+// value of a feature.
 //
-// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles).  One warp copies the rows of a stage
-// into a ring in shared memory (bulk copies) and, once the 16 other warps have multiplied them, adds up their results; each
-// of those holds 256 values of K of a tile, for which its activations stay in registers while the expert lasts.  Nothing
-// waits for another CTA.  The results do not depend on the order in which CTAs run.
+// A block's codes enter as they are (integers in fp16) and its scales and offsets are applied to the sums of 16 or 32
+// products, in fp32: offsets as one more product of the offsets with the activations' sums over their groups.
+//
+// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles), whose rows bulk copies bring into a
+// ring in shared memory.  Each of its 16 warps holds 256 values of K of a tile, for which its activations stay in registers
+// while the expert lasts.  The warps take turns at a stage's end: one stage later, one of them adds up the 16 results, has the
+// slot filled again and writes (a 17th warp for that would cost every thread a quarter of its registers).  Nothing waits for
+// another CTA.  The results do not depend on the order in which CTAs run.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -29,7 +34,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kMaxTokens = 64, kMaxTop = 16, kMaxStepExperts = 256, kMaxPairs = kMaxTokens * kMaxTop;
-constexpr int kWorkers = 16, kStepThreads = (kWorkers + 1) * 32, kMaxRing = 8;
+constexpr int kWorkers = 16, kStepThreads = kWorkers * 32, kMaxRing = 8;
 constexpr int kRouteCluster = 8, kRouteThreads = 256;
 constexpr int kMaxHidden = 16384;
 
@@ -41,7 +46,7 @@ struct StepArgs {
   float* dst;                  // UP: a [P][F];  DOWN: partial results [chunks][P][H]
   unsigned* dst_max;           // UP: the largest magnitude of a, as bits
   float* part;                 // UP with several chunks: partial results [chunks][P][2F]
-  int* tickets;                // of each group of tiles (DOWN), of each (pair group, group of tiles) (UP with chunks)
+  int* tickets;                // of each group of tiles (DOWN; null: k_moe_step_sum follows), of each segment's (UP with chunks)
   const int* top_e;            // [T][k], ascending
   const float* top_w;
   int T, k, E, act;
@@ -57,8 +62,9 @@ struct StepArgs {
 
 struct alignas(128) StepShared {
   uint64_t full[kMaxRing], done[kMaxRing];
-  int n_seg, last;
+  int n_seg;
   int cnt[kMaxStepExperts], off[kMaxStepExperts];
+  unsigned short expert[kMaxPairs], rank[kMaxPairs];   // of a pair: its expert, how many of the expert's pairs are before it
   unsigned short pair[kMaxPairs];                      // pairs (token * k + slot) by expert, then token
   unsigned short seg_e[kMaxPairs], seg_at[kMaxPairs], seg_n[kMaxPairs];
 };
@@ -84,14 +90,15 @@ XM_DEV double warp_sum_d(double v) {
   return v;
 }
 
-// A cluster of 8 CTAs a token: each has the whole row and an eighth of the experts.
+// A cluster of 8 CTAs a token: each has the whole row and an eighth of the experts, one for each warp, or for several warps
+// where there are few (which then take parts of the row).
 template <typename XT>
 __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
+  constexpr int WARPS = kRouteThreads / 32, MINE = kMaxStepExperts / kRouteCluster;
   extern __shared__ __align__(16) float row[];
   __shared__ float red[32];
-  __shared__ double part[kMaxStepExperts / kRouteCluster][kRouteThreads / 32], logit[kMaxStepExperts / kRouteCluster];
-  __shared__ int chosen[kMaxTop];
-  __shared__ float weight[kMaxTop];
+  __shared__ double part[WARPS], logit[MINE], all[kMaxStepExperts], val[kMaxTop];
+  __shared__ unsigned chosen[WARPS];
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), t = (int)(blockIdx.x / kRouteCluster), tid = threadIdx.x, lane = tid & 31,
             warp = tid >> 5;
@@ -99,101 +106,108 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
   grid_dep_launch();
   for (int i = blockIdx.x * kRouteThreads + tid; i < a.n_tickets; i += gridDim.x * kRouteThreads) a.tickets[i] = 0;
   if (rank == 0 && tid < a.k) a.a_max[t * a.k + tid] = 0u;
+  const int mine = (a.E - rank + kRouteCluster - 1) / kRouteCluster;       // experts rank, rank + 8, ...
+  const int most = (a.E + kRouteCluster - 1) / kRouteCluster;
+  const int split = most <= 1 ? 8 : most <= 2 ? 4 : most <= 4 ? 2 : 1;     // warps an expert
+  const int at_once = WARPS / split, slice = warp % split;
+  const int n4 = a.H / 4 / split;                                          // (H is a multiple of 256)
+  constexpr int AHEAD = 4;                 // the first loads of the first expert go out before the row is there
+  float4 first[AHEAD];
+  {
+    const int j = warp / split;
+    const float4* g = reinterpret_cast<const float4*>(a.gate + (int64_t)(rank + j * kRouteCluster) * a.H) + slice * n4;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      first[i] = j < mine && lane + 32 * i < n4 ? __ldg(g + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   const XT* x = (const XT*)a.x + (int64_t)t * a.stride;
-  float s = 0.f;
+  float s = 0.f, m = 0.f;
+#pragma unroll 4
   for (int i = tid; i < a.H; i += kRouteThreads) {
     const float v = to_f32<XT>(x[i]);
-    row[i] = v;
+    row[i] = a.norm_w ? v * a.norm_w[i] : v;
     s = fmaf(v, v, s);
+    m = fmaxf(m, fabsf(row[i]));
   }
-  if (a.norm_w) {
-    s = block_sum<kRouteThreads>(s, red);
-    const float r = 1.0f / sqrtf(s / (float)a.H + a.eps);
-    for (int i = tid; i < a.H; i += kRouteThreads) row[i] = row[i] * r * a.norm_w[i];
-  }
-  float m = 0.f;
-  for (int i = tid; i < a.H; i += kRouteThreads) m = fmaxf(m, fabsf(row[i]));
-  m = block_max<kRouteThreads>(m, red);                        // (all of the row is there)
-  for (int i = rank * kRouteThreads + tid; i < a.H; i += kRouteCluster * kRouteThreads) a.v[(int64_t)t * a.H + i] = row[i];
-  if (rank == 0 && tid == 0) a.v_max[t] = m;
-  const int mine = (a.E - rank + kRouteCluster - 1) / kRouteCluster;       // experts rank, rank + 8, ...
-#pragma unroll 2
-  for (int j = 0; j < mine; ++j) {
-    const float4* g = reinterpret_cast<const float4*>(a.gate + (int64_t)(rank + j * kRouteCluster) * a.H);
-    double d = 0.;
-#pragma unroll 4
-    for (int i = tid; i < a.H / 4; i += kRouteThreads) {
-      const float4 w = __ldg(g + i), v = *reinterpret_cast<const float4*>(row + 4 * i);
-      d = fma((double)v.x, (double)w.x, d);
-      d = fma((double)v.y, (double)w.y, d);
-      d = fma((double)v.z, (double)w.z, d);
-      d = fma((double)v.w, (double)w.w, d);
-    }
-    d = warp_sum_d(d);
-    if (lane == 0) part[j][warp] = d;
+  s = warp_sum(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (lane == 0) {
+    red[warp] = s;
+    red[8 + warp] = m;
   }
   __syncthreads();
-  if (tid < mine) {
+  s = m = 0.f;
+  for (int w = 0; w < WARPS; ++w) {
+    s += red[w];
+    m = fmaxf(m, red[8 + w]);
+  }
+  const float r = a.norm_w ? 1.0f / sqrtf(s / (float)a.H + a.eps) : 1.0f;
+  for (int i = rank * kRouteThreads + tid; i < a.H; i += kRouteCluster * kRouteThreads) a.v[(int64_t)t * a.H + i] = row[i] * r;
+  if (rank == 0 && tid == 0) a.v_max[t] = m * r;
+  for (int j0 = 0; j0 < mine; j0 += at_once) {
+    const int j = j0 + warp / split;
     double d = 0.;
-    for (int w = 0; w < kRouteThreads / 32; ++w) d += part[tid][w];
-    logit[tid] = d;
+    if (j < mine) {
+      const float4* g = reinterpret_cast<const float4*>(a.gate + (int64_t)(rank + j * kRouteCluster) * a.H) + slice * n4;
+      const float* v = row + 4 * slice * n4;
+      double q[4] = {0., 0., 0., 0.};
+      auto add = [&](const float4& w, int i) {
+        const float4 u = *reinterpret_cast<const float4*>(v + 4 * i);
+        q[0] = fma((double)u.x, (double)w.x, q[0]);
+        q[1] = fma((double)u.y, (double)w.y, q[1]);
+        q[2] = fma((double)u.z, (double)w.z, q[2]);
+        q[3] = fma((double)u.w, (double)w.w, q[3]);
+      };
+      int i = lane;
+      if (j0 == 0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u, i += 32)
+          if (i < n4) add(first[u], i);
+      }
+#pragma unroll 8
+      for (; i < n4; i += 32) add(__ldg(g + i), i);
+      d = warp_sum_d((q[0] + q[1]) + (q[2] + q[3]));
+    }
+    if (lane == 0) part[warp] = d;
+    __syncthreads();
+    if (tid < at_once && j0 + tid < mine) {
+      double z = 0.;
+      for (int w = 0; w < split; ++w) z += part[tid * split + w];
+      logit[j0 + tid] = z * (double)r;
+    }
+    __syncthreads();
   }
   cl.sync();
-  if (rank == 0 && warp == 0) {
-    constexpr int EACH = kMaxStepExperts / 32;
-    double l[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int e = lane + 32 * i;
-      l[i] = e < a.E ? cl.map_shared_rank(logit, e % kRouteCluster)[e / kRouteCluster] : 0.;
+  if (rank == 0) {
+    // an expert a thread: how many come before it
+    double l = 0., key = 0.;
+    if (tid < a.E) {
+      l = cl.map_shared_rank(logit, tid % kRouteCluster)[tid / kRouteCluster];
+      key = l == l ? l : -INFINITY;                                     // (NaN: not before any other)
+      all[tid] = key;
     }
-    unsigned left = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) left |= (lane + 32 * i < a.E ? 1u : 0u) << i;
-    double top = 0., val = 0.;
-    int expert = 0;
-    for (int j = 0; j < a.k; ++j) {
-      double best = -INFINITY;
-      int at = 1 << 30;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const double q = l[i] == l[i] ? l[i] : -INFINITY;             // (NaN: not before any other)
-        if ((left >> i & 1) && (at == 1 << 30 || q > best)) {
-          best = q;
-          at = lane + 32 * i;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double q = __shfl_xor_sync(~0u, best, o);
-        const int i = __shfl_xor_sync(~0u, at, o);
-        if (i != 1 << 30 && (at == 1 << 30 || q > best || (q == best && i < at))) {
-          best = q;
-          at = i;
-        }
-      }
-      if ((at & 31) == lane) left &= ~(1u << (at >> 5));
-      double q = 0.;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i)
-        if (i == at >> 5) q = l[i];
-      q = __shfl_sync(~0u, q, at & 31);                                // (itself, a NaN too)
-      if (j == 0) top = best;
-      if (lane == j) {
-        expert = at;
-        val = q;
-      }
+    __syncthreads();
+    int before = a.E;
+    if (tid < a.E) {
+      before = 0;
+#pragma unroll 4
+      for (int e = 0; e < a.E; ++e) before += all[e] > key || (all[e] == key && e < tid);
     }
-    if (!(fabs(top) < INFINITY)) top = 0.;
-    const float w = lane < a.k ? expf((float)(val - top)) : 0.f;
-    const float sum = warp_sum(w) + 1e-12f;
-    if (lane < a.k) chosen[lane] = expert;
-    __syncwarp();
-    if (lane < a.k) {
-      int place = 0;
-      for (int j = 0; j < a.k; ++j) place += chosen[j] < expert;
-      a.top_e[t * a.k + place] = expert;
-      a.top_w[t * a.k + place] = w / sum;
+    const bool in = before < a.k;
+    const unsigned b = __ballot_sync(~0u, in);
+    if (lane == 0) chosen[warp] = b;
+    if (in) val[before] = l;
+    __syncthreads();
+    if (in) {
+      double top = val[0];
+      if (!(fabs(top) < INFINITY)) top = 0.;
+      float sum = 1e-12f;
+      for (int j = 0; j < a.k; ++j) sum += expf((float)(val[j] - top));
+      int place = __popc(b & ((1u << lane) - 1));
+      for (int w = 0; w < warp; ++w) place += __popc(chosen[w]);
+      a.top_e[t * a.k + place] = tid;
+      a.top_w[t * a.k + place] = expf((float)(l - top)) / sum;
     }
   }
   cl.sync();                                                  // rank 0 has read the others' logits
@@ -202,345 +216,688 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
 // ---------------------------------------------------------------------------
 // Products
 // ---------------------------------------------------------------------------
+// out[token][row] from the second products' partial results
+XM_DEV void step_output(const StepArgs& a, int token, int row) {
+  const int P = a.T * a.k;
+  float y = 0.f;
+  for (int j = 0; j < a.k; ++j) {
+    float q = 0.f;
+    for (int c = 0; c < a.chunks; ++c) q += __ldcg(a.dst + ((int64_t)c * P + token * a.k + j) * a.N + row);
+    y = fmaf(q, __ldcg(a.top_w + token * a.k + j), y);
+  }
+  if (a.residual) y += a.residual[token * a.residual_stride + row];
+  a.out[token * a.out_stride + row] = y;
+}
+
 XM_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+XM_DEV void mma_f16_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {       // the first of a sum
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+XM_DEV void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
 }
 XM_DEV uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The 256 values of K that a warp holds, of its columns: for each group of 32 the thread's 8 (8 t .. 8 t + 7 of the group,
-// t = lane % 4) as pairs (0, 2), (1, 3), (4, 6), (5, 7): the order in which words of 4-bit codes fall apart under masks.
-template <int NT>
+// How a thread's 8 values of a group of 32 of K lie (t = lane % 4): 8 t .. 8 t + 7, or, for types whose groups have 16 values
+// or whose blocks are not 8-byte aligned, 4 t .. 4 t + 3 of each half.  Either way they enter the products as the pairs (0, 2),
+// (1, 3), (4, 6), (5, 7): the order in which words of codes fall apart under masks.
+template <int T>
+constexpr bool halves() { return T == T_Q6_K || T == T_Q8_0; }
+
+// The 256 values of K that a warp holds, of M tokens: column g (= lane / 4) is token g / 2, hi or lo by g % 2 (M = 4), or token
+// g in two parts (M = 8).  By groups of 32 their pairs, and the sums over groups of 32 or 16 times 2^-5, of groups 2 t, 2 t + 1
+// (and 2 t + 8, 2 t + 9).
+template <int M>
 struct Columns {
-  uint32_t b[NT][8][4];
+  static constexpr int PARTS = M == 4 ? 1 : 2;
+  uint32_t b[PARTS][8][4];
+  uint32_t sum[PARTS][2];
 };
+// What a thread has of a tile's results: of its two rows (g, g + 8) the token t (M = 4), or the tokens 2 t, 2 t + 1 (M = 8).
+template <int M>
+struct Result {
+  static constexpr int N = M == 4 ? 1 : 2;
+  float v[2][N];
+  XM_DEV void clear() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[0][i] = v[1][i] = 0.f;
+  }
+  // v += s0 times the first row's sums, s1 times the second's
+  XM_DEV void add(const float (&c)[4], float s0, float s1) {
+    if constexpr (M == 4) {
+      v[0][0] = fmaf(s0, c[0] + c[1], v[0][0]);
+      v[1][0] = fmaf(s1, c[2] + c[3], v[1][0]);
+    } else {
+      v[0][0] = fmaf(s0, c[0], v[0][0]);
+      v[0][1] = fmaf(s0, c[1], v[0][1]);
+      v[1][0] = fmaf(s1, c[2], v[1][0]);
+      v[1][1] = fmaf(s1, c[3], v[1][1]);
+    }
+  }
+};
+
+// c = the products of 16 values of K (a: of the two rows; i: a pair of pairs of group j)
+template <int M, bool FIRST>
+XM_DEV void mma_group(float (&c)[4], const uint32_t (&a)[4], const Columns<M>& x, int j, int i) {
+  if constexpr (FIRST) mma_f16_zero(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
+  else mma_f16(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
+  if constexpr (M == 8) mma_f16(c, a, x.b[1][j][2 * i], x.b[1][j][2 * i + 1]);
+}
 
 // Types whose weights enter with the block's own value, not rounded to fp16 as dequantisation rounds it.
 template <int T>
 constexpr bool own_value() { return T == T_Q4_K || T == T_Q5_K || T == T_Q6_K || T == T_Q8_0; }
 
-// 256 values of K of sixteen rows, value by value: fp16 weights, or two fp16 each (hi + 2^-11 lo).
-template <int T, int NT>
-XM_DEV void unit_any(const uint8_t* lo_row, const uint8_t* hi_row, int t, const Columns<NT>& x, float (&acc)[NT][2]) {
+// 256 values of K of sixteen rows (r0: the thread's first row, r1: its second).
+
+// Any type, value by value: weights rounded to fp16.
+template <int T, int M>
+XM_DEV void unit_any(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = 0.f;
-#pragma unroll 1
-  for (int part = 0; part < (own_value<T>() ? 2 : 1); ++part) {
-    float c[NT][4];
+  for (int j = 0; j < 8; ++j) {
+    uint32_t w[2][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t w[2][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint8_t* p = r ? hi_row : lo_row;
-        float v[8];
-        if constexpr (QT<T>::QK == 256) QT<T>::decode8(p, 32 * j + 8 * t, v);
-        else QT<T>::decode8(p + j * QT<T>::REC, 8 * t, v);
-        if (part) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = (v[i] - __half2float(__float2half_rn(v[i]))) * 2048.f;
-        }
-        w[r][0] = pack2(v[0], v[2]);
-        w[r][1] = pack2(v[1], v[3]);
-        w[r][2] = pack2(v[4], v[6]);
-        w[r][3] = pack2(v[5], v[7]);
-      }
-      const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma_f16(c[n], a0, x.b[n][j][0], x.b[n][j][1]);
-        mma_f16(c[n], a1, x.b[n][j][2], x.b[n][j][3]);
-      }
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* p = r ? r1 : r0;
+      float v[8];
+      if constexpr (QT<T>::QK == 256) QT<T>::decode8(p, 32 * j + 8 * t, v);
+      else QT<T>::decode8(p + j * QT<T>::REC, 8 * t, v);
+      w[r][0] = pack2(v[0], v[2]);
+      w[r][1] = pack2(v[1], v[3]);
+      w[r][2] = pack2(v[4], v[6]);
+      w[r][3] = pack2(v[5], v[7]);
     }
-    const float scale = part ? 0x1p-11f : 1.f;
+    const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
+    mma_group<M, false>(c, a0, x, j, 0);
+    mma_group<M, false>(c, a1, x, j, 1);
+  }
+  acc.clear();
+  acc.add(c, 1.f, 1.f);
+}
+
+XM_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// Q4_K, and Q5_K (FIVE): w = d s_j c - dmin m_j.  A word's codes under the mask 0x000f000f are fp16 subnormals c 2^-24, under
+// 0x00f000f0 c 2^-20: no instruction makes them numbers.  s_j comes from its byte as (2^23 + s) - 2^23, for the upper codes as
+// (2^19 + s / 16) - 2^19; both are exact.
+template <bool FIVE, int M>
+XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, BIT = 0x00100010u;
+  constexpr int QS = FIVE ? 48 : 16;
+  uint32_t sc[2][2], am[2], qh[2][4];
+  float d[2], dm[2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n][0] = fmaf(scale, fmaf(c[n][1], 0x1p-11f, c[n][0]), acc[n][0]);
-      acc[n][1] = fmaf(scale, fmaf(c[n][3], 0x1p-11f, c[n][2]), acc[n][1]);
+  for (int r = 0; r < 2; ++r) {
+    const uint4 h = lds128(r ? r1 : r0);
+    const float2 dd = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
+    d[r] = dd.x * 0x1p24f;
+    dm[r] = dd.y * -0x1p29f;
+    sc[r][0] = h.y & 0x3f3f3f3fu;
+    sc[r][1] = (h.w & 0x0f0f0f0fu) | ((h.y >> 2) & 0x30303030u);
+    const uint32_t m = t < 2 ? h.z & 0x3f3f3f3fu : ((h.w >> 4) & 0x0f0f0f0fu) | ((h.z >> 2) & 0x30303030u);
+    am[r] = __byte_perm(m, 0u, t & 1 ? 0x4342 : 0x4140);      // (m_2t, m_2t+1) 2^-24
+    if constexpr (FIVE) {
+      const uint4 q = lds128((r ? r1 : r0) + 16);             // the fifth bits of groups 2 j, 2 j + 1: word j, bit = value
+      qh[r][0] = (q.x >> (8 * t)) & 0xffu;
+      qh[r][1] = (q.y >> (8 * t)) & 0xffu;
+      qh[r][2] = (q.z >> (8 * t)) & 0xffu;
+      qh[r][3] = (q.w >> (8 * t)) & 0xffu;
     }
   }
+  Result<M> sum;
+  sum.clear();
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    uint32_t lo[2][4], hi[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint2 q = *reinterpret_cast<const uint2*>((r ? r1 : r0) + QS + 32 * jj + 8 * t);
+      const uint32_t w[4] = {q.x, q.x >> 8, q.y, q.y >> 8};
+      if constexpr (FIVE) {
+        const uint32_t b = qh[r][jj], f[4] = {(b * ((1u << 4) + (1u << 18))) & BIT, (b * ((1u << 3) + (1u << 17))) & BIT,
+                                              (b * (1u + (1u << 14))) & BIT, ((b >> 1) * (1u + (1u << 14))) & BIT};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[r][i] = (w[i] & LOW) | f[i];
+          hi[r][i] = (w[i] & HIGH) | (f[i] << 4);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[r][i] = w[i] & LOW;
+          hi[r][i] = w[i] & HIGH;
+        }
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int j = 2 * jj + half;
+      const uint32_t(&q)[2][4] = half ? hi : lo;
+      const uint32_t a0[4] = {q[0][0], q[1][0], q[0][1], q[1][1]}, a1[4] = {q[0][2], q[1][2], q[0][3], q[1][3]};
+      float c[4], s[2];
+      mma_group<M, true>(c, a0, x, j, 0);
+      mma_group<M, false>(c, a1, x, j, 1);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t b = __byte_perm(sc[r][j >> 2], half ? 0x49000000u : 0x4B000000u, 0x7650 | (j & 3));
+        s[r] = __uint_as_float(b) - (half ? 0x1p19f : 0x1p23f);
+      }
+      sum.add(c, s[0], s[1]);
+    }
+  }
+  float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16_k8(c, am[0], am[1], x.sum[i][0]);
+  acc.clear();
+  acc.add(c, dm[0], dm[1]);
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int i = 0; i < Result<M>::N; ++i) acc.v[r][i] = fmaf(d[r], sum.v[r][i], acc.v[r][i]);
+}
+
+// The 32-bit word at a 2-byte aligned address.
+XM_DEV uint32_t lds_word(const uint8_t* p) {
+  const uint32_t sh = ((uint32_t)(uintptr_t)p & 2) * 8;
+  const uint32_t* a = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+  return __funnelshift_r(a[0], a[1], sh);
+}
+
+// Q6_K: w = d s_g (c - 32), groups of 16, records at any even address.  Codes are put together as bytes, four at a time.
+template <int M>
+XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  uint32_t sc[2][4];                       // s + 128, bytes
+  float d[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const uint8_t* p = r ? r1 : r0;
+    // words of the scales at 192 and of d behind them
+    const uint32_t sh = ((uint32_t)(uintptr_t)p & 2) * 8;
+    const uint32_t* a = reinterpret_cast<const uint32_t*>((reinterpret_cast<uintptr_t>(p) + 192) & ~(uintptr_t)3);
+    const uint32_t w[5] = {a[0], a[1], a[2], a[3], a[4]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[r][i] = __funnelshift_r(w[i], w[i + 1], sh) ^ 0x80808080u;
+    const uint32_t dw = w[4] >> sh;
+    d[r] = __half2float(__ushort_as_half((unsigned short)dw)) * 0x1p24f;
+  }
+  Result<M> sum;
+  sum.clear();
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t low[2][2], high[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint8_t* q = r ? r1 : r0;
+        low[r][0] = lds_word(q + 64 * h + 16 * p + 4 * t);
+        low[r][1] = lds_word(q + 64 * h + 32 + 16 * p + 4 * t);
+        high[r] = lds_word(q + 128 + 32 * h + 16 * p + 4 * t);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int g = 8 * h + 2 * i + p;                          // the group of 16
+        uint32_t q[2][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t nib = (i < 2 ? low[r][i & 1] : low[r][i & 1] >> 4) & 0x0f0f0f0fu;
+          const uint32_t two = (i == 0 ? high[r] << 4 : i == 1 ? high[r] << 2 : i == 2 ? high[r] : high[r] >> 2) & 0x30303030u;
+          const uint32_t c4 = nib | two;
+          q[r][0] = c4 & 0x00ff00ffu;
+          q[r][1] = (c4 >> 8) & 0x00ff00ffu;
+        }
+        const uint32_t a[4] = {q[0][0], q[1][0], q[0][1], q[1][1]};
+        float c[4], s[2];
+        mma_group<M, true>(c, a, x, g >> 1, g & 1);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          s[r] = __uint_as_float(__byte_perm(sc[r][g >> 2], 0x4B000000u, 0x7650 | (g & 3))) - (0x1p23f + 128.f);
+        sum.add(c, s[0], s[1]);
+      }
+    }
+  // offsets: -32 sum s_g S_g, the scales as fp16 (1024 + byte) - 1152
+  uint32_t o[2][2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t w = t < 2 ? sc[r][2 * i] : sc[r][2 * i + 1];
+      const uint32_t u = __byte_perm(w, 0x64646464u, t & 1 ? 0x4342 : 0x4140);
+      const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
+      o[r][i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  float c[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t a[4] = {o[0][0], o[1][0], o[0][1], o[1][1]};
+#pragma unroll
+  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16(c, a, x.sum[i][0], x.sum[i][1]);
+  acc.clear();
+  acc.add(c, d[0] * -0x1p-14f, d[1] * -0x1p-14f);                 // (2^-24 of d, 2^5 of the sums, 2^5)
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int i = 0; i < Result<M>::N; ++i) acc.v[r][i] = fmaf(d[r], sum.v[r][i], acc.v[r][i]);
+}
+
+// Q8_0: w = d_j c, eight records of 34 bytes; the codes enter as c + 128, and -128 sum d_j S_j as the offsets' product.
+template <int M>
+XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  uint32_t dd[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const uint8_t* p = (r ? r1 : r0) + 68 * t;
+    dd[r] = (uint32_t)*reinterpret_cast<const unsigned short*>(p) | (uint32_t)*reinterpret_cast<const unsigned short*>(p + 34) << 16;
+  }
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16_k8(o, dd[0], dd[1], x.sum[i][0]);
+  acc.clear();
+  acc.add(o, -0x1p12f, -0x1p12f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t w[2][2];
+    float s[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* p = (r ? r1 : r0) + 34 * j + 2 + 4 * t;
+      if (j & 1) {
+        w[r][0] = *reinterpret_cast<const uint32_t*>(p);
+        w[r][1] = *reinterpret_cast<const uint32_t*>(p + 16);
+      } else {
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(p - 2);
+        w[r][0] = __funnelshift_r(a[0], a[1], 16);
+        w[r][1] = __funnelshift_r(a[4], a[5], 16);
+      }
+      w[r][0] ^= 0x80808080u;
+      w[r][1] ^= 0x80808080u;
+      const uint32_t u = __shfl_sync(~0u, dd[r], (threadIdx.x & 28) | (j >> 1));
+      s[r] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xffffu))) * 0x1p24f;
+    }
+    constexpr uint32_t K = 0x00ff00ffu;
+    const uint32_t a0[4] = {w[0][0] & K, w[1][0] & K, (w[0][0] >> 8) & K, (w[1][0] >> 8) & K};
+    const uint32_t a1[4] = {w[0][1] & K, w[1][1] & K, (w[0][1] >> 8) & K, (w[1][1] >> 8) & K};
+    float c[4];
+    mma_group<M, true>(c, a0, x, j, 0);
+    mma_group<M, false>(c, a1, x, j, 1);
+    acc.add(c, s[0], s[1]);
+  }
+}
+
+template <int T, int M>
+XM_DEV void unit(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  if constexpr (T == T_Q4_K) unit_k<false, M>(r0, r1, t, x, acc);
+  else if constexpr (T == T_Q5_K) unit_k<true, M>(r0, r1, t, x, acc);
+  else if constexpr (T == T_Q6_K) unit_q6k<M>(r0, r1, t, x, acc);
+  else if constexpr (T == T_Q8_0) unit_q80<M>(r0, r1, t, x, acc);
+  else unit_any<T, M>(r0, r1, t, x, acc);
 }
 
 template <int T>
 constexpr int block_bytes() { return QT<T>::QK == 256 ? QT<T>::REC : 8 * QT<T>::REC; }   // of 256 values
 
-template <int T, int NT, bool UP>
+template <int T, int M, bool UP>
+struct Step {
+  static constexpr int RB = block_bytes<T>(), N = Result<M>::N;
+  const StepArgs& a;
+  StepShared& sm;
+  uint8_t* ring;
+  float* red;                              // [ring][warp][lane][2 N]
+  int lane, warp, g, t, P, per_seg, stage_bytes, s0, s1;
+
+  XM_DEV Step(const StepArgs& a_, StepShared& s, uint8_t* dyn) : a(a_), sm(s), ring(dyn) {
+    lane = threadIdx.x & 31;
+    warp = threadIdx.x >> 5;
+    g = lane >> 2;
+    t = lane & 3;
+    P = a.T * a.k;
+    stage_bytes = 16 * a.tps * a.pitch;
+    red = reinterpret_cast<float*>(dyn + a.ring * stage_bytes);
+    per_seg = a.chunks * a.groups;         // stages of a segment: (chunk, group of tiles)
+  }
+  // A stage's place, and the next one's.
+  struct Where {
+    int seg, chunk, group, slot, lap;
+  };
+  XM_DEV Where where(int s) const {
+    Where w;
+    w.seg = s / per_seg;
+    const int in = s - w.seg * per_seg;
+    w.chunk = in / a.groups;
+    w.group = in - w.chunk * a.groups;
+    w.lap = (s - s0) / a.ring;
+    w.slot = (s - s0) - w.lap * a.ring;
+    return w;
+  }
+  XM_DEV void next(Where& w) const {
+    if (++w.group == a.groups) {
+      w.group = 0;
+      if (++w.chunk == a.chunks) {
+        w.chunk = 0;
+        ++w.seg;
+      }
+    }
+    if (++w.slot == a.ring) {
+      w.slot = 0;
+      ++w.lap;
+    }
+  }
+  XM_DEV int tiles_of(const Where& w) const { return min(a.tps, a.tiles - w.group * a.tps); }
+
+  // Which pairs go to which expert, and the segments: an expert and up to M of its pairs.
+  XM_DEV void segments() {
+    for (int i = threadIdx.x; i < P; i += kStepThreads) sm.expert[i] = (unsigned short)__ldcg(a.top_e + i);
+    for (int e = threadIdx.x; e < a.E; e += kStepThreads) sm.cnt[e] = 0;
+    __syncthreads();
+    if (warp == 0) {
+      for (int i0 = 0; i0 < P; i0 += 32) {
+        const int i = i0 + lane, e = i < P ? sm.expert[i] : -1 - lane;
+        const unsigned same = __match_any_sync(~0u, e);
+        const int before = i < P ? sm.cnt[e] : 0;
+        __syncwarp();
+        if (i < P) {
+          sm.rank[i] = (unsigned short)(before + __popc(same & ((1u << lane) - 1)));
+          if (lane == __ffs(same) - 1) sm.cnt[e] = before + __popc(same);
+        }
+        __syncwarp();
+      }
+      int at = 0, segs = 0;
+      for (int e0 = 0; e0 < a.E; e0 += 32) {
+        const int e = e0 + lane, n = e < a.E ? sm.cnt[e] : 0, s = (n + M - 1) / M;
+        int sum = n | s << 16;             // (both sums stay below 2^15)
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(~0u, sum, o);
+          if (lane >= o) sum += u;
+        }
+        const int first = at + (sum & 0xffff) - n, seg = segs + (sum >> 16) - s;
+        if (e < a.E) sm.off[e] = first;
+        for (int i = 0; i < s; ++i) {
+          sm.seg_e[seg + i] = (unsigned short)e;
+          sm.seg_at[seg + i] = (unsigned short)(first + i * M);
+          sm.seg_n[seg + i] = (unsigned short)min(M, n - i * M);
+        }
+        const int all = __shfl_sync(~0u, sum, 31);
+        at += all & 0xffff;
+        segs += all >> 16;
+      }
+      if (lane == 0) sm.n_seg = segs;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < P; i += kStepThreads) sm.pair[sm.off[sm.expert[i]] + sm.rank[i]] = (unsigned short)i;
+    const int64_t total = (int64_t)sm.n_seg * per_seg;
+    s0 = (int)(total * blockIdx.x / gridDim.x);
+    s1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    __syncthreads();
+  }
+
+  // Has the stage's rows copied to its slot (one warp).
+  XM_DEV void fill(int s) {
+    const Where w = where(s);
+    const int e = sm.seg_e[w.seg], rows = 16 * tiles_of(w), len = min(a.kc, a.nsb - w.chunk * a.kc) * RB;
+    const int first = w.group * a.tps * (UP ? 8 : 16);                    // the stage's first row
+    const int64_t col = (int64_t)w.chunk * a.kc * RB;
+    const uint8_t* w1 = (const uint8_t*)a.w1[e] + col;
+    const uint8_t* w3 = UP ? (const uint8_t*)a.w3[e] + col : nullptr;
+    auto from = [&](int r) {               // row r of the stage: its address
+      if (UP) return (r & 8 ? w3 : w1) + (int64_t)(first + (r >> 4) * 8 + (r & 7)) * a.row_bytes;
+      return w1 + (int64_t)(first + r) * a.row_bytes;
+    };
+    // (whole units of 16 bytes; only types whose 256 values do not fill them begin inside one)
+    auto size = [&](const uint8_t* p) { return (uint32_t)(((uintptr_t)p & 15) + len + 15) & ~15u; };
+    uint32_t bytes = 0;
+    if (RB % 16 == 0) {
+      bytes = rows * len;
+    } else {
+      for (int r = lane; r < rows; r += 32) bytes += size(from(r));
+      bytes = __reduce_add_sync(~0u, bytes);
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&sm.full[w.slot], bytes);
+    __syncwarp();
+    for (int r = lane; r < rows; r += 32) {
+      const uint8_t* p = from(r);
+      bulk_g2s(ring + w.slot * stage_bytes + r * a.pitch, (const void*)((uintptr_t)p & ~(uintptr_t)15), size(p), &sm.full[w.slot]);
+    }
+  }
+
+  // This warp's activations of a segment and a chunk.
+  XM_DEV void load_columns(Columns<M>& x, int seg, int k0, bool mine) {
+    const int col = M == 4 ? g >> 1 : g;
+    const bool there = mine && col < sm.seg_n[seg], rest = M == 4 && (g & 1);      // (this column has the low parts)
+    const int pair = there ? sm.pair[sm.seg_at[seg] + col] : 0, row = UP ? pair / a.k : pair;
+    const float inv = ldexpf(1.0f, -fp16_row_shift(there ? __ldcg(a.src_max + row) : 0.f));
+    const float* p = a.src + (int64_t)row * a.K + k0 + (halves<T>() ? 4 : 8) * t;
+    auto low = [](float v) { return v - __half2float(__float2half_rn(v)); };
+    float part[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v[8];
+      if (there) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(p + 32 * j)),
+                     w = __ldcg(reinterpret_cast<const float4*>(p + 32 * j + (halves<T>() ? 16 : 4)));
+        v[0] = u.x * inv; v[1] = u.y * inv; v[2] = u.z * inv; v[3] = u.w * inv;
+        v[4] = w.x * inv; v[5] = w.y * inv; v[6] = w.z * inv; v[7] = w.w * inv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      }
+      part[2 * j] = (v[0] + v[1]) + (v[2] + v[3]);
+      part[2 * j + 1] = (v[4] + v[5]) + (v[6] + v[7]);
+#pragma unroll
+      for (int q = 0; q < Columns<M>::PARTS; ++q) {
+        if (q || rest) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = low(v[i]);
+        }
+        x.b[q][j][0] = pack2(v[0], v[2]);
+        x.b[q][j][1] = pack2(v[1], v[3]);
+        x.b[q][j][2] = pack2(v[4], v[6]);
+        x.b[q][j][3] = pack2(v[5], v[7]);
+      }
+    }
+    if constexpr (own_value<T>()) {
+      constexpr int G = T == T_Q6_K ? 16 : 8;
+      float q[4] = {0.f, 0.f, 0.f, 0.f};                       // sums of groups 2 t, 2 t + 1 (, 2 t + 8, 2 t + 9)
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        float z = G == 16 ? part[i] : part[2 * i] + part[2 * i + 1];
+        z += __shfl_xor_sync(~0u, z, 1);
+        z += __shfl_xor_sync(~0u, z, 2);
+        if ((i & 7) >> 1 == t) q[(i >> 3) * 2 + (i & 1)] = z * 0x1p-5f;
+      }
+#pragma unroll
+      for (int c = 0; c < Columns<M>::PARTS; ++c) {
+        if (c || rest) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = low(q[i]);
+        }
+        x.sum[c][0] = pack2(q[0], q[1]);
+        x.sum[c][1] = pack2(q[2], q[3]);
+      }
+    }
+  }
+
+  // Whether this warp is the one that writes the last of `all` results under a ticket.
+  XM_DEV bool last(int* ticket, int all) {
+    __threadfence();
+    __syncwarp();
+    int old = 0;
+    if (lane == 0) old = atomicAdd(ticket, 1);
+    old = __shfl_sync(~0u, old, 0);
+    if (old != all - 1) return false;
+    __threadfence();
+    return true;
+  }
+
+  // The stage's end: its results are added up, its slot is filled again, the results are written (one warp).
+  XM_DEV void finish(int s, float (&most)[N], int& most_of) {
+    const Where w = where(s);
+    const int at = sm.seg_at[w.seg], n_pairs = sm.seg_n[w.seg], kc = min(a.kc, a.nsb - w.chunk * a.kc);
+    const int tiles = tiles_of(w), tile0 = w.group * a.tps;
+    int pair[N];
+    float scale[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = M == 4 ? t : 2 * t + n;
+      pair[n] = i < n_pairs ? sm.pair[at + i] : -1;
+      scale[n] = pair[n] < 0 ? 0.f : ldexpf(1.0f, fp16_row_shift(__ldcg(a.src_max + (UP ? pair[n] / a.k : pair[n]))));
+    }
+    if (UP && most_of != w.seg) {
+      most_of = w.seg;
+#pragma unroll
+      for (int n = 0; n < N; ++n) most[n] = 0.f;
+    }
+    auto result = [&](int n, int i, float gate, float up) {       // a feature of the first products
+      const float y = xm_act(a.act, gate) * up;
+      a.dst[(int64_t)pair[n] * a.N + (tile0 + i) * 8 + g] = y;
+      if (fabsf(y) > most[n]) {
+        most[n] = fabsf(y);
+        atomicMax(a.dst_max + pair[n], __float_as_uint(most[n]));
+      }
+    };
+    mbar_wait_bounded(&sm.done[w.slot], w.lap & 1);
+    for (int i = 0; i < tiles; ++i) {
+      Result<M> v;
+      v.clear();
+      const float* r = red + ((w.slot * kWorkers + i * a.kc) * 32 + lane) * 2 * N;
+#pragma unroll 4
+      for (int q = 0; q < kc; ++q) {
+        if constexpr (N == 1) {
+          const float2 u = *reinterpret_cast<const float2*>(r + q * 64);
+          v.v[0][0] += u.x;
+          v.v[1][0] += u.y;
+        } else {
+          const float4 u = *reinterpret_cast<const float4*>(r + q * 128);
+          v.v[0][0] += u.x;
+          v.v[0][1] += u.y;
+          v.v[1][0] += u.z;
+          v.v[1][1] += u.w;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (pair[n] < 0) continue;
+        const float y0 = v.v[0][n] * scale[n], y1 = v.v[1][n] * scale[n];
+        if (!UP) {
+          float* p = a.dst + ((int64_t)w.chunk * P + pair[n]) * a.N + (tile0 + i) * 16 + g;
+          p[0] = y0;
+          p[8] = y1;
+        } else if (a.chunks == 1) {
+          result(n, i, y0, y1);
+        } else {
+          float* p = a.part + ((int64_t)w.chunk * P + pair[n]) * 2 * a.N + (tile0 + i) * 8 + g;
+          p[0] = y0;
+          p[a.N] = y1;
+        }
+      }
+    }
+    __syncwarp();
+    if (s + a.ring < s1) fill(s + a.ring);
+    if (UP && a.chunks > 1 && last(a.tickets + w.seg * a.groups + w.group, a.chunks)) {
+      for (int i = 0; i < tiles; ++i) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (pair[n] < 0) continue;
+          float gate = 0.f, up = 0.f;
+          for (int q = 0; q < a.chunks; ++q) {
+            const float* p = a.part + ((int64_t)q * P + pair[n]) * 2 * a.N + (tile0 + i) * 8 + g;
+            gate += __ldcg(p);
+            up += __ldcg(p + a.N);
+          }
+          result(n, i, gate, up);
+        }
+      }
+      __syncwarp();
+    }
+    if (!UP && a.tickets && last(a.tickets + w.group, sm.n_seg * a.chunks)) {
+      const int rows = 16 * tiles;
+      for (int i = lane; i < rows * a.T; i += 32) {
+        const int tok = i / rows;
+        step_output(a, tok, tile0 * 16 + i - tok * rows);
+      }
+      __syncwarp();
+    }
+  }
+
+  XM_DEV void run() {
+    const int my_tile = warp / a.kc, my_sb = warp - my_tile * a.kc;
+    const int mine_at = (my_tile * 16 + g) * a.pitch + my_sb * RB;
+    Columns<M> x;
+    int held = -1, most_of = -1;
+    float most[N];
+    Where w = where(s0);
+    // a stage's end one stage after it: by then the other warps have done it too
+    for (int s = s0; s <= s1 && s0 < s1; ++s, next(w)) {
+      if (s < s1) {
+        const bool in_k = my_tile < a.tps && w.chunk * a.kc + my_sb < a.nsb;
+        const int k = w.seg * a.chunks + w.chunk;
+        if (held != k) {
+          held = k;
+          load_columns(x, w.seg, (w.chunk * a.kc + my_sb) * 256, in_k);
+        }
+        mbar_wait_bounded(&sm.full[w.slot], w.lap & 1);
+        if (in_k && my_tile < tiles_of(w)) {
+          const uint8_t* r0 = ring + w.slot * stage_bytes + mine_at;
+          const uint8_t* r1 = r0 + 8 * a.pitch;
+          if constexpr (RB % 16 != 0) {    // (a row's bytes begin where they do in 16 bytes of the weight)
+            const int tile = w.group * a.tps + my_tile, n = UP ? tile * 8 + g : tile * 16 + g;
+            const int64_t col = (int64_t)w.chunk * a.kc * RB;
+            r0 += (int)(n * a.row_bytes + col) & 15;
+            r1 += (int)((UP ? n : n + 8) * a.row_bytes + col) & 15;
+          }
+          Result<M> acc;
+          unit<T, M>(r0, r1, t, x, acc);
+          float* r = red + ((w.slot * kWorkers + warp) * 32 + lane) * 2 * N;
+          if constexpr (N == 1) *reinterpret_cast<float2*>(r) = make_float2(acc.v[0][0], acc.v[1][0]);
+          else *reinterpret_cast<float4*>(r) = make_float4(acc.v[0][0], acc.v[0][1], acc.v[1][0], acc.v[1][1]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.done[w.slot]);
+      }
+      if (s > s0 && (s - 1 - s0) % kWorkers == warp) finish(s - 1, most, most_of);
+    }
+  }
+};
+
+template <int T, int M, bool UP>
 __global__ void __launch_bounds__(kStepThreads, 1) k_moe_step(StepArgs a) {
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ StepShared sm;
-  constexpr int RB = block_bytes<T>(), COLS = 4 * NT;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int stage_bytes = 16 * a.tps * a.pitch;
-  uint8_t* ring = dyn;
-  float* red = reinterpret_cast<float*>(dyn + a.ring * stage_bytes);       // [ring][worker][lane][2 NT]
-  if (UP) grid_dep_wait();
-  grid_dep_launch();
-  // Which pairs go to which expert, and the segments (an expert and up to COLS of its pairs): from the routing, which is
-  // complete before the launch of DOWN can begin (UP waits for it before it lets DOWN start).
-  const int P = a.T * a.k;
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
     for (int i = 0; i < a.ring; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.done[i], kWorkers);
     }
     fence_mbar_init();
   }
-  for (int e = warp; e < a.E; e += kWorkers + 1) {
-    int n = 0;
-    for (int i = lane; i < (P + 31) / 32 * 32; i += 32) n += __popc(__ballot_sync(~0u, i < P && __ldcg(a.top_e + i) == e));
-    if (lane == 0) sm.cnt[e] = n;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int at = 0, segs = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 32) {
-      const int e = e0 + lane, n = e < a.E ? sm.cnt[e] : 0, s = (n + COLS - 1) / COLS;
-      int pn = n, ps = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(~0u, pn, o), v = __shfl_up_sync(~0u, ps, o);
-        if (lane >= o) {
-          pn += u;
-          ps += v;
-        }
-      }
-      if (e < a.E) sm.off[e] = at + pn - n;
-      for (int i = 0; i < s; ++i) {
-        const int g = segs + ps - s + i;
-        sm.seg_e[g] = (unsigned short)e;
-        sm.seg_at[g] = (unsigned short)(at + pn - n + i * COLS);
-        sm.seg_n[g] = (unsigned short)min(COLS, n - i * COLS);
-      }
-      at += __shfl_sync(~0u, pn, 31);
-      segs += __shfl_sync(~0u, ps, 31);
-    }
-    if (lane == 0) sm.n_seg = segs;
-  }
-  __syncthreads();
-  for (int e = warp; e < a.E; e += kWorkers + 1) {
-    if (sm.cnt[e] == 0) continue;
-    int at = sm.off[e];
-    for (int i = lane; i < (P + 31) / 32 * 32; i += 32) {
-      const bool is = i < P && __ldcg(a.top_e + i) == e;
-      const unsigned b = __ballot_sync(~0u, is);
-      if (is) sm.pair[at + __popc(b & ((1u << lane) - 1))] = (unsigned short)i;
-      at += __popc(b);
-    }
-  }
-  __syncthreads();
-  const int per_seg = a.chunks * a.groups;                     // stages of a segment: (chunk, group of tiles)
-  const int64_t total = (int64_t)sm.n_seg * per_seg;
-  const int s0 = (int)(total * blockIdx.x / gridDim.x), s1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-
-  if (warp == kWorkers) {
-    // -- copies and results ------------------------------------------------
-    const int g = lane >> 2, t = lane & 3;
-    auto issue = [&](int s) {
-      const int slot = (s - s0) % a.ring, seg = s / per_seg, c = s % per_seg / a.groups, grp = s % a.groups;
-      const int e = sm.seg_e[seg], tile0 = grp * a.tps, rows = 16 * min(a.tps, a.tiles - tile0);
-      const int len = min(a.kc, a.nsb - c * a.kc) * RB;
-      const uint8_t* w1 = (const uint8_t*)a.w1[e];
-      const uint8_t* w3 = UP ? (const uint8_t*)a.w3[e] : nullptr;
-      uint32_t bytes = 0;
-      auto from = [&](int r) {                                 // row r of the stage: its address
-        const int tile = tile0 + r / 16, i = r % 16;
-        const uint8_t* base = UP && i >= 8 ? w3 : w1;
-        const int64_t n = UP ? tile * 8 + i % 8 : tile * 16 + i;
-        return base + n * a.row_bytes + (int64_t)c * a.kc * RB;
-      };
-      auto size = [&](const uint8_t* p) { return (uint32_t)(((uintptr_t)p & 15) + len + 15) & ~15u; };
-      for (int r = lane; r < rows; r += 32) bytes += size(from(r));
-      bytes = __reduce_add_sync(~0u, bytes);
-      if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], bytes);
-      __syncwarp();
-      for (int r = lane; r < rows; r += 32) {
-        const uint8_t* p = from(r);
-        bulk_g2s(ring + slot * stage_bytes + r * a.pitch, (const void*)((uintptr_t)p & ~(uintptr_t)15), size(p), &sm.full[slot]);
-      }
-    };
-    for (int s = s0; s < min(s1, s0 + a.ring); ++s) issue(s);
-    if (!UP) grid_dep_wait();
-    float most[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) most[n] = 0.f;
-    for (int s = s0; s < s1; ++s) {
-      const int slot = (s - s0) % a.ring, lap = (s - s0) / a.ring;
-      const int seg = s / per_seg, c = s % per_seg / a.groups, grp = s % a.groups;
-      const int tile0 = grp * a.tps, tiles = min(a.tps, a.tiles - tile0);
-      const int at = sm.seg_at[seg], n_pairs = sm.seg_n[seg], kc = min(a.kc, a.nsb - c * a.kc);
-      mbar_wait_bounded(&sm.done[slot], lap & 1);
-      for (int i = 0; i < tiles; ++i) {
-        float v[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) v[n][0] = v[n][1] = 0.f;
-        const float* r = red + ((slot * kWorkers + i * a.kc) * 32 + lane) * 2 * NT;
-        for (int w = 0; w < kc; ++w) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float2 q = *reinterpret_cast<const float2*>(r + w * 64 * NT + 2 * n);
-            v[n][0] += q.x;
-            v[n][1] += q.y;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (4 * n + t >= n_pairs) continue;
-          const int pair = sm.pair[at + 4 * n + t];
-          const float scale = ldexpf(1.0f, fp16_row_shift(__ldcg(a.src_max + (UP ? pair / a.k : pair))));
-          if (UP) {
-            const int f = (tile0 + i) * 8 + g;
-            const float gate = v[n][0] * scale, up = v[n][1] * scale;
-            if (a.chunks == 1) {
-              const float y = xm_act(a.act, gate) * up;
-              a.dst[(int64_t)pair * a.N + f] = y;
-              most[n] = fmaxf(most[n], fabsf(y));
-            } else {
-              float* p = a.part + ((int64_t)c * P + pair) * 2 * a.N + f;
-              p[0] = gate;
-              p[a.N] = up;
-            }
-          } else {
-            float* p = a.dst + ((int64_t)c * P + pair) * a.N + (tile0 + i) * 16 + g;
-            p[0] = v[n][0] * scale;
-            p[8] = v[n][1] * scale;
-          }
-        }
-      }
-      __syncwarp();
-      if (s + a.ring < s1) issue(s + a.ring);
-      const bool ends = s + 1 == s1 || (s + 1) / per_seg != seg;
-      if (UP && a.chunks > 1) {
-        // the last chunk's writer of these tiles takes the chunks together
-        __threadfence();
-        __syncwarp();
-        int old = 0;
-        if (lane == 0) old = atomicAdd(a.tickets + seg * a.groups + grp, 1);
-        old = __shfl_sync(~0u, old, 0);
-        if (old == a.chunks - 1) {
-          __threadfence();
-          for (int i = 0; i < tiles; ++i) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if (4 * n + t >= n_pairs) continue;
-              const int pair = sm.pair[at + 4 * n + t], f = (tile0 + i) * 8 + g;
-              float gate = 0.f, up = 0.f;
-              for (int q = 0; q < a.chunks; ++q) {
-                const float* p = a.part + ((int64_t)q * P + pair) * 2 * a.N + f;
-                gate += __ldcg(p);
-                up += __ldcg(p + a.N);
-              }
-              const float y = xm_act(a.act, gate) * up;
-              a.dst[(int64_t)pair * a.N + f] = y;
-              most[n] = fmaxf(most[n], fabsf(y));
-            }
-          }
-          __syncwarp();
-        }
-      }
-      if (UP && ends) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float m = most[n];
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-          if (g == 0 && 4 * n + t < n_pairs) atomicMax(a.dst_max + sm.pair[at + 4 * n + t], __float_as_uint(m));
-          most[n] = 0.f;
-        }
-      }
-      if (!UP) {
-        __threadfence();
-        __syncwarp();
-        int old = 0;
-        if (lane == 0) old = atomicAdd(a.tickets + grp, 1);
-        old = __shfl_sync(~0u, old, 0);
-        if (old == sm.n_seg * a.chunks - 1) {
-          __threadfence();
-          const int rows = 16 * tiles;
-          for (int i = lane; i < rows * a.T; i += 32) {
-            const int tok = i / rows, row = tile0 * 16 + i % rows;
-            float y = 0.f;
-            for (int j = 0; j < a.k; ++j) {
-              float q = 0.f;
-              for (int ch = 0; ch < a.chunks; ++ch) q += __ldcg(a.dst + ((int64_t)ch * P + tok * a.k + j) * a.N + row);
-              y = fmaf(q, __ldcg(a.top_w + tok * a.k + j), y);
-            }
-            if (a.residual) y += a.residual[tok * a.residual_stride + row];
-            a.out[tok * a.out_stride + row] = y;
-          }
-          __syncwarp();
-        }
-      }
-    }
-    return;
-  }
-
-  // -- products --------------------------------------------------------------
+  // DOWN reads the routing before its wait: it is complete before DOWN can start, since UP waits for it and only then lets
+  // DOWN start
+  if (UP) grid_dep_wait();
+  grid_dep_launch();
+  Step<T, M, UP> step(a, sm, dyn);
+  step.segments();
+  if (step.warp == 0)
+    for (int s = step.s0; s < min(step.s1, step.s0 + a.ring); ++s) step.fill(s);
   if (!UP) grid_dep_wait();
-  const int g = lane >> 2, t = lane & 3;
-  const int my_tile = warp / a.kc, my_sb = warp % a.kc;
-  Columns<NT> x;
-  int held = -1;
-  for (int s = s0; s < s1; ++s) {
-    const int slot = (s - s0) % a.ring, lap = (s - s0) / a.ring;
-    const int seg = s / per_seg, c = s % per_seg / a.groups, grp = s % a.groups;
-    const bool mine = my_tile < min(a.tps, a.tiles - grp * a.tps) && my_tile < a.tps && c * a.kc + my_sb < a.nsb;
-    if (held != s / a.groups) {
-      // this segment's activations: column g is token g / 2 of the segment's, hi or lo
-      held = s / a.groups;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int col = 4 * n + (g >> 1);
-        const bool there = mine && col < sm.seg_n[seg];
-        const int pair = there ? sm.pair[sm.seg_at[seg] + col] : 0, row = UP ? pair / a.k : pair;
-        const float inv = ldexpf(1.0f, -fp16_row_shift(there ? __ldcg(a.src_max + row) : 0.f));
-        const float* p = a.src + (int64_t)row * a.K + (int64_t)(c * a.kc + my_sb) * 256 + 8 * t;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float v[8];
-          if (there) {
-            const float4 u = __ldcg(reinterpret_cast<const float4*>(p + 32 * j)),
-                         w = __ldcg(reinterpret_cast<const float4*>(p + 32 * j + 4));
-            v[0] = u.x * inv; v[1] = u.y * inv; v[2] = u.z * inv; v[3] = u.w * inv;
-            v[4] = w.x * inv; v[5] = w.y * inv; v[6] = w.z * inv; v[7] = w.w * inv;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-          }
-          if (g & 1) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (v[i] - __half2float(__float2half_rn(v[i]))) * 2048.f;
-          }
-          x.b[n][j][0] = pack2(v[0], v[2]);
-          x.b[n][j][1] = pack2(v[1], v[3]);
-          x.b[n][j][2] = pack2(v[4], v[6]);
-          x.b[n][j][3] = pack2(v[5], v[7]);
-        }
-      }
-    }
-    mbar_wait_bounded(&sm.full[slot], lap & 1);
-    if (mine) {
-      const uint8_t* rows = ring + slot * stage_bytes + my_tile * 16 * a.pitch + my_sb * RB;
-      // (a row's bytes begin where they do in 16 bytes of the weight)
-      const int tile = grp * a.tps + my_tile;
-      auto start = [&](int i) {
-        const int64_t n = UP ? tile * 8 + i % 8 : tile * 16 + i;
-        return rows + i * a.pitch + (int)((n * a.row_bytes + (int64_t)c * a.kc * RB) & 15);
-      };
-      float acc[NT][2];
-      unit_any<T, NT>(start(g), start(g + 8), t, x, acc);
-      float* r = red + ((slot * kWorkers + warp) * 32 + lane) * 2 * NT;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(r + 2 * n) = make_float2(acc[n][0], acc[n][1]);
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.done[slot]);
-  }
+  step.run();
+}
+
+// The outputs by themselves, a thread each: for so many that the last writer's warp would be long at it.
+__global__ void __launch_bounds__(256) k_moe_step_sum(StepArgs a) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  step_output(a, blockIdx.y, row);
 }
 
 // ---------------------------------------------------------------------------
@@ -550,8 +907,8 @@ struct Plan {
   int nsb, chunks, kc, tps, tiles, groups, pitch, ring, smem;
 };
 
-// K values a row, `tiles` tiles of sixteen rows, rb bytes of 256 values, NT groups of four columns
-Plan plan(int64_t K, int64_t tiles, int rb, int NT) {
+// K values a row, `tiles` tiles of sixteen rows, rb bytes of 256 values, M tokens
+Plan plan(int64_t K, int64_t tiles, int rb, int M, bool half) {
   Plan p;
   p.nsb = (int)(K / 256);
   p.chunks = (p.nsb + kWorkers - 1) / kWorkers;
@@ -560,10 +917,12 @@ Plan plan(int64_t K, int64_t tiles, int rb, int NT) {
   p.tps = kWorkers / p.kc;
   p.tiles = (int)tiles;
   p.groups = (p.tiles + p.tps - 1) / p.tps;
-  // rows 32 bytes apart modulo 64: four rows of the words that four lanes read fall on different banks
-  p.pitch = (p.kc * rb + 15 + 31) / 32 * 32;
-  if (p.pitch % 64 == 0) p.pitch += 32;
-  const int stage = 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * NT * 4;
+  // what the four lanes of a row read falls on other banks than the next rows': 8 bytes each, rows 32 bytes apart modulo 64;
+  // of types read by 4 bytes (half) 16 bytes apart modulo 32
+  p.pitch = (p.kc * rb + 15 + 15) / 16 * 16;
+  if (half) p.pitch += p.pitch % 32 == 0 ? 16 : 0;
+  else p.pitch += p.pitch % 64 == 32 ? 0 : (96 - p.pitch % 64) % 64;
+  const int stage = 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M / 4) * 4;
   p.ring = std::min(kMaxRing, (int)(212 * 1024 / (stage + red)));
   p.smem = p.ring * (stage + red);
   return p;
@@ -573,6 +932,7 @@ struct Layout {
   int64_t top_e, top_w, v, v_max, a, a_max, part, tickets, up_part, bytes;
   int n_tickets;
 };
+// (pitch, ring and smem of these plans are not used)
 Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb) {
   Layout l;
   int64_t at = 0;
@@ -582,7 +942,7 @@ Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb) {
     return o;
   };
   const int64_t P = T * k;
-  const Plan up = plan(H, F / 8, rb, 1), down = plan(F, H / 16, rb, 1);
+  const Plan up = plan(H, F / 8, rb, 4, false), down = plan(F, H / 16, rb, 4, false);
   l.top_e = take(P);
   l.top_w = take(P);
   l.v = take(T * H);
@@ -617,7 +977,7 @@ cudaError_t step_launch(void (*kernel)(KArgs...), dim3 grid, int threads, int sm
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int T, int NT>
+template <int T, int M>
 cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cudaStream_t st) {
   const int sms = xm_sm_count();
   auto fill = [](StepArgs& a, const Plan& p) {
@@ -631,12 +991,19 @@ cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cuda
     a.ring = p.ring;
     a.row_bytes = (int64_t)p.nsb * block_bytes<T>();
   };
-  const Plan pu = plan(H, F / 8, block_bytes<T>(), NT), pd = plan(F, H / 16, block_bytes<T>(), NT);
+  const Plan pu = plan(H, F / 8, block_bytes<T>(), M, halves<T>()), pd = plan(F, H / 16, block_bytes<T>(), M, halves<T>());
   fill(up, pu);
   fill(down, pd);
-  cudaError_t e = step_launch(k_moe_step<T, NT, true>, dim3(sms), kStepThreads, pu.smem, 1, st, up);
-  if (e != cudaSuccess) return e;
-  return step_launch(k_moe_step<T, NT, false>, dim3(sms), kStepThreads, pd.smem, 1, st, down);
+  if (pu.ring < 2 || pd.ring < 2) return cudaErrorInvalidConfiguration;    // (a stage's end comes one stage later)
+  // the last writer of some rows adds them up, unless that is more than some 64 loads a lane: the last ones all end in the
+  // last expert's CTAs
+  const bool apart = (int64_t)16 * pd.tps * down.T * down.k * pd.chunks > 64 * 32;
+  if (apart) down.tickets = nullptr;
+  cudaError_t e = step_launch(k_moe_step<T, M, true>, dim3(sms), kStepThreads, pu.smem, 1, st, up);
+  if (e == cudaSuccess) e = step_launch(k_moe_step<T, M, false>, dim3(sms), kStepThreads, pd.smem, 1, st, down);
+  if (e == cudaSuccess && apart)
+    e = step_launch(k_moe_step_sum, dim3((unsigned)(H / 256), (unsigned)down.T), 256, 0, 1, st, down);
+  return e;
 }
 
 }  // namespace
@@ -700,7 +1067,7 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     up.dst = f32(l.a);
     up.dst_max = reinterpret_cast<unsigned*>(ws + l.a_max);
     up.part = f32(l.up_part);
-    const Plan pd = plan(F, H / 16, 256 / qk * rec, 1);
+    const Plan pd = plan(F, H / 16, 256 / qk * rec, 4, false);
     up.tickets = i32(l.tickets) + pd.groups;
     up.top_e = i32(l.top_e);
     up.top_w = f32(l.top_w);
@@ -724,7 +1091,7 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     down.out = d_out;
     down.out_stride = out_stride;
     dispatch_quant(qtype, [&]<int Q>() {
-      e = T <= 4 ? step_products<Q, 1>(up, down, H, F, st) : step_products<Q, 2>(up, down, H, F, st);
+      e = T <= 4 ? step_products<Q, 4>(up, down, H, F, st) : step_products<Q, 8>(up, down, H, F, st);
     });
   }
   if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "moe_step launch: %s", cudaGetErrorString(e));

@@ -304,10 +304,13 @@ int xm_moe_combine(const float* d_rows, int64_t T, int64_t H, int E, int k, int6
  * x [T][H] of x_dtype, residual (fp32, may be null) and out (fp32) with row
  * pitches in elements; out may be x or the residual.  Routing as in
  * xm_moe_forward, with the logits summed in 64 bits and equal ones decided for
- * the lower expert.  d_w1 / d_w3 / d_w2 are DEVICE arrays of E device pointers
- * (16-byte aligned) to GGUF blocks of `qtype`, any block type; weights of Q4_K,
- * Q5_K, Q6_K and Q8_0 enter with the block's own value, those of the other
- * types rounded to fp16 as dequantisation rounds them; activations keep 22 bits.
+ * the lower expert.  The experts' weights are GGUF blocks of `qtype`, any block
+ * type; those of Q4_K, Q5_K, Q6_K and Q8_0 enter with the block's own value, those of
+ * the other types rounded to fp16 as dequantisation rounds them; activations keep
+ * 22 bits.  d_table (64-byte aligned, device memory): xm_moe_step_table's table,
+ * made once for a layer from HOST arrays of E device pointers (16-byte aligned;
+ * w1, w3 [F][H], w2 [H][F]) in host memory of xm_moe_step_table_size bytes, which
+ * the caller copies to the device and keeps as long as the weights.
  * E <= 256, k <= 16; H (<= 16384) and F multiples of 256.  d_workspace (256-byte
  * aligned, xm_moe_step_workspace_size bytes, no initial contents): one for each
  * call that may run at the same time.  Three launches, no host synchronisation;
@@ -316,10 +319,13 @@ int xm_moe_combine(const float* d_rows, int64_t T, int64_t H, int E, int k, int6
  * Replaces moe.py:54-115 with the norm and the residual add of forward.py:113-116.
  */
 int64_t xm_moe_step_workspace_size(int64_t T, int64_t H, int64_t F, int E, int k, int qtype);
+int64_t xm_moe_step_table_size(int E);
+int xm_moe_step_table(int qtype, int64_t H, int64_t F, int E, const void* const* h_w1, const void* const* h_w3,
+                      const void* const* h_w2, void* h_table);
 int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_stride, const float* d_norm_w, float eps,
-                const float* d_gate, int E, int k, int64_t F, const void* const* d_w1, const void* const* d_w3,
-                const void* const* d_w2, int qtype, int activation, const float* d_residual, int64_t residual_stride,
-                float* d_out, int64_t out_stride, void* d_workspace, int64_t workspace_bytes, void* stream);
+                const float* d_gate, int E, int k, int64_t F, const void* d_table, int qtype, int activation,
+                const float* d_residual, int64_t residual_stride, float* d_out, int64_t out_stride, void* d_workspace,
+                int64_t workspace_bytes, void* stream);
 
 /*
  * xm_qgemv without a workspace argument, for callers that cannot allocate

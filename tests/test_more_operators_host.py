@@ -1,13 +1,15 @@
 """CPU: what the C entries of the mixture-of-experts step, the norms between blocks and the log-probabilities refuse, before
 any launch."""
 
+import ctypes
+
 from xanosmerks_b200 import _lib
 
 L, BAD, NO = _lib.lib, _lib.XM_ERR_INVALID, _lib.XM_ERR_UNSUPPORTED
 
 
 def step(T=1, H=512, F=512, E=4, k=2, qtype=12, act=0, xs=None, rs=0, os=None, x=256, ws=256, n=1 << 40, dt=0, gate=256, w=256):
-    return L.xm_moe_step(x, dt, T, H, H if xs is None else xs, None, 1e-5, gate, E, k, F, w, w, w, qtype, act, None, rs, 256,
+    return L.xm_moe_step(x, dt, T, H, H if xs is None else xs, None, 1e-5, gate, E, k, F, w, qtype, act, None, rs, 256,
                          H if os is None else os, ws, n, None)
 
 
@@ -18,11 +20,26 @@ def test_moe_step():
     assert step(E=257) == NO and step(k=5) == NO and step(E=64, k=17) == NO and step(k=0) == NO
     assert step(qtype=0) == NO and step(qtype=16) == NO and step(act=4) == BAD and step(dt=3) == BAD
     assert step(xs=511) == BAD and step(os=511) == BAD
-    assert step(x=None) == BAD and step(x=258) == BAD and step(ws=128) == BAD and step(gate=260) == BAD and step(w=4) == BAD
+    assert step(x=None) == BAD and step(x=258) == BAD and step(ws=128) == BAD and step(gate=260) == BAD and step(w=32) == BAD
     need = L.xm_moe_step_workspace_size(1, 512, 512, 4, 2, 12)
     assert need > 0 and step(n=need - 1) == BAD and b"workspace" in L.xm_last_error()
     assert L.xm_moe_step_workspace_size(65, 512, 512, 4, 2, 12) == 0
     assert L.xm_moe_step_workspace_size(1, 500, 512, 4, 2, 12) == 0
+
+
+def test_moe_step_table():
+    E = 2
+    assert L.xm_moe_step_table_size(0) == 0 and L.xm_moe_step_table_size(257) == 0
+    host = ctypes.create_string_buffer(L.xm_moe_step_table_size(E))
+    good, odd = (ctypes.c_void_p * E)(256, 512), (ctypes.c_void_p * E)(256, 520)
+
+    def table(qtype=14, H=768, F=768, w1=good, w3=good, w2=good, to=host):
+        return L.xm_moe_step_table(qtype, H, F, E, w1, w3, w2, to)
+
+    assert table() == 0                                # (rows of 630 bytes: no tensor maps, the addresses alone)
+    assert list((ctypes.c_uint64 * (3 * E)).from_buffer_copy(host.raw[-24 * E:])) == [256, 512] * 3
+    assert table(w3=odd) == BAD and b"expert 1" in L.xm_last_error() and table(w1=None) == BAD and table(to=None) == BAD
+    assert table(qtype=1) == NO and table(H=700) == NO
 
 
 def norm(rows=1, D=64, ht=0, yt=0, hp=64, yp=64, op=64, gate=None, gt=0, gp=0, per=1, pre=None, nt=0, np_=64, h=256, nxt=None):

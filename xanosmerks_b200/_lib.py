@@ -85,8 +85,10 @@ SIGNATURES = {
     "xm_residual_norm": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _i64, _int, _i64, _f32, _vp,
                                 _f32, _vp, _i64, _vp, _int, _i64, _vp]),
     "xm_moe_step_workspace_size": (_i64, [_i64, _i64, _i64, _int, _int, _int]),
-    "xm_moe_step": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _int, _int, _i64, _vp, _vp, _vp, _int, _int, _vp,
-                           _i64, _vp, _i64, _vp, _i64, _vp]),
+    "xm_moe_step_table_size": (_i64, [_int]),
+    "xm_moe_step_table": (_int, [_int, _i64, _i64, _int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_vp), _vp]),
+    "xm_moe_step": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _f32, _vp, _int, _int, _i64, _vp, _int, _int, _vp, _i64, _vp,
+                           _i64, _vp, _i64, _vp]),
     "xm_comm_destroy": (_int, [_vp]),
     "xm_allreduce_add": (_int, [_vp, _vp, _vp, _i64, _vp]),
 }

@@ -18,14 +18,19 @@
 // A block's codes enter as they are (integers in fp16) and its scales and offsets are applied to the sums of 16 or 32
 // products, in fp32: offsets as one more product of the offsets with the activations' sums over their groups.
 //
-// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles), whose rows bulk copies bring into a
-// ring in shared memory.  Each of its 16 warps holds 256 values of K of a tile, for which its activations stay in registers
+// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles), whose rows tensor copies bring into a
+// ring in shared memory (one or two instructions for the rows of a matrix; a bulk copy for each row takes some 180 clocks to
+// issue, 2900 a stage).  Each of its 16 warps holds 256 values of K of a tile, for which its activations stay in registers
 // while the expert lasts.  The warps take turns at a stage's end: one stage later, one of them adds up the 16 results, has the
-// slot filled again and writes (a 17th warp for that would cost every thread a quarter of its registers).  Nothing waits for
-// another CTA.  The results do not depend on the order in which CTAs run.
+// slot filled again and writes (a 17th warp for that would cost every thread a quarter of its registers; each warp's own
+// loads by cp.async, 700 to 1300 clocks a stage in the load/store unit, of the 1640 in which 37 KB can come from HBM).
+// Nothing waits for another CTA.  The results do not depend on the order in which CTAs run.
 #include <cooperative_groups.h>
+#include <cuda.h>
 
 #include <algorithm>
+#include <cstring>
+#include <mutex>
 
 #include "xm_gemv_dot.cuh"
 
@@ -38,9 +43,16 @@ constexpr int kWorkers = 16, kStepThreads = kWorkers * 32, kMaxRing = 8;
 constexpr int kRouteCluster = 8, kRouteThreads = 256;
 constexpr int kMaxHidden = 16384;
 
+// How the rows of a stage get into shared memory.
+enum Copies {
+  kTensor,                     // by tensor maps: rows are whole units of 16 bytes
+  kWhole,                      // they are not, but a stage has whole rows: as they lie in the weight
+  kRows                        // neither: row by row, from the unit that a row begins in to the one that it ends in
+};
+
 struct StepArgs {
-  const void* const* w1;       // (device arrays of E pointers; DOWN: w1 = the second products' weights)
-  const void* const* w3;
+  const CUtensorMap *map1, *map3;        // of the E weights (DOWN: map1 of the second products')
+  const uint8_t *const *w1, *const *w3;  // their bytes
   const float* src;            // [rows][K]: v of a token (UP), a of a pair (DOWN)
   const float* src_max;        // its largest magnitudes
   float* dst;                  // UP: a [P][F];  DOWN: partial results [chunks][P][H]
@@ -54,7 +66,9 @@ struct StepArgs {
   int nsb, chunks, kc, tps;    // 256-blocks of K, parts of K, their 256-blocks, tiles a stage
   int tiles, groups;           // row tiles, and stages that hold them
   int64_t row_bytes;
-  int pitch, ring;
+  // In shared memory a stage is `boxes` times [rows][pitch bytes], each with box_sb 256-blocks of K of its rows (UP: those of
+  // W1, then those of W3).
+  int boxes, box_sb, pitch, ring, copies;
   const float* residual;       // DOWN
   int64_t residual_stride, out_stride;
   float* out;
@@ -63,10 +77,11 @@ struct StepArgs {
 struct alignas(128) StepShared {
   uint64_t full[kMaxRing], done[kMaxRing];
   int n_seg;
+  const uint8_t *w1[kMaxStepExperts], *w3[kMaxStepExperts];
   int cnt[kMaxStepExperts], off[kMaxStepExperts];
-  unsigned short expert[kMaxPairs], rank[kMaxPairs];   // of a pair: its expert, how many of the expert's pairs are before it
-  unsigned short pair[kMaxPairs];                      // pairs (token * k + slot) by expert, then token
-  unsigned short seg_e[kMaxPairs], seg_at[kMaxPairs], seg_n[kMaxPairs];
+  unsigned short pair[kMaxPairs], seg_at[kMaxPairs];   // pairs (token * k + slot) by expert, then token; a segment's first
+  uint8_t expert[kMaxPairs], rank[kMaxPairs];          // of a pair: its expert, how many of the expert's pairs are before it
+  uint8_t seg_e[kMaxPairs], seg_n[kMaxPairs];
 };
 
 // ---------------------------------------------------------------------------
@@ -216,6 +231,18 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
 // ---------------------------------------------------------------------------
 // Products
 // ---------------------------------------------------------------------------
+// a box of a tensor map to shared memory, completing on `bar`
+XM_DEV void tensor_g2s(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar)) : "memory");
+}
+XM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {        // (half as long as a try_wait, where the phase is complete)
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // out[token][row] from the second products' partial results
 XM_DEV void step_output(const StepArgs& a, int token, int row) {
   const int P = a.T * a.k;
@@ -552,22 +579,23 @@ struct Step {
   const StepArgs& a;
   StepShared& sm;
   uint8_t* ring;
-  float* red;                              // [ring][warp][lane][2 N]
+  float* red;                              // [slot][warp][lane][2 N]
   int lane, warp, g, t, P, per_seg, stage_bytes, s0, s1;
 
-  XM_DEV Step(const StepArgs& a_, StepShared& s, uint8_t* dyn) : a(a_), sm(s), ring(dyn) {
+  XM_DEV Step(const StepArgs& a_, StepShared& s, uint8_t* dyn) : a(a_), sm(s) {
     lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
     g = lane >> 2;
     t = lane & 3;
     P = a.T * a.k;
-    stage_bytes = 16 * a.tps * a.pitch;
+    ring = dyn;
+    stage_bytes = a.boxes * 16 * a.tps * a.pitch;
     red = reinterpret_cast<float*>(dyn + a.ring * stage_bytes);
     per_seg = a.chunks * a.groups;         // stages of a segment: (chunk, group of tiles)
   }
   // A stage's place, and the next one's.
   struct Where {
-    int seg, chunk, group, slot, lap;
+    int seg, chunk, group;
   };
   XM_DEV Where where(int s) const {
     Where w;
@@ -575,28 +603,34 @@ struct Step {
     const int in = s - w.seg * per_seg;
     w.chunk = in / a.groups;
     w.group = in - w.chunk * a.groups;
-    w.lap = (s - s0) / a.ring;
-    w.slot = (s - s0) - w.lap * a.ring;
     return w;
   }
-  XM_DEV void next(Where& w) const {
-    if (++w.group == a.groups) {
-      w.group = 0;
-      if (++w.chunk == a.chunks) {
-        w.chunk = 0;
-        ++w.seg;
-      }
+  // (true: another segment or chunk)
+  XM_DEV bool next(Where& w) const {
+    if (++w.group < a.groups) return false;
+    w.group = 0;
+    if (++w.chunk == a.chunks) {
+      w.chunk = 0;
+      ++w.seg;
     }
-    if (++w.slot == a.ring) {
-      w.slot = 0;
-      ++w.lap;
-    }
+    return true;
   }
-  XM_DEV int tiles_of(const Where& w) const { return min(a.tps, a.tiles - w.group * a.tps); }
+  XM_DEV int tiles_of(int group) const { return min(a.tps, a.tiles - group * a.tps); }
 
   // Which pairs go to which expert, and the segments: an expert and up to M of its pairs.
   XM_DEV void segments() {
-    for (int i = threadIdx.x; i < P; i += kStepThreads) sm.expert[i] = (unsigned short)__ldcg(a.top_e + i);
+    if (a.T == 1) {                        // (in order as they are)
+      if ((int)threadIdx.x < P) {
+        sm.seg_e[threadIdx.x] = (uint8_t)__ldcg(a.top_e + threadIdx.x);
+        sm.seg_at[threadIdx.x] = sm.pair[threadIdx.x] = (unsigned short)threadIdx.x;
+        sm.seg_n[threadIdx.x] = 1;
+      }
+      if (threadIdx.x == 0) sm.n_seg = P;
+      __syncthreads();
+      share();
+      return;
+    }
+    for (int i = threadIdx.x; i < P; i += kStepThreads) sm.expert[i] = (uint8_t)__ldcg(a.top_e + i);
     for (int e = threadIdx.x; e < a.E; e += kStepThreads) sm.cnt[e] = 0;
     __syncthreads();
     if (warp == 0) {
@@ -606,7 +640,7 @@ struct Step {
         const int before = i < P ? sm.cnt[e] : 0;
         __syncwarp();
         if (i < P) {
-          sm.rank[i] = (unsigned short)(before + __popc(same & ((1u << lane) - 1)));
+          sm.rank[i] = (uint8_t)(before + __popc(same & ((1u << lane) - 1)));
           if (lane == __ffs(same) - 1) sm.cnt[e] = before + __popc(same);
         }
         __syncwarp();
@@ -623,9 +657,9 @@ struct Step {
         const int first = at + (sum & 0xffff) - n, seg = segs + (sum >> 16) - s;
         if (e < a.E) sm.off[e] = first;
         for (int i = 0; i < s; ++i) {
-          sm.seg_e[seg + i] = (unsigned short)e;
+          sm.seg_e[seg + i] = (uint8_t)e;
           sm.seg_at[seg + i] = (unsigned short)(first + i * M);
-          sm.seg_n[seg + i] = (unsigned short)min(M, n - i * M);
+          sm.seg_n[seg + i] = (uint8_t)min(M, n - i * M);
         }
         const int all = __shfl_sync(~0u, sum, 31);
         at += all & 0xffff;
@@ -635,38 +669,58 @@ struct Step {
     }
     __syncthreads();
     for (int i = threadIdx.x; i < P; i += kStepThreads) sm.pair[sm.off[sm.expert[i]] + sm.rank[i]] = (unsigned short)i;
+    __syncthreads();
+    share();
+  }
+  // This CTA's stages.
+  XM_DEV void share() {
     const int64_t total = (int64_t)sm.n_seg * per_seg;
     s0 = (int)(total * blockIdx.x / gridDim.x);
     s1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    __syncthreads();
   }
 
-  // Has the stage's rows copied to its slot (one warp).
+  // Has the stage's rows copied to its slot (one thread).
   XM_DEV void fill(int s) {
     const Where w = where(s);
-    const int e = sm.seg_e[w.seg], rows = 16 * tiles_of(w), len = min(a.kc, a.nsb - w.chunk * a.kc) * RB;
-    const int first = w.group * a.tps * (UP ? 8 : 16);                    // the stage's first row
-    const int64_t col = (int64_t)w.chunk * a.kc * RB;
-    const uint8_t* w1 = (const uint8_t*)a.w1[e] + col;
-    const uint8_t* w3 = UP ? (const uint8_t*)a.w3[e] + col : nullptr;
-    auto from = [&](int r) {               // row r of the stage: its address
-      if (UP) return (r & 8 ? w3 : w1) + (int64_t)(first + (r >> 4) * 8 + (r & 7)) * a.row_bytes;
-      return w1 + (int64_t)(first + r) * a.row_bytes;
-    };
-    // (whole units of 16 bytes; only types whose 256 values do not fill them begin inside one)
-    auto size = [&](const uint8_t* p) { return (uint32_t)(((uintptr_t)p & 15) + len + 15) & ~15u; };
-    uint32_t bytes = 0;
-    if (RB % 16 == 0) {
-      bytes = rows * len;
-    } else {
-      for (int r = lane; r < rows; r += 32) bytes += size(from(r));
-      bytes = __reduce_add_sync(~0u, bytes);
+    const int slot = (s - s0) % a.ring, e = sm.seg_e[w.seg];
+    uint8_t* to = ring + slot * stage_bytes;
+    uint64_t* bar = &sm.full[slot];
+    constexpr int ROWS = UP ? 8 : 16;      // of a tile, of one matrix
+    const int block = ROWS * a.tps * a.pitch, first = w.group * a.tps * ROWS;
+    if (a.copies == kTensor) {
+      // (rows past the weight's last and columns past a row's end arrive as zeros; boxes wholly past it are left out)
+      const int sbs = min(a.kc, a.nsb - w.chunk * a.kc), n = (sbs + a.box_sb - 1) / a.box_sb;
+      mbar_arrive_expect_tx(bar, n * 16 * a.tps * a.pitch);
+      for (int b = 0; b < n; ++b) {
+        const int col = (w.chunk * a.kc + b * a.box_sb) * RB / 8;
+        tensor_g2s(to, a.map1 + e, col, first, bar);
+        to += block;
+        if (UP) {
+          tensor_g2s(to, a.map3 + e, col, first, bar);
+          to += block;
+        }
+      }
+      return;
     }
-    if (lane == 0) mbar_arrive_expect_tx(&sm.full[w.slot], bytes);
-    __syncwarp();
-    for (int r = lane; r < rows; r += 32) {
-      const uint8_t* p = from(r);
-      bulk_g2s(ring + w.slot * stage_bytes + r * a.pitch, (const void*)((uintptr_t)p & ~(uintptr_t)15), size(p), &sm.full[w.slot]);
+    const int len = min(a.kc, a.nsb - w.chunk * a.kc) * RB, rows = ROWS * tiles_of(w.group);
+    const int64_t from = first * a.row_bytes + (int64_t)w.chunk * a.kc * RB;
+    if (a.copies == kWhole) {              // (rows by eights are whole units of 16 bytes)
+      mbar_arrive_expect_tx(bar, (UP ? 2 : 1) * rows * len);
+      bulk_g2s(to, sm.w1[e] + from, rows * len, bar);
+      if (UP) bulk_g2s(to + block, sm.w3[e] + from, rows * len, bar);
+      return;
+    }
+    auto size = [&](const uint8_t* q) { return (uint32_t)(((uintptr_t)q & 15) + len + 15) & ~15u; };
+    uint32_t bytes = 0;
+    for (int r = 0; r < rows; ++r)
+      bytes += size(sm.w1[e] + from + r * a.row_bytes) + (UP ? size(sm.w3[e] + from + r * a.row_bytes) : 0);
+    mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll 1
+    for (int h = 0; h < (UP ? 2 : 1); ++h) {
+      const uint8_t* q = (h ? sm.w3[e] : sm.w1[e]) + from;
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r, q += a.row_bytes)
+        bulk_g2s(to + h * block + r * a.pitch, (const void*)((uintptr_t)q & ~(uintptr_t)15), size(q), bar);
     }
   }
 
@@ -742,8 +796,9 @@ struct Step {
   // The stage's end: its results are added up, its slot is filled again, the results are written (one warp).
   XM_DEV void finish(int s, float (&most)[N], int& most_of) {
     const Where w = where(s);
+    const int lap = (s - s0) / a.ring, slot = (s - s0) - lap * a.ring;
     const int at = sm.seg_at[w.seg], n_pairs = sm.seg_n[w.seg], kc = min(a.kc, a.nsb - w.chunk * a.kc);
-    const int tiles = tiles_of(w), tile0 = w.group * a.tps;
+    const int tiles = tiles_of(w.group), tile0 = w.group * a.tps;
     int pair[N];
     float scale[N];
 #pragma unroll
@@ -765,11 +820,11 @@ struct Step {
         atomicMax(a.dst_max + pair[n], __float_as_uint(most[n]));
       }
     };
-    mbar_wait_bounded(&sm.done[w.slot], w.lap & 1);
+    mbar_wait_bounded(&sm.done[slot], lap & 1);
     for (int i = 0; i < tiles; ++i) {
       Result<M> v;
       v.clear();
-      const float* r = red + ((w.slot * kWorkers + i * a.kc) * 32 + lane) * 2 * N;
+      const float* r = red + ((slot * kWorkers + i * a.kc) * 32 + lane) * 2 * N;
 #pragma unroll 4
       for (int q = 0; q < kc; ++q) {
         if constexpr (N == 1) {
@@ -802,7 +857,8 @@ struct Step {
       }
     }
     __syncwarp();
-    if (s + a.ring < s1) fill(s + a.ring);
+    if (lane == 0 && s + a.ring < s1) fill(s + a.ring);
+    __syncwarp();
     if (UP && a.chunks > 1 && last(a.tickets + w.seg * a.groups + w.group, a.chunks)) {
       for (int i = 0; i < tiles; ++i) {
 #pragma unroll
@@ -831,40 +887,44 @@ struct Step {
 
   XM_DEV void run() {
     const int my_tile = warp / a.kc, my_sb = warp - my_tile * a.kc;
-    const int mine_at = (my_tile * 16 + g) * a.pitch + my_sb * RB;
+    const int my_box = my_sb / a.box_sb, second = (UP ? 8 * a.tps : 8) * a.pitch;      // (from a row to the one with g + 8)
+    const int mine_at = my_box * 16 * a.tps * a.pitch + (my_tile * (UP ? 8 : 16) + g) * a.pitch + (my_sb - my_box * a.box_sb) * RB;
+    float* mine_red = red + (warp * 32 + lane) * 2 * N;
     Columns<M> x;
-    int held = -1, most_of = -1;
+    int most_of = -1, slot = 0, lap = 0;
     float most[N];
     Where w = where(s0);
+    bool fresh = true;
     // a stage's end one stage after it: by then the other warps have done it too
-    for (int s = s0; s <= s1 && s0 < s1; ++s, next(w)) {
+    for (int s = s0; s <= s1 && s0 < s1; ++s) {
       if (s < s1) {
         const bool in_k = my_tile < a.tps && w.chunk * a.kc + my_sb < a.nsb;
-        const int k = w.seg * a.chunks + w.chunk;
-        if (held != k) {
-          held = k;
-          load_columns(x, w.seg, (w.chunk * a.kc + my_sb) * 256, in_k);
-        }
-        mbar_wait_bounded(&sm.full[w.slot], w.lap & 1);
-        if (in_k && my_tile < tiles_of(w)) {
-          const uint8_t* r0 = ring + w.slot * stage_bytes + mine_at;
-          const uint8_t* r1 = r0 + 8 * a.pitch;
-          if constexpr (RB % 16 != 0) {    // (a row's bytes begin where they do in 16 bytes of the weight)
-            const int tile = w.group * a.tps + my_tile, n = UP ? tile * 8 + g : tile * 16 + g;
+        if (fresh) load_columns(x, w.seg, (w.chunk * a.kc + my_sb) * 256, in_k);
+        if (!mbar_test(&sm.full[slot], lap & 1)) mbar_wait_bounded(&sm.full[slot], lap & 1);
+        if (in_k && my_tile < tiles_of(w.group)) {
+          const uint8_t* r0 = ring + slot * stage_bytes + mine_at;
+          const uint8_t* r1 = r0 + second;
+          if (RB % 16 != 0 && a.copies == kRows) {  // (a row's bytes begin where they do in 16 bytes of the weight)
+            const int tile = w.group * a.tps + my_tile, n = tile * (UP ? 8 : 16) + g;
             const int64_t col = (int64_t)w.chunk * a.kc * RB;
             r0 += (int)(n * a.row_bytes + col) & 15;
             r1 += (int)((UP ? n : n + 8) * a.row_bytes + col) & 15;
           }
           Result<M> acc;
           unit<T, M>(r0, r1, t, x, acc);
-          float* r = red + ((w.slot * kWorkers + warp) * 32 + lane) * 2 * N;
+          float* r = mine_red + slot * (kWorkers * 32 * 2 * N);
           if constexpr (N == 1) *reinterpret_cast<float2*>(r) = make_float2(acc.v[0][0], acc.v[1][0]);
           else *reinterpret_cast<float4*>(r) = make_float4(acc.v[0][0], acc.v[0][1], acc.v[1][0], acc.v[1][1]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.done[w.slot]);
+        if (lane == 0) mbar_arrive(&sm.done[slot]);
+        if (++slot == a.ring) {
+          slot = 0;
+          ++lap;
+        }
+        fresh = next(w);
       }
-      if (s > s0 && (s - 1 - s0) % kWorkers == warp) finish(s - 1, most, most_of);
+      if (((s - 1 - s0) & (kWorkers - 1)) == warp && s > s0) finish(s - 1, most, most_of);
     }
   }
 };
@@ -880,14 +940,20 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_moe_step(StepArgs a) {
     }
     fence_mbar_init();
   }
-  // DOWN reads the routing before its wait: it is complete before DOWN can start, since UP waits for it and only then lets
-  // DOWN start
+  if (a.copies != kTensor)
+    for (int e = threadIdx.x; e < a.E; e += kStepThreads) {
+      sm.w1[e] = a.w1[e];
+      if (UP) sm.w3[e] = a.w3[e];
+    }
+  // DOWN reads the routing, and the weights that it names, before its wait: it is complete before DOWN can start, since UP
+  // waits for it and only then lets DOWN start
   if (UP) grid_dep_wait();
   grid_dep_launch();
   Step<T, M, UP> step(a, sm, dyn);
   step.segments();
-  if (step.warp == 0)
+  if (threadIdx.x == 0)
     for (int s = step.s0; s < min(step.s1, step.s0 + a.ring); ++s) step.fill(s);
+  __syncwarp();
   if (!UP) grid_dep_wait();
   step.run();
 }
@@ -904,36 +970,65 @@ __global__ void __launch_bounds__(256) k_moe_step_sum(StepArgs a) {
 // Host
 // ---------------------------------------------------------------------------
 struct Plan {
-  int nsb, chunks, kc, tps, tiles, groups, pitch, ring, smem;
+  int nsb, chunks, kc, tps, tiles, groups, boxes, box_sb, pitch, ring, smem, copies;
 };
 
-// K values a row, `tiles` tiles of sixteen rows, rb bytes of 256 values, M tokens
-Plan plan(int64_t K, int64_t tiles, int rb, int M, bool half) {
+// K values a row, `tiles` tiles of sixteen rows; rb: bytes of 256 values, read by 4 bytes (half) or 8; M tokens; up: the first
+// products, whose parts of K cost more to put together.
+Plan plan(int64_t K, int64_t tiles, int rb, bool half, int M, bool up) {
   Plan p;
   p.nsb = (int)(K / 256);
-  p.chunks = (p.nsb + kWorkers - 1) / kWorkers;
-  p.kc = (p.nsb + p.chunks - 1) / p.chunks;
-  p.chunks = (p.nsb + p.kc - 1) / p.kc;
+  p.copies = (int64_t)p.nsb * rb % 16 == 0 ? kTensor : p.nsb <= kWorkers ? kWhole : kRows;
+  // parts of K: of as many 256-blocks as leave the fewest warps without work; parts and boxes begin at whole units of 16 bytes
+  const int step = p.copies == kTensor ? 16 / std::__gcd(rb, 16) : 1;
+  double best = 1e9;
+  for (int kc = step; kc <= kWorkers; kc += step) {
+    const int chunks = (p.nsb + kc - 1) / kc;
+    if (p.copies == kWhole && chunks > 1) continue;
+    const double cost = (double)chunks / (kWorkers / kc) * (1 + (up ? 0.25 : 0.04) * (chunks - 1));
+    if (cost < best - 1e-9 || (cost < best + 1e-9 && chunks < p.chunks)) {
+      best = cost;
+      p.kc = kc;
+      p.chunks = chunks;
+    }
+  }
+  p.kc = std::min(p.kc, p.nsb);
   p.tps = kWorkers / p.kc;
   p.tiles = (int)tiles;
   p.groups = (p.tiles + p.tps - 1) / p.tps;
-  // what the four lanes of a row read falls on other banks than the next rows': 8 bytes each, rows 32 bytes apart modulo 64;
-  // of types read by 4 bytes (half) 16 bytes apart modulo 32
-  p.pitch = (p.kc * rb + 15 + 15) / 16 * 16;
-  if (half) p.pitch += p.pitch % 32 == 0 ? 16 : 0;
-  else p.pitch += p.pitch % 64 == 32 ? 0 : (96 - p.pitch % 64) % 64;
-  const int stage = 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M / 4) * 4;
-  p.ring = std::min(kMaxRing, (int)(212 * 1024 / (stage + red)));
+  // What the four lanes of a row read should fall on other banks than the next rows': 8 bytes each, rows 32 bytes apart modulo
+  // 64; 4 bytes each, 16 apart modulo 32.
+  const int odd = half ? 32 : 64, rest = half ? 16 : 32;
+  auto pitched = [&](int bytes) {
+    bytes = (bytes + 15) / 16 * 16;
+    return bytes + (odd + rest - bytes % odd) % odd;
+  };
+  p.boxes = 1;
+  p.box_sb = p.kc;
+  if (p.copies == kTensor) {
+    // (a box row is at most 256 elements of 8 bytes)
+    while (pitched(p.box_sb * rb) > 2048) {
+      ++p.boxes;
+      p.box_sb = ((p.kc + p.boxes - 1) / p.boxes + step - 1) / step * step;
+    }
+    p.boxes = (p.kc + p.box_sb - 1) / p.box_sb;
+    p.pitch = pitched(p.box_sb * rb);
+  } else {
+    p.pitch = p.copies == kWhole ? p.kc * rb : pitched(p.kc * rb + 15);
+  }
+  const int stage = p.boxes * 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M / 4) * 4;
+  p.ring = std::min(kMaxRing, (int)((227 * 1024 - (int)sizeof(StepShared) - 1024) / (stage + red)));
   p.smem = p.ring * (stage + red);
   return p;
 }
+Plan plan_up(int64_t H, int64_t F, int rb, bool half, int M) { return plan(H, F / 8, rb, half, M, true); }
+Plan plan_down(int64_t H, int64_t F, int rb, bool half, int M) { return plan(F, H / 16, rb, half, M, false); }
 
 struct Layout {
   int64_t top_e, top_w, v, v_max, a, a_max, part, tickets, up_part, bytes;
-  int n_tickets;
+  int n_tickets, down_groups;
 };
-// (pitch, ring and smem of these plans are not used)
-Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb) {
+Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb, bool half) {
   Layout l;
   int64_t at = 0;
   auto take = [&](int64_t n) {
@@ -942,7 +1037,7 @@ Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb) {
     return o;
   };
   const int64_t P = T * k;
-  const Plan up = plan(H, F / 8, rb, 4, false), down = plan(F, H / 16, rb, 4, false);
+  const Plan up = plan_up(H, F, rb, half, 4), down = plan_down(H, F, rb, half, 4);    // (parts and groups go by neither M)
   l.top_e = take(P);
   l.top_w = take(P);
   l.v = take(T * H);
@@ -950,6 +1045,7 @@ Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb) {
   l.a = take(P * F);
   l.a_max = take(P);
   l.part = take((int64_t)down.chunks * P * H);
+  l.down_groups = down.groups;
   l.n_tickets = down.groups + (up.chunks > 1 ? (int)P * up.groups : 0);
   l.tickets = take(l.n_tickets);
   l.up_part = take(up.chunks > 1 ? (int64_t)up.chunks * P * 2 * F : 0);
@@ -987,11 +1083,14 @@ cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cuda
     a.tps = p.tps;
     a.tiles = p.tiles;
     a.groups = p.groups;
+    a.row_bytes = (int64_t)p.nsb * block_bytes<T>();
+    a.boxes = p.boxes;
+    a.box_sb = p.box_sb;
     a.pitch = p.pitch;
     a.ring = p.ring;
-    a.row_bytes = (int64_t)p.nsb * block_bytes<T>();
+    a.copies = p.copies;
   };
-  const Plan pu = plan(H, F / 8, block_bytes<T>(), M, halves<T>()), pd = plan(F, H / 16, block_bytes<T>(), M, halves<T>());
+  const Plan pu = plan_up(H, F, block_bytes<T>(), halves<T>(), M), pd = plan_down(H, F, block_bytes<T>(), halves<T>(), M);
   fill(up, pu);
   fill(down, pd);
   if (pu.ring < 2 || pd.ring < 2) return cudaErrorInvalidConfiguration;    // (a stage's end comes one stage later)
@@ -1006,45 +1105,114 @@ cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cuda
   return e;
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  return fn;
+}
+
+// Sizes that the step takes; qk and record bytes of the type.
+int check_sizes(int64_t H, int64_t F, int E, int qtype, int* qk, int* rec) {
+  if (!host_qtype_geometry(qtype, qk, rec) || *qk < 32)
+    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: expert weights of type id %d", qtype);
+  if (H < 256 || H % 256 || H > kMaxHidden || F < 256 || F % 256 || F > (1 << 20))
+    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: experts of %lld -> %lld (multiples of 256; hidden up to %d)",
+                        (long long)H, (long long)F, kMaxHidden);
+  if (E < 1 || E > kMaxStepExperts)
+    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: %d experts (up to %d)", E, kMaxStepExperts);
+  return XM_OK;
+}
+bool by_halves(int qtype) { return qtype == T_Q6_K || qtype == T_Q8_0; }
+static_assert(halves<T_Q6_K>() && halves<T_Q8_0>() && !halves<T_Q4_K>(), "by_halves() says what halves() does");
+
+// A table: 3 E tensor maps (w1, w3, w2), then 3 E pointers.
+struct Table {
+  const CUtensorMap* maps;
+  const uint8_t* const* weights;
+};
+Table table_at(const void* d, int E) {
+  return {(const CUtensorMap*)d, (const uint8_t* const*)((const uint8_t*)d + (int64_t)3 * E * sizeof(CUtensorMap))};
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t xm_moe_step_workspace_size(int64_t T, int64_t H, int64_t F, int E, int k, int qtype) {
   int qk = 0, rec = 0;
-  if (T < 1 || T > kMaxTokens || H < 256 || H % 256 || H > kMaxHidden || F < 256 || F % 256 || F > (1 << 20) || E < 1 ||
-      E > kMaxStepExperts || k < 1 || k > E || k > kMaxTop || !host_qtype_geometry(qtype, &qk, &rec) || qk < 32)
-    return 0;
-  return layout(T, H, F, k, 256 / qk * rec).bytes;
+  if (T < 1 || T > kMaxTokens || k < 1 || k > E || k > kMaxTop || check_sizes(H, F, E, qtype, &qk, &rec) != XM_OK) return 0;
+  return layout(T, H, F, k, 256 / qk * rec, by_halves(qtype)).bytes;
+}
+
+int64_t xm_moe_step_table_size(int E) {
+  return E < 1 || E > kMaxStepExperts ? 0 : (int64_t)3 * E * (sizeof(CUtensorMap) + sizeof(void*));
+}
+
+int xm_moe_step_table(int qtype, int64_t H, int64_t F, int E, const void* const* h_w1, const void* const* h_w3,
+                      const void* const* h_w2, void* h_table) {
+  int qk = 0, rec = 0;
+  const int st = check_sizes(H, F, E, qtype, &qk, &rec);
+  if (st != XM_OK) return st;
+  if (!h_w1 || !h_w3 || !h_w2 || !h_table) return xm_set_error(XM_ERR_INVALID, "moe_step_table: null pointer");
+  const int rb = 256 / qk * rec;
+  const Plan up = plan_up(H, F, rb, by_halves(qtype), 4), down = plan_down(H, F, rb, by_halves(qtype), 4);
+  std::memset(h_table, 0, (size_t)xm_moe_step_table_size(E));
+  CUtensorMap* maps = (CUtensorMap*)h_table;
+  const void** weights = (const void**)(maps + 3 * E);
+  for (int i = 0; i < 3 * E; ++i) {
+    const void* w = i < E ? h_w1[i] : i < 2 * E ? h_w3[i - E] : h_w2[i - 2 * E];
+    if (!w || ((uintptr_t)w & 15))
+      return xm_set_error(XM_ERR_INVALID, "moe_step_table: weight %d of expert %d is null or not 16-byte aligned", i / E, i % E);
+    weights[i] = w;
+    const Plan& p = i < 2 * E ? up : down;
+    if (p.copies != kTensor) continue;
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return xm_set_error(XM_ERR_CUDA, "moe_step_table: cuTensorMapEncodeTiled unavailable");
+    CUtensorMap map;                       // (64-byte aligned, which the caller's memory need not be)
+    const cuuint64_t dims[2] = {(cuuint64_t)p.nsb * rb / 8, (cuuint64_t)(i < 2 * E ? F : H)};
+    const cuuint64_t strides[1] = {(cuuint64_t)p.nsb * rb};
+    const cuuint32_t box[2] = {(cuuint32_t)p.pitch / 8, (cuuint32_t)((i < 2 * E ? 8 : 16) * p.tps)}, one[2] = {1, 1};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<void*>(w), dims, strides, box, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return xm_set_error(XM_ERR_CUDA, "moe_step_table: tensor map (%d)", (int)r);
+    std::memcpy(&maps[i], &map, sizeof(map));
+  }
+  return XM_OK;
 }
 
 int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_stride, const float* d_norm_w, float eps,
-                const float* d_gate, int E, int k, int64_t F, const void* const* d_w1, const void* const* d_w3,
-                const void* const* d_w2, int qtype, int activation, const float* d_residual, int64_t residual_stride,
-                float* d_out, int64_t out_stride, void* d_workspace, int64_t workspace_bytes, void* stream) {
+                const float* d_gate, int E, int k, int64_t F, const void* d_table, int qtype, int activation,
+                const float* d_residual, int64_t residual_stride, float* d_out, int64_t out_stride, void* d_workspace,
+                int64_t workspace_bytes, void* stream) {
   if (x_dtype != XM_DT_F32 && x_dtype != XM_DT_F16 && x_dtype != XM_DT_BF16)
     return xm_set_error(XM_ERR_INVALID, "moe_step: bad element type %d", x_dtype);
   int qk = 0, rec = 0;
-  if (!host_qtype_geometry(qtype, &qk, &rec) || qk < 32)
-    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: expert weights of type id %d", qtype);
+  const int ok = check_sizes(H, F, E, qtype, &qk, &rec);
+  if (ok != XM_OK) return ok;
   if (T < 0 || T > kMaxTokens) return xm_set_error(XM_ERR_INVALID, "moe_step: %lld tokens (up to %d)", (long long)T, kMaxTokens);
-  if (H < 256 || H % 256 || H > kMaxHidden || F < 256 || F % 256 || F > (1 << 20))
-    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: experts of %lld -> %lld (multiples of 256; hidden up to %d)",
-                        (long long)H, (long long)F, kMaxHidden);
-  if (E < 1 || E > kMaxStepExperts || k < 1 || k > E || k > kMaxTop)
-    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: %d of %d experts (up to %d of up to %d)", k, E, kMaxTop, kMaxStepExperts);
+  if (k < 1 || k > E || k > kMaxTop)
+    return xm_set_error(XM_ERR_UNSUPPORTED, "moe_step: %d of %d experts (up to %d)", k, E, kMaxTop);
   if (activation < XM_ACT_SILU || activation > XM_ACT_IDENTITY)
     return xm_set_error(XM_ERR_INVALID, "moe_step: unknown activation %d", activation);
   if (x_stride < H || out_stride < H || (d_residual && residual_stride < H))
     return xm_set_error(XM_ERR_INVALID, "moe_step: a row pitch is below %lld values", (long long)H);
   if (T == 0) return XM_OK;
-  if (!d_x || !d_gate || !d_w1 || !d_w3 || !d_w2 || !d_out || !d_workspace)
-    return xm_set_error(XM_ERR_INVALID, "moe_step: null pointer");
+  if (!d_x || !d_gate || !d_table || !d_out || !d_workspace) return xm_set_error(XM_ERR_INVALID, "moe_step: null pointer");
   if (((uintptr_t)d_x & (x_dtype == XM_DT_F32 ? 3 : 1)) || ((uintptr_t)d_gate & 15) || ((uintptr_t)d_workspace & 255) ||
-      (((uintptr_t)d_norm_w | (uintptr_t)d_residual | (uintptr_t)d_out) & 3) ||
-      (((uintptr_t)d_w1 | (uintptr_t)d_w3 | (uintptr_t)d_w2) & 7))
+      ((uintptr_t)d_table & 63) || (((uintptr_t)d_norm_w | (uintptr_t)d_residual | (uintptr_t)d_out) & 3))
     return xm_set_error(XM_ERR_INVALID, "moe_step: unaligned pointer");
-  const Layout l = layout(T, H, F, k, 256 / qk * rec);
+  const Layout l = layout(T, H, F, k, 256 / qk * rec, by_halves(qtype));
   if (workspace_bytes < l.bytes)
     return xm_set_error(XM_ERR_INVALID, "moe_step: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                         (long long)l.bytes);
@@ -1059,16 +1227,18 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
                                       : k_moe_step_route<__nv_bfloat16>;
   cudaError_t e = step_launch(route, dim3((unsigned)T * kRouteCluster), kRouteThreads, (int)H * 4, kRouteCluster, st, r);
   if (e == cudaSuccess) {
+    const Table t = table_at(d_table, E);
     StepArgs up = {}, down = {};
-    up.w1 = d_w1;
-    up.w3 = d_w3;
+    up.map1 = t.maps;
+    up.map3 = t.maps + E;
+    up.w1 = t.weights;
+    up.w3 = t.weights + E;
     up.src = f32(l.v);
     up.src_max = f32(l.v_max);
     up.dst = f32(l.a);
     up.dst_max = reinterpret_cast<unsigned*>(ws + l.a_max);
     up.part = f32(l.up_part);
-    const Plan pd = plan(F, H / 16, 256 / qk * rec, 4, false);
-    up.tickets = i32(l.tickets) + pd.groups;
+    up.tickets = i32(l.tickets) + l.down_groups;
     up.top_e = i32(l.top_e);
     up.top_w = f32(l.top_w);
     up.T = (int)T;
@@ -1078,8 +1248,8 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     up.K = (int)H;
     up.N = (int)F;
     down = up;
-    down.w1 = d_w2;
-    down.w3 = nullptr;
+    down.map1 = t.maps + 2 * E;
+    down.w1 = t.weights + 2 * E;
     down.src = f32(l.a);
     down.src_max = f32(l.a_max);
     down.dst = f32(l.part);

@@ -74,11 +74,20 @@ class MoELayer:
         self._p3 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w3])
         self._p2 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w2])
         self._is_dense = self.num_experts_per_tok == self.num_experts
-        # the same pointers on the device, for step(): w1, w3, w2
-        self._table = torch.tensor([[w.data.data_ptr() for w in ws] for ws in (self.w1, self.w3, self.w2)],
-                                   dtype=torch.int64, device=self.device) if self.device.type == "cuda" else None
+        self._table = None                 # step()'s, made by its first call
 
     STEP_TOKENS = 64   # tokens of a step at most
+
+    def _step_table(self) -> torch.Tensor:
+        """The weights' addresses and tensor maps on the device."""
+        if self._table is None:
+            E = self.num_experts
+            host = torch.empty(max(lib.xm_moe_step_table_size(E), 1), dtype=torch.uint8)
+            with torch.cuda.device(self.device):
+                check(lib.xm_moe_step_table(self.qtype, self.hidden, self.intermediate, E, self._p1, self._p3, self._p2,
+                                            host.data_ptr()), "moe step")
+                self._table = host.to(self.device)      # (done when it returns: any stream may read it)
+        return self._table
 
     def step(self, x: torch.Tensor, norm_weight: torch.Tensor | None = None, eps: float = 1e-5,
              residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -112,10 +121,10 @@ class MoELayer:
         # a workspace for each call: two captured graphs, or two streams, never share one
         need = _step_workspace(T, H, F, E, k, self.qtype)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        table = self._table.data_ptr()
+        table = self._table if self._table is not None else self._step_table()
         check(call_on(dev, lib.xm_moe_step, x.data_ptr(), dt, T, H, pitch[0],
-                      None if norm_weight is None else norm_weight.data_ptr(), eps, self.gate.data_ptr(), E, k, F, table,
-                      table + 8 * E, table + 16 * E, self.qtype, ACT[self.activation],
+                      None if norm_weight is None else norm_weight.data_ptr(), eps, self.gate.data_ptr(), E, k, F,
+                      table.data_ptr(), self.qtype, ACT[self.activation],
                       None if residual is None else residual.data_ptr(), pitch[1], out.data_ptr(), pitch[2], ws.data_ptr(),
                       need), "moe step")
         return out

@@ -11,19 +11,19 @@
 //   k_moe_step<DOWN>   W2 a; whoever writes the last partial result of some output rows adds them up
 //
 // The products run on mma.sync (m16n8k16, fp16 with fp32 sums): sixteen weight rows by eight columns.  An activation is
-// 2^s (hi + lo), both fp16, which keeps some 22 bits: up to 4 tokens have a column for each part, up to 8 tokens a column each
+// 2^s (hi + lo), both fp16 (a power of two for each 256 of them), which keeps some 22 bits: up to 4 tokens have a column for each part, up to 8 tokens a column each
 // and two products.  A tile of UP is eight rows of W1 and the same eight of W3, so that one thread holds the gate and the up
 // value of a feature.
 //
 // A block's codes enter as they are (integers in fp16) and its scales and offsets are applied to the sums of 16 or 32
 // products, in fp32: offsets as one more product of the offsets with the activations' sums over their groups.
 //
-// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles), whose rows tensor copies bring into a
-// ring in shared memory (one or two instructions for the rows of a matrix; a bulk copy for each row takes some 180 clocks to
-// issue, 2900 a stage).  Each of its 16 warps holds 256 values of K of a tile, for which its activations stay in registers
-// while the expert lasts.  The warps take turns at a stage's end: one stage later, one of them adds up the 16 results, has the
-// slot filled again and writes (a 17th warp for that would cost every thread a quarter of its registers; each warp's own
-// loads by cp.async, 700 to 1300 clocks a stage in the load/store unit, of the 1640 in which 37 KB can come from HBM).
+// A CTA takes a contiguous range of the stages (expert, part of K, group of row tiles).  Two warps have a stage's rows copied
+// into a ring in shared memory by tensor copies (one or two instructions a matrix of some 340 clocks each; a bulk copy for each
+// row takes 180 to issue, 2900 a stage; each warp's own loads by cp.async 700 to 1300 in the load/store unit; of the 1640 in
+// which a stage's 37 KB can come from HBM).  Sixteen warps multiply, each 256 values of K of a tile, for which its activations
+// stay in registers while the expert lasts.  Two more add up their results and write.  (Warps that multiply and take turns at
+// the copies and sums need no registers for others, but every stage then waits for the one that is late.)
 // Nothing waits for another CTA.  The results do not depend on the order in which CTAs run.
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -39,7 +39,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kMaxTokens = 64, kMaxTop = 16, kMaxStepExperts = 256, kMaxPairs = kMaxTokens * kMaxTop;
-constexpr int kWorkers = 16, kStepThreads = kWorkers * 32, kMaxRing = 8;
+constexpr int kWorkers = 16, kCopiers = 2, kFinishers = 2, kStepThreads = (kWorkers + kCopiers + kFinishers) * 32, kMaxRing = 8;
 constexpr int kRouteCluster = 8, kRouteThreads = 256;
 constexpr int kMaxHidden = 16384;
 
@@ -54,9 +54,7 @@ struct StepArgs {
   const CUtensorMap *map1, *map3;        // of the E weights (DOWN: map1 of the second products')
   const uint8_t *const *w1, *const *w3;  // their bytes
   const float* src;            // [rows][K]: v of a token (UP), a of a pair (DOWN)
-  const float* src_max;        // its largest magnitudes
   float* dst;                  // UP: a [P][F];  DOWN: partial results [chunks][P][H]
-  unsigned* dst_max;           // UP: the largest magnitude of a, as bits
   float* part;                 // UP with several chunks: partial results [chunks][P][2F]
   int* tickets;                // of each group of tiles (DOWN; null: k_moe_step_sum follows), of each segment's (UP with chunks)
   const int* top_e;            // [T][k], ascending
@@ -75,7 +73,7 @@ struct StepArgs {
 };
 
 struct alignas(128) StepShared {
-  uint64_t full[kMaxRing], done[kMaxRing];
+  uint64_t full[kMaxRing], done[kMaxRing], empty[kMaxRing];   // a stage's rows are there, its results are, they are added up
   int n_seg;
   const uint8_t *w1[kMaxStepExperts], *w3[kMaxStepExperts];
   int cnt[kMaxStepExperts], off[kMaxStepExperts];
@@ -93,9 +91,8 @@ struct RouteArgs {
   const float *norm_w, *gate;
   float eps;
   int T, H, E, k;
-  float *v, *v_max, *top_w;
+  float *v, *top_w;
   int* top_e;
-  unsigned* a_max;             // [T * k], zeroed
   int *tickets, n_tickets;     // zeroed
 };
 
@@ -105,28 +102,31 @@ XM_DEV double warp_sum_d(double v) {
   return v;
 }
 
+XM_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+XM_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // A cluster of 8 CTAs a token: each has the whole row and an eighth of the experts, one for each warp, or for several warps
-// where there are few (which then take parts of the row).
+// where there are few (which then take parts of the row).  The logits go to the first CTA's shared memory, the others end.
 template <typename XT>
 __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
-  constexpr int WARPS = kRouteThreads / 32, MINE = kMaxStepExperts / kRouteCluster;
+  constexpr int WARPS = kRouteThreads / 32;
   extern __shared__ __align__(16) float row[];
-  __shared__ float red[32];
-  __shared__ double part[WARPS], logit[MINE], all[kMaxStepExperts], val[kMaxTop];
+  __shared__ float red[WARPS];
+  __shared__ double part[WARPS], all[kMaxStepExperts], val[kMaxTop];
   __shared__ unsigned chosen[WARPS];
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), t = (int)(blockIdx.x / kRouteCluster), tid = threadIdx.x, lane = tid & 31,
             warp = tid >> 5;
+  cluster_arrive();                        // (the first CTA runs before anything is written to it)
   grid_dep_wait();
   grid_dep_launch();
   for (int i = blockIdx.x * kRouteThreads + tid; i < a.n_tickets; i += gridDim.x * kRouteThreads) a.tickets[i] = 0;
-  if (rank == 0 && tid < a.k) a.a_max[t * a.k + tid] = 0u;
   const int mine = (a.E - rank + kRouteCluster - 1) / kRouteCluster;       // experts rank, rank + 8, ...
   const int most = (a.E + kRouteCluster - 1) / kRouteCluster;
   const int split = most <= 1 ? 8 : most <= 2 ? 4 : most <= 4 ? 2 : 1;     // warps an expert
   const int at_once = WARPS / split, slice = warp % split;
   const int n4 = a.H / 4 / split;                                          // (H is a multiple of 256)
-  constexpr int AHEAD = 4;                 // the first loads of the first expert go out before the row is there
+  constexpr int AHEAD = 8;                 // the first loads of the first expert go out before the row is there
   float4 first[AHEAD];
   {
     const int j = warp / split;
@@ -136,30 +136,22 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
       first[i] = j < mine && lane + 32 * i < n4 ? __ldg(g + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const XT* x = (const XT*)a.x + (int64_t)t * a.stride;
-  float s = 0.f, m = 0.f;
-#pragma unroll 4
+  float s = 0.f;
+#pragma unroll 8
   for (int i = tid; i < a.H; i += kRouteThreads) {
     const float v = to_f32<XT>(x[i]);
     row[i] = a.norm_w ? v * a.norm_w[i] : v;
     s = fmaf(v, v, s);
-    m = fmaxf(m, fabsf(row[i]));
   }
   s = warp_sum(s);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  if (lane == 0) {
-    red[warp] = s;
-    red[8 + warp] = m;
-  }
+  if (lane == 0) red[warp] = s;
   __syncthreads();
-  s = m = 0.f;
-  for (int w = 0; w < WARPS; ++w) {
-    s += red[w];
-    m = fmaxf(m, red[8 + w]);
-  }
+  s = 0.f;
+  for (int w = 0; w < WARPS; ++w) s += red[w];
   const float r = a.norm_w ? 1.0f / sqrtf(s / (float)a.H + a.eps) : 1.0f;
   for (int i = rank * kRouteThreads + tid; i < a.H; i += kRouteCluster * kRouteThreads) a.v[(int64_t)t * a.H + i] = row[i] * r;
-  if (rank == 0 && tid == 0) a.v_max[t] = m * r;
+  cluster_wait();
+  double* to = cl.map_shared_rank(all, 0);
   for (int j0 = 0; j0 < mine; j0 += at_once) {
     const int j = j0 + warp / split;
     double d = 0.;
@@ -184,48 +176,52 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
       for (; i < n4; i += 32) add(__ldg(g + i), i);
       d = warp_sum_d((q[0] + q[1]) + (q[2] + q[3]));
     }
+    if (split == 1) {
+      if (lane == 0 && j < mine) to[rank + j * kRouteCluster] = d * (double)r;
+      continue;
+    }
     if (lane == 0) part[warp] = d;
     __syncthreads();
     if (tid < at_once && j0 + tid < mine) {
       double z = 0.;
       for (int w = 0; w < split; ++w) z += part[tid * split + w];
-      logit[j0 + tid] = z * (double)r;
+      to[rank + (j0 + tid) * kRouteCluster] = z * (double)r;
     }
     __syncthreads();
   }
-  cl.sync();
-  if (rank == 0) {
-    // an expert a thread: how many come before it
-    double l = 0., key = 0.;
-    if (tid < a.E) {
-      l = cl.map_shared_rank(logit, tid % kRouteCluster)[tid / kRouteCluster];
-      key = l == l ? l : -INFINITY;                                     // (NaN: not before any other)
-      all[tid] = key;
-    }
-    __syncthreads();
-    int before = a.E;
-    if (tid < a.E) {
-      before = 0;
+  cluster_arrive();
+  if (rank != 0) return;
+  cluster_wait();
+  // an expert a thread: how many come before it
+  double l = 0., key = 0.;
+  if (tid < a.E) {
+    l = all[tid];
+    key = l == l ? l : -INFINITY;                                       // (NaN: not before any other)
+  }
+  int before = a.E;
+  if (tid < a.E) {
+    before = 0;
 #pragma unroll 4
-      for (int e = 0; e < a.E; ++e) before += all[e] > key || (all[e] == key && e < tid);
-    }
-    const bool in = before < a.k;
-    const unsigned b = __ballot_sync(~0u, in);
-    if (lane == 0) chosen[warp] = b;
-    if (in) val[before] = l;
-    __syncthreads();
-    if (in) {
-      double top = val[0];
-      if (!(fabs(top) < INFINITY)) top = 0.;
-      float sum = 1e-12f;
-      for (int j = 0; j < a.k; ++j) sum += expf((float)(val[j] - top));
-      int place = __popc(b & ((1u << lane) - 1));
-      for (int w = 0; w < warp; ++w) place += __popc(chosen[w]);
-      a.top_e[t * a.k + place] = tid;
-      a.top_w[t * a.k + place] = expf((float)(l - top)) / sum;
+    for (int e = 0; e < a.E; ++e) {
+      const double o = all[e] == all[e] ? all[e] : -INFINITY;
+      before += o > key || (o == key && e < tid);
     }
   }
-  cl.sync();                                                  // rank 0 has read the others' logits
+  const bool in = before < a.k;
+  const unsigned b = __ballot_sync(~0u, in);
+  if (lane == 0) chosen[warp] = b;
+  if (in) val[before] = l;
+  __syncthreads();
+  if (in) {
+    double top = val[0];
+    if (!(fabs(top) < INFINITY)) top = 0.;
+    float sum = 1e-12f;
+    for (int j = 0; j < a.k; ++j) sum += expf((float)(val[j] - top));
+    int place = __popc(b & ((1u << lane) - 1));
+    for (int w = 0; w < warp; ++w) place += __popc(chosen[w]);
+    a.top_e[t * a.k + place] = tid;
+    a.top_w[t * a.k + place] = expf((float)(l - top)) / sum;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -290,6 +286,7 @@ struct Columns {
   static constexpr int PARTS = M == 4 ? 1 : 2;
   uint32_t b[PARTS][8][4];
   uint32_t sum[PARTS][2];
+  float scale[M == 4 ? 1 : 2];             // 2^s of the tokens that this thread has results of
 };
 // What a thread has of a tile's results: of its two rows (g, g + 8) the token t (M = 4), or the tokens 2 t, 2 t + 1 (M = 8).
 template <int M>
@@ -357,14 +354,15 @@ XM_DEV void unit_any(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
 XM_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // Q4_K, and Q5_K (FIVE): w = d s_j c - dmin m_j.  A word's codes under the mask 0x000f000f are fp16 subnormals c 2^-24, under
-// 0x00f000f0 c 2^-20: no instruction makes them numbers.  s_j comes from its byte as (2^23 + s) - 2^23, for the upper codes as
-// (2^19 + s / 16) - 2^19; both are exact.
+// 0x00f000f0 c 2^-20: no instruction makes them numbers.  The scales of a pair of groups come from their bytes as fp16
+// (1024 + s_2j) - 1024 and, for the upper codes, (64 + s_2j+1 / 16) - 64: exact.
 template <bool FIVE, int M>
 XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
   constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, BIT = 0x00100010u;
   constexpr int QS = FIVE ? 48 : 16;
   uint32_t sc[2][2], am[2], qh[2][4];
   float d[2], dm[2];
+  const __half2 bias = __floats2half2_rn(-1024.f, -64.f);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const uint4 h = lds128(r ? r1 : r0);
@@ -408,20 +406,21 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
         }
       }
     }
+    float2 s[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t b = __byte_perm(sc[r][jj >> 1], 0x54006400u, jj & 1 ? 0x7352 : 0x7150);
+      s[r] = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&b), bias));
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int j = 2 * jj + half;
       const uint32_t(&q)[2][4] = half ? hi : lo;
       const uint32_t a0[4] = {q[0][0], q[1][0], q[0][1], q[1][1]}, a1[4] = {q[0][2], q[1][2], q[0][3], q[1][3]};
-      float c[4], s[2];
+      float c[4];
       mma_group<M, true>(c, a0, x, j, 0);
       mma_group<M, false>(c, a1, x, j, 1);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t b = __byte_perm(sc[r][j >> 2], half ? 0x49000000u : 0x4B000000u, 0x7650 | (j & 3));
-        s[r] = __uint_as_float(b) - (half ? 0x1p19f : 0x1p23f);
-      }
-      sum.add(c, s[0], s[1]);
+      sum.add(c, half ? s[0].y : s[0].x, half ? s[1].y : s[1].x);
     }
   }
   float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -579,7 +578,7 @@ struct Step {
   const StepArgs& a;
   StepShared& sm;
   uint8_t* ring;
-  float* red;                              // [slot][warp][lane][2 N]
+  float* red;                              // [ring][warp][lane][2 N]
   int lane, warp, g, t, P, per_seg, stage_bytes, s0, s1;
 
   XM_DEV Step(const StepArgs& a_, StepShared& s, uint8_t* dyn) : a(a_), sm(s) {
@@ -593,7 +592,7 @@ struct Step {
     red = reinterpret_cast<float*>(dyn + a.ring * stage_bytes);
     per_seg = a.chunks * a.groups;         // stages of a segment: (chunk, group of tiles)
   }
-  // A stage's place, and the next one's.
+  // A stage's place.
   struct Where {
     int seg, chunk, group;
   };
@@ -604,16 +603,6 @@ struct Step {
     w.chunk = in / a.groups;
     w.group = in - w.chunk * a.groups;
     return w;
-  }
-  // (true: another segment or chunk)
-  XM_DEV bool next(Where& w) const {
-    if (++w.group < a.groups) return false;
-    w.group = 0;
-    if (++w.chunk == a.chunks) {
-      w.chunk = 0;
-      ++w.seg;
-    }
-    return true;
   }
   XM_DEV int tiles_of(int group) const { return min(a.tps, a.tiles - group * a.tps); }
 
@@ -679,48 +668,40 @@ struct Step {
     s1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
   }
 
-  // Has the stage's rows copied to its slot (one thread).
-  XM_DEV void fill(int s) {
+  // One of two threads that have the stage's rows copied to its slot: UP the first those of W1, the second those of W3; DOWN
+  // the even and the odd boxes.
+  XM_DEV void fill(int s, int slot, int which) {
     const Where w = where(s);
-    const int slot = (s - s0) % a.ring, e = sm.seg_e[w.seg];
-    uint8_t* to = ring + slot * stage_bytes;
+    const int e = sm.seg_e[w.seg];
     uint64_t* bar = &sm.full[slot];
     constexpr int ROWS = UP ? 8 : 16;      // of a tile, of one matrix
     const int block = ROWS * a.tps * a.pitch, first = w.group * a.tps * ROWS;
+    uint8_t* to = ring + slot * stage_bytes + (UP ? which * block : 0);
     if (a.copies == kTensor) {
       // (rows past the weight's last and columns past a row's end arrive as zeros; boxes wholly past it are left out)
       const int sbs = min(a.kc, a.nsb - w.chunk * a.kc), n = (sbs + a.box_sb - 1) / a.box_sb;
-      mbar_arrive_expect_tx(bar, n * 16 * a.tps * a.pitch);
-      for (int b = 0; b < n; ++b) {
-        const int col = (w.chunk * a.kc + b * a.box_sb) * RB / 8;
-        tensor_g2s(to, a.map1 + e, col, first, bar);
-        to += block;
-        if (UP) {
-          tensor_g2s(to, a.map3 + e, col, first, bar);
-          to += block;
-        }
-      }
+      const int mine = UP ? n : (n + 1 - which) / 2;
+      mbar_arrive_expect_tx(bar, mine * block);
+      const CUtensorMap* map = (UP && which ? a.map3 : a.map1) + e;
+      for (int b = UP ? 0 : which; b < n; b += UP ? 1 : 2)
+        tensor_g2s(to + b * (UP ? 2 : 1) * block, map, (w.chunk * a.kc + b * a.box_sb) * RB / 8, first, bar);
       return;
     }
     const int len = min(a.kc, a.nsb - w.chunk * a.kc) * RB, rows = ROWS * tiles_of(w.group);
-    const int64_t from = first * a.row_bytes + (int64_t)w.chunk * a.kc * RB;
-    if (a.copies == kWhole) {              // (rows by eights are whole units of 16 bytes)
-      mbar_arrive_expect_tx(bar, (UP ? 2 : 1) * rows * len);
-      bulk_g2s(to, sm.w1[e] + from, rows * len, bar);
-      if (UP) bulk_g2s(to + block, sm.w3[e] + from, rows * len, bar);
-      return;
-    }
-    auto size = [&](const uint8_t* q) { return (uint32_t)(((uintptr_t)q & 15) + len + 15) & ~15u; };
-    uint32_t bytes = 0;
-    for (int r = 0; r < rows; ++r)
-      bytes += size(sm.w1[e] + from + r * a.row_bytes) + (UP ? size(sm.w3[e] + from + r * a.row_bytes) : 0);
-    mbar_arrive_expect_tx(bar, bytes);
+    const uint8_t* p = (UP && which ? sm.w3[e] : sm.w1[e]) + first * a.row_bytes + (int64_t)w.chunk * a.kc * RB;
+    if (!UP && which) {
+      mbar_arrive(bar);
+    } else if (a.copies == kWhole) {       // (rows by eights are whole units of 16 bytes)
+      mbar_arrive_expect_tx(bar, rows * len);
+      bulk_g2s(to, p, rows * len, bar);
+    } else {
+      auto size = [&](const uint8_t* q) { return (uint32_t)(((uintptr_t)q & 15) + len + 15) & ~15u; };
+      uint32_t bytes = 0;
+      for (int r = 0; r < rows; ++r) bytes += size(p + r * a.row_bytes);
+      mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll 1
-    for (int h = 0; h < (UP ? 2 : 1); ++h) {
-      const uint8_t* q = (h ? sm.w3[e] : sm.w1[e]) + from;
-#pragma unroll 1
-      for (int r = 0; r < rows; ++r, q += a.row_bytes)
-        bulk_g2s(to + h * block + r * a.pitch, (const void*)((uintptr_t)q & ~(uintptr_t)15), size(q), bar);
+      for (int r = 0; r < rows; ++r, p += a.row_bytes)
+        bulk_g2s(to + r * a.pitch, (const void*)((uintptr_t)p & ~(uintptr_t)15), size(p), bar);
     }
   }
 
@@ -729,22 +710,37 @@ struct Step {
     const int col = M == 4 ? g >> 1 : g;
     const bool there = mine && col < sm.seg_n[seg], rest = M == 4 && (g & 1);      // (this column has the low parts)
     const int pair = there ? sm.pair[sm.seg_at[seg] + col] : 0, row = UP ? pair / a.k : pair;
-    const float inv = ldexpf(1.0f, -fp16_row_shift(there ? __ldcg(a.src_max + row) : 0.f));
     const float* p = a.src + (int64_t)row * a.K + k0 + (halves<T>() ? 4 : 8) * t;
     auto low = [](float v) { return v - __half2float(__float2half_rn(v)); };
+    // all of the column's 256 values first: their power of two
+    float4 u[8][2];
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        u[j][i] = there ? __ldcg(reinterpret_cast<const float4*>(p + 32 * j + i * (halves<T>() ? 16 : 4)))
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(u[j][i].x), fabsf(u[j][i].y)), fmaxf(fabsf(u[j][i].z), fabsf(u[j][i].w))));
+    m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+    const int shift = fp16_row_shift(m);
+    const float inv = ldexpf(1.0f, -shift), own = ldexpf(1.0f, shift);
+    if constexpr (M == 4) {
+      x.scale[0] = __shfl_sync(~0u, own, 8 * t);
+    } else {
+      x.scale[0] = __shfl_sync(~0u, own, 8 * t);
+      x.scale[1] = __shfl_sync(~0u, own, 8 * t + 4);
+    }
     float part[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float v[8];
-      if (there) {
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(p + 32 * j)),
-                     w = __ldcg(reinterpret_cast<const float4*>(p + 32 * j + (halves<T>() ? 16 : 4)));
-        v[0] = u.x * inv; v[1] = u.y * inv; v[2] = u.z * inv; v[3] = u.w * inv;
-        v[4] = w.x * inv; v[5] = w.y * inv; v[6] = w.z * inv; v[7] = w.w * inv;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
+      float v[8] = {u[j][0].x * inv, u[j][0].y * inv, u[j][0].z * inv, u[j][0].w * inv,
+                    u[j][1].x * inv, u[j][1].y * inv, u[j][1].z * inv, u[j][1].w * inv};
       part[2 * j] = (v[0] + v[1]) + (v[2] + v[3]);
       part[2 * j + 1] = (v[4] + v[5]) + (v[6] + v[7]);
 #pragma unroll
@@ -793,32 +789,19 @@ struct Step {
     return true;
   }
 
-  // The stage's end: its results are added up, its slot is filled again, the results are written (one warp).
-  XM_DEV void finish(int s, float (&most)[N], int& most_of) {
+  // The stage's results are added up and written (one warp).
+  XM_DEV void finish(int s, int slot, int lap) {
     const Where w = where(s);
-    const int lap = (s - s0) / a.ring, slot = (s - s0) - lap * a.ring;
     const int at = sm.seg_at[w.seg], n_pairs = sm.seg_n[w.seg], kc = min(a.kc, a.nsb - w.chunk * a.kc);
     const int tiles = tiles_of(w.group), tile0 = w.group * a.tps;
     int pair[N];
-    float scale[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int i = M == 4 ? t : 2 * t + n;
       pair[n] = i < n_pairs ? sm.pair[at + i] : -1;
-      scale[n] = pair[n] < 0 ? 0.f : ldexpf(1.0f, fp16_row_shift(__ldcg(a.src_max + (UP ? pair[n] / a.k : pair[n]))));
-    }
-    if (UP && most_of != w.seg) {
-      most_of = w.seg;
-#pragma unroll
-      for (int n = 0; n < N; ++n) most[n] = 0.f;
     }
     auto result = [&](int n, int i, float gate, float up) {       // a feature of the first products
-      const float y = xm_act(a.act, gate) * up;
-      a.dst[(int64_t)pair[n] * a.N + (tile0 + i) * 8 + g] = y;
-      if (fabsf(y) > most[n]) {
-        most[n] = fabsf(y);
-        atomicMax(a.dst_max + pair[n], __float_as_uint(most[n]));
-      }
+      a.dst[(int64_t)pair[n] * a.N + (tile0 + i) * 8 + g] = xm_act(a.act, gate) * up;
     };
     mbar_wait_bounded(&sm.done[slot], lap & 1);
     for (int i = 0; i < tiles; ++i) {
@@ -839,10 +822,14 @@ struct Step {
           v.v[1][1] += u.w;
         }
       }
+      if (i + 1 == tiles) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[slot]);
+      }
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         if (pair[n] < 0) continue;
-        const float y0 = v.v[0][n] * scale[n], y1 = v.v[1][n] * scale[n];
+        const float y0 = v.v[0][n], y1 = v.v[1][n];
         if (!UP) {
           float* p = a.dst + ((int64_t)w.chunk * P + pair[n]) * a.N + (tile0 + i) * 16 + g;
           p[0] = y0;
@@ -856,8 +843,6 @@ struct Step {
         }
       }
     }
-    __syncwarp();
-    if (lane == 0 && s + a.ring < s1) fill(s + a.ring);
     __syncwarp();
     if (UP && a.chunks > 1 && last(a.tickets + w.seg * a.groups + w.group, a.chunks)) {
       for (int i = 0; i < tiles; ++i) {
@@ -885,46 +870,73 @@ struct Step {
     }
   }
 
-  XM_DEV void run() {
+  XM_DEV void copy(int which) {            // (one thread)
+    int slot = 0, lap = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (lap > 0) mbar_wait_bounded(&sm.empty[slot], (lap - 1) & 1);
+      fill(s, slot, which);
+      if (++slot == a.ring) {
+        slot = 0;
+        ++lap;
+      }
+    }
+  }
+
+  XM_DEV void finishes(int which) {        // (every other stage)
+    int slot = 0, lap = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (((s - s0) & 1) == which) finish(s, slot, lap);
+      if (++slot == a.ring) {
+        slot = 0;
+        ++lap;
+      }
+    }
+  }
+
+  XM_DEV void multiply() {
     const int my_tile = warp / a.kc, my_sb = warp - my_tile * a.kc;
     const int my_box = my_sb / a.box_sb, second = (UP ? 8 * a.tps : 8) * a.pitch;      // (from a row to the one with g + 8)
     const int mine_at = my_box * 16 * a.tps * a.pitch + (my_tile * (UP ? 8 : 16) + g) * a.pitch + (my_sb - my_box * a.box_sb) * RB;
-    float* mine_red = red + (warp * 32 + lane) * 2 * N;
+    float* const mine_red = red + (warp * 32 + lane) * 2 * N;
     Columns<M> x;
-    int most_of = -1, slot = 0, lap = 0;
-    float most[N];
-    Where w = where(s0);
-    bool fresh = true;
-    // a stage's end one stage after it: by then the other warps have done it too
-    for (int s = s0; s <= s1 && s0 < s1; ++s) {
-      if (s < s1) {
-        const bool in_k = my_tile < a.tps && w.chunk * a.kc + my_sb < a.nsb;
-        if (fresh) load_columns(x, w.seg, (w.chunk * a.kc + my_sb) * 256, in_k);
-        if (!mbar_test(&sm.full[slot], lap & 1)) mbar_wait_bounded(&sm.full[slot], lap & 1);
-        if (in_k && my_tile < tiles_of(w.group)) {
-          const uint8_t* r0 = ring + slot * stage_bytes + mine_at;
-          const uint8_t* r1 = r0 + second;
-          if (RB % 16 != 0 && a.copies == kRows) {  // (a row's bytes begin where they do in 16 bytes of the weight)
-            const int tile = w.group * a.tps + my_tile, n = tile * (UP ? 8 : 16) + g;
-            const int64_t col = (int64_t)w.chunk * a.kc * RB;
-            r0 += (int)(n * a.row_bytes + col) & 15;
-            r1 += (int)((UP ? n : n + 8) * a.row_bytes + col) & 15;
-          }
-          Result<M> acc;
-          unit<T, M>(r0, r1, t, x, acc);
-          float* r = mine_red + slot * (kWorkers * 32 * 2 * N);
-          if constexpr (N == 1) *reinterpret_cast<float2*>(r) = make_float2(acc.v[0][0], acc.v[1][0]);
-          else *reinterpret_cast<float4*>(r) = make_float4(acc.v[0][0], acc.v[0][1], acc.v[1][0], acc.v[1][1]);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.done[slot]);
-        if (++slot == a.ring) {
-          slot = 0;
-          ++lap;
-        }
-        fresh = next(w);
+    int slot = 0, lap = 0, left = 0, tile = 0, chunk = 0;
+    bool in_k = false;
+    for (int s = s0; s < s1; ++s) {
+      if (left == 0) {                     // another segment or part of K
+        const Where w = where(s);
+        left = a.groups - w.group;
+        chunk = w.chunk;
+        tile = w.group * a.tps + my_tile;
+        in_k = my_tile < a.tps && chunk * a.kc + my_sb < a.nsb;
+        load_columns(x, w.seg, (chunk * a.kc + my_sb) * 256, in_k);
       }
-      if (((s - 1 - s0) & (kWorkers - 1)) == warp && s > s0) finish(s - 1, most, most_of);
+      if (!mbar_test(&sm.full[slot], lap & 1)) mbar_wait_bounded(&sm.full[slot], lap & 1);
+      if (in_k && tile < a.tiles) {
+        const uint8_t* r0 = ring + slot * stage_bytes + mine_at;
+        const uint8_t* r1 = r0 + second;
+        if (RB % 16 != 0 && a.copies == kRows) {    // (a row's bytes begin where they do in 16 bytes of the weight)
+          const int n = tile * (UP ? 8 : 16) + g;
+          const int64_t col = (int64_t)chunk * a.kc * RB;
+          r0 += (int)(n * a.row_bytes + col) & 15;
+          r1 += (int)((UP ? n : n + 8) * a.row_bytes + col) & 15;
+        }
+        Result<M> acc;
+        unit<T, M>(r0, r1, t, x, acc);
+        float* r = mine_red + slot * (kWorkers * 32 * 2 * N);
+        if constexpr (N == 1)
+          *reinterpret_cast<float2*>(r) = make_float2(acc.v[0][0] * x.scale[0], acc.v[1][0] * x.scale[0]);
+        else
+          *reinterpret_cast<float4*>(r) = make_float4(acc.v[0][0] * x.scale[0], acc.v[0][1] * x.scale[N - 1],
+                                                      acc.v[1][0] * x.scale[0], acc.v[1][1] * x.scale[N - 1]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.done[slot]);
+      if (++slot == a.ring) {
+        slot = 0;
+        ++lap;
+      }
+      --left;
+      tile += a.tps;
     }
   }
 };
@@ -935,8 +947,9 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_moe_step(StepArgs a) {
   __shared__ StepShared sm;
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.ring; ++i) {
-      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.full[i], kCopiers);
       mbar_init(&sm.done[i], kWorkers);
+      mbar_init(&sm.empty[i], 1);
     }
     fence_mbar_init();
   }
@@ -951,11 +964,15 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_moe_step(StepArgs a) {
   grid_dep_launch();
   Step<T, M, UP> step(a, sm, dyn);
   step.segments();
-  if (threadIdx.x == 0)
-    for (int s = step.s0; s < min(step.s1, step.s0 + a.ring); ++s) step.fill(s);
-  __syncwarp();
-  if (!UP) grid_dep_wait();
-  step.run();
+  if (step.warp < kWorkers) {
+    if (!UP) grid_dep_wait();
+    step.multiply();
+  } else if (step.warp < kWorkers + kCopiers) {
+    if (step.lane == 0) step.copy(step.warp - kWorkers);
+  } else {
+    if (!UP) grid_dep_wait();
+    step.finishes(step.warp - kWorkers - kCopiers);
+  }
 }
 
 // The outputs by themselves, a thread each: for so many that the last writer's warp would be long at it.
@@ -1006,18 +1023,22 @@ Plan plan(int64_t K, int64_t tiles, int rb, bool half, int M, bool up) {
   p.boxes = 1;
   p.box_sb = p.kc;
   if (p.copies == kTensor) {
-    // (a box row is at most 256 elements of 8 bytes)
-    while (pitched(p.box_sb * rb) > 2048) {
-      ++p.boxes;
-      p.box_sb = ((p.kc + p.boxes - 1) / p.boxes + step - 1) / step * step;
+    // a box row is at most 256 elements of 8 bytes; of the numbers of boxes that allow it the one that wastes least
+    int least = 1 << 30;
+    for (int boxes = 1; boxes <= p.kc; ++boxes) {
+      const int sb = ((p.kc + boxes - 1) / boxes + step - 1) / step * step, n = (p.kc + sb - 1) / sb, pitch = pitched(sb * rb);
+      if (pitch <= 2048 && n * pitch + 64 * n < least) {       // (64 bytes a row for another instruction)
+        least = n * pitch + 64 * n;
+        p.boxes = n;
+        p.box_sb = sb;
+        p.pitch = pitch;
+      }
     }
-    p.boxes = (p.kc + p.box_sb - 1) / p.box_sb;
-    p.pitch = pitched(p.box_sb * rb);
   } else {
     p.pitch = p.copies == kWhole ? p.kc * rb : pitched(p.kc * rb + 15);
   }
   const int stage = p.boxes * 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M / 4) * 4;
-  p.ring = std::min(kMaxRing, (int)((227 * 1024 - (int)sizeof(StepShared) - 1024) / (stage + red)));
+  p.ring = std::min(kMaxRing, (227 * 1024 - (int)sizeof(StepShared) - 1024) / (stage + red));
   p.smem = p.ring * (stage + red);
   return p;
 }
@@ -1025,7 +1046,7 @@ Plan plan_up(int64_t H, int64_t F, int rb, bool half, int M) { return plan(H, F 
 Plan plan_down(int64_t H, int64_t F, int rb, bool half, int M) { return plan(F, H / 16, rb, half, M, false); }
 
 struct Layout {
-  int64_t top_e, top_w, v, v_max, a, a_max, part, tickets, up_part, bytes;
+  int64_t top_e, top_w, v, a, part, tickets, up_part, bytes;
   int n_tickets, down_groups;
 };
 Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb, bool half) {
@@ -1041,9 +1062,7 @@ Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb, bool half) {
   l.top_e = take(P);
   l.top_w = take(P);
   l.v = take(T * H);
-  l.v_max = take(T);
   l.a = take(P * F);
-  l.a_max = take(P);
   l.part = take((int64_t)down.chunks * P * H);
   l.down_groups = down.groups;
   l.n_tickets = down.groups + (up.chunks > 1 ? (int)P * up.groups : 0);
@@ -1093,7 +1112,7 @@ cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cuda
   const Plan pu = plan_up(H, F, block_bytes<T>(), halves<T>(), M), pd = plan_down(H, F, block_bytes<T>(), halves<T>(), M);
   fill(up, pu);
   fill(down, pd);
-  if (pu.ring < 2 || pd.ring < 2) return cudaErrorInvalidConfiguration;    // (a stage's end comes one stage later)
+  if (pu.ring < 2 || pd.ring < 2) return cudaErrorInvalidConfiguration;    // (no type and size has so few)
   // the last writer of some rows adds them up, unless that is more than some 64 loads a lane: the last ones all end in the
   // last expert's CTAs
   const bool apart = (int64_t)16 * pd.tps * down.T * down.k * pd.chunks > 64 * 32;
@@ -1220,8 +1239,8 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
   auto f32 = [&](int64_t o) { return reinterpret_cast<float*>(ws + o); };
   auto i32 = [&](int64_t o) { return reinterpret_cast<int*>(ws + o); };
   cudaStream_t st = (cudaStream_t)stream;
-  const RouteArgs r{d_x, x_stride, d_norm_w, d_gate, eps, (int)T, (int)H, E, k, f32(l.v), f32(l.v_max), f32(l.top_w),
-                    i32(l.top_e), reinterpret_cast<unsigned*>(ws + l.a_max), i32(l.tickets), l.n_tickets};
+  const RouteArgs r{d_x, x_stride, d_norm_w, d_gate, eps, (int)T, (int)H, E, k, f32(l.v), f32(l.top_w), i32(l.top_e),
+                    i32(l.tickets), l.n_tickets};
   auto route = x_dtype == XM_DT_F32   ? k_moe_step_route<float>
                : x_dtype == XM_DT_F16 ? k_moe_step_route<__half>
                                       : k_moe_step_route<__nv_bfloat16>;
@@ -1234,9 +1253,7 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     up.w1 = t.weights;
     up.w3 = t.weights + E;
     up.src = f32(l.v);
-    up.src_max = f32(l.v_max);
     up.dst = f32(l.a);
-    up.dst_max = reinterpret_cast<unsigned*>(ws + l.a_max);
     up.part = f32(l.up_part);
     up.tickets = i32(l.tickets) + l.down_groups;
     up.top_e = i32(l.top_e);
@@ -1251,7 +1268,6 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     down.map1 = t.maps + 2 * E;
     down.w1 = t.weights + 2 * E;
     down.src = f32(l.a);
-    down.src_max = f32(l.a_max);
     down.dst = f32(l.part);
     down.tickets = i32(l.tickets);
     down.K = (int)F;

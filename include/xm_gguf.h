@@ -313,7 +313,7 @@ int xm_moe_combine(const float* d_rows, int64_t T, int64_t H, int E, int k, int6
  * the caller copies to the device and keeps as long as the weights.
  * E <= 256, k <= 16; H (<= 16384) and F multiples of 256.  d_workspace (256-byte
  * aligned, xm_moe_step_workspace_size bytes, no initial contents): one for each
- * call that may run at the same time.  Three launches, no host synchronisation;
+ * call that may run at the same time.  Four launches, no host synchronisation;
  * the same result for every launch.
  *
  * Replaces moe.py:54-115 with the norm and the residual add of forward.py:113-116.

@@ -3,16 +3,19 @@
 //   v = x, or x w / sqrt(mean x^2 + eps);  l = gate v;  the k largest l, p = softmax over them;
 //   out = residual + sum over the k experts e, ascending, of p_e W2_e (act(W1_e v) * (W3_e v))
 //
-// Bound: HBM, the blocks of the experts that some token chose (each read once for up to M = 4 or 8 tokens of an expert).
+// Bound: HBM, the blocks of the experts that some token chose (each read once for up to M tokens of an expert).
 //
-// Three launches, each starting while the one before it ends:
+// Four launches, each starting while the one before it ends:
 //   k_moe_step_route   a cluster a token: norm, logits in 64 bits (a near tie of two experts goes one way), top k, softmax
 //   k_moe_step<UP>     a = act(W1 v) * (W3 v) of every (token, expert) pair
-//   k_moe_step<DOWN>   W2 a; whoever writes the last partial result of some output rows adds them up
+//   k_moe_step<DOWN>   W2 a
+//   k_moe_step_sum     the weighted sum and the residual
 //
 // The products run on mma.sync (m16n8k16, fp16 with fp32 sums): sixteen weight rows by eight columns.  An activation is
-// 2^s (hi + lo), both fp16 (a power of two for each 256 of them), which keeps some 22 bits: up to 4 tokens have a column for each part, up to 8 tokens a column each
-// and two products.  A tile of UP is eight rows of W1 and the same eight of W3, so that one thread holds the gate and the up
+// 2^s (hi + lo), both fp16 (a power of two for each 256 of them), which keeps some 22 bits: up to 4 tokens have a column for
+// each part (M = 4), up to 8 tokens a column each and two products (M = 8).  A single token (M = 1) has the two columns of its
+// parts four times, for every fourth group of values: a thread then has the sums of one group in four, and a quarter of the
+// scales to apply.  A tile of UP is eight rows of W1 and the same eight of W3, so that one thread holds the gate and the up
 // value of a feature.
 //
 // A block's codes enter as they are (integers in fp16) and its scales and offsets are applied to the sums of 16 or 32
@@ -56,7 +59,7 @@ struct StepArgs {
   const float* src;            // [rows][K]: v of a token (UP), a of a pair (DOWN)
   float* dst;                  // UP: a [P][F];  DOWN: partial results [chunks][P][H]
   float* part;                 // UP with several chunks: partial results [chunks][P][2F]
-  int* tickets;                // of each group of tiles (DOWN; null: k_moe_step_sum follows), of each segment's (UP with chunks)
+  int* tickets;                // UP with chunks: of each segment's groups of tiles
   const int* top_e;            // [T][k], ascending
   const float* top_w;
   int T, k, E, act;
@@ -278,20 +281,22 @@ XM_DEV uint32_t pack2(float lo, float hi) {
 template <int T>
 constexpr bool halves() { return T == T_Q6_K || T == T_Q8_0; }
 
-// The 256 values of K that a warp holds, of M tokens: column g (= lane / 4) is token g / 2, hi or lo by g % 2 (M = 4), or token
-// g in two parts (M = 8).  By groups of 32 their pairs, and the sums over groups of 32 or 16 times 2^-5, of groups 2 t, 2 t + 1
-// (and 2 t + 8, 2 t + 9).
+// The 256 values of K that a warp holds, of M tokens: column g (= lane / 4) is token g / 2, hi or lo by g % 2 (M = 4), token g
+// in two parts (M = 8), or hi or lo of the one token in the groups g / 2, g / 2 + 4, ... and zero in the others (M = 1).  By
+// groups of 32 their pairs, and the sums over groups of 32 or 16 times 2^-5, of groups 2 t, 2 t + 1 (and 2 t + 8, 2 t + 9; M = 1:
+// in columns 0 and 1).
 template <int M>
 struct Columns {
-  static constexpr int PARTS = M == 4 ? 1 : 2;
+  static constexpr int PARTS = M == 8 ? 2 : 1;
   uint32_t b[PARTS][8][4];
   uint32_t sum[PARTS][2];
-  float scale[M == 4 ? 1 : 2];             // 2^s of the tokens that this thread has results of
+  float scale[M == 8 ? 2 : 1];             // 2^s of the tokens that this thread has results of
 };
-// What a thread has of a tile's results: of its two rows (g, g + 8) the token t (M = 4), or the tokens 2 t, 2 t + 1 (M = 8).
+// What a thread has of a tile's results: of its two rows (g, g + 8) the token t (M = 4), the tokens 2 t, 2 t + 1 (M = 8), or a
+// quarter of the one token's (M = 1).
 template <int M>
 struct Result {
-  static constexpr int N = M == 4 ? 1 : 2;
+  static constexpr int N = M == 8 ? 2 : 1;
   float v[2][N];
   XM_DEV void clear() {
 #pragma unroll
@@ -299,7 +304,7 @@ struct Result {
   }
   // v += s0 times the first row's sums, s1 times the second's
   XM_DEV void add(const float (&c)[4], float s0, float s1) {
-    if constexpr (M == 4) {
+    if constexpr (M != 8) {
       v[0][0] = fmaf(s0, c[0] + c[1], v[0][0]);
       v[1][0] = fmaf(s1, c[2] + c[3], v[1][0]);
     } else {
@@ -353,6 +358,13 @@ XM_DEV void unit_any(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
 
 XM_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
+// Codes of 8 bits of which the upper four count sixteenfold: those bits alone (a - b of fp16 subnormals is exact, and the
+// pipe of the logic operations is the busier one).
+XM_DEV uint32_t minus(uint32_t a, uint32_t b) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
 // Q4_K, and Q5_K (FIVE): w = d s_j c - dmin m_j.  A word's codes under the mask 0x000f000f are fp16 subnormals c 2^-24, under
 // 0x00f000f0 c 2^-20: no instruction makes them numbers.  The scales of a pair of groups come from their bytes as fp16
 // (1024 + s_2j) - 1024 and, for the upper codes, (64 + s_2j+1 / 16) - 64: exact.
@@ -362,7 +374,6 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
   constexpr int QS = FIVE ? 48 : 16;
   uint32_t sc[2][2], am[2], qh[2][4];
   float d[2], dm[2];
-  const __half2 bias = __floats2half2_rn(-1024.f, -64.f);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const uint4 h = lds128(r ? r1 : r0);
@@ -381,6 +392,7 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
       qh[r][3] = (q.w >> (8 * t)) & 0xffu;
     }
   }
+  float one[2][4];                         // M = 1: the sums of groups t and t + 4
   Result<M> sum;
   sum.clear();
 #pragma unroll
@@ -389,38 +401,64 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint2 q = *reinterpret_cast<const uint2*>((r ? r1 : r0) + QS + 32 * jj + 8 * t);
-      const uint32_t w[4] = {q.x, q.x >> 8, q.y, q.y >> 8};
+      uint32_t f[4] = {0u, 0u, 0u, 0u};
       if constexpr (FIVE) {
-        const uint32_t b = qh[r][jj], f[4] = {(b * ((1u << 4) + (1u << 18))) & BIT, (b * ((1u << 3) + (1u << 17))) & BIT,
-                                              (b * (1u + (1u << 14))) & BIT, ((b >> 1) * (1u + (1u << 14))) & BIT};
+        const uint32_t b = qh[r][jj];
+        f[0] = (b * ((1u << 4) + (1u << 18))) & BIT;
+        f[1] = (b * ((1u << 3) + (1u << 17))) & BIT;
+        f[2] = (b * (1u + (1u << 14))) & BIT;
+        f[3] = ((b >> 1) * (1u + (1u << 14))) & BIT;
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[r][i] = (w[i] & LOW) | f[i];
-          hi[r][i] = (w[i] & HIGH) | (f[i] << 4);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? q.x : q.y;
+        if (i & 1) {
+          const uint32_t two = __byte_perm(w, 0u, 0x4341);      // bytes 1 and 3
+          lo[r][i] = two & LOW;
+          hi[r][i] = minus(two, lo[r][i]);
+        } else {
+          lo[r][i] = w & LOW;
+          hi[r][i] = w & HIGH;
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[r][i] = w[i] & LOW;
-          hi[r][i] = w[i] & HIGH;
+        if constexpr (FIVE) {
+          lo[r][i] |= f[i];
+          hi[r][i] |= f[i] << 4;
         }
       }
     }
     float2 s[2];
+    if constexpr (M != 1) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint32_t b = __byte_perm(sc[r][jj >> 1], 0x54006400u, jj & 1 ? 0x7352 : 0x7150);
-      s[r] = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&b), bias));
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t b = __byte_perm(sc[r][jj >> 1], 0x54006400u, jj & 1 ? 0x7352 : 0x7150);
+        s[r] = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&b), __floats2half2_rn(-1024.f, -64.f)));
+      }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int j = 2 * jj + half;
       const uint32_t(&q)[2][4] = half ? hi : lo;
       const uint32_t a0[4] = {q[0][0], q[1][0], q[0][1], q[1][1]}, a1[4] = {q[0][2], q[1][2], q[0][3], q[1][3]};
-      float c[4];
-      mma_group<M, true>(c, a0, x, j, 0);
-      mma_group<M, false>(c, a1, x, j, 1);
-      sum.add(c, half ? s[0].y : s[0].x, half ? s[1].y : s[1].x);
+      if constexpr (M == 1) {
+        if (j % 4 == 0) mma_group<M, true>(one[j / 4], a0, x, j, 0);
+        else mma_group<M, false>(one[j / 4], a0, x, j, 0);
+        mma_group<M, false>(one[j / 4], a1, x, j, 1);
+      } else {
+        float c[4];
+        mma_group<M, true>(c, a0, x, j, 0);
+        mma_group<M, false>(c, a1, x, j, 1);
+        sum.add(c, half ? s[0].y : s[0].x, half ? s[1].y : s[1].x);
+      }
+    }
+  }
+  if constexpr (M == 1) {
+    const float odd = t & 1 ? 0.0625f : 1.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float s[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) s[r] = __uint_as_float(__byte_perm(sc[r][i], 0x4B000000u, 0x7650 | t)) - 0x1p23f;
+      sum.add(one[i], s[0] * odd, s[1] * odd);
     }
   }
   float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -458,6 +496,7 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
     const uint32_t dw = w[4] >> sh;
     d[r] = __half2float(__ushort_as_half((unsigned short)dw)) * 0x1p24f;
   }
+  float one[4][4];                         // M = 1: the sums of groups t, t + 4, ...
   Result<M> sum;
   sum.clear();
 #pragma unroll
@@ -485,14 +524,30 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
           q[r][1] = (c4 >> 8) & 0x00ff00ffu;
         }
         const uint32_t a[4] = {q[0][0], q[1][0], q[0][1], q[1][1]};
-        float c[4], s[2];
-        mma_group<M, true>(c, a, x, g >> 1, g & 1);
+        if constexpr (M == 1) {
+          // (groups 4 i + p, then 4 i + 2 + p: the first of a four is p = 0, i even)
+          if (p == 0 && !(i & 1)) mma_group<M, true>(one[g >> 2], a, x, g >> 1, g & 1);
+          else mma_group<M, false>(one[g >> 2], a, x, g >> 1, g & 1);
+        } else {
+          float c[4], s[2];
+          mma_group<M, true>(c, a, x, g >> 1, g & 1);
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          s[r] = __uint_as_float(__byte_perm(sc[r][g >> 2], 0x4B000000u, 0x7650 | (g & 3))) - (0x1p23f + 128.f);
-        sum.add(c, s[0], s[1]);
+          for (int r = 0; r < 2; ++r)
+            s[r] = __uint_as_float(__byte_perm(sc[r][g >> 2], 0x4B000000u, 0x7650 | (g & 3))) - (0x1p23f + 128.f);
+          sum.add(c, s[0], s[1]);
+        }
       }
     }
+  if constexpr (M == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float s[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        s[r] = __uint_as_float(__byte_perm(sc[r][i], 0x4B000000u, 0x7650 | t)) - (0x1p23f + 128.f);
+      sum.add(one[i], s[0], s[1]);
+    }
+  }
   // offsets: -32 sum s_g S_g, the scales as fp16 (1024 + byte) - 1152
   uint32_t o[2][2];
 #pragma unroll
@@ -530,6 +585,7 @@ XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
   for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16_k8(o, dd[0], dd[1], x.sum[i][0]);
   acc.clear();
   acc.add(o, -0x1p12f, -0x1p12f);
+  float one[2][4];                         // M = 1: the sums of groups t and t + 4
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     uint32_t w[2][2];
@@ -547,21 +603,40 @@ XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
       }
       w[r][0] ^= 0x80808080u;
       w[r][1] ^= 0x80808080u;
-      const uint32_t u = __shfl_sync(~0u, dd[r], (threadIdx.x & 28) | (j >> 1));
-      s[r] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xffffu))) * 0x1p24f;
+      if constexpr (M != 1) {
+        const uint32_t u = __shfl_sync(~0u, dd[r], (threadIdx.x & 28) | (j >> 1));
+        s[r] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xffffu))) * 0x1p24f;
+      }
     }
     constexpr uint32_t K = 0x00ff00ffu;
     const uint32_t a0[4] = {w[0][0] & K, w[1][0] & K, (w[0][0] >> 8) & K, (w[1][0] >> 8) & K};
     const uint32_t a1[4] = {w[0][1] & K, w[1][1] & K, (w[0][1] >> 8) & K, (w[1][1] >> 8) & K};
-    float c[4];
-    mma_group<M, true>(c, a0, x, j, 0);
-    mma_group<M, false>(c, a1, x, j, 1);
-    acc.add(c, s[0], s[1]);
+    if constexpr (M == 1) {
+      if (j % 4 == 0) mma_group<M, true>(one[j / 4], a0, x, j, 0);
+      else mma_group<M, false>(one[j / 4], a0, x, j, 0);
+      mma_group<M, false>(one[j / 4], a1, x, j, 1);
+    } else {
+      float c[4];
+      mma_group<M, true>(c, a0, x, j, 0);
+      mma_group<M, false>(c, a1, x, j, 1);
+      acc.add(c, s[0], s[1]);
+    }
+  }
+  if constexpr (M == 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float s[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        s[r] = __half2float(*reinterpret_cast<const __half*>((r ? r1 : r0) + 34 * (t + 4 * i))) * 0x1p24f;
+      acc.add(one[i], s[0], s[1]);
+    }
   }
 }
 
 template <int T, int M>
 XM_DEV void unit(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
+  static_assert(M != 1 || own_value<T>(), "one scale for a group of values");
   if constexpr (T == T_Q4_K) unit_k<false, M>(r0, r1, t, x, acc);
   else if constexpr (T == T_Q5_K) unit_k<true, M>(r0, r1, t, x, acc);
   else if constexpr (T == T_Q6_K) unit_q6k<M>(r0, r1, t, x, acc);
@@ -707,6 +782,74 @@ struct Step {
 
   // This warp's activations of a segment and a chunk.
   XM_DEV void load_columns(Columns<M>& x, int seg, int k0, bool mine) {
+    if constexpr (M == 1) load_one(x, seg, k0, mine);
+    else load_several(x, seg, k0, mine);
+  }
+  // The one token's: a lane has the groups g / 2, g / 2 + 4, ... alone.
+  XM_DEV void load_one(Columns<M>& x, int seg, int k0, bool mine) {
+    constexpr int G = T == T_Q6_K ? 16 : 8, V = 256 / G / 4;     // groups, a lane's values of one
+    const int pair = sm.pair[sm.seg_at[seg]], row = UP ? pair / a.k : pair, own = g >> 1;
+    const float* p = a.src + (int64_t)row * a.K + k0;
+    float v[G / 4][V], m = 0.f;
+#pragma unroll
+    for (int i = 0; i < G / 4; ++i)
+#pragma unroll
+      for (int q = 0; q < V; q += 4) {
+        // (values 8 t .. 8 t + 7 of a group of 32, or 4 t .. 4 t + 3 of each 16)
+        const int at = (own + 4 * i) * (256 / G) + (halves<T>() ? 4 * q + 4 * t : 8 * t + q);
+        const float4 u = mine ? __ldcg(reinterpret_cast<const float4*>(p + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i][q] = u.x;
+        v[i][q + 1] = u.y;
+        v[i][q + 2] = u.z;
+        v[i][q + 3] = u.w;
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))));
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const int shift = fp16_row_shift(m);
+    const float inv = ldexpf(1.0f, -shift);
+    x.scale[0] = ldexpf(1.0f, shift);
+    auto part = [&](float f) { return g & 1 ? f - __half2float(__float2half_rn(f)) : f; };
+    float sum[G / 4];
+#pragma unroll
+    for (int i = 0; i < G / 4; ++i) {
+      float z = 0.f;
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        v[i][q] *= inv;
+        z += v[i][q];
+      }
+      z += __shfl_xor_sync(~0u, z, 1);
+      z += __shfl_xor_sync(~0u, z, 2);
+      sum[i] = z * 0x1p-5f;
+#pragma unroll
+      for (int q = 0; q < V; q += 4) {
+        const uint32_t b0 = pack2(part(v[i][q]), part(v[i][q + 2])), b1 = pack2(part(v[i][q + 1]), part(v[i][q + 3]));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {      // (zero in the groups that are others')
+          const int at = 4 * i + c;        // the group
+          const int j = G == 16 ? at / 2 : at, w = G == 16 ? 2 * (at & 1) : q / 2;
+          x.b[0][j][w] = c == own ? b0 : 0u;
+          x.b[0][j][w + 1] = c == own ? b1 : 0u;
+        }
+      }
+    }
+    // sums of groups 2 t, 2 t + 1 (, 2 t + 8, 2 t + 9) in columns 0 and 1: group n is with the lanes of g / 2 = n % 4
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = 2 * t + (i & 1);       // (+ 8 for i >= 2)
+      float z[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        z[h] = 2 * (i / 2) + h < G / 4 ? __shfl_sync(~0u, sum[2 * (i / 2) + h < G / 4 ? 2 * (i / 2) + h : 0], (n & 3) * 8) : 0.f;
+      q[i] = n < 4 ? z[0] : z[1];
+      q[i] = g < 2 ? part(q[i]) : 0.f;
+    }
+    x.sum[0][0] = pack2(q[0], q[1]);
+    x.sum[0][1] = pack2(q[2], q[3]);
+  }
+  XM_DEV void load_several(Columns<M>& x, int seg, int k0, bool mine) {
     const int col = M == 4 ? g >> 1 : g;
     const bool there = mine && col < sm.seg_n[seg], rest = M == 4 && (g & 1);      // (this column has the low parts)
     const int pair = there ? sm.pair[sm.seg_at[seg] + col] : 0, row = UP ? pair / a.k : pair;
@@ -797,7 +940,7 @@ struct Step {
     int pair[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int i = M == 4 ? t : 2 * t + n;
+      const int i = M == 8 ? 2 * t + n : t;
       pair[n] = i < n_pairs ? sm.pair[at + i] : -1;
     }
     auto result = [&](int n, int i, float gate, float up) {       // a feature of the first products
@@ -820,6 +963,13 @@ struct Step {
           v.v[0][1] += u.y;
           v.v[1][0] += u.z;
           v.v[1][1] += u.w;
+        }
+      }
+      if constexpr (M == 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v.v[h][0] += __shfl_xor_sync(~0u, v.v[h][0], 1);
+          v.v[h][0] += __shfl_xor_sync(~0u, v.v[h][0], 2);
         }
       }
       if (i + 1 == tiles) {
@@ -857,14 +1007,6 @@ struct Step {
           }
           result(n, i, gate, up);
         }
-      }
-      __syncwarp();
-    }
-    if (!UP && a.tickets && last(a.tickets + w.group, sm.n_seg * a.chunks)) {
-      const int rows = 16 * tiles;
-      for (int i = lane; i < rows * a.T; i += 32) {
-        const int tok = i / rows;
-        step_output(a, tok, tile0 * 16 + i - tok * rows);
       }
       __syncwarp();
     }
@@ -975,7 +1117,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_moe_step(StepArgs a) {
   }
 }
 
-// The outputs by themselves, a thread each: for so many that the last writer's warp would be long at it.
+// The outputs, a thread each.  (The last writer of some rows could add them up in DOWN, but its fence and its ticket cost more
+// than a launch that is there when DOWN ends: one token, 2 of 8 experts, 7 us.)
 __global__ void __launch_bounds__(256) k_moe_step_sum(StepArgs a) {
   grid_dep_wait();
   grid_dep_launch();
@@ -1037,7 +1180,7 @@ Plan plan(int64_t K, int64_t tiles, int rb, bool half, int M, bool up) {
   } else {
     p.pitch = p.copies == kWhole ? p.kc * rb : pitched(p.kc * rb + 15);
   }
-  const int stage = p.boxes * 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M / 4) * 4;
+  const int stage = p.boxes * 16 * p.tps * p.pitch, red = kWorkers * 32 * 2 * (M == 8 ? 2 : 1) * 4;
   p.ring = std::min(kMaxRing, (227 * 1024 - (int)sizeof(StepShared) - 1024) / (stage + red));
   p.smem = p.ring * (stage + red);
   return p;
@@ -1047,7 +1190,7 @@ Plan plan_down(int64_t H, int64_t F, int rb, bool half, int M) { return plan(F, 
 
 struct Layout {
   int64_t top_e, top_w, v, a, part, tickets, up_part, bytes;
-  int n_tickets, down_groups;
+  int n_tickets;
 };
 Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb, bool half) {
   Layout l;
@@ -1064,18 +1207,27 @@ Layout layout(int64_t T, int64_t H, int64_t F, int64_t k, int rb, bool half) {
   l.v = take(T * H);
   l.a = take(P * F);
   l.part = take((int64_t)down.chunks * P * H);
-  l.down_groups = down.groups;
-  l.n_tickets = down.groups + (up.chunks > 1 ? (int)P * up.groups : 0);
+  l.n_tickets = up.chunks > 1 ? (int)P * up.groups : 0;
   l.tickets = take(l.n_tickets);
   l.up_part = take(up.chunks > 1 ? (int64_t)up.chunks * P * 2 * F : 0);
   l.bytes = at;
   return l;
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t step_launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, int cluster, cudaStream_t st, Args... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto KERNEL, typename... Args>
+cudaError_t step_launch(dim3 grid, int threads, int smem, int cluster, cudaStream_t st, Args... args) {
+  static bool done[64] = {};               // (the kernel may have all shared memory, by device)
+  int dev = 0;
+  cudaError_t e = smem > 0 ? cudaGetDevice(&dev) : cudaSuccess;
   if (e != cudaSuccess) return e;
+  if (smem > 0 && (dev >= 64 || !done[dev])) {
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, KERNEL);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)at.sharedSizeBytes);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -1089,7 +1241,7 @@ cudaError_t step_launch(void (*kernel)(KArgs...), dim3 grid, int threads, int sm
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  return cudaLaunchKernelEx(&cfg, KERNEL, args...);
 }
 
 template <int T, int M>
@@ -1113,14 +1265,9 @@ cudaError_t step_products(StepArgs up, StepArgs down, int64_t H, int64_t F, cuda
   fill(up, pu);
   fill(down, pd);
   if (pu.ring < 2 || pd.ring < 2) return cudaErrorInvalidConfiguration;    // (no type and size has so few)
-  // the last writer of some rows adds them up, unless that is more than some 64 loads a lane: the last ones all end in the
-  // last expert's CTAs
-  const bool apart = (int64_t)16 * pd.tps * down.T * down.k * pd.chunks > 64 * 32;
-  if (apart) down.tickets = nullptr;
-  cudaError_t e = step_launch(k_moe_step<T, M, true>, dim3(sms), kStepThreads, pu.smem, 1, st, up);
-  if (e == cudaSuccess) e = step_launch(k_moe_step<T, M, false>, dim3(sms), kStepThreads, pd.smem, 1, st, down);
-  if (e == cudaSuccess && apart)
-    e = step_launch(k_moe_step_sum, dim3((unsigned)(H / 256), (unsigned)down.T), 256, 0, 1, st, down);
+  cudaError_t e = step_launch<k_moe_step<T, M, true>>(dim3(sms), kStepThreads, pu.smem, 1, st, up);
+  if (e == cudaSuccess) e = step_launch<k_moe_step<T, M, false>>(dim3(sms), kStepThreads, pd.smem, 1, st, down);
+  if (e == cudaSuccess) e = step_launch<k_moe_step_sum>(dim3((unsigned)(H / 256), (unsigned)down.T), 256, 0, 1, st, down);
   return e;
 }
 
@@ -1241,10 +1388,11 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
   cudaStream_t st = (cudaStream_t)stream;
   const RouteArgs r{d_x, x_stride, d_norm_w, d_gate, eps, (int)T, (int)H, E, k, f32(l.v), f32(l.top_w), i32(l.top_e),
                     i32(l.tickets), l.n_tickets};
-  auto route = x_dtype == XM_DT_F32   ? k_moe_step_route<float>
-               : x_dtype == XM_DT_F16 ? k_moe_step_route<__half>
-                                      : k_moe_step_route<__nv_bfloat16>;
-  cudaError_t e = step_launch(route, dim3((unsigned)T * kRouteCluster), kRouteThreads, (int)H * 4, kRouteCluster, st, r);
+  const dim3 routes((unsigned)T * kRouteCluster);
+  cudaError_t e =
+      x_dtype == XM_DT_F32   ? step_launch<k_moe_step_route<float>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r)
+      : x_dtype == XM_DT_F16 ? step_launch<k_moe_step_route<__half>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r)
+                             : step_launch<k_moe_step_route<__nv_bfloat16>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r);
   if (e == cudaSuccess) {
     const Table t = table_at(d_table, E);
     StepArgs up = {}, down = {};
@@ -1255,7 +1403,7 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     up.src = f32(l.v);
     up.dst = f32(l.a);
     up.part = f32(l.up_part);
-    up.tickets = i32(l.tickets) + l.down_groups;
+    up.tickets = i32(l.tickets);
     up.top_e = i32(l.top_e);
     up.top_w = f32(l.top_w);
     up.T = (int)T;
@@ -1269,7 +1417,6 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     down.w1 = t.weights + 2 * E;
     down.src = f32(l.a);
     down.dst = f32(l.part);
-    down.tickets = i32(l.tickets);
     down.K = (int)F;
     down.N = (int)H;
     down.residual = d_residual;
@@ -1277,7 +1424,11 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
     down.out = d_out;
     down.out_stride = out_stride;
     dispatch_quant(qtype, [&]<int Q>() {
-      e = T <= 4 ? step_products<Q, 4>(up, down, H, F, st) : step_products<Q, 8>(up, down, H, F, st);
+      // Four tokens a pass while an expert has some 2.5 of them on average (five and more are then one in twenty): the registers
+      // for eight do not fit, and a pass for four takes two thirds of the time.
+      if (own_value<Q>() && T == 1) e = step_products<Q, own_value<Q>() ? 1 : 4>(up, down, H, F, st);
+      else if (T <= 4 || 2 * T * k <= 5 * E) e = step_products<Q, 4>(up, down, H, F, st);
+      else e = step_products<Q, 8>(up, down, H, F, st);
     });
   }
   if (e != cudaSuccess) return xm_set_error(XM_ERR_CUDA, "moe_step launch: %s", cudaGetErrorString(e));

@@ -115,21 +115,26 @@ lib = _load()
 
 
 
+_torch = _stream_of = None
+
+
+def _bind():
+    global _torch, _stream_of
+    import torch
+    # (torch's own accessor where this build has it: a fifth of a microsecond instead of two)
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _stream_of = get if get is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
+    _torch = torch
+
+
 def call_on(dev, fn, *args) -> int:
     """fn(*args, stream) with `dev` (a CUDA device with an index) current and its current stream."""
-    import torch
-    if torch.cuda.current_device() == dev.index:
-        return fn(*args, _raw_stream(dev.index))
-    with torch.cuda.device(dev):
-        return fn(*args, _raw_stream(dev.index))
-
-
-def _raw_stream(index):
-    """The current stream's handle (torch's own accessor where this build has it: a fifth of a microsecond
-    instead of two)."""
-    import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+    if _torch is None:
+        _bind()
+    if _torch.cuda.current_device() == dev.index:
+        return fn(*args, _stream_of(dev.index))
+    with _torch.cuda.device(dev):
+        return fn(*args, _stream_of(dev.index))
 
 
 def check_device(what: str = "") -> None:

@@ -101,33 +101,43 @@ class MoELayer:
         blocks' own values (of Q4_K, Q5_K, Q6_K and Q8_0) with activations of 22 bits."""
         H, F, E, k, dev = self.hidden, self.intermediate, self.num_experts, self.num_experts_per_tok, self.device
         dt = _DT.get(x.dtype) if isinstance(x, torch.Tensor) else None
-        if dt is None or x.dim() != 2 or x.shape[1] != H or x.device != dev or (x.stride(1) != 1 and H > 1):
+        if dt is None or x.dim() != 2 or x.shape[1] != H or x.device != dev or x.stride(1) != 1:
             raise ValueError(f"step: x must be an fp32, fp16 or bf16 tensor [tokens, {H}] on {dev} with unit stride in its last "
                              f"dimension")
         T = x.shape[0]
         if T > self.STEP_TOKENS:
             raise ValueError(f"step: {T} tokens (up to {self.STEP_TOKENS}; forward_device takes more)")
-        if norm_weight is not None and (norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (H,)
-                                        or not norm_weight.is_contiguous() or norm_weight.device != dev):
-            raise ValueError(f"step: norm_weight must be a contiguous fp32 tensor [{H}] on {dev}")
-        for name, t in (("residual", residual), ("out", out)):
-            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (T, H) or t.device != dev or t.stride(1) != 1):
-                raise ValueError(f"step: {name} must be an fp32 tensor [{T}, {H}] on {dev} with unit stride in its last dimension")
+        norm = res = None
+        if norm_weight is not None:
+            if (norm_weight.dtype is not torch.float32 or norm_weight.dim() != 1 or norm_weight.shape[0] != H
+                    or not norm_weight.is_contiguous() or norm_weight.device != dev):
+                raise ValueError(f"step: norm_weight must be a contiguous fp32 tensor [{H}] on {dev}")
+            norm = norm_weight.data_ptr()
+        res_pitch = H
+        if residual is not None:
+            res, res_pitch = self._step_rows(residual, T, "residual")
         if out is None:
-            out = torch.empty((T, H), dtype=torch.float32, device=dev)
+            out = self.gate.new_empty((T, H))
+            out_ptr, out_pitch = out.data_ptr(), H
+        else:
+            out_ptr, out_pitch = self._step_rows(out, T, "out")
         if T == 0:
             return out
-        pitch = [t.stride(0) if t is not None and T > 1 else H for t in (x, residual, out)]
         # a workspace for each call: two captured graphs, or two streams, never share one
         need = _step_workspace(T, H, F, E, k, self.qtype)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = self.gate.new_empty((need + 3) // 4)
         table = self._table if self._table is not None else self._step_table()
-        check(call_on(dev, lib.xm_moe_step, x.data_ptr(), dt, T, H, pitch[0],
-                      None if norm_weight is None else norm_weight.data_ptr(), eps, self.gate.data_ptr(), E, k, F,
-                      table.data_ptr(), self.qtype, ACT[self.activation],
-                      None if residual is None else residual.data_ptr(), pitch[1], out.data_ptr(), pitch[2], ws.data_ptr(),
-                      need), "moe step")
+        check(call_on(dev, lib.xm_moe_step, x.data_ptr(), dt, T, H, x.stride(0) if T > 1 else H, norm, eps,
+                      self.gate.data_ptr(), E, k, F, table.data_ptr(), self.qtype, ACT[self.activation], res, res_pitch, out_ptr,
+                      out_pitch, ws.data_ptr(), need), "moe step")
         return out
+
+    def _step_rows(self, t, T, what):
+        """(address, row pitch) of the fp32 rows [T, hidden] t."""
+        if t.dtype is not torch.float32 or t.dim() != 2 or tuple(t.shape) != (T, self.hidden) or t.device != self.device or t.stride(1) != 1:
+            raise ValueError(f"step: {what} must be an fp32 tensor [{T}, {self.hidden}] on {self.device} with unit stride in its last "
+                             f"dimension")
+        return t.data_ptr(), t.stride(0) if T > 1 else self.hidden
 
     def forward_device(self, x: torch.Tensor) -> torch.Tensor:
         """x: CUDA tensor (..., H) -> fp32 CUDA tensor of the same shape."""

@@ -179,6 +179,30 @@ def _as_rows(t, d):
     return t if d == 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _rows_and_pitch(t, d):
+    """(a tensor that holds t's rows, their pitch in elements)."""
+    if t.is_contiguous():
+        return t, d
+    t = _as_rows(t, d)
+    return t, t.stride(0) if t.shape[0] > 1 else d
+
+
+def _gate_rows(gate, shape, dev):
+    """gate (anything that broadcasts to shape) as (rows [n, 1 or D], whether wide)."""
+    if not isinstance(gate, torch.Tensor) or gate.dtype not in _DT or gate.device != dev or not 1 <= gate.dim() <= len(shape):
+        raise ValueError(f"residual_norm: gate must be an fp32, fp16 or bf16 tensor on {dev} that broadcasts to {tuple(shape)}")
+    lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
+    if any(n not in (1, s) for n, s in zip(lead, shape)):
+        raise ValueError(f"residual_norm: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+    gate = gate.reshape(lead)
+    last = len(lead) - 1                                  # leading sizes that the gate has, then ones
+    while last > 0 and lead[last - 1] == 1:
+        last -= 1
+    if any(n != s for n, s in zip(lead[:last], shape)):
+        gate = gate.expand(*shape[:-1], lead[-1])
+    return _as_rows(gate, lead[-1]), int(lead[-1] == shape[-1])
+
+
 def residual_norm(stream: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor | None = None,
                   gate: torch.Tensor | None = None, scale: float = 1.0, pre_weight: torch.Tensor | None = None,
                   eps: float = 1e-5, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
@@ -191,52 +215,50 @@ def residual_norm(stream: torch.Tensor, y: torch.Tensor, post_weight: torch.Tens
     that broadcasts to the stream's shape: [D], [batch, 1, D] for one gate a sequence, [..., 1] for one value a row.
     h has the stream's type and goes to ``out`` if given (``stream`` itself: in place); next has ``out_dtype`` (default: y's
     type).  All in fp32; each result is rounded once, so that next comes from h before its rounding."""
-    if not isinstance(stream, torch.Tensor) or not stream.is_cuda or stream.dtype not in _DT or stream.dim() < 1:
+    ht = _DT.get(stream.dtype) if isinstance(stream, torch.Tensor) else None
+    if ht is None or not stream.is_cuda or stream.dim() < 1:
         raise ValueError("residual_norm: the stream must be an fp32, fp16 or bf16 CUDA tensor")
-    dev, shape, d = stream.device, stream.shape, stream.shape[-1]
-    if not isinstance(y, torch.Tensor) or y.shape != shape or y.dtype not in _DT or y.device != dev:
+    dev, shape = stream.device, stream.shape
+    d = shape[-1]
+    yt = _DT.get(y.dtype) if isinstance(y, torch.Tensor) else None
+    if yt is None or y.shape != shape or y.device != dev:
         raise ValueError(f"residual_norm: y must be an fp32, fp16 or bf16 tensor {tuple(shape)} on {dev}")
-    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if w is not None and (w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != d or w.device != dev
-                              or not w.is_contiguous()):
-            raise ValueError(f"residual_norm: {name} must be a contiguous fp32 tensor [{d}] on {dev}")
-    if out_dtype is None:
-        out_dtype = y.dtype
-    if out_dtype not in _DT:
+    weights = [None, None]
+    for i, w in enumerate((post_weight, pre_weight)):
+        if w is not None:
+            if w.dtype is not torch.float32 or w.dim() != 1 or w.shape[0] != d or w.device != dev or not w.is_contiguous():
+                raise ValueError(f"residual_norm: {('post', 'pre')[i]}_weight must be a contiguous fp32 tensor [{d}] on {dev}")
+            weights[i] = w.data_ptr()
+    ot = yt if out_dtype is None else _DT.get(out_dtype)
+    if ot is None:
         raise ValueError(f"residual_norm: out_dtype {out_dtype} (fp32, fp16 or bf16)")
+    h2, h_pitch = _rows_and_pitch(stream, d)
+    y2, y_pitch = _rows_and_pitch(y, d)
     if out is None:
-        out = torch.empty(shape, dtype=stream.dtype, device=dev)
-    elif out.shape != shape or out.dtype != stream.dtype or out.device != dev:
-        raise ValueError(f"residual_norm: out must be {stream.dtype} {tuple(shape)} on {dev}")
-    o2 = out if out.dim() == 2 else out.view(-1, d)
-    if d > 1 and o2.stride(1) != 1:
-        raise ValueError("residual_norm: out must have unit stride in its last dimension")
-    h2, y2 = _as_rows(stream, d), _as_rows(y, d)
-    rows = h2.shape[0]
-    after = None if pre_weight is None else torch.empty(shape, dtype=out_dtype, device=dev)
+        out = torch.empty_like(stream) if h2 is stream else torch.empty(shape, dtype=stream.dtype, device=dev)
+        o2, o_pitch = out, d
+    else:
+        if out.shape != shape or out.dtype != stream.dtype or out.device != dev:
+            raise ValueError(f"residual_norm: out must be {stream.dtype} {tuple(shape)} on {dev}")
+        o2 = out if out.dim() == 2 else out.view(-1, d)
+        if d > 1 and o2.stride(1) != 1:
+            raise ValueError("residual_norm: out must have unit stride in its last dimension")
+        o_pitch = o2.stride(0) if o2.shape[0] > 1 else d
+    after = None
+    if pre_weight is not None:
+        after = (torch.empty_like(y) if ot == yt and y2 is y else
+                 torch.empty(shape, dtype=y.dtype if out_dtype is None else out_dtype, device=dev))
+    rows = stream.numel() // d if d else 0
     if rows == 0:
         return out, after
     g_ptr, g_type, g_pitch, g_wide, per = None, 0, 0, 0, 1
     if gate is not None:
-        if not isinstance(gate, torch.Tensor) or gate.dtype not in _DT or gate.device != dev or gate.dim() > len(shape):
-            raise ValueError(f"residual_norm: gate must be an fp32, fp16 or bf16 tensor on {dev} that broadcasts to {tuple(shape)}")
-        lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
-        if gate.dim() == 0 or any(n not in (1, s) for n, s in zip(lead, shape)):
-            raise ValueError(f"residual_norm: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-        gate = gate.reshape(lead)
-        last = len(lead) - 1                              # leading sizes that the gate has, then ones
-        while last > 0 and lead[last - 1] == 1:
-            last -= 1
-        if any(n != s for n, s in zip(lead[:last], shape)):
-            gate, last = gate.expand(*shape[:-1], lead[-1]), len(shape) - 1
-        g2 = _as_rows(gate, lead[-1])
+        g2, g_wide = _gate_rows(gate, shape, dev)
         per = rows // g2.shape[0]
-        g_ptr, g_type, g_wide = g2.data_ptr(), _DT[g2.dtype], int(lead[-1] == d)
-        g_pitch = g2.stride(0) if g2.shape[0] > 1 else 0
-    check(call_on(dev, lib.xm_residual_norm, h2.data_ptr(), _DT[h2.dtype], h2.stride(0) if rows > 1 else d, y2.data_ptr(),
-                  _DT[y2.dtype], y2.stride(0) if rows > 1 else d, rows, d, _ptr(post_weight), g_ptr, g_type, g_pitch, g_wide,
-                  per, scale, _ptr(pre_weight), eps, o2.data_ptr(), o2.stride(0) if rows > 1 else d, _ptr(after),
-                  _DT[out_dtype], d), "residual_norm")
+        g_ptr, g_type, g_pitch = g2.data_ptr(), _DT[g2.dtype], g2.stride(0) if g2.shape[0] > 1 else 0
+    check(call_on(dev, lib.xm_residual_norm, h2.data_ptr(), ht, h_pitch, y2.data_ptr(), yt, y_pitch, rows, d, weights[0], g_ptr,
+                  g_type, g_pitch, g_wide, per, scale, weights[1], eps, o2.data_ptr(), o_pitch,
+                  None if after is None else after.data_ptr(), ot, d), "residual_norm")
     return out, after
 
 

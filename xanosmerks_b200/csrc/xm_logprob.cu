@@ -14,8 +14,8 @@
 // spread over the whole part, so that few hundred of 128000 pass).  A list that runs over, or a threshold of -inf, sends the
 // CTA to the slow way: one pass a place.
 //
-// C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM for many rows (each logit is read once; some seven
-// instructions and one exponential a logit), latency for few.
+// C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
+// eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
 #include <cooperative_groups.h>
 
 #include "xm_gemv_dot.cuh"
@@ -41,6 +41,7 @@ struct LogpArgs {
 
 struct alignas(16) LogpSmem {
   u64 list[kListCap];
+  int vectors[kListCap];                   // those with a logit for the list
   u64 best[kTopMax];                       // this CTA's largest, in order; 0: none
   u64 merge[kClusterMax * kTopMax];
   float red[kWarps][4];
@@ -51,6 +52,10 @@ struct alignas(16) LogpSmem {
   double r;                                // c x reference (log2)
   float S, E, mx;
   int above;
+  // the row's
+  double lse;
+  bool inf;
+  int rank;
 };
 
 // order-preserving key of a logit: NaN and -inf below everything else
@@ -68,6 +73,20 @@ XM_DEV float exp2_fast(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
+}
+// two fp32 operations in one instruction
+XM_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+XM_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 // the next larger number (of +inf: NaN, which compares as nothing does)
@@ -202,6 +221,52 @@ XM_DEV bool best_of_list(LogpSmem& sm, int n, int top) {
   return true;
 }
 
+// How many logits of a vector reach a threshold, and their maximum: of 16-bit logits two at a time, in their own type (a
+// threshold that is no number of the type is never reached).
+template <typename XT>
+struct Ranks {
+  typedef float Threshold;
+  int n = 0;
+  XM_DEV static Threshold threshold(float t) { return t; }
+  XM_DEV static float max_of(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  XM_DEV void add(const uint4& u, Threshold t, float most) {
+    if (most >= t)
+      n += (__uint_as_float(u.x) >= t) + (__uint_as_float(u.y) >= t) + (__uint_as_float(u.z) >= t) + (__uint_as_float(u.w) >= t);
+  }
+  XM_DEV void flush() {}
+};
+template <typename T2, typename T1>
+struct Ranks16 {
+  typedef T2 Threshold;
+  int n = 0;
+  T2 part;                                 // counts of up to 64 vectors: whole numbers of bf16 too (4 a vector and half)
+  XM_DEV Ranks16() { memset(&part, 0, 4); }
+  XM_DEV static T2 two(uint32_t w) {
+    T2 t;
+    memcpy(&t, &w, 4);
+    return t;
+  }
+  XM_DEV static float max_of(const uint4& u) {
+    const T2 m = __hmax2(__hmax2(two(u.x), two(u.y)), __hmax2(two(u.z), two(u.w)));
+    return fmaxf((float)m.x, (float)m.y);
+  }
+  XM_DEV void add(const uint4& u, Threshold t, float) {
+    part = __hadd2(part, __hadd2(__hadd2(__hge2(two(u.x), t), __hge2(two(u.y), t)), __hadd2(__hge2(two(u.z), t), __hge2(two(u.w), t))));
+  }
+  XM_DEV void flush() {
+    n += (int)((float)part.x + (float)part.y);
+    memset(&part, 0, 4);
+  }
+};
+template <> struct Ranks<__half> : Ranks16<__half2, __half> {
+  XM_DEV static __half2 threshold(float t) { return __half2half2(__float2half_ru(t)); }
+};
+template <> struct Ranks<__nv_bfloat16> : Ranks16<__nv_bfloat162, __nv_bfloat16> {
+  XM_DEV static __nv_bfloat162 threshold(float t) { return __bfloat162bfloat162(__float2bfloat16_ru(t)); }
+};
+
 template <typename XT>
 __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   constexpr int VE = Part<XT>::VE;
@@ -230,28 +295,28 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   const float thr_hi = seen ? above(xt) : -3.402823466e38f, thr_lo = seen ? xt : thr_hi;
   const int tv = valid ? (p.mis + (int)token) / VE : 0;
 
-  // rounds of kUnroll vectors a thread; the vectors of a round lie spread over the part
-  const int chunks = (p.nv + 31) / 32, rounds = (chunks + kWarps * kUnroll - 1) / (kWarps * kUnroll);
-  auto vec = [&](int r, int u) { return p.v0 + (r + rounds * (u * kWarps + warp)) * 32 + lane; };
-  const int end = p.v0 + p.nv;
+  // Rounds of kUnroll vectors a thread; the vectors of a round lie spread over the part.  Vectors at the row's ends, which may
+  // hold others' logits too, are the last warp's last.
+  const int lo = p.v0 + (p.nv > 0 && !p.inner(p.v0)), end = p.v0 + p.nv - (p.nv > 0 && !p.inner(p.v0 + p.nv - 1) && p.nv > lo - p.v0);
+  const int chunks = (end - lo + 31) / 32, rounds = (chunks + kWarps * kUnroll - 1) / (kWarps * kUnroll);
+  const int first = lo + rounds * warp * 32 + lane, apart = rounds * kWarps * 32;      // vector u of round r: first + u apart + 32 r
+  const uint4* const vectors_at = reinterpret_cast<const uint4*>(p.base);
   const uint4 none = sizeof(XT) == 4 ? make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu)
                                      : make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-  uint4 cur[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int v = vec(0, u);
-    cur[u] = rounds > 0 && v < end ? p.load(v) : none;
+  uint4 cur[kUnroll], edge = none;
+  int edge_v = -1;
+  if (warp == kWarps - 1 && lane < 2) {
+    edge_v = lane == 0 ? (lo > p.v0 ? p.v0 : -1) : (end < p.v0 + p.nv ? p.v0 + p.nv - 1 : -1);
+    if (edge_v >= 0) edge = p.edge(edge_v);
   }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) cur[u] = first + u * apart < end ? ldg_stream_v4(vectors_at + first + u * apart) : none;
   if (tid == 0) sm.n = 0;
   // the reference and the list's threshold
-  float m = -INFINITY;
+  float m = Ranks<XT>::max_of(edge);
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    float x[VE];
-    Part<XT>::values(cur[u], x);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) m = fmaxf(m, x[i]);
-  }
+  for (int u = 0; u < kUnroll; ++u) m = fmaxf(m, Ranks<XT>::max_of(cur[u]));
+  m = fmaxf(m, -INFINITY);                           // (NaN: nothing)
   float thr_top = __uint_as_float(0x7fffffffu);
   const bool whole = p.nv * VE <= kListCap;          // a part that the list holds
   bool slow = false;
@@ -263,44 +328,47 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   m = block_max_f(m, sm);
   const float ref = m > -INFINITY && m < INFINITY ? m : 0.f;
   const float rc = greedy ? 0.f : ref * c;
-  float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
-  int count = 0;
   const float cc = greedy ? 0.f : c;
+  float2 S = make_float2(0.f, 0.f), E = S;
+  Ranks<XT> ranks;
+  typename Ranks<XT>::Threshold at_least_lo = Ranks<XT>::threshold(thr_lo), at_least_hi = Ranks<XT>::threshold(thr_hi);
+  // (their conversion is long: not once a vector)
+  asm volatile("" : "+r"(reinterpret_cast<uint32_t&>(at_least_lo)), "+r"(reinterpret_cast<uint32_t&>(at_least_hi)));
+  auto take = [&](const uint4& raw, int v) {
+    float x[VE];
+    Part<XT>::values(raw, x);
+#pragma unroll
+    for (int i = 0; i < VE; i += 2) {
+      float2 t = fma2(make_float2(x[i], x[i + 1]), make_float2(cc, cc), make_float2(-rc, -rc));
+      t.x = fmaxf(t.x, -200.f);
+      t.y = fmaxf(t.y, -200.f);
+      const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+      S = add2(S, e);
+      E = fma2(e, t, E);
+    }
+    const float most = Ranks<XT>::max_of(raw);
+    ranks.add(raw, v < tv ? at_least_lo : at_least_hi, most);
+    if (most >= thr_top) {                           // (which of its logits: later, for all such vectors together)
+      const int at = atomicAdd(&sm.n, 1);
+      if (at < kListCap) sm.vectors[at] = v;
+    }
+  };
   for (int r = 0; r < rounds; ++r) {
     uint4 next[kUnroll];
+    const int v = first + 32 * r;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = vec(r + 1, u);
-      next[u] = r + 1 < rounds && v < end ? p.load(v) : none;
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      next[u] = r + 1 < rounds && v + 32 + u * apart < end ? ldg_stream_v4(vectors_at + v + 32 + u * apart) : none;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[VE], vm = -INFINITY;
-      Part<XT>::values(cur[u], x);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const float t = fmaxf(fmaf(x[i], cc, -rc), -200.f), e = exp2_fast(t);
-        S[i & 1] += e;
-        E[i & 1] = fmaf(e, t, E[i & 1]);
-        vm = fmaxf(vm, x[i]);
-      }
-      const int v = vec(r, u);
-      const float thr = v < tv ? thr_lo : thr_hi;
-      if (vm >= fminf(thr, thr_top)) {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          count += x[i] >= thr;
-          if (x[i] >= thr_top) {
-            const int at = atomicAdd(&sm.n, 1);
-            if (at < kListCap) sm.list[at] = entry(x[i], p.index(v) + i);
-          }
-        }
-      }
-    }
+    for (int u = 0; u < kUnroll; ++u) take(cur[u], v + u * apart);
+    if ((r & 15) == 15) ranks.flush();
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) cur[u] = next[u];
   }
-  float s = block_sum_f(S[0] + S[1], sm), e = block_sum_f(E[0] + E[1], sm);
+  if (edge_v >= 0) take(edge, edge_v);
+  ranks.flush();
+  int count = ranks.n;
+  float s = block_sum_f(S.x + S.y, sm), e = block_sum_f(E.x + E.y, sm);
   double r2 = (double)rc;
   float mx = ref;
   if (greedy) {
@@ -311,18 +379,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     mx = -INFINITY;
     p.each([&](float x, int) { mx = fmaxf(mx, x); });
     mx = block_max_f(mx, sm);
-    S[0] = E[0] = 0.f;
+    s = e = 0.f;
     if (mx > -INFINITY) {
       p.each([&](float x, int) {
         const float t = x == mx ? 0.f : fmaxf((x - mx) * c, -200.f), w = exp2_fast(t);
         if (x == mx || mx < INFINITY) {
-          S[0] += w;
-          E[0] = fmaf(w, t, E[0]);
+          s += w;
+          e = fmaf(w, t, e);
         }
       });
     }
-    s = block_sum_f(S[0], sm);
-    e = block_sum_f(E[0], sm);
+    s = block_sum_f(s, sm);
+    e = block_sum_f(e, sm);
     r2 = (double)mx * (double)c;
   }
   if (!seen) p.each([&](float x, int i) { count += i < token && !(x > -INFINITY); });
@@ -340,9 +408,27 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   }
   if (a.top > 0) {
     if (tid < kTopMax) sm.best[tid] = 0ull;
-    if (whole) p.each([&](float x, int i) { sm.list[atomicAdd(&sm.n, 1)] = entry(x, i); });
+    const int listed = sm.n;
     __syncthreads();
-    const int n = sm.n;
+    if (tid == 0) sm.n = 0;
+    __syncthreads();
+    if (whole) {
+      p.each([&](float x, int i) { sm.list[atomicAdd(&sm.n, 1)] = entry(x, i); });
+    } else if (listed <= kListCap) {
+      for (int l = tid; l < listed; l += kThreads) {
+        const int v = sm.vectors[l];
+        float x[VE];
+        Part<XT>::values(p.load(v), x);
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          if (x[i] >= thr_top) {
+            const int at = atomicAdd(&sm.n, 1);
+            if (at < kListCap) sm.list[at] = entry(x[i], p.index(v) + i);
+          }
+      }
+    }
+    __syncthreads();
+    const int n = listed <= kListCap ? sm.n : listed;
     __syncthreads();
     if (!slow) slow = n > kListCap || !best_of_list(sm, n, a.top);
     if (slow) {
@@ -370,31 +456,43 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   if (C > 1) cl.sync();
   else __syncthreads();
   if (cr == 0) {
-    // the parts' sums, on the largest reference
-    double R = -INFINITY;
-    bool inf = false;
-    int rank = 0;
-    for (int i = 0; i < C; ++i) {
-      const LogpSmem* o = C > 1 ? cl.map_shared_rank(&sm, i) : &sm;
-      if (o->S > 0.f) {
-        R = fmax(R, o->r);
-        inf = inf || !(o->mx < INFINITY);
+    // the parts' sums, on the largest reference (a part a lane of the first warp)
+    if (warp == 0) {
+      const LogpSmem* o = C > 1 && lane < C ? cl.map_shared_rank(&sm, lane) : &sm;
+      const bool there = lane < C && o->S > 0.f;
+      double R = there ? o->r : -INFINITY, part_S = there ? (double)o->S : 0., part_E = there ? (double)o->E : 0.;
+      const bool inf_part = there && !(o->mx < INFINITY), inf = __any_sync(~0u, inf_part);
+      int rank = lane < C ? o->above : 0;
+      const double mine_r = R;
+#pragma unroll
+      for (int i = kClusterMax / 2; i > 0; i >>= 1) {
+        R = fmax(R, __shfl_xor_sync(~0u, R, i));
+        rank += __shfl_xor_sync(~0u, rank, i);
       }
-      rank += o->above;
-    }
-    double SS = 0., EE = 0.;
-    for (int i = 0; i < C; ++i) {
-      const LogpSmem* o = C > 1 ? cl.map_shared_rank(&sm, i) : &sm;
-      if (!(o->S > 0.f)) continue;
       if (inf) {
-        if (!(o->mx < INFINITY)) SS += (double)o->S;
-      } else {
-        const double d = o->r - R, f = exp2(d);
-        SS += f * (double)o->S;
-        EE += f * ((double)o->E + d * (double)o->S);
+        part_S = inf_part ? part_S : 0.;
+        part_E = 0.;
+      } else if (there) {
+        const double d = mine_r - R, f = d < 0. ? exp2(d) : 1.;
+        part_E = f * (part_E + d * part_S);
+        part_S *= f;
+      }
+#pragma unroll
+      for (int i = kClusterMax / 2; i > 0; i >>= 1) {
+        part_S += __shfl_xor_sync(~0u, part_S, i);
+        part_E += __shfl_xor_sync(~0u, part_E, i);
+      }
+      if (lane == 0) {
+        sm.lse = inf ? log2(part_S) : R + log2(part_S);
+        sm.inf = inf;
+        sm.rank = rank;
+        a.entropy[b] = greedy || !(part_S > 0.) ? 0.f : (float)fmax(0.0, 0.6931471805599453 * (log2(part_S) - part_E / part_S));
       }
     }
-    const double lse = inf ? log2(SS) : R + log2(SS);
+    __syncthreads();
+    const double lse = sm.lse;
+    const bool inf = sm.inf;
+    int rank = sm.rank;
     auto logp = [&](float x, bool first) -> float {
       if (!(x > -INFINITY)) return greedy && first ? 0.f : -INFINITY;
       if (greedy) return first ? 0.f : -INFINITY;
@@ -408,7 +506,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
       }
       a.rank[b] = valid ? rank : -1;
       a.logprob[b] = valid ? logp(xt, rank == 0 && seen) : __uint_as_float(0x7fffffffu);
-      a.entropy[b] = greedy || !(SS > 0.) ? 0.f : (float)fmax(0.0, 0.6931471805599453 * (log2(SS) - EE / SS));
     }
     if (a.top > 0) {
       const int all = C * a.top;

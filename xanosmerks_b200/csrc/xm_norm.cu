@@ -94,9 +94,10 @@ XM_DEV float row_sum(float v, float* red, bool block) {
 }
 
 // V: values a load; NP: packs of 8 values a thread.  Vector j of the row's thread t is vector j * (threads of the row) + t.
-// MAXT: threads of a block at most.
+// MAXT: threads of a block at most; three blocks on an SM where the registers allow it, for the loads that are on their way
+// together.
 template <typename HT, typename YT, int V, int NP, int MAXT>
-__global__ void __launch_bounds__(MAXT) k_residual_norm(NormArgs a) {
+__global__ void __launch_bounds__(MAXT, MAXT == 128 || (MAXT == 256 && NP == 2) ? 3 : 1) k_residual_norm(NormArgs a) {
   constexpr int NV = 8 / V * NP;
   __shared__ float red[2][32];
   grid_dep_wait();
@@ -219,6 +220,7 @@ cudaError_t norm_np(const NormArgs& a, cudaStream_t st) {
   if (a.D <= 256) return norm_launch<HT, YT, V, 1, 128>(a, st);
   if (a.D <= 1024) return norm_launch<HT, YT, V, 4, 128>(a, st);
   if (a.D <= 2048) return norm_launch<HT, YT, V, 1, 256>(a, st);
+  if (a.D <= 4096) return norm_launch<HT, YT, V, 2, 256>(a, st);
   if (a.D <= 8192) return norm_launch<HT, YT, V, 2, 512>(a, st);
   if (a.D <= 16384) return norm_launch<HT, YT, V, 2, 1024>(a, st);
   return norm_launch<HT, YT, V, 4, 1024>(a, st);

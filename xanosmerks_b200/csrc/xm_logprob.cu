@@ -9,10 +9,10 @@
 // part of the row again with its own maximum.  A weight's exponent is held above -200, which also gives -inf and NaN logits
 // the weight 0 (and 0 in E).
 //
-// Alternatives: after the first round every warp knows the j-th largest of its lanes' maxima; the least of these over the
-// warps, j = ceil(top / warps), has at least `top` logits at or above it.  Only those go to a list (the round's logits are
-// spread over the whole part, so that few hundred of 128000 pass).  A list that runs over, or a threshold of -inf, sends the
-// CTA to the slow way: one pass a place.
+// Alternatives: every warp knows the j-th largest of its lanes' maxima so far; the least of these over the warps, j = ceil(top
+// / warps), has at least `top` logits at or above it.  Only vectors with such logits go to a list, and the threshold is raised
+// whenever twice as much has been seen (a round's logits are spread over the whole part), so that a few hundred of 128000
+// pass.  A list that runs over, or a threshold of -inf, sends the CTA to the slow way: one pass a place.
 //
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
@@ -231,8 +231,8 @@ struct Ranks {
   XM_DEV static float max_of(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
-  XM_DEV void add(const uint4& u, Threshold t, float most) {
-    if (most >= t)
+  XM_DEV void add(const uint4& u, Threshold t) {
+    if (max_of(u) >= t)
       n += (__uint_as_float(u.x) >= t) + (__uint_as_float(u.y) >= t) + (__uint_as_float(u.z) >= t) + (__uint_as_float(u.w) >= t);
   }
   XM_DEV void flush() {}
@@ -252,7 +252,7 @@ struct Ranks16 {
     const T2 m = __hmax2(__hmax2(two(u.x), two(u.y)), __hmax2(two(u.z), two(u.w)));
     return fmaxf((float)m.x, (float)m.y);
   }
-  XM_DEV void add(const uint4& u, Threshold t, float) {
+  XM_DEV void add(const uint4& u, Threshold t) {
     part = __hadd2(part, __hadd2(__hadd2(__hge2(two(u.x), t), __hge2(two(u.y), t)), __hadd2(__hge2(two(u.z), t), __hge2(two(u.w), t))));
   }
   XM_DEV void flush() {
@@ -267,7 +267,8 @@ template <> struct Ranks<__nv_bfloat16> : Ranks16<__nv_bfloat162, __nv_bfloat16>
   XM_DEV static __nv_bfloat162 threshold(float t) { return __bfloat162bfloat162(__float2bfloat16_ru(t)); }
 };
 
-template <typename XT>
+// TOP: whether there are alternatives to find.
+template <typename XT, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   constexpr int VE = Part<XT>::VE;
   __shared__ LogpSmem sm;
@@ -320,11 +321,12 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   float thr_top = __uint_as_float(0x7fffffffu);
   const bool whole = p.nv * VE <= kListCap;          // a part that the list holds
   bool slow = false;
-  if (a.top > 0 && !whole) {
+  if (TOP && !whole) {
     const uint32_t t = block_threshold(logit_key(m), a.top, sm);
     slow = t == 0;
     if (!slow) thr_top = key_logit(t);
   }
+  float peak = -INFINITY;                            // of what this thread has seen
   m = block_max_f(m, sm);
   const float ref = m > -INFINITY && m < INFINITY ? m : 0.f;
   const float rc = greedy ? 0.f : ref * c;
@@ -346,11 +348,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
       S = add2(S, e);
       E = fma2(e, t, E);
     }
-    const float most = Ranks<XT>::max_of(raw);
-    ranks.add(raw, v < tv ? at_least_lo : at_least_hi, most);
-    if (most >= thr_top) {                           // (which of its logits: later, for all such vectors together)
-      const int at = atomicAdd(&sm.n, 1);
-      if (at < kListCap) sm.vectors[at] = v;
+    ranks.add(raw, v < tv ? at_least_lo : at_least_hi);
+    if constexpr (TOP) {
+      const float most = Ranks<XT>::max_of(raw);
+      peak = fmaxf(peak, most);
+      if (most >= thr_top) {                         // (which of its logits: later, for all such vectors together)
+        const int at = atomicAdd(&sm.n, 1);
+        if (at < kListCap) sm.vectors[at] = v;
+      }
     }
   };
   for (int r = 0; r < rounds; ++r) {
@@ -362,6 +367,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) take(cur[u], v + u * apart);
     if ((r & 15) == 15) ranks.flush();
+    if constexpr (TOP)
+      if (!slow && !whole && r > 0 && (r & (r + 1)) == 0 && r + 1 < rounds) {
+        const uint32_t t = block_threshold(logit_key(peak), a.top, sm);
+        if (t) thr_top = fmaxf(thr_top, key_logit(t));
+      }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) cur[u] = next[u];
   }
@@ -406,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     sm.E = e;
     sm.mx = mx;
   }
-  if (a.top > 0) {
+  if constexpr (TOP) {
     if (tid < kTopMax) sm.best[tid] = 0ull;
     const int listed = sm.n;
     __syncthreads();
@@ -507,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
       a.rank[b] = valid ? rank : -1;
       a.logprob[b] = valid ? logp(xt, rank == 0 && seen) : __uint_as_float(0x7fffffffu);
     }
-    if (a.top > 0) {
+    if constexpr (TOP) {
       const int all = C * a.top;
       for (int i = tid; i < all; i += kThreads) {
         const LogpSmem* o = C > 1 ? cl.map_shared_rank(&sm, i / a.top) : &sm;
@@ -549,7 +559,7 @@ cudaError_t logp_launch(const LogpArgs& a, int64_t B, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_logprobs<XT>, a);
+  return a.top > 0 ? cudaLaunchKernelEx(&cfg, k_logprobs<XT, true>, a) : cudaLaunchKernelEx(&cfg, k_logprobs<XT, false>, a);
 }
 
 }  // namespace

@@ -111,9 +111,9 @@ XM_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;
 // A cluster of 8 CTAs a token: each has the whole row and an eighth of the experts, one for each warp, or for several warps
 // where there are few (which then take parts of the row).  The logits go to the first CTA's shared memory, the others end.
 template <typename XT>
-__global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
+__global__ void __launch_bounds__(kRouteThreads, 3) k_moe_step_route(RouteArgs a) {
   constexpr int WARPS = kRouteThreads / 32;
-  extern __shared__ __align__(16) float row[];
+  extern __shared__ __align__(16) double row[];               // (converted once, not for each expert)
   __shared__ float red[WARPS];
   __shared__ double part[WARPS], all[kMaxStepExperts], val[kMaxTop];
   __shared__ unsigned chosen[WARPS];
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
 #pragma unroll 8
   for (int i = tid; i < a.H; i += kRouteThreads) {
     const float v = to_f32<XT>(x[i]);
-    row[i] = a.norm_w ? v * a.norm_w[i] : v;
+    row[i] = (double)(a.norm_w ? v * a.norm_w[i] : v);
     s = fmaf(v, v, s);
   }
   s = warp_sum(s);
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
   s = 0.f;
   for (int w = 0; w < WARPS; ++w) s += red[w];
   const float r = a.norm_w ? 1.0f / sqrtf(s / (float)a.H + a.eps) : 1.0f;
-  for (int i = rank * kRouteThreads + tid; i < a.H; i += kRouteCluster * kRouteThreads) a.v[(int64_t)t * a.H + i] = row[i] * r;
+  for (int i = rank * kRouteThreads + tid; i < a.H; i += kRouteCluster * kRouteThreads) a.v[(int64_t)t * a.H + i] = (float)row[i] * r;
   cluster_wait();
   double* to = cl.map_shared_rank(all, 0);
   for (int j0 = 0; j0 < mine; j0 += at_once) {
@@ -160,14 +160,14 @@ __global__ void __launch_bounds__(kRouteThreads) k_moe_step_route(RouteArgs a) {
     double d = 0.;
     if (j < mine) {
       const float4* g = reinterpret_cast<const float4*>(a.gate + (int64_t)(rank + j * kRouteCluster) * a.H) + slice * n4;
-      const float* v = row + 4 * slice * n4;
+      const double* v = row + 4 * slice * n4;
       double q[4] = {0., 0., 0., 0.};
       auto add = [&](const float4& w, int i) {
-        const float4 u = *reinterpret_cast<const float4*>(v + 4 * i);
-        q[0] = fma((double)u.x, (double)w.x, q[0]);
-        q[1] = fma((double)u.y, (double)w.y, q[1]);
-        q[2] = fma((double)u.z, (double)w.z, q[2]);
-        q[3] = fma((double)u.w, (double)w.w, q[3]);
+        const double2 u = *reinterpret_cast<const double2*>(v + 4 * i), z = *reinterpret_cast<const double2*>(v + 4 * i + 2);
+        q[0] = fma(u.x, (double)w.x, q[0]);
+        q[1] = fma(u.y, (double)w.y, q[1]);
+        q[2] = fma(z.x, (double)w.z, q[2]);
+        q[3] = fma(z.y, (double)w.w, q[3]);
       };
       int i = lane;
       if (j0 == 0) {
@@ -472,15 +472,18 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
     for (int i = 0; i < Result<M>::N; ++i) acc.v[r][i] = fmaf(d[r], sum.v[r][i], acc.v[r][i]);
 }
 
-// The 32-bit word at a 2-byte aligned address.
+// The 32-bit word at a 4-byte (FOUR) or 2-byte aligned address.
+template <bool FOUR>
 XM_DEV uint32_t lds_word(const uint8_t* p) {
+  if constexpr (FOUR) return *reinterpret_cast<const uint32_t*>(p);
   const uint32_t sh = ((uint32_t)(uintptr_t)p & 2) * 8;
   const uint32_t* a = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
   return __funnelshift_r(a[0], a[1], sh);
 }
 
-// Q6_K: w = d s_g (c - 32), groups of 16, records at any even address.  Codes are put together as bytes, four at a time.
-template <int M>
+// Q6_K: w = d s_g (c - 32), groups of 16, records at any even address (every other one at a multiple of four: FOUR).  Codes are
+// put together as bytes, four at a time.
+template <int M, bool FOUR>
 XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
   uint32_t sc[2][4];                       // s + 128, bytes
   float d[2];
@@ -507,9 +510,9 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint8_t* q = r ? r1 : r0;
-        low[r][0] = lds_word(q + 64 * h + 16 * p + 4 * t);
-        low[r][1] = lds_word(q + 64 * h + 32 + 16 * p + 4 * t);
-        high[r] = lds_word(q + 128 + 32 * h + 16 * p + 4 * t);
+        low[r][0] = lds_word<FOUR>(q + 64 * h + 16 * p + 4 * t);
+        low[r][1] = lds_word<FOUR>(q + 64 * h + 32 + 16 * p + 4 * t);
+        high[r] = lds_word<FOUR>(q + 128 + 32 * h + 16 * p + 4 * t);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -517,11 +520,12 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
         uint32_t q[2][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t nib = (i < 2 ? low[r][i & 1] : low[r][i & 1] >> 4) & 0x0f0f0f0fu;
-          const uint32_t two = (i == 0 ? high[r] << 4 : i == 1 ? high[r] << 2 : i == 2 ? high[r] : high[r] >> 2) & 0x30303030u;
-          const uint32_t c4 = nib | two;
-          q[r][0] = c4 & 0x00ff00ffu;
-          q[r][1] = (c4 >> 8) & 0x00ff00ffu;
+          // (one selection: what it leaves above the sixth bit goes with the masks of the pairs)
+          const uint32_t nib = i < 2 ? low[r][i & 1] : low[r][i & 1] >> 4;
+          const uint32_t two = i == 0 ? high[r] << 4 : i == 1 ? high[r] << 2 : i == 2 ? high[r] : high[r] >> 2;
+          const uint32_t c4 = (nib & 0x0f0f0f0fu) | (two & 0xf0f0f0f0u);
+          q[r][0] = c4 & 0x003f003fu;
+          q[r][1] = __byte_perm(c4, 0u, 0x4341) & 0x003f003fu;
         }
         const uint32_t a[4] = {q[0][0], q[1][0], q[0][1], q[1][1]};
         if constexpr (M == 1) {
@@ -639,7 +643,10 @@ XM_DEV void unit(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& 
   static_assert(M != 1 || own_value<T>(), "one scale for a group of values");
   if constexpr (T == T_Q4_K) unit_k<false, M>(r0, r1, t, x, acc);
   else if constexpr (T == T_Q5_K) unit_k<true, M>(r0, r1, t, x, acc);
-  else if constexpr (T == T_Q6_K) unit_q6k<M>(r0, r1, t, x, acc);
+  else if constexpr (T == T_Q6_K) {
+    if (__all_sync(~0u, (((uintptr_t)r0 | (uintptr_t)r1) & 2) == 0)) unit_q6k<M, true>(r0, r1, t, x, acc);
+    else unit_q6k<M, false>(r0, r1, t, x, acc);
+  }
   else if constexpr (T == T_Q8_0) unit_q80<M>(r0, r1, t, x, acc);
   else unit_any<T, M>(r0, r1, t, x, acc);
 }
@@ -1390,9 +1397,9 @@ int xm_moe_step(const void* d_x, int x_dtype, int64_t T, int64_t H, int64_t x_st
                     i32(l.tickets), l.n_tickets};
   const dim3 routes((unsigned)T * kRouteCluster);
   cudaError_t e =
-      x_dtype == XM_DT_F32   ? step_launch<k_moe_step_route<float>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r)
-      : x_dtype == XM_DT_F16 ? step_launch<k_moe_step_route<__half>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r)
-                             : step_launch<k_moe_step_route<__nv_bfloat16>>(routes, kRouteThreads, (int)H * 4, kRouteCluster, st, r);
+      x_dtype == XM_DT_F32   ? step_launch<k_moe_step_route<float>>(routes, kRouteThreads, (int)H * 8, kRouteCluster, st, r)
+      : x_dtype == XM_DT_F16 ? step_launch<k_moe_step_route<__half>>(routes, kRouteThreads, (int)H * 8, kRouteCluster, st, r)
+                             : step_launch<k_moe_step_route<__nv_bfloat16>>(routes, kRouteThreads, (int)H * 8, kRouteCluster, st, r);
   if (e == cudaSuccess) {
     const Table t = table_at(d_table, E);
     StepArgs up = {}, down = {};

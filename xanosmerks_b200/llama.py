@@ -15,7 +15,11 @@ GEMV), and so are gate and up; the caches are fp16 ``[B][Hk][max_ctx][128]``,
 or, with ``kv_type``, a :class:`~xanosmerks_b200.kvcache.PagedKVCache` per layer
 (fp16 or 4-bit), which also takes models that normalise the heads of queries and
 keys.  The next token is the first maximum (greedy) or sampled
-(:meth:`LlamaDecoder.set_sampling`).
+(:meth:`LlamaDecoder.set_sampling`).  The MLP of a layer may be a mixture of experts
+(:meth:`~xanosmerks_b200.moe.MoELayer.step` in a decode step), blocks may have a norm
+behind them too and a scale in front of the residual add
+(:func:`~xanosmerks_b200.ops.residual_norm`), and whole sequences are scored by
+:meth:`LlamaDecoder.score`.
 
 Tensor parallelism (``world_size > 1``, one process per GPU): attention heads
 and FFN columns are split across ranks (QKV and gate/up column-parallel, O and
@@ -34,8 +38,9 @@ import torch
 from . import qtypes
 from ._lib import DT_F16, DT_F32, PRO_NONE, PRO_RMSNORM, PRO_SWIGLU, check, check_device, lib
 from .kvcache import PagedKVCache, rope_table
-from .ops import GGUFTensor, gemm_supported
-from .sampling import sample
+from .moe import MoELayer
+from .ops import GGUFTensor, gemm_supported, residual_norm
+from .sampling import TokenLogprobs, logprobs, sample
 from .synth import make_weight_device
 
 __all__ = ["LlamaConfig", "LlamaWeights", "LlamaDecoder", "synth_llama_weights", "shard_rows", "shard_cols"]
@@ -62,6 +67,11 @@ class LlamaConfig:
     output_qtype: str = "Q6_K"
     embed_qtype: str = "Q4_K"
     qk_norm: bool = False                # RMSNorm of each query and key head before the rotation
+    num_experts: int = 0                 # > 0: every MLP is a mixture of that many experts of intermediate_size
+    num_experts_per_tok: int = 2
+    expert_qtype: str = "Q4_K"           # of an expert's three weights
+    post_norms: bool = False             # RMSNorm of each block's output before the residual add
+    residual_scale: float = 1.0          # of a block's output in the residual add
 
     def reference_config(self) -> dict:
         """The keys the reference's model classes read (forward.py, attention.py)."""
@@ -76,8 +86,11 @@ class LlamaConfig:
         D, F, V = self.hidden_size, self.intermediate_size, self.vocab_size
         qkv = (self.num_heads + 2 * self.num_kv_heads) * self.head_dim
         rb = lambda q, n, k: n * qtypes.row_bytes(qtypes.normalize(q), k)  # noqa: E731
-        layer = (rb(self.attn_qtype, qkv, D) + rb(self.attn_qtype, D, self.num_heads * self.head_dim)
-                 + rb(self.gate_up_qtype, 2 * F, D) + rb(self.down_qtype, D, F))
+        layer = rb(self.attn_qtype, qkv, D) + rb(self.attn_qtype, D, self.num_heads * self.head_dim)
+        if self.num_experts:
+            layer += self.num_experts_per_tok * (2 * rb(self.expert_qtype, F, D) + rb(self.expert_qtype, D, F))
+        else:
+            layer += rb(self.gate_up_qtype, 2 * F, D) + rb(self.down_qtype, D, F)
         return self.num_layers * layer + rb(self.output_qtype, V, D)
 
 
@@ -117,7 +130,9 @@ class LlamaWeights:
     heads), ``o`` [D, Hq*128 / world], ``gate_up`` [2F / world, D] (gate rows then
     up rows), ``down`` [D, F / world], ``attn_norm`` / ``ffn_norm`` fp32 [D];
     ``embed`` [V, D], ``norm`` fp32 [D], ``output`` [V, D]; with ``cfg.qk_norm`` also
-    ``q_norm`` / ``k_norm`` fp32 [head_dim] per layer."""
+    ``q_norm`` / ``k_norm`` fp32 [head_dim] per layer, with ``cfg.post_norms``
+    ``post_attn_norm`` / ``post_ffn_norm`` fp32 [D]; with ``cfg.num_experts`` a ``moe``
+    (:class:`~xanosmerks_b200.moe.MoELayer`) instead of ``gate_up`` and ``down``."""
 
     def __init__(self, cfg: LlamaConfig, embed, layers, norm, output, rank=0, world=1):
         self.cfg, self.embed, self.layers, self.norm, self.output = cfg, embed, layers, norm, output
@@ -126,10 +141,14 @@ class LlamaWeights:
     @classmethod
     def from_full(cls, cfg: LlamaConfig, full: dict, rank: int = 0, world: int = 1) -> "LlamaWeights":
         """Shard full per-layer tensors ``wq, wk, wv, wo, wg, wu, wd`` (GGUFTensor)
-        and ``n1, n2`` (with ``cfg.qk_norm`` also ``qn, kn``) for ``rank`` of ``world``."""
+        and ``n1, n2`` (with ``cfg.qk_norm`` also ``qn, kn``, with ``cfg.post_norms`` ``pn1, pn2``; with
+        ``cfg.num_experts`` ``moe``, the nested dict of ``MoELayer``, instead of ``wg, wu, wd``) for ``rank`` of ``world``."""
         hq, hk, hd, F = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.intermediate_size
         if hq % world or hk % world or F % world:
             raise ValueError(f"heads {hq}/{hk} and FFN {F} must divide by the world size {world}")
+        if world > 1 and (cfg.num_experts or cfg.post_norms or cfg.residual_scale != 1.0):
+            raise NotImplementedError("LlamaWeights: experts, norms behind blocks and residual scales on one rank only (a "
+                                      "tensor-parallel block's output is summed into the residual stream as it is)")
         hq_l, hk_l, f_l = hq // world, hk // world, F // world
         layers = []
         for lw in full["layers"]:
@@ -137,13 +156,19 @@ class LlamaWeights:
                              shard_rows(lw["wk"], rank * hk_l * hd, (rank + 1) * hk_l * hd),
                              shard_rows(lw["wv"], rank * hk_l * hd, (rank + 1) * hk_l * hd)])
             o = lw["wo"] if world == 1 else shard_cols(lw["wo"], rank * hq_l * hd, (rank + 1) * hq_l * hd)
-            gu = _cat_rows([shard_rows(lw["wg"], rank * f_l, (rank + 1) * f_l),
-                            shard_rows(lw["wu"], rank * f_l, (rank + 1) * f_l)])
-            down = lw["wd"] if world == 1 else shard_cols(lw["wd"], rank * f_l, (rank + 1) * f_l)
-            layers.append({"qkv": qkv, "o": o, "gate_up": gu, "down": down,
-                           "attn_norm": lw["n1"], "ffn_norm": lw["n2"]})
+            layers.append({"qkv": qkv, "o": o, "attn_norm": lw["n1"], "ffn_norm": lw["n2"]})
+            if cfg.num_experts:
+                layers[-1]["moe"] = MoELayer({"num_experts": cfg.num_experts,
+                                              "num_experts_per_tok": cfg.num_experts_per_tok, "hidden_act": "silu"}, lw["moe"])
+            else:
+                gu = _cat_rows([shard_rows(lw["wg"], rank * f_l, (rank + 1) * f_l),
+                                shard_rows(lw["wu"], rank * f_l, (rank + 1) * f_l)])
+                down = lw["wd"] if world == 1 else shard_cols(lw["wd"], rank * f_l, (rank + 1) * f_l)
+                layers[-1].update(gate_up=gu, down=down)
             if cfg.qk_norm:
                 layers[-1].update(q_norm=lw["qn"], k_norm=lw["kn"])
+            if cfg.post_norms:
+                layers[-1].update(post_attn_norm=lw["pn1"], post_ffn_norm=lw["pn2"])
         return cls(cfg, full["embed"], layers, full["norm"], full["output"], rank, world)
 
 
@@ -168,13 +193,21 @@ def synth_llama_weights(cfg: LlamaConfig, seed: int = 0, device="cuda"):
         layers.append({"wq": w(cfg.attn_qtype, cfg.num_heads * hd, D, b + 0),
                        "wk": w(cfg.attn_qtype, cfg.num_kv_heads * hd, D, b + 1),
                        "wv": w(cfg.attn_qtype, cfg.num_kv_heads * hd, D, b + 2),
-                       "wo": w(cfg.attn_qtype, D, cfg.num_heads * hd, b + 3),
-                       "wg": w(cfg.gate_up_qtype, F, D, b + 4),
-                       "wu": w(cfg.gate_up_qtype, F, D, b + 5),
-                       "wd": w(cfg.down_qtype, D, F, b + 6),
-                       "n1": norm_w(), "n2": norm_w()})
+                       "wo": w(cfg.attn_qtype, D, cfg.num_heads * hd, b + 3)})
+        if cfg.num_experts:
+            shape = {"w1": (F, D), "w2": (D, F), "w3": (F, D)}
+            layers[-1]["moe"] = {
+                "gate": {"weight": torch.randn(cfg.num_experts, D, generator=g, device=device) / D ** 0.5},
+                "experts": {str(e): {n: {"weight": w(cfg.expert_qtype, *shape[n], 100000 * (e + 1) + b + 4 + j)}
+                                     for j, n in enumerate(shape)} for e in range(cfg.num_experts)}}
+        else:
+            layers[-1].update(wg=w(cfg.gate_up_qtype, F, D, b + 4), wu=w(cfg.gate_up_qtype, F, D, b + 5),
+                              wd=w(cfg.down_qtype, D, F, b + 6))
+        layers[-1].update(n1=norm_w(), n2=norm_w())
         if cfg.qk_norm:
             layers[-1].update(qn=norm_w(hd), kn=norm_w(hd))
+        if cfg.post_norms:
+            layers[-1].update(pn1=norm_w(), pn2=norm_w())
     return {"embed": w(cfg.embed_qtype, V, D, 1), "layers": layers, "norm": norm_w(),
             "output": w(cfg.output_qtype, V, D, 2)}
 
@@ -351,6 +384,36 @@ class LlamaDecoder:
                          k_norm=lw.get("k_norm"), eps=self.cfg.norm_eps)
         return cache.attend(q, self.block_table, self.kv_lens, cu).flatten(1)
 
+    def _add(self, h: torch.Tensor, y: torch.Tensor, post: torch.Tensor | None, pre: torch.Tensor | None = None):
+        """h += scale * y, or the norm of y (in place); the norm of the new h with ``pre``."""
+        return residual_norm(h, y, post_weight=post, scale=self.cfg.residual_scale, pre_weight=pre, eps=self.cfg.norm_eps,
+                             out=h)[1]
+
+    @property
+    def _plain_residual(self) -> bool:
+        """Whether blocks add their output to the stream as it is (then in the epilogue of their last product)."""
+        return not self.cfg.post_norms and self.cfg.residual_scale == 1.0
+
+    def _experts(self, lw, h: torch.Tensor):
+        """The mixture-of-experts block of a decode step on the rows h of the stream, a few at a time."""
+        moe, eps = lw["moe"], self.cfg.norm_eps
+        for r0 in range(0, h.shape[0], moe.STEP_TOKENS):
+            x = h[r0:r0 + moe.STEP_TOKENS]
+            if self._plain_residual:
+                moe.step(x, norm_weight=lw["ffn_norm"], eps=eps, residual=x, out=x)
+            else:
+                self._add(x, moe.step(x, norm_weight=lw["ffn_norm"], eps=eps), lw.get("post_ffn_norm"))
+
+    def _experts_prefill(self, lw, h: torch.Tensor, o: torch.Tensor):
+        """The attention block's output o into the stream h, and the mixture-of-experts block of many rows."""
+        moe = lw["moe"]
+        if h.shape[0] <= moe.STEP_TOKENS or moe.num_experts > 32:          # (forward_device takes up to 32 experts)
+            self._add(h, o, lw.get("post_attn_norm"))
+            self._experts(lw, h)
+            return
+        x = self._add(h, o, lw.get("post_attn_norm"), lw["ffn_norm"])
+        self._add(h, moe.forward_device(x), lw.get("post_ffn_norm"))
+
     def _layers(self, lq: int):
         cfg, B = self.cfg, self.B
         rows = B * lq
@@ -369,15 +432,24 @@ class LlamaDecoder:
                                        cfg.head_dim, cfg.rope_theta, self.max_ctx, self.attn.data_ptr(),
                                        self.hq * cfg.head_dim, self.attn_ws.data_ptr(), self.attn_ws.numel(), st),
                       "attention")
-            if self.world == 1:
+            if self.world == 1 and self._plain_residual:
                 self._proj(lw["o"], attn, rows, self.h, accumulate=True)
+            elif self.world == 1:
+                self._proj(lw["o"], attn, rows, self.part)
+                self._add(self.h[:rows], self.part[:rows], lw.get("post_attn_norm"))
             else:
                 self._proj(lw["o"], attn, rows, self.part)
                 self._allreduce_add(rows)
             # MLP block (forward.py:113-116)
+            if "moe" in lw:
+                self._experts(lw, self.h[:rows])
+                continue
             self._proj(lw["gate_up"], self.h, rows, self.gu, PRO_RMSNORM, lw["ffn_norm"])
-            if self.world == 1:
+            if self.world == 1 and self._plain_residual:
                 self._proj(lw["down"], self.gu, rows, self.h, PRO_SWIGLU, accumulate=True)
+            elif self.world == 1:
+                self._proj(lw["down"], self.gu, rows, self.part, PRO_SWIGLU)
+                self._add(self.h[:rows], self.part[:rows], lw.get("post_ffn_norm"))
             else:
                 self._proj(lw["down"], self.gu, rows, self.part, PRO_SWIGLU)
                 self._allreduce_add(rows)
@@ -520,6 +592,17 @@ class LlamaDecoder:
             self._gemv(wt, x, rows, y, prologue, norm, accumulate)
 
     def _prefill_gemm(self, ids: torch.Tensor) -> torch.Tensor:
+        B, S = self.B, ids.shape[1]
+        h = self._prefill_rows(ids)
+        # the output head on each sequence's last token (the decode state keeps those rows)
+        self.h[:B].copy_(h.view(B, S, self.cfg.hidden_size)[:, S - 1])
+        self._head(1)
+        self.pos0.fill_(S)
+        self.length = S
+        return self.next_ids
+
+    def _prefill_rows(self, ids: torch.Tensor) -> torch.Tensor:
+        """The residual stream [B * S, hidden] behind the last layer of a prompt entering an empty cache."""
         cfg, B = self.cfg, self.B
         S = ids.shape[1]
         if ids.shape[0] != B:
@@ -535,8 +618,8 @@ class LlamaDecoder:
         h = torch.empty(rows, D, **f32)
         qkv = torch.empty(rows, self.qkv_dim, **f32)
         attn = torch.empty(rows, self.hq * hd, **f32)
-        gu = torch.empty(rows, 2 * self.f_l, **f32)
-        part = torch.empty(rows, D, **f32) if self.world > 1 else None
+        gu = None if cfg.num_experts else torch.empty(rows, 2 * self.f_l, **f32)
+        part = torch.empty(rows, D, **f32) if self.world > 1 or cfg.num_experts or not self._plain_residual else None
         idv = ids.reshape(-1).to(self.dev, torch.int32).contiguous()
         chunk_pos = torch.arange(0, S, self.PREFILL_CHUNK, dtype=torch.int32, device=self.dev)
         st = self._stream()
@@ -567,30 +650,62 @@ class LlamaDecoder:
                                            self.hk, hd, cfg.rope_theta, self.max_ctx, attn[r0].data_ptr(),
                                            self.hq * hd, self.attn_ws.data_ptr(), self.attn_ws.numel(), st),
                           "attention")
-            if self.world == 1:
+            if "moe" in lw:
+                self._gemm(lw["o"], attn, rows, part)
+                self._experts_prefill(lw, h, part)
+                continue
+            if part is None:
                 self._gemm(lw["o"], attn, rows, h, accumulate=True)
             else:
                 self._gemm(lw["o"], attn, rows, part)
-                self._allreduce_rows(h, part)
+                if self.world == 1:
+                    self._add(h, part, lw.get("post_attn_norm"))
+                else:
+                    self._allreduce_rows(h, part)
             self._gemm(lw["gate_up"], h, rows, gu, PRO_RMSNORM, lw["ffn_norm"])
-            if self.world == 1:
+            if part is None:
                 self._gemm(lw["down"], gu, rows, h, PRO_SWIGLU, accumulate=True)
             else:
                 self._gemm(lw["down"], gu, rows, part, PRO_SWIGLU)
-                self._allreduce_rows(h, part)
-        # the output head on each sequence's last token (the decode state keeps those rows)
-        last = h.view(B, S, D)[:, S - 1]
-        self.h[:B].copy_(last)
-        self._head(1)
-        self.pos0.fill_(S)
-        self.length = S
-        return self.next_ids
+                if self.world == 1:
+                    self._add(h, part, lw.get("post_ffn_norm"))
+                else:
+                    self._allreduce_rows(h, part)
+        return h
 
     def _allreduce_rows(self, h, part):
         """h += sum over ranks of part (the prefill's row-parallel outputs, NCCL all-reduce)."""
         import torch.distributed as dist
         dist.all_reduce(part, group=self.pg)
         h.add_(part)
+
+    SCORE_ROWS = 512        # logits at a time: 64 MB of 32000 fp32 ones
+
+    def score(self, ids, temperature: float = 1.0, top: int = 0) -> TokenLogprobs:
+        """Log-probabilities of sequences ids [B, S], 2 <= S <= max_ctx: what each token i + 1 has behind the tokens 0 .. i, with
+        the entropy there, the token's rank and the ``top`` largest alternatives (see
+        :func:`~xanosmerks_b200.sampling.logprobs`); every tensor begins [B, S - 1].  The decoder is reset before and after."""
+        ids = torch.as_tensor(np.asarray(ids) if not isinstance(ids, torch.Tensor) else ids)
+        if ids.dim() != 2 or ids.shape[1] < 2:
+            raise ValueError(f"score: ids must be [{self.B}, S] with two tokens or more, got {tuple(ids.shape)}")
+        self.reset()
+        B, S = ids.shape
+        h = self._prefill_rows(ids)
+        self.reset()
+        ow, V = self.w.output, self.cfg.vocab_size
+        target = ids.to(self.dev).roll(-1, 1).reshape(-1).contiguous().to(torch.int32)
+        parts = []
+        for r0 in range(0, B * S, self.SCORE_ROWS):
+            rows = min(self.SCORE_ROWS, B * S - r0)
+            logits = torch.empty(rows, V, dtype=torch.float32, device=self.dev)
+            self._gemm(ow, h[r0:r0 + rows], rows, logits, PRO_RMSNORM, self.w.norm)
+            parts.append(logprobs(logits, target[r0:r0 + rows], temperature=temperature, top=top))
+        whole = [None if p[0] is None else torch.cat(p).unflatten(0, (B, S))[:, :-1] for p in zip(*parts)]
+        return TokenLogprobs(*whole)
+
+    def token_logprobs(self, top: int = 0) -> TokenLogprobs:
+        """Of the tokens that the last step or prefill chose (``next_ids``), under its logits."""
+        return logprobs(self.logits, self.next_ids, top=top)
 
     def decode_step(self):
         """One step from device state: the token in next_ids enters at pos0."""

@@ -239,3 +239,40 @@ def test_nothing_to_do_and_refusals():
                {"out": good.half()}, {"norm_weight": good[0].half()}):
         with pytest.raises(ValueError):
             b.layer.step(good, **kw)
+
+
+class Sparse(Block):
+    """Weights that are 0 but for one in 64, which are 1: codes of little and of the middle of their range."""
+
+    def __init__(self, qtype, H, F, seed=0):
+        shape = {"w1": (F, H), "w3": (F, H), "w2": (H, F)}
+        rng = np.random.default_rng(seed)
+        exp = {}
+        for n, s in shape.items():
+            one = rng.random((s[0] * s[1] // 64, 64)).argmin(1)             # the place in 64 values
+            if qtype == "Q8_0":
+                raw = np.zeros((s[0] * s[1] // 32, 34), np.uint8)
+                raw[:, 1] = 0x3C                                             # fp16 1.0
+                at = 64 * np.arange(len(one)) + one
+                raw[at // 32, 2 + at % 32] = 1
+            else:                                                            # code 32 is 0: two upper bits 10, four lower ones 0
+                raw = np.zeros((s[0] * s[1] // 256, 210), np.uint8)
+                raw[:, 128:192] = 0xAA
+                raw[:, 192:208] = 1
+                raw[:, 209] = 0x3C
+                raw[np.arange(len(one)) // 4, 32 * (np.arange(len(one)) % 4) + one % 32] |= np.where(one < 32, 1, 16).astype(np.uint8)
+            exp[n] = {"weight": GGUFTensor(torch.from_numpy(raw.reshape(-1)).cuda(), qtype, s)}
+        self.gate = torch.zeros(1, H, device="cuda")
+        self.layer = MoELayer({"num_experts": 1, "num_experts_per_tok": 1, "hidden_act": "identity"},
+                              {"gate": {"weight": self.gate}, "experts": {"0": exp}})
+        self.experts, self.qtype, self.act, self.k, self.E, self.cache = {"0": exp}, qtype, "identity", 1, 1, {}
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16])
+@pytest.mark.parametrize("qtype", ["Q8_0", "Q6_K"])
+def test_few_weights_of_small_codes(qtype, tokens):
+    """What a sum loses is measured by its weights, not by the range of their codes."""
+    b = Sparse(qtype, 1024, 512)
+    assert 0 < float(b.weights(0)[0].sum()) <= 1024 * 512 / 64 and float(b.weights(0)[0].max()) == 1
+    x = rows(tokens, 1024, 7)
+    check(b.layer.step(x), b.want(x))

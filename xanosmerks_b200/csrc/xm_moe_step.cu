@@ -12,7 +12,7 @@
 //   k_moe_step_sum     the weighted sum and the residual
 //
 // The products run on mma.sync (m16n8k16, fp16 with fp32 sums): sixteen weight rows by eight columns.  An activation is
-// 2^s (hi + lo), both fp16 (a power of two for each 256 of them), which keeps some 22 bits: up to 4 tokens have a column for
+// 2^s (hi + lo), both fp16 (a power of two for each 256 of them), which keeps 22 bits of the largest: up to 4 tokens have a column for
 // each part (M = 4), up to 8 tokens a column each and two products (M = 8).  A single token (M = 1) has the two columns of its
 // parts four times, for every fourth group of values: a thread then has the sums of one group in four, and a quarter of the
 // scales to apply.  A tile of UP is eight rows of W1 and the same eight of W3, so that one thread holds the gate and the up
@@ -283,13 +283,13 @@ constexpr bool halves() { return T == T_Q6_K || T == T_Q8_0; }
 
 // The 256 values of K that a warp holds, of M tokens: column g (= lane / 4) is token g / 2, hi or lo by g % 2 (M = 4), token g
 // in two parts (M = 8), or hi or lo of the one token in the groups g / 2, g / 2 + 4, ... and zero in the others (M = 1).  By
-// groups of 32 their pairs, and the sums over groups of 32 or 16 times 2^-5, of groups 2 t, 2 t + 1 (and 2 t + 8, 2 t + 9; M = 1:
-// in columns 0 and 1).
+// groups of 32 their pairs, and the sums over groups times 2^-5, of groups 2 t, 2 t + 1 (M = 1: in columns 0 and 1), for the types
+// whose weights have offsets.
 template <int M>
 struct Columns {
   static constexpr int PARTS = M == 8 ? 2 : 1;
   uint32_t b[PARTS][8][4];
-  uint32_t sum[PARTS][2];
+  uint32_t sum[PARTS];
   float scale[M == 8 ? 2 : 1];             // 2^s of the tokens that this thread has results of
 };
 // What a thread has of a tile's results: of its two rows (g, g + 8) the token t (M = 4), the tokens 2 t, 2 t + 1 (M = 8), or a
@@ -316,12 +316,54 @@ struct Result {
   }
 };
 
-// c = the products of 16 values of K (a: of the two rows; i: a pair of pairs of group j)
+// c (+)= the products of 16 values of K (a: of the two rows; i: a pair of pairs of group j); M = 8: of the upper parts
 template <int M, bool FIRST>
 XM_DEV void mma_group(float (&c)[4], const uint32_t (&a)[4], const Columns<M>& x, int j, int i) {
   if constexpr (FIRST) mma_f16_zero(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
   else mma_f16(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
-  if constexpr (M == 8) mma_f16(c, a, x.b[1][j][2 * i], x.b[1][j][2 * i + 1]);
+}
+// c = the products of a group of 32.  (M = 8: the lower parts first: added to the sum of the upper ones, each product would lose
+// what lies below that sum's 24 bits.)
+template <int M>
+XM_DEV void mma_32(float (&c)[4], const uint32_t (&a0)[4], const uint32_t (&a1)[4], const Columns<M>& x, int j) {
+  if constexpr (M == 8) {
+    mma_f16_zero(c, a0, x.b[1][j][0], x.b[1][j][1]);
+    mma_f16(c, a1, x.b[1][j][2], x.b[1][j][3]);
+    mma_f16(c, a0, x.b[0][j][0], x.b[0][j][1]);
+    mma_f16(c, a1, x.b[0][j][2], x.b[0][j][3]);
+  } else {
+    mma_f16_zero(c, a0, x.b[0][j][0], x.b[0][j][1]);
+    mma_f16(c, a1, x.b[0][j][2], x.b[0][j][3]);
+  }
+}
+// The same of a group of 16 (the half i of group j).
+template <int M>
+XM_DEV void mma_16(float (&c)[4], const uint32_t (&a)[4], const Columns<M>& x, int j, int i) {
+  if constexpr (M == 8) {
+    mma_f16_zero(c, a, x.b[1][j][2 * i], x.b[1][j][2 * i + 1]);
+    mma_f16(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
+  } else {
+    mma_f16_zero(c, a, x.b[0][j][2 * i], x.b[0][j][2 * i + 1]);
+  }
+}
+
+// Codes as factors.  A matrix instruction cuts products off some 26 bits below the largest by the exponents of their factors,
+// and a subnormal has the exponent of a number up to 2^10 times as large: of codes that enter as the subnormals that their bits
+// are, 2^-20 of the largest product was lost, against 2^-26 as numbers, and results were off by 1.4e-6 against 4e-7.  So they
+// are made numbers, by one subtraction a pair, or the products are made to end above the cut: with whole numbers below 2^15
+// nothing is lost of codes below 2^10 (measured over 250000 sums of 16).  The latter is what one token takes, whose kernel waits
+// for its instructions (Q4_K, 8 experts of 14336 x 4096: 59 us a step against 68 with the subtractions, off by 3e-7 to 8e-7
+// against 3e-7 to 4e-7); with more tokens both take as long.
+
+// The upper part of an activation, or of a sum of them: what fp16 holds of it, or of its whole number.
+template <bool WHOLE>
+XM_DEV float upper(float v) { return __half2float(__float2half_rn(WHOLE ? rintf(v) : v)); }
+
+// (1024 + c) - (1024 + bias) of two fp16, exact: numbers from codes below 1024 that lie under fp16 words of 1024.
+constexpr uint32_t OVER = 0x64006400u;
+XM_DEV uint32_t less(uint32_t u, float bias) {
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1024.f + bias));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Types whose weights enter with the block's own value, not rounded to fp16 as dequantisation rounds it.
@@ -333,7 +375,7 @@ constexpr bool own_value() { return T == T_Q4_K || T == T_Q5_K || T == T_Q6_K ||
 // Any type, value by value: weights rounded to fp16.
 template <int T, int M>
 XM_DEV void unit_any(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
-  float c[4] = {0.f, 0.f, 0.f, 0.f};
+  float c[4] = {0.f, 0.f, 0.f, 0.f}, lower[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     uint32_t w[2][4];
@@ -351,39 +393,38 @@ XM_DEV void unit_any(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
     const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
     mma_group<M, false>(c, a0, x, j, 0);
     mma_group<M, false>(c, a1, x, j, 1);
+    if constexpr (M == 8) {
+      mma_f16(lower, a0, x.b[1][j][0], x.b[1][j][1]);
+      mma_f16(lower, a1, x.b[1][j][2], x.b[1][j][3]);
+    }
   }
   acc.clear();
   acc.add(c, 1.f, 1.f);
+  if constexpr (M == 8) acc.add(lower, 1.f, 1.f);
 }
 
 XM_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// Codes of 8 bits of which the upper four count sixteenfold: those bits alone (a - b of fp16 subnormals is exact, and the
-// pipe of the logic operations is the busier one).
-XM_DEV uint32_t minus(uint32_t a, uint32_t b) {
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
-
-// Q4_K, and Q5_K (FIVE): w = d s_j c - dmin m_j.  A word's codes under the mask 0x000f000f are fp16 subnormals c 2^-24, under
-// 0x00f000f0 c 2^-20: no instruction makes them numbers.  The scales of a pair of groups come from their bytes as fp16
-// (1024 + s_2j) - 1024 and, for the upper codes, (64 + s_2j+1 / 16) - 64: exact.
+// Q4_K, and Q5_K (FIVE): w = d s_j c - dmin m_j.  A word's codes under the masks 0x000f000f and 0x00f000f0: c and 16 c.  The
+// scales of a pair of groups come from their bytes as fp16 (1024 + s_2j) - 1024 and, for the upper codes,
+// (64 + s_2j+1 / 16) - 64: exact.
 template <bool FIVE, int M>
 XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
-  constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, BIT = 0x00100010u;
+  constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, FIFTH = 0x00100010u;
   constexpr int QS = FIVE ? 48 : 16;
+  constexpr bool NUMBERS = M != 1;         // codes as numbers, not as subnormals c 2^-24
   uint32_t sc[2][2], am[2], qh[2][4];
   float d[2], dm[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const uint4 h = lds128(r ? r1 : r0);
     const float2 dd = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
-    d[r] = dd.x * 0x1p24f;
-    dm[r] = dd.y * -0x1p29f;
+    d[r] = NUMBERS ? dd.x : dd.x * 0x1p24f;
+    dm[r] = dd.y * -0x1p5f;
     sc[r][0] = h.y & 0x3f3f3f3fu;
     sc[r][1] = (h.w & 0x0f0f0f0fu) | ((h.y >> 2) & 0x30303030u);
     const uint32_t m = t < 2 ? h.z & 0x3f3f3f3fu : ((h.w >> 4) & 0x0f0f0f0fu) | ((h.z >> 2) & 0x30303030u);
-    am[r] = __byte_perm(m, 0u, t & 1 ? 0x4342 : 0x4140);      // (m_2t, m_2t+1) 2^-24
+    am[r] = less(__byte_perm(m, OVER, t & 1 ? 0x7372 : 0x7170), 0.f);      // m_2t, m_2t+1
     if constexpr (FIVE) {
       const uint4 q = lds128((r ? r1 : r0) + 16);             // the fifth bits of groups 2 j, 2 j + 1: word j, bit = value
       qh[r][0] = (q.x >> (8 * t)) & 0xffu;
@@ -401,28 +442,24 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint2 q = *reinterpret_cast<const uint2*>((r ? r1 : r0) + QS + 32 * jj + 8 * t);
-      uint32_t f[4] = {0u, 0u, 0u, 0u};
+      // (the fifth bits: one product puts two of them where the codes of a pair have theirs)
+      constexpr uint32_t BASE = NUMBERS ? OVER : 0u;
+      uint32_t f[4] = {BASE, BASE, BASE, BASE};
       if constexpr (FIVE) {
         const uint32_t b = qh[r][jj];
-        f[0] = (b * ((1u << 4) + (1u << 18))) & BIT;
-        f[1] = (b * ((1u << 3) + (1u << 17))) & BIT;
-        f[2] = (b * (1u + (1u << 14))) & BIT;
-        f[3] = ((b >> 1) * (1u + (1u << 14))) & BIT;
+        f[0] |= (b * ((1u << 4) + (1u << 18))) & FIFTH;
+        f[1] |= (b * ((1u << 3) + (1u << 17))) & FIFTH;
+        f[2] |= (b * (1u + (1u << 14))) & FIFTH;
+        f[3] |= ((b >> 1) * (1u + (1u << 14))) & FIFTH;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w = i < 2 ? q.x : q.y;
-        if (i & 1) {
-          const uint32_t two = __byte_perm(w, 0u, 0x4341);      // bytes 1 and 3
-          lo[r][i] = two & LOW;
-          hi[r][i] = minus(two, lo[r][i]);
-        } else {
-          lo[r][i] = w & LOW;
-          hi[r][i] = w & HIGH;
-        }
-        if constexpr (FIVE) {
-          lo[r][i] |= f[i];
-          hi[r][i] |= f[i] << 4;
+        const uint32_t w = i < 2 ? q.x : q.y, v = i & 1 ? __byte_perm(w, 0u, 0x4341) : w;      // (bytes 1 and 3)
+        lo[r][i] = (v & LOW) | f[i];
+        hi[r][i] = (v & HIGH) | (FIVE ? (f[i] ^ BASE) << 4 : 0u) | BASE;
+        if constexpr (NUMBERS) {
+          lo[r][i] = less(lo[r][i], 0.f);
+          hi[r][i] = less(hi[r][i], 0.f);
         }
       }
     }
@@ -445,8 +482,7 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
         mma_group<M, false>(one[j / 4], a1, x, j, 1);
       } else {
         float c[4];
-        mma_group<M, true>(c, a0, x, j, 0);
-        mma_group<M, false>(c, a1, x, j, 1);
+        mma_32(c, a0, a1, x, j);
         sum.add(c, half ? s[0].y : s[0].x, half ? s[1].y : s[1].x);
       }
     }
@@ -463,7 +499,7 @@ XM_DEV void unit_k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>
   }
   float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16_k8(c, am[0], am[1], x.sum[i][0]);
+  for (int i = Columns<M>::PARTS - 1; i >= 0; --i) mma_f16_k8(c, am[0], am[1], x.sum[i]);
   acc.clear();
   acc.add(c, dm[0], dm[1]);
 #pragma unroll
@@ -481,8 +517,13 @@ XM_DEV uint32_t lds_word(const uint8_t* p) {
   return __funnelshift_r(a[0], a[1], sh);
 }
 
+// The bytes 0 and 2, or 1 and 3, of w as numbers less BIAS.
+template <int BIAS>
+XM_DEV uint32_t signed_pair(uint32_t w, bool odd) { return less(__byte_perm(w, OVER, odd ? 0x7371 : 0x7270), BIAS); }
+
 // Q6_K: w = d s_g (c - 32), groups of 16, records at any even address (every other one at a multiple of four: FOUR).  Codes are
-// put together as bytes, four at a time.
+// put together as bytes, four at a time.  (Offsets by the sums of groups, as Q4_K has them, would cost small weights their
+// bits: those are differences there.)
 template <int M, bool FOUR>
 XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
   uint32_t sc[2][4];                       // s + 128, bytes
@@ -497,7 +538,7 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
 #pragma unroll
     for (int i = 0; i < 4; ++i) sc[r][i] = __funnelshift_r(w[i], w[i + 1], sh) ^ 0x80808080u;
     const uint32_t dw = w[4] >> sh;
-    d[r] = __half2float(__ushort_as_half((unsigned short)dw)) * 0x1p24f;
+    d[r] = __half2float(__ushort_as_half((unsigned short)dw));
   }
   float one[4][4];                         // M = 1: the sums of groups t, t + 4, ...
   Result<M> sum;
@@ -520,12 +561,11 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
         uint32_t q[2][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          // (one selection: what it leaves above the sixth bit goes with the masks of the pairs)
           const uint32_t nib = i < 2 ? low[r][i & 1] : low[r][i & 1] >> 4;
           const uint32_t two = i == 0 ? high[r] << 4 : i == 1 ? high[r] << 2 : i == 2 ? high[r] : high[r] >> 2;
-          const uint32_t c4 = (nib & 0x0f0f0f0fu) | (two & 0xf0f0f0f0u);
-          q[r][0] = c4 & 0x003f003fu;
-          q[r][1] = __byte_perm(c4, 0u, 0x4341) & 0x003f003fu;
+          const uint32_t c4 = (nib & 0x0f0f0f0fu) | (two & 0x30303030u);
+          q[r][0] = signed_pair<32>(c4, false);
+          q[r][1] = signed_pair<32>(c4, true);
         }
         const uint32_t a[4] = {q[0][0], q[1][0], q[0][1], q[1][1]};
         if constexpr (M == 1) {
@@ -534,7 +574,7 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
           else mma_group<M, false>(one[g >> 2], a, x, g >> 1, g & 1);
         } else {
           float c[4], s[2];
-          mma_group<M, true>(c, a, x, g >> 1, g & 1);
+          mma_16(c, a, x, g >> 1, g & 1);
 #pragma unroll
           for (int r = 0; r < 2; ++r)
             s[r] = __uint_as_float(__byte_perm(sc[r][g >> 2], 0x4B000000u, 0x7650 | (g & 3))) - (0x1p23f + 128.f);
@@ -552,43 +592,26 @@ XM_DEV void unit_q6k(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
       sum.add(one[i], s[0], s[1]);
     }
   }
-  // offsets: -32 sum s_g S_g, the scales as fp16 (1024 + byte) - 1152
-  uint32_t o[2][2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t w = t < 2 ? sc[r][2 * i] : sc[r][2 * i + 1];
-      const uint32_t u = __byte_perm(w, 0x64646464u, t & 1 ? 0x4342 : 0x4140);
-      const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
-      o[r][i] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  float c[4] = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t a[4] = {o[0][0], o[1][0], o[0][1], o[1][1]};
-#pragma unroll
-  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16(c, a, x.sum[i][0], x.sum[i][1]);
   acc.clear();
-  acc.add(c, d[0] * -0x1p-14f, d[1] * -0x1p-14f);                 // (2^-24 of d, 2^5 of the sums, 2^5)
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int i = 0; i < Result<M>::N; ++i) acc.v[r][i] = fmaf(d[r], sum.v[r][i], acc.v[r][i]);
+    for (int i = 0; i < Result<M>::N; ++i) acc.v[r][i] = d[r] * sum.v[r][i];
 }
 
-// Q8_0: w = d_j c, eight records of 34 bytes; the codes enter as c + 128, and -128 sum d_j S_j as the offsets' product.
+// Q8_0: w = d_j c, eight records of 34 bytes.
 template <int M>
 XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<M>& x, Result<M>& acc) {
-  uint32_t dd[2];
+  uint32_t dd[2] = {0u, 0u};               // d_2t, d_2t+1
+  if constexpr (M != 1) {
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const uint8_t* p = (r ? r1 : r0) + 68 * t;
-    dd[r] = (uint32_t)*reinterpret_cast<const unsigned short*>(p) | (uint32_t)*reinterpret_cast<const unsigned short*>(p + 34) << 16;
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* p = (r ? r1 : r0) + 68 * t;
+      dd[r] = (uint32_t)*reinterpret_cast<const unsigned short*>(p) |
+              (uint32_t)*reinterpret_cast<const unsigned short*>(p + 34) << 16;
+    }
   }
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < Columns<M>::PARTS; ++i) mma_f16_k8(o, dd[0], dd[1], x.sum[i][0]);
   acc.clear();
-  acc.add(o, -0x1p12f, -0x1p12f);
   float one[2][4];                         // M = 1: the sums of groups t and t + 4
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -609,20 +632,20 @@ XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
       w[r][1] ^= 0x80808080u;
       if constexpr (M != 1) {
         const uint32_t u = __shfl_sync(~0u, dd[r], (threadIdx.x & 28) | (j >> 1));
-        s[r] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xffffu))) * 0x1p24f;
+        s[r] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xffffu)));
       }
     }
-    constexpr uint32_t K = 0x00ff00ffu;
-    const uint32_t a0[4] = {w[0][0] & K, w[1][0] & K, (w[0][0] >> 8) & K, (w[1][0] >> 8) & K};
-    const uint32_t a1[4] = {w[0][1] & K, w[1][1] & K, (w[0][1] >> 8) & K, (w[1][1] >> 8) & K};
+    const uint32_t a0[4] = {signed_pair<128>(w[0][0], false), signed_pair<128>(w[1][0], false),
+                            signed_pair<128>(w[0][0], true), signed_pair<128>(w[1][0], true)};
+    const uint32_t a1[4] = {signed_pair<128>(w[0][1], false), signed_pair<128>(w[1][1], false),
+                            signed_pair<128>(w[0][1], true), signed_pair<128>(w[1][1], true)};
     if constexpr (M == 1) {
       if (j % 4 == 0) mma_group<M, true>(one[j / 4], a0, x, j, 0);
       else mma_group<M, false>(one[j / 4], a0, x, j, 0);
       mma_group<M, false>(one[j / 4], a1, x, j, 1);
     } else {
       float c[4];
-      mma_group<M, true>(c, a0, x, j, 0);
-      mma_group<M, false>(c, a1, x, j, 1);
+      mma_32(c, a0, a1, x, j);
       acc.add(c, s[0], s[1]);
     }
   }
@@ -632,7 +655,7 @@ XM_DEV void unit_q80(const uint8_t* r0, const uint8_t* r1, int t, const Columns<
       float s[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        s[r] = __half2float(*reinterpret_cast<const __half*>((r ? r1 : r0) + 34 * (t + 4 * i))) * 0x1p24f;
+        s[r] = __half2float(*reinterpret_cast<const __half*>((r ? r1 : r0) + 34 * (t + 4 * i)));
       acc.add(one[i], s[0], s[1]);
     }
   }
@@ -788,6 +811,7 @@ struct Step {
   }
 
   // This warp's activations of a segment and a chunk.
+  static constexpr bool OFFSETS = T == T_Q4_K || T == T_Q5_K;
   XM_DEV void load_columns(Columns<M>& x, int seg, int k0, bool mine) {
     if constexpr (M == 1) load_one(x, seg, k0, mine);
     else load_several(x, seg, k0, mine);
@@ -816,7 +840,7 @@ struct Step {
     const int shift = fp16_row_shift(m);
     const float inv = ldexpf(1.0f, -shift);
     x.scale[0] = ldexpf(1.0f, shift);
-    auto part = [&](float f) { return g & 1 ? f - __half2float(__float2half_rn(f)) : f; };
+    auto part = [&](float f) { return g & 1 ? f - upper<OFFSETS>(f) : upper<OFFSETS>(f); };
     float sum[G / 4];
 #pragma unroll
     for (int i = 0; i < G / 4; ++i) {
@@ -841,27 +865,22 @@ struct Step {
         }
       }
     }
-    // sums of groups 2 t, 2 t + 1 (, 2 t + 8, 2 t + 9) in columns 0 and 1: group n is with the lanes of g / 2 = n % 4
-    float q[4];
+    if constexpr (OFFSETS) {               // groups 2 t, 2 t + 1 in columns 0 and 1: group n is with the lanes of g / 2 = n % 4
+      float q[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = 2 * t + (i & 1);       // (+ 8 for i >= 2)
-      float z[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        z[h] = 2 * (i / 2) + h < G / 4 ? __shfl_sync(~0u, sum[2 * (i / 2) + h < G / 4 ? 2 * (i / 2) + h : 0], (n & 3) * 8) : 0.f;
-      q[i] = n < 4 ? z[0] : z[1];
-      q[i] = g < 2 ? part(q[i]) : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const int n = 2 * t + i;
+        const float z0 = __shfl_sync(~0u, sum[0], (n & 3) * 8), z1 = __shfl_sync(~0u, sum[1], (n & 3) * 8);
+        q[i] = g < 2 ? part(n < 4 ? z0 : z1) : 0.f;
+      }
+      x.sum[0] = pack2(q[0], q[1]);
     }
-    x.sum[0][0] = pack2(q[0], q[1]);
-    x.sum[0][1] = pack2(q[2], q[3]);
   }
   XM_DEV void load_several(Columns<M>& x, int seg, int k0, bool mine) {
     const int col = M == 4 ? g >> 1 : g;
     const bool there = mine && col < sm.seg_n[seg], rest = M == 4 && (g & 1);      // (this column has the low parts)
     const int pair = there ? sm.pair[sm.seg_at[seg] + col] : 0, row = UP ? pair / a.k : pair;
     const float* p = a.src + (int64_t)row * a.K + k0 + (halves<T>() ? 4 : 8) * t;
-    auto low = [](float v) { return v - __half2float(__float2half_rn(v)); };
     // all of the column's 256 values first: their power of two
     float4 u[8][2];
     float m = 0.f;
@@ -886,43 +905,40 @@ struct Step {
       x.scale[0] = __shfl_sync(~0u, own, 8 * t);
       x.scale[1] = __shfl_sync(~0u, own, 8 * t + 4);
     }
-    float part[16];
+    float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float v[8] = {u[j][0].x * inv, u[j][0].y * inv, u[j][0].z * inv, u[j][0].w * inv,
                     u[j][1].x * inv, u[j][1].y * inv, u[j][1].z * inv, u[j][1].w * inv};
-      part[2 * j] = (v[0] + v[1]) + (v[2] + v[3]);
-      part[2 * j + 1] = (v[4] + v[5]) + (v[6] + v[7]);
+      sum[j] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      float top[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        top[i] = upper<false>(v[i]);
+        v[i] -= top[i];
+      }
 #pragma unroll
       for (int q = 0; q < Columns<M>::PARTS; ++q) {
-        if (q || rest) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = low(v[i]);
-        }
-        x.b[q][j][0] = pack2(v[0], v[2]);
-        x.b[q][j][1] = pack2(v[1], v[3]);
-        x.b[q][j][2] = pack2(v[4], v[6]);
-        x.b[q][j][3] = pack2(v[5], v[7]);
+        const bool lower = q || rest;
+        x.b[q][j][0] = pack2(lower ? v[0] : top[0], lower ? v[2] : top[2]);
+        x.b[q][j][1] = pack2(lower ? v[1] : top[1], lower ? v[3] : top[3]);
+        x.b[q][j][2] = pack2(lower ? v[4] : top[4], lower ? v[6] : top[6]);
+        x.b[q][j][3] = pack2(lower ? v[5] : top[5], lower ? v[7] : top[7]);
       }
     }
-    if constexpr (own_value<T>()) {
-      constexpr int G = T == T_Q6_K ? 16 : 8;
-      float q[4] = {0.f, 0.f, 0.f, 0.f};                       // sums of groups 2 t, 2 t + 1 (, 2 t + 8, 2 t + 9)
+    if constexpr (OFFSETS) {
+      float q[2] = {0.f, 0.f};             // sums of groups 2 t, 2 t + 1
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        float z = G == 16 ? part[i] : part[2 * i] + part[2 * i + 1];
+      for (int j = 0; j < 8; ++j) {
+        float z = sum[j];
         z += __shfl_xor_sync(~0u, z, 1);
         z += __shfl_xor_sync(~0u, z, 2);
-        if ((i & 7) >> 1 == t) q[(i >> 3) * 2 + (i & 1)] = z * 0x1p-5f;
+        if (j >> 1 == t) q[j & 1] = z * 0x1p-5f;
       }
 #pragma unroll
       for (int c = 0; c < Columns<M>::PARTS; ++c) {
-        if (c || rest) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = low(q[i]);
-        }
-        x.sum[c][0] = pack2(q[0], q[1]);
-        x.sum[c][1] = pack2(q[2], q[3]);
+        const bool lower = c || rest;
+        x.sum[c] = pack2(lower ? q[0] - upper<false>(q[0]) : upper<false>(q[0]), lower ? q[1] - upper<false>(q[1]) : upper<false>(q[1]));
       }
     }
   }

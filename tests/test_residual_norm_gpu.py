@@ -140,3 +140,16 @@ def test_refusals():
                   ((torch.zeros(1, 32769, device="cuda"),) * 2, {})):
         with pytest.raises(ValueError):
             residual_norm(*a, **kw)
+
+
+def test_broadcast_inputs():
+    """One row, or one sequence, for all of them: rows that lie on one another are read as such, never written."""
+    s, y, post, pre = make((3, 5, 512), seed=4)
+    compare(s, y[:1, :1].expand(3, 5, 512), post=post, pre=pre)
+    compare(s[:1].expand(3, 5, 512), y, pre=pre)
+    compare(s[0, :1].expand(5, 512), y[0, :1].expand(5, 512), post=post, pre=pre)
+    flat = s[0, :1].expand(5, 512)
+    with pytest.raises((ValueError, RuntimeError)):
+        residual_norm(flat, y[0], out=flat)
+    one, z, post, pre = make((4, 1), seed=5)
+    compare(one[:1].expand(4, 1), z, pre=pre)

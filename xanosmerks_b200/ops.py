@@ -173,10 +173,10 @@ def qlinear(weight: GGUFTensor, x: torch.Tensor, bias: torch.Tensor | None = Non
 
 
 def _as_rows(t, d):
-    """t [..., d] as rows [n, d] with unit stride in the last dimension (a copy where the strides do not allow it)."""
+    """t [..., d] as rows [n, d] of their own, with unit stride in the last dimension (a copy where the strides do not allow it)."""
     if t.dim() != 2:
         t = t.reshape(-1, d)
-    return t if d == 1 or t.stride(1) == 1 else t.contiguous()
+    return t if (d == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= d) else t.contiguous()
 
 
 def _rows_and_pitch(t, d):

@@ -314,7 +314,8 @@ int xm_moe_combine(const float* d_rows, int64_t T, int64_t H, int E, int k, int6
  * E <= 256, k <= 16; H (<= 16384) and F multiples of 256.  d_workspace (256-byte
  * aligned, xm_moe_step_workspace_size bytes, no initial contents): one for each
  * call that may run at the same time.  Four launches, no host synchronisation;
- * the same result for every launch.
+ * the same call gives the same bits (T and k decide how an activation's two parts
+ * enter the products, and with it the last bits).
  *
  * Replaces moe.py:54-115 with the norm and the residual add of forward.py:113-116.
  */
@@ -464,7 +465,8 @@ int xm_sample(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t str
  * and rank -1.  NaN logits count as -inf (log-probability -inf); a row of
  * nothing else has entropy 0.  Logits of +inf share the mass.  T <= 0: the first
  * maximum has log-probability 0, the others -inf.  T is per row where
- * d_temperature is given.  Same result for any launch.  (The log-probability
+ * d_temperature is given.  The same call gives the same bits; B decides how many
+ * CTAs share a row, and with it the last bits of its sums.  (The log-probability
  * that sampling.py:94-158 draws from, before its filters.)
  */
 int xm_logprobs(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t stride, const void* d_tokens,

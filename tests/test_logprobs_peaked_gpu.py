@@ -33,8 +33,12 @@ def want(x, t, T, top):
 
 def compare(x, t, T=1.0, top=3):
     r = logprobs(x, t, temperature=T, top=top)
+    check((r.logprob, r.entropy, r.top_logprobs), x, t, T, top)
+
+
+def check(results, x, t, T, top):
     ref = want(x.float().cpu().numpy(), t.cpu().numpy(), float(np.float32(T)), top)
-    for got, v in zip((r.logprob, r.entropy, r.top_logprobs), ref):
+    for got, v in zip(results, ref):
         rel = np.where(np.abs(v) < 2.0 ** -31, 2.0 ** -15, 2.0 ** -16)
         off = np.abs(got.double().cpu().numpy() - v)
         bad = off > rel * np.abs(v) + 2.0 ** -100
@@ -94,3 +98,15 @@ def test_a_first_round_far_below_the_peak():
             x[:, 600] = lift - 1.5
             compare(x, t)
             compare(x[:2], t[:2])
+
+
+def test_many_logits_above_what_was_seen():
+    """So many vectors reach the largest logit seen that the row is taken again: a flat rest, each thread's in one long sum."""
+    for v, dtype in ((1 << 18, torch.float32), (260001, torch.bfloat16)):
+        x = torch.zeros(300, v, dtype=dtype, device="cuda")
+        lift = torch.linspace(7, 14, 300, device="cuda")[:, None]
+        x[:, 1000:3000:8] = (lift - torch.linspace(6, 0, 250, device="cuda")).to(dtype)
+        t = torch.arange(300, device="cuda") + 900
+        r = logprobs(x, t, top=3)                      # (300 rows: one CTA each)
+        some = [0, 100, 299]
+        check([v[some] for v in (r.logprob, r.entropy, r.top_logprobs)], x[some], t[some], 1.0, 3)

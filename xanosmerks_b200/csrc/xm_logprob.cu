@@ -453,12 +453,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
     float mx = -INFINITY;
     p.each([&](float x, int) { mx = fmaxf(mx, x); });
     mx = block_max_f(mx, sm);
-    sum_S = sum_E = 0.f;
+    double s = 0., e = 0.;                           // (one chain of additions through the part)
     p.each([&](float x, int) {
-      if (x == mx && own != mx) own = mx;
-      else if (x == mx) join(0.f);
-      else if (mx < INFINITY && x > -INFINITY) join((x - mx) * c);
+      const float t = x == mx ? 0.f : mx < INFINITY && x > -INFINITY ? fmaxf((x - mx) * c, -200.f) : -200.f, w = exp2_fast(t);
+      if (x == mx && own != mx) {
+        own = mx;
+      } else {
+        s += (double)w;
+        e += (double)(w * t);
+      }
     });
+    sum_S = (float)s;
+    sum_E = (float)e;
     r2 = (double)mx * (double)c;
   } else {
     // the vectors left out, by their place (the order in which they came must not matter)

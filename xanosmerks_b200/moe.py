@@ -70,6 +70,14 @@ class MoELayer:
             raise NotImplementedError("all expert weights must share one block type")
         self.qtype = qt.pop()
         E = self.num_experts
+        # (the kernels go by these sizes alone)
+        if self.gate.shape[0] != E:
+            raise ValueError(f"MoELayer: gate.weight has {self.gate.shape[0]} rows for {E} experts")
+        up, down = (self.intermediate, self.hidden), (self.hidden, self.intermediate)
+        for i in range(E):
+            for name, w, shape in (("w1", self.w1[i], up), ("w3", self.w3[i], up), ("w2", self.w2[i], down)):
+                if w.shape != shape or w.device != self.device:
+                    raise ValueError(f"MoELayer: {name} of expert {i} is {w.shape} on {w.device}, not {shape} on {self.device}")
         self._p1 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w1])
         self._p3 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w3])
         self._p2 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w2])

@@ -40,7 +40,7 @@ from ._lib import DT_F16, DT_F32, PRO_NONE, PRO_RMSNORM, PRO_SWIGLU, check, chec
 from .kvcache import PagedKVCache, rope_table
 from .moe import MoELayer
 from .ops import GGUFTensor, gemm_supported, residual_norm
-from .sampling import TokenLogprobs, logprobs, sample
+from .sampling import MAX_TOP, TokenLogprobs, logprobs, sample
 from .synth import make_weight_device
 
 __all__ = ["LlamaConfig", "LlamaWeights", "LlamaDecoder", "synth_llama_weights", "shard_rows", "shard_cols"]
@@ -592,8 +592,10 @@ class LlamaDecoder:
             self._gemv(wt, x, rows, y, prologue, norm, accumulate)
 
     def _prefill_gemm(self, ids: torch.Tensor) -> torch.Tensor:
+        self._check_prompt(ids)
         B, S = self.B, ids.shape[1]
         h = self._prefill_rows(ids)
+        self._draw()
         # the output head on each sequence's last token (the decode state keeps those rows)
         self.h[:B].copy_(h.view(B, S, self.cfg.hidden_size)[:, S - 1])
         self._head(1)
@@ -601,17 +603,20 @@ class LlamaDecoder:
         self.length = S
         return self.next_ids
 
-    def _prefill_rows(self, ids: torch.Tensor) -> torch.Tensor:
-        """The residual stream [B * S, hidden] behind the last layer of a prompt entering an empty cache."""
-        cfg, B = self.cfg, self.B
-        S = ids.shape[1]
+    def _check_prompt(self, ids: torch.Tensor):
+        B, S = self.B, ids.shape[1]
         if ids.shape[0] != B:
             raise ValueError(f"ids must be [{B}, S], got {tuple(ids.shape)}")
         if S > self.max_ctx:
             raise ValueError(f"context overflow: {S} > {self.max_ctx}")
         lo, hi = int(ids.min()), int(ids.max())
-        if lo < 0 or hi >= cfg.vocab_size:
-            raise ValueError(f"token ids must lie in [0, {cfg.vocab_size}), got [{lo}, {hi}]")
+        if lo < 0 or hi >= self.cfg.vocab_size:
+            raise ValueError(f"token ids must lie in [0, {self.cfg.vocab_size}), got [{lo}, {hi}]")
+
+    def _prefill_rows(self, ids: torch.Tensor) -> torch.Tensor:
+        """The residual stream [B * S, hidden] behind the last layer of a prompt (checked) entering an empty cache."""
+        cfg, B = self.cfg, self.B
+        S = ids.shape[1]
         rows = B * S                                       # row b*S + s: token s of sequence b
         D, hd = cfg.hidden_size, cfg.head_dim
         f32 = dict(dtype=torch.float32, device=self.dev)
@@ -630,7 +635,6 @@ class LlamaDecoder:
         whole = S >= 16 or self.kv_type is not None
         if self.kv_type is not None:
             self.kv_lens.fill_(S)
-        self._draw()
         zeros_b = torch.zeros(B, dtype=torch.int32, device=self.dev)
         for li, lw in enumerate(self.w.layers):
             self._gemm(lw["qkv"], h, rows, qkv, PRO_RMSNORM, lw["attn_norm"])
@@ -684,10 +688,15 @@ class LlamaDecoder:
     def score(self, ids, temperature: float = 1.0, top: int = 0) -> TokenLogprobs:
         """Log-probabilities of sequences ids [B, S], 2 <= S <= max_ctx: what each token i + 1 has behind the tokens 0 .. i, with
         the entropy there, the token's rank and the ``top`` largest alternatives (see
-        :func:`~xanosmerks_b200.sampling.logprobs`); every tensor begins [B, S - 1].  The decoder is reset before and after."""
+        :func:`~xanosmerks_b200.sampling.logprobs`); every tensor begins [B, S - 1].  The decoder is reset before and after; a refused
+        call leaves it as it was, and the random numbers of ``set_sampling`` go on where they were."""
         ids = torch.as_tensor(np.asarray(ids) if not isinstance(ids, torch.Tensor) else ids)
         if ids.dim() != 2 or ids.shape[1] < 2:
             raise ValueError(f"score: ids must be [{self.B}, S] with two tokens or more, got {tuple(ids.shape)}")
+        self._check_prompt(ids)
+        most = min(MAX_TOP, self.cfg.vocab_size)
+        if not 0 <= top <= most:
+            raise ValueError(f"score: {top} alternatives (0 to {most})")
         self.reset()
         B, S = ids.shape
         h = self._prefill_rows(ids)

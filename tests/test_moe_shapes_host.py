@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from xanosmerks_b200 import qtypes
+from xanosmerks_b200._lib import XMError
 from xanosmerks_b200.moe import MoELayer
 from xanosmerks_b200.ops import GGUFTensor
 
@@ -45,3 +46,14 @@ def test_gate():
 def test_device():
     with pytest.raises(ValueError, match="of expert 2"):
         layer(w3_2=weight(F, H, device="meta"))
+
+
+def test_a_layer_without_steps_table(monkeypatch):
+    """Where the table of the step cannot be made, the layer is there for the block of many tokens."""
+    def fails(self):
+        raise XMError("moe step: tensor map")
+    monkeypatch.setattr(MoELayer, "_step_table", fails)
+    made = layer()
+    assert made._table is None and made.hidden == H
+    with pytest.raises(XMError):
+        made.step(torch.zeros(1, H))

@@ -16,6 +16,7 @@ they chose, with the norm before the layer and the residual add behind it.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -82,11 +83,12 @@ class MoELayer:
         self._p3 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w3])
         self._p2 = (ctypes.c_void_p * E)(*[w.data.data_ptr() for w in self.w2])
         self._is_dense = self.num_experts_per_tok == self.num_experts
-        # step()'s, made here where it takes these sizes (not by a first call inside a capture)
+        # step()'s, made here where it takes these sizes (not by a first call inside a capture); a failure is step()'s to raise
         self._table = None
         if lib.xm_moe_step_workspace_size(1, self.hidden, self.intermediate, E, self.num_experts_per_tok, self.qtype) > 0 \
                 and not any(w.data.data_ptr() & 15 for w in self.w1 + self.w3 + self.w2):
-            self._step_table()
+            with contextlib.suppress(XMError):
+                self._step_table()
 
     STEP_TOKENS = 64   # tokens of a step at most
 

@@ -135,8 +135,15 @@ class LlamaWeights:
     (:class:`~xanosmerks_b200.moe.MoELayer`) instead of ``gate_up`` and ``down``."""
 
     def __init__(self, cfg: LlamaConfig, embed, layers, norm, output, rank=0, world=1):
+        self._check_world(cfg, world)
         self.cfg, self.embed, self.layers, self.norm, self.output = cfg, embed, layers, norm, output
         self.rank, self.world = rank, world
+
+    @staticmethod
+    def _check_world(cfg: LlamaConfig, world: int):
+        if world > 1 and (cfg.num_experts or cfg.post_norms or cfg.residual_scale != 1.0):
+            raise NotImplementedError("LlamaWeights: experts, norms behind blocks and residual scales on one rank only (a "
+                                      "tensor-parallel block's output is summed into the residual stream as it is)")
 
     @classmethod
     def from_full(cls, cfg: LlamaConfig, full: dict, rank: int = 0, world: int = 1) -> "LlamaWeights":
@@ -146,9 +153,7 @@ class LlamaWeights:
         hq, hk, hd, F = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.intermediate_size
         if hq % world or hk % world or F % world:
             raise ValueError(f"heads {hq}/{hk} and FFN {F} must divide by the world size {world}")
-        if world > 1 and (cfg.num_experts or cfg.post_norms or cfg.residual_scale != 1.0):
-            raise NotImplementedError("LlamaWeights: experts, norms behind blocks and residual scales on one rank only (a "
-                                      "tensor-parallel block's output is summed into the residual stream as it is)")
+        cls._check_world(cfg, world)
         hq_l, hk_l, f_l = hq // world, hk // world, F // world
         layers = []
         for lw in full["layers"]:

@@ -187,6 +187,14 @@ def _rows_and_pitch(t, d):
     return t, t.stride(0) if t.shape[0] > 1 else d
 
 
+def _rows_of(out, d):
+    """The rows [n, d] of out, or as many of their own where no one pitch leads from each to the next (a part of each sequence)."""
+    try:
+        return out.view(-1, d)
+    except RuntimeError:
+        return out.new_empty((out.numel() // d if d else 0, d))
+
+
 def _gate_rows(gate, shape, dev):
     """gate (anything that broadcasts to shape) as (rows [n, 1 or D], whether wide)."""
     if not isinstance(gate, torch.Tensor) or gate.dtype not in _DT or gate.device != dev or not 1 <= gate.dim() <= len(shape):
@@ -240,7 +248,7 @@ def residual_norm(stream: torch.Tensor, y: torch.Tensor, post_weight: torch.Tens
     else:
         if out.shape != shape or out.dtype != stream.dtype or out.device != dev:
             raise ValueError(f"residual_norm: out must be {stream.dtype} {tuple(shape)} on {dev}")
-        o2 = out if out.dim() == 2 else out.view(-1, d)
+        o2 = out if out.dim() == 2 else _rows_of(out, d)
         if d > 1 and o2.stride(1) != 1:
             raise ValueError("residual_norm: out must have unit stride in its last dimension")
         o_pitch = o2.stride(0) if o2.shape[0] > 1 else d
@@ -259,6 +267,8 @@ def residual_norm(stream: torch.Tensor, y: torch.Tensor, post_weight: torch.Tens
     check(call_on(dev, lib.xm_residual_norm, h2.data_ptr(), ht, h_pitch, y2.data_ptr(), yt, y_pitch, rows, d, weights[0], g_ptr,
                   g_type, g_pitch, g_wide, per, scale, weights[1], eps, o2.data_ptr(), o_pitch,
                   None if after is None else after.data_ptr(), ot, d), "residual_norm")
+    if out.data_ptr() != o2.data_ptr():
+        out.copy_(o2.view(shape))
     return out, after
 
 

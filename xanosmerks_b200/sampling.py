@@ -105,6 +105,8 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature=1.0, top: i
     pitch, one = logits.stride()
     if v > 1 and one != 1:
         raise ValueError("logprobs: logits must have unit stride in the last dimension")
+    if b > 1 and pitch < v:                            # rows that lie on one another (expanded: tokens under one row)
+        logits, pitch = logits.contiguous(), v
     if (not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1
             or tokens.shape[0] != b or tokens.device != dev or not tokens.is_contiguous()):
         raise ValueError(f"logprobs: tokens must be a contiguous int32 or int64 tensor [{b}] on {dev}")

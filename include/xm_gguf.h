@@ -465,9 +465,17 @@ int xm_sample(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t str
  * and rank -1.  NaN logits count as -inf (log-probability -inf); a row of
  * nothing else has entropy 0.  Logits of +inf share the mass.  T <= 0: the first
  * maximum has log-probability 0, the others -inf.  T is per row where
- * d_temperature is given.  The same call gives the same bits; B decides how many
- * CTAs share a row, and with it the last bits of its sums.  (The log-probability
- * that sampling.py:94-158 draws from, before its filters.)
+ * d_temperature is given.  Log-probabilities and entropies are good to 2^-16 of
+ * themselves, next to 0 too (to 2^-15 below 2^-31; a token whose share is below
+ * 2^-126 of the largest counts as 0).  The same call gives the same bits; B
+ * decides how many CTAs share a row, and with it the last bits of its sums.  A
+ * row is read once, some rows more often: a part of it (there are up to 8) in
+ * which more than 32 vectors of 16 bytes reach the largest logit seen so far
+ * (equal or rising logits throughout), one with a weight 2^100 times the
+ * first-seen ones' and one with +inf three times; and once for each alternative a
+ * part with some 2000 candidates for them (equal or rising logits, or a mask that
+ * leaves thousands of neighbouring tokens and nothing elsewhere).  (The
+ * log-probability that sampling.py:94-158 draws from, before its filters.)
  */
 int xm_logprobs(const void* d_logits, int dtype, int64_t B, int64_t V, int64_t stride, const void* d_tokens,
                 int token_bytes, float temperature, const float* d_temperature, int top, float* d_logprob,

@@ -8,7 +8,7 @@
 //
 // M is known at the end only.  Until then weights are relative to r, the largest logit that a CTA sees first (rounds of nothing
 // but -inf and NaN are passed over), and vectors with a logit at or above the largest one seen (r, raised whenever twice as much
-// has been seen: some six vectors of 16000) stay out of the sums.  Their logits are taken at the end, a thread each, and all but
+// has been seen: a few vectors of 16000) stay out of the sums.  Their logits are taken at the end, a thread each, and all but
 // one of M join; sums on other references meet by the difference of those, in 64 bits.  Where a weight reaches 2^100, a logit is +inf, or too many
 // vectors are left out (equal or rising logits throughout), the CTA takes its part of the row again with its own maximum.  A
 // weight's exponent is held above -200, which also gives -inf and NaN logits the weight 0 (and 0 in E).
@@ -23,7 +23,7 @@
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
 //
-// Measured, cold: 2048 rows of 32000 fp32 logits 53 to 56 us (4.7 to 4.9 TB/s); 2000 of 128001 fp16 with 8 alternatives 134 us
+// Measured, cold: 2048 rows of 32000 fp32 logits 53 to 56 us (4.7 to 4.9 TB/s); 2000 of 128001 fp16 with 8 alternatives 135 us
 // (3.8 TB/s); 64 of 128000 bf16 with 20, 19 us; one of 32000, 9 us in a captured graph.  (With the largest logit in the sums, and
 // entropies below 1e-4 good to three digits or none: 54 to 56, 129, 18.6 and 8.5.)
 #include <cooperative_groups.h>

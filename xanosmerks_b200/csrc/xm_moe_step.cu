@@ -30,7 +30,7 @@
 // Nothing waits for another CTA.  The results do not depend on the order in which CTAs run.
 //
 // Measured, a step from Python with its inputs and weights cold in L2: Q4_K, 4096 -> 14336, 2 of 8 experts, one token 58 us (the
-// chosen blocks at 3.4 TB/s), 7 bf16 tokens 170 to 190 us (3.6 to 3.8 TB/s); Q4_K, 8 of 128 experts, one token 30 us (26 in a
+// chosen blocks at 3.4 TB/s), 7 bf16 tokens 170 to 196 us (3.5 to 3.8 TB/s); Q4_K, 8 of 128 experts, one token 30 us (26 in a
 // captured graph); Q6_K, 8 of 128 experts, 33 tokens 177 us.  At most 58 % of the copy bandwidth: the products' instructions, which
 // take up to three quarters of the issue slots while a stage's bytes are there, are what a faster step would have fewer of.
 #include <cooperative_groups.h>

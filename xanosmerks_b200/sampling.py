@@ -96,7 +96,9 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature=1.0, top: i
 
     ``temperature``: a number, or an fp32 tensor [B]; 0: the first maximum has log-probability 0, the others -inf.  A token
     outside the vocabulary (-1 for padding, say) gives NaN and rank -1.  NaN logits count as -inf, which have
-    log-probability -inf; a row of nothing else has entropy 0.  Logits of +inf share the mass."""
+    log-probability -inf; a row of nothing else has entropy 0.  Logits of +inf share the mass.  Results are good to 2^-16 of
+    themselves, those of confident rows too.  Rows that lie on one another (``row.expand(B, -1)``: tokens under one row) are
+    copied.  With alternatives, rows of equal or rising logits throughout are read once for each of them."""
     dt = _DT.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
     if dt is None or logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1:
         raise ValueError("logprobs: logits must be a 2-D fp32, fp16 or bf16 CUDA tensor")

@@ -110,3 +110,15 @@ def test_many_logits_above_what_was_seen():
         r = logprobs(x, t, top=3)                      # (300 rows: one CTA each)
         some = [0, 100, 299]
         check([v[some] for v in (r.logprob, r.entropy, r.top_logprobs)], x[some], t[some], 1.0, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parts_whose_first_round_is_far_below_their_own_largest(dtype):
+    """A cluster's part with a largest logit far above what it sees first, and far below another part's."""
+    for most, second in ((100.0, 60.0), (80.0, 66.0), (140.0, 68.0), (60.0, 59.0)):
+        x = torch.randn(2, 128000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)) * 0.5
+        x[:, 5] = most
+        x[:, 16400:16460:7] = second + torch.linspace(-1, 1, 9, device="cuda")
+        x[1, 70000] = second - 0.5
+        compare(x.to(dtype), torch.tensor([5, 16400], device="cuda"))
+        compare((x * 0.1).to(dtype), torch.tensor([16407, 5], device="cuda"), T=0.1)

@@ -584,11 +584,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(LogpArgs a) {
             if (k == largest) s += q[h].S + (own ? 0.f : 1.f);
             continue;
           }
-          auto add = [&](double d, float S, float E) {          // sums on a reference of d + the largest
-            if (!(d > -200.)) return;
-            const float f = exp2f((float)d);
-            s = fmaf(f, S, s);
-            e += f * fmaf((float)d, S, E);
+          // sums on a reference of d + the largest, up to 2^100 and more: 2^d alone may be below fp32's numbers
+          auto add = [&](double d, float S, float E) {
+            if (!(d > -250.)) return;
+            const float whole = rintf((float)d);
+            const double f = (double)exp2f((float)(d - (double)whole)) * __hiloint2double((1023 + (int)whole) << 20, 0);
+            s += (float)(f * (double)S);
+            e += (float)(f * ((double)E + d * (double)S));
           };
           if (q[h].S > 0.f) add(o[h]->r - R, q[h].S, q[h].E);
           if (k && !own) add((double)q[h].peak * (double)c - R, 1.f, 0.f);

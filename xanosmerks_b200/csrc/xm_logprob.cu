@@ -23,8 +23,8 @@
 // C CTAs (a cluster) share a row where rows are few or long.  Bound: HBM and issue for many rows (each logit is read once; some
 // eight instructions a logit, sums and exponents two at a time, ranks and maxima of 16-bit logits too), latency for few.
 //
-// Measured, cold: 2048 rows of 32000 fp32 logits 53 to 56 us (4.7 to 4.9 TB/s); 2000 of 128001 fp16 with 8 alternatives 135 us
-// (3.8 TB/s); 64 of 128000 bf16 with 20, 19 us; one of 32000, 9 us in a captured graph.  (With the largest logit in the sums, and
+// Measured, cold: 2048 rows of 32000 fp32 logits 53 to 57 us (4.6 to 4.9 TB/s); 2000 of 128001 fp16 with 8 alternatives 135 to 142 us
+// (3.6 to 3.8 TB/s); 64 of 128000 bf16 with 20, 19.6 us, and one of 32000, 9.2 us, in a captured graph.  (With the largest logit in the sums, and
 // entropies below 1e-4 good to three digits or none: 54 to 56, 129, 18.6 and 8.5.)
 #include <cooperative_groups.h>
 
